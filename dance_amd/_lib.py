@@ -151,6 +151,17 @@ def _declare(lib):
         "dh_block_cells_static": (c_int, [i64, i64, i64, P, P, P, P, P, P, P, P, P, c_size_t, P]),
         "dh_csr_degree_scales_f32": (c_int, [i64, i64, i64, P, P, i32, P, P, P, P]),
         "dh_adam_step_f32": (c_int, [i32, P, P, P, P, P, P, c_float, c_float, c_float, c_float, c_float, P]),
+        "dh_grad_norm_workspace_bytes": (c_size_t, [i32, P]),
+        "dh_grad_norm": (c_int, [i32, P, P, P, i32, P, P, c_size_t, P]),
+        "dh_grad_clip": (c_int, [i32, P, P, P, P, P, i32, c_double, P, P, c_size_t, P]),
+        "dh_residual_norm_forward": (c_int, [i64, i64, i32, P, i64, P, i64, P, i64, i32, i32, c_float, i32, c_float, i32, P, P, i32, P, P, P, i64, P, i64,
+                                             P, P]),
+        "dh_residual_norm_backward_workspace_bytes": (c_size_t, [i64, i64]),
+        "dh_residual_norm_backward": (c_int, [i64, i64, i32, P, i64, P, i64, P, i64, i32, i32, c_float, i32, i32, P, P, i32, P, P, P, i64, P, i64, P, i64,
+                                              P, i64, P, i64, P, P, P, P, P, c_size_t, P]),
+        "dh_gemm_grouped": (c_int, [i64, i64, i64, i64, i32, i32, P, i64, P, i64, i64, P, P, i64, i32, P, i64, i32, i32, P]),
+        "dh_gemm_grouped_wgrad_workspace_bytes": (c_size_t, [i64, i64, i64]),
+        "dh_gemm_grouped_wgrad": (c_int, [i64, i64, i64, i64, i32, P, i64, P, i64, P, P, i64, i64, i32, P, i64, P, c_size_t, P]),
         "dh_sage_alpha_grad_f32": (c_int, [i64, i64, i64, i64, P, P, P, P, P, P, i64, P, i64, P, P]),
         "dh_dec_target_f32": (c_int, [i64, i64, P, i64, P, P, i64, P]),
         "dh_dec_kl_workspace_bytes": (c_size_t, []),

@@ -695,3 +695,114 @@ def student_t_assign(z: torch.Tensor, mu: torch.Tensor, *, a: float, eps: float,
     q = 1.0 / ((1.0 + torch.sum((z.unsqueeze(1) - mu)**2, dim=2) / a) + eps)
     q = q**pw * scale
     return q / torch.sum(q, dim=1, keepdim=True)
+
+
+class _GroupedLinearFn(torch.autograd.Function):
+    """y[i] = act(W_g x[i] + b_g) over rows sorted by group (csrc/gemm_grouped.hip), with the gradients of x, W and b.
+
+    fp32, or bf16 rows with bf16 or fp32 weights (fp32 ones are rounded to bf16 for the products, as in _LinearFn; dW then comes back in
+    fp32).  Accumulation is fp32; with a ReLU the mask is the sign of the stored y."""
+
+    @staticmethod
+    def forward(ctx, x, weight, group_ptr, bias, relu):
+        x = _rows(x)
+        w = weight.detach()
+        if x.dtype == torch.bfloat16 and w.dtype == torch.float32:
+            w = w.to(torch.bfloat16)
+        w = w if w.dim() == 3 and (w.numel() == 0 or w.stride(-1) == 1) else w.contiguous()
+        b = None if bias is None else bias.detach().float().contiguous()
+        y = kernels.gemm_grouped(x, w, group_ptr, trans_b=True, bias=b, act=kernels.ACT_RELU if relu else kernels.ACT_NONE)
+        ctx.relu, ctx.w_dtype, ctx.b_dtype = relu, weight.dtype, None if bias is None else bias.dtype
+        ctx.save_for_backward(x, w, group_ptr, y if relu else None)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, w, group_ptr, y = ctx.saved_tensors
+        dy = _rows(dy)
+        if ctx.relu:
+            dy = kernels.relu_backward_bf16(y, dy) if dy.dtype == torch.bfloat16 else kernels.relu_backward(y, dy)
+        dx = dw = db = None
+        if ctx.needs_input_grad[0]:
+            dx = kernels.gemm_grouped(dy, w, group_ptr, trans_b=False)
+        want_b = ctx.b_dtype is not None and ctx.needs_input_grad[3]
+        if ctx.needs_input_grad[1] or want_b:
+            dw = kernels.gemm_grouped_wgrad(dy, x, group_ptr, out_dtype=ctx.w_dtype, want_bias=want_b)
+            if want_b:
+                dw, db = dw
+                db = db.to(ctx.b_dtype)
+        return dx, dw if ctx.needs_input_grad[1] else None, None, db, None
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """t itself where its rows are contiguous and do not overlap, else a contiguous copy (expanded and transposed tensors)."""
+    if t.dim() == 2 and (t.numel() == 0 or (t.stride(1) == 1 and (t.shape[0] == 1 or t.stride(0) >= t.shape[1]))):
+        return t
+    return t.contiguous()
+
+
+def grouped_linear(x: torch.Tensor, weight: torch.Tensor, group_ptr: torch.Tensor, bias: Optional[torch.Tensor] = None, *, relu: bool = False):
+    """``linear`` with one weight per row type: y[i] = act(x[i] weight[g]^T + bias[g]) for group_ptr[g] <= i < group_ptr[g + 1].
+
+    x [M, K] (fp32 or bf16) with rows sorted by type, weight [G, N, K], bias [G, N], group_ptr int32 [G + 1] on the device.  Rows of no
+    type (before group_ptr[0], from group_ptr[G] on) give zeros and receive zero gradients."""
+    return _GroupedLinearFn.apply(x, weight, group_ptr, bias, relu)
+
+
+class _ResidualNormFn(torch.autograd.Function):
+    """(r, h) of ``residual_norm`` in one pass over f and x; backward in one pass over f, x, dr, dh (csrc/residual_norm.hip)."""
+
+    @staticmethod
+    def forward(ctx, f, x, gate, w1, b1, w2, b2, opts):
+        has_post, has_pre, kind, gate_sigmoid, scale, eps = opts
+        ctx.set_materialize_grads(False)
+        f, x = _rows(f), None if x is None else _rows(x)
+        if gate is not None and gate.dim() == 2:
+            gate = _rows(gate)
+        elif gate is not None:
+            gate = gate.contiguous()
+        params = [None if p is None else p.contiguous() for p in (w1, b1, w2, b2)]
+        post = (params[0], params[1]) if has_post else None
+        pre = (params[2], params[3]) if has_pre else None
+        r, h, stats = kernels.residual_norm_forward(f, x, post=post, gate=gate, gate_sigmoid=gate_sigmoid, scale=scale, pre=pre, kind=kind, eps=eps,
+                                                    want_stats=any(ctx.needs_input_grad))
+        ctx.opts = opts
+        ctx.save_for_backward(f, x, gate, *params, stats)
+        return (r, h) if has_pre else r
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dr, dh=None):
+        f, x, gate, w1, b1, w2, b2, stats = ctx.saved_tensors
+        has_post, has_pre, kind, gate_sigmoid, scale, _ = ctx.opts
+        names = ("f", "x", "gate", "w1", "b1", "w2", "b2")
+        if dr is None and dh is None:
+            return (None, ) * 8
+        want = [n for n, need in zip(names, ctx.needs_input_grad) if need]
+        g = kernels.residual_norm_backward(None if dr is None else _rows(dr), None if dh is None else _rows(dh), f, x, stats,
+                                           post=(w1, b1) if has_post else None, gate=gate, gate_sigmoid=gate_sigmoid, scale=scale,
+                                           pre=(w2, b2) if has_pre else None, kind=kind, want=want)
+        return tuple(g.get(n) for n in names) + (None, )
+
+
+def residual_norm(f: torch.Tensor, x: Optional[torch.Tensor] = None, *, post=None, gate: Optional[torch.Tensor] = None, gate_act: str = "none",
+                  scale: float = 1.0, pre=None, kind: str = "layer", eps: float = 1e-5):
+    """What stands between two blocks of a residual network, in one kernel: with f the output of a block and x the stream it was taken from,
+
+        r = x + scale * act(gate) * norm(f; post)        (norm left out without ``post``, x = 0 without x)
+        h = norm(r; pre)                                 (None without ``pre``): the next block's input
+
+    Returns (r, h).  f, x [M, D] fp32 or bf16 (D <= 4096); ``post`` / ``pre``: (weight, bias), fp32 [D], None for no weight or no bias;
+    ``kind``: "layer" or "rms"; gate: fp32 [] / [1] (one for all) or [D] (per column), or of f's dtype [M, 1] (per row) or [M, D];
+    ``gate_act``: "none" or "sigmoid".  h is computed from the unrounded r.  Gradients of f, x, gate and all parameters."""
+    if kind not in ("layer", "rms"):
+        raise ValueError(f"residual_norm: kind must be 'layer' or 'rms', got {kind!r}")
+    if gate_act not in ("none", "sigmoid"):
+        raise ValueError(f"residual_norm: gate_act must be 'none' or 'sigmoid', got {gate_act!r}")
+    w1, b1 = post if post is not None else (None, None)
+    w2, b2 = pre if pre is not None else (None, None)
+    opts = (post is not None, pre is not None, kernels.NORM_LAYER if kind == "layer" else kernels.NORM_RMS, gate_act == "sigmoid", float(scale),
+            float(eps))
+    out = _ResidualNormFn.apply(f, x, gate, w1, b1, w2, b2, opts)
+    return out if pre is not None else (out, None)

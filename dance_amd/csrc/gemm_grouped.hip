@@ -1,0 +1,568 @@
+// Products grouped by row type with ragged group sizes: one weight per type (tissue, donor, node type), rows sorted by type.
+//
+//   forward     Y[i] = act(X[i] op(W_g) + b_g)            op(W_g) = W_g^T (W [G][N][K], torch.nn.Linear's layout) or W_g (W [G][K][N])
+//   gradient    dX   = the same product with the other op;   dW_g = sum_i dY[i]^T X[i],  db_g = sum_i dY[i]
+//   for the rows ptr[g] <= i < ptr[g + 1] of group g.
+//
+// The bounds ptr stay on the device: no launch depends on their values.  A launch covers every possible raggedness with a closed form of
+// them: group g owns the row slots [floor(ptr[g] / R) + g, floor(ptr[g + 1] / R) + g + 1), R rows each, always enough for its
+// ceil(len / R) tiles and monotone in g, so a workgroup finds its group with one 64-wide search per 64 groups instead of a prefix sum;
+// at most one slot per group and none of the work is wasted on it.
+#include <type_traits>
+
+#include "common.h"
+
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned int u32x4u __attribute__((ext_vector_type(4), aligned(2)));  // 16 bytes at an element's own alignment
+
+__device__ __forceinline__ float bf16_f32(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
+__device__ __forceinline__ uint16_t f32_bf16(float x) {  // nearest even; NaN stays a quiet NaN
+  const uint32_t u = __float_as_uint(x);
+  if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)((u >> 16) | 0x40u);
+  return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
+}
+
+// ---- groups --------------------------------------------------------------------------------------------------------------------------
+// The bounds with a group of "no weight" in front (rows before ptr[0]) and behind (rows from ptr[G] on): edge(0) = 0, edge(i) = ptr[i - 1],
+// edge(G + 2) = M.  Values outside [0, M] are clamped, so a wrong table can cost wrong rows but no access out of bounds.
+struct Groups {
+  const int32_t* ptr;
+  int64_t M;
+  int G;
+  __device__ __forceinline__ int64_t edge(int i) const {
+    if (i <= 0) return 0;
+    if (i >= G + 2) return M;
+    const int64_t v = ptr[i - 1];
+    return v < 0 ? 0 : v > M ? M : v;
+  }
+};
+
+// the last i in [0, n) with key(i) <= s, key non-decreasing and key(0) <= s: 64 probes at a time
+template <class Key>
+__device__ __forceinline__ int search(int n, int64_t s, Key key) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, len = n;
+  while (len > 1) {
+    const int step = (len + 63) / 64, i = lo + lane * step;
+    const bool le = i < lo + len && key(i) <= s;
+    const unsigned long long mask = __ballot(le);
+    const int last = mask ? 63 - __builtin_clzll(mask) : 0;
+    const int next = lo + last * step;
+    len = min(step, lo + len - next);
+    lo = next;
+  }
+  return __builtin_amdgcn_readfirstlane(lo);
+}
+
+struct Slot {
+  int group;       // -1: rows that belong to no group
+  int64_t begin, end, start;  // the slot's rows; start: the group's first row
+  int index;       // number of the slot within its group
+  bool live;
+};
+
+// slot s of R rows (R a power of two: shift)
+__device__ __forceinline__ Slot find_slot(const Groups& gr, int64_t s, int shift) {
+  const int n = gr.G + 2;
+  const int i = search(n, s, [&](int j) { return (gr.edge(j) >> shift) + j; });
+  const int64_t a = gr.edge(i), b = gr.edge(i + 1);
+  const int64_t first = (a >> shift) + i;
+  Slot r;
+  r.group = i == 0 || i == n - 1 ? -1 : i - 1;
+  r.start = a;
+  r.index = (int)(s - first);
+  r.begin = a + ((int64_t)r.index << shift);
+  r.end = min(b, r.begin + ((int64_t)1 << shift));
+  r.live = r.index >= 0 && r.begin < b;
+  return r;
+}
+
+// the logical number of a workgroup: the dispatcher deals workgroups round robin to the 8 XCDs; handing each XCD a contiguous run keeps
+// the tiles that share an operand panel on one L2
+__device__ __forceinline__ int64_t xcd_run(int64_t bid, int64_t n) {
+  const int64_t q = n / 8, r = n % 8, xcd = bid % 8;
+  return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + bid / 8;
+}
+
+// ---- operand tiles -------------------------------------------------------------------------------------------------------------------
+template <class T>
+struct Geo;
+template <>
+struct Geo<uint16_t> {
+  static constexpr int VEC = 8, BK = 64, LD_MK = 72;  // 144-byte rows: the 16-byte fragment reads of 32 rows fall on distinct banks
+};
+template <>
+struct Geo<float> {
+  static constexpr int VEC = 4, BK = 32, LD_MK = 36;
+};
+
+// R rows (m or n) x BK of an operand.  KM = false: memory is [row][k]; true: [k][row].  Both stay as they lie in memory in LDS too:
+// a [k][row] image is read back transposed (bf16: ds_read_b64_tr_b16) or by single elements (fp32).
+template <class T, bool KM, int R, int THREADS>
+struct Operand {
+  static constexpr int VEC = Geo<T>::VEC, BK = Geo<T>::BK;
+  // [k][row] images: bf16 rows of R + 32 elements (64 bytes past a multiple of 256: the four k rows that one transposing read takes from
+  // lie on distinct banks); fp32 rows of R + 8 (the two half waves read rows 4 apart: 32 banks apart)
+  static constexpr int LD = KM ? (sizeof(T) == 2 ? R + 32 : R + 8) : Geo<T>::LD_MK;
+  static constexpr int ELEMS = KM ? BK * LD : R * LD;
+  static constexpr int CPR = KM ? R / VEC : 8;                        // 16-byte pieces per image row
+  static constexpr int PIECES = (KM ? BK : R) * CPR / THREADS;        // per thread
+  static constexpr int ROWS_PER_PASS = THREADS / CPR;
+  static_assert(PIECES >= 1 && PIECES * THREADS == (KM ? BK : R) * CPR, "tile does not divide among the threads");
+
+  u32x4 reg[PIECES];
+
+  static __device__ __forceinline__ u32x4 guarded(const T* p, int64_t n_valid) {
+    if (n_valid >= VEC) return *reinterpret_cast<const u32x4u*>(p);
+    T e[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) e[i] = i < n_valid ? p[i] : T(0);
+    u32x4 v;
+    __builtin_memcpy(&v, e, 16);
+    return v;
+  }
+  // rows [r0, rlim) of the operand, k in [k0, klim).  Rows beyond rlim read some row below it (their products are never stored);
+  // k beyond klim reads as zero.  FULL: the whole BK lies below klim (and for KM all R rows below rlim).
+  template <bool FULL>
+  __device__ __forceinline__ void load(const T* base, int64_t ld, int64_t r0, int64_t rlim, int64_t k0, int64_t klim) {
+    const int tid = threadIdx.x;
+#pragma unroll
+    for (int q = 0; q < PIECES; ++q) {
+      const int ir = tid / CPR + q * ROWS_PER_PASS, ic = (tid % CPR) * VEC;
+      if (!KM) {
+        const int64_t row = min(r0 + ir, rlim - 1), k = k0 + ic;
+        const T* p = base + row * ld + k;
+        if (FULL) reg[q] = *reinterpret_cast<const u32x4u*>(p);
+        else reg[q] = guarded(p, klim - k);
+      } else {
+        const int64_t k = k0 + ir, row = r0 + ic;
+        const T* p = base + k * ld + row;
+        if (FULL) reg[q] = *reinterpret_cast<const u32x4u*>(p);
+        else reg[q] = guarded(p, k < klim ? rlim - row : 0);
+      }
+    }
+  }
+  __device__ __forceinline__ void store(T* img) const {
+    const int tid = threadIdx.x;
+#pragma unroll
+    for (int q = 0; q < PIECES; ++q) {
+      const int ir = tid / CPR + q * ROWS_PER_PASS, ic = (tid % CPR) * VEC;
+      *reinterpret_cast<u32x4*>(img + ir * LD + ic) = reg[q];
+    }
+  }
+  // bf16: the 32x32x16 fragment of rows [row, row + 32), k [kk, kk + 16): lane l holds row l & 31, k (l >> 5) * 8 .. + 8
+  static __device__ __forceinline__ bf16x8 frag_bf16(const uint16_t* img, int row, int kk) {
+    const int lane = threadIdx.x & 63;
+    if (!KM) return *reinterpret_cast<const bf16x8*>(img + (row + (lane & 31)) * LD + kk + (lane >> 5) * 8);
+    // ds_read_b64_tr_b16: 16 lanes fetch a 4 (k) x 16 (row) block, lane 4 r + c the four elements c of row r, and each receives one column of it
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef s16x4 __attribute__((address_space(3))) * lds_s16x4;
+    const int b = lane >> 4, i = lane & 15;
+    const uint16_t* p = img + (kk + (b >> 1) * 8 + (i >> 2)) * LD + row + (b & 1) * 16 + (i & 3) * 4;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)p);
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(p + 4 * LD));
+    bf16x8 f;
+    __builtin_memcpy(&f, &lo, 8);
+    __builtin_memcpy(reinterpret_cast<char*>(&f) + 8, &hi, 8);
+    return f;
+  }
+  // fp32: k = kk + 4 (lane >> 5) + s for the four 32x32x2 steps s (the same permutation of k on both operands)
+  static __device__ __forceinline__ f32x4 frag_f32(const float* img, int row, int kk) {
+    const int lane = threadIdx.x & 63, r = row + (lane & 31), k = kk + 4 * (lane >> 5);
+    if (!KM) return *reinterpret_cast<const f32x4*>(img + r * LD + k);
+    f32x4 f;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) f[s] = img[(k + s) * LD + r];
+    return f;
+  }
+};
+
+// ---- the tile ------------------------------------------------------------------------------------------------------------------------
+// BM x BN of C = A B^T over k in [0, K): WR x WC waves of MI x NI 32 x 32 accumulators.  Two LDS stages: while the products of one step
+// run, the next one's pieces (requested a step earlier) are written and the ones after that requested.
+template <class T, bool A_KM, bool B_KM, int MI, int NI, int WR, int WC>
+struct Tile {
+  static constexpr int BM = MI * WR * 32, BN = NI * WC * 32, THREADS = WR * WC * 64, BK = Geo<T>::BK;
+  typedef Operand<T, A_KM, BM, THREADS> OpA;
+  typedef Operand<T, B_KM, BN, THREADS> OpB;
+  static constexpr int STAGE = OpA::ELEMS + OpB::ELEMS, LDS_BYTES = 2 * STAGE * (int)sizeof(T);
+
+  f32x16 acc[MI][NI];
+
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NI; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+  }
+  __device__ __forceinline__ void products(const T* st) {
+    const int wave = threadIdx.x >> 6, wm = (wave / WC) * MI * 32, wn = (wave % WC) * NI * 32;
+    const T *ia = st, *ib = st + OpA::ELEMS;
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int kk = 0; kk < BK; kk += 16) {
+        bf16x8 a[MI], b[NI];
+#pragma unroll
+        for (int i = 0; i < MI; ++i) a[i] = OpA::frag_bf16(ia, wm + i * 32, kk);
+#pragma unroll
+        for (int j = 0; j < NI; ++j) b[j] = OpB::frag_bf16(ib, wn + j * 32, kk);
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+          for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], b[j], acc[i][j], 0, 0, 0);
+      }
+    } else {
+#pragma unroll
+      for (int kk = 0; kk < BK; kk += 8) {
+        f32x4 a[MI], b[NI];
+#pragma unroll
+        for (int i = 0; i < MI; ++i) a[i] = OpA::frag_f32(ia, wm + i * 32, kk);
+#pragma unroll
+        for (int j = 0; j < NI; ++j) b[j] = OpB::frag_f32(ib, wn + j * 32, kk);
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+          for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i][s], b[j][s], acc[i][j], 0, 0, 0);
+      }
+    }
+  }
+  // seen(opB or opA): called with the A operand's registers of every step (the bias gradient's column sums)
+  template <class Seen>
+  __device__ __forceinline__ void run(const T* A, int64_t lda, int64_t m0, int64_t mlim, const T* B, int64_t ldb, int64_t n0, int64_t nlim,
+                                      int64_t k_begin, int64_t k_end, T* lds, Seen&& seen) {
+    zero();
+    if (k_end <= k_begin) return;
+    const bool whole = (!A_KM || m0 + BM <= mlim) && (!B_KM || n0 + BN <= nlim);
+    OpA a;
+    OpB b;
+    auto fetch = [&](int64_t k0) __attribute__((always_inline)) {
+      if (whole && k0 + BK <= k_end) {
+        a.template load<true>(A, lda, m0, mlim, k0, k_end);
+        b.template load<true>(B, ldb, n0, nlim, k0, k_end);
+      } else {
+        a.template load<false>(A, lda, m0, mlim, k0, k_end);
+        b.template load<false>(B, ldb, n0, nlim, k0, k_end);
+      }
+    };
+    auto put = [&](int stage) __attribute__((always_inline)) {
+      a.store(lds + stage * STAGE);
+      b.store(lds + stage * STAGE + OpA::ELEMS);
+      seen(a);
+    };
+    const int64_t steps = (k_end - k_begin + BK - 1) / BK;
+    fetch(k_begin);
+    put(0);
+    if (steps > 1) fetch(k_begin + BK);
+    __syncthreads();
+    for (int64_t t = 0; t < steps; ++t) {
+      if (t + 1 < steps) {
+        put((t + 1) & 1);
+        if (t + 2 < steps) fetch(k_begin + (t + 2) * BK);
+      }
+      products(lds + (t & 1) * STAGE);
+      __syncthreads();
+    }
+  }
+  // f(m, n, value) for the tile's elements: 32x32 accumulator layout: column lane & 31, row (r & 3) + 8 (r >> 2) + 4 (lane >> 5)
+  template <class F>
+  __device__ __forceinline__ void each(int64_t m0, int64_t mlim, int64_t n0, int64_t nlim, F&& f) const {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NI; ++j) {
+        const int64_t n = n0 + (wave % WC) * NI * 32 + j * 32 + (lane & 31);
+        if (n >= nlim) continue;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int64_t m = m0 + (wave / WC) * MI * 32 + i * 32 + (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5);
+          if (m < mlim) f(m, n, acc[i][j][r]);
+        }
+      }
+  }
+};
+
+// ---- forward (and dX) ----------------------------------------------------------------------------------------------------------------
+struct FwdArgs {
+  Groups gr;
+  int64_t N, K;
+  const void *X, *W;
+  int64_t ldx, ldw, stride_w;
+  const float* bias;  // [G][N]
+  int64_t ld_bias;
+  void* Y;
+  int64_t ldy;
+  int act, y_bf16, zero_outside;
+};
+
+template <class T, bool W_KM, int MI, int NI, int WR, int WC>
+__global__ __launch_bounds__(WR* WC * 64) void grouped_forward_kernel(const FwdArgs a) {
+  typedef Tile<T, false, W_KM, MI, NI, WR, WC> TileT;
+  extern __shared__ __attribute__((aligned(16))) unsigned char raw_lds[];
+  const int64_t tiles_n = (a.N + TileT::BN - 1) / TileT::BN;
+  const int64_t id = xcd_run(blockIdx.x, gridDim.x);
+  const Slot s = find_slot(a.gr, id / tiles_n, __builtin_ctz(TileT::BM));
+  if (!s.live) return;
+  const int64_t n0 = (id % tiles_n) * TileT::BN;
+  auto put = [&](int64_t m, int64_t n, float v) __attribute__((always_inline)) {
+    if (a.y_bf16) static_cast<uint16_t*>(a.Y)[m * a.ldy + n] = f32_bf16(v);
+    else static_cast<float*>(a.Y)[m * a.ldy + n] = v;
+  };
+  TileT t;
+  if (s.group < 0) {
+    if (!a.zero_outside) return;
+    t.zero();
+    t.each(s.begin, s.end, n0, a.N, put);
+    return;
+  }
+  t.run(static_cast<const T*>(a.X), a.ldx, s.begin, s.end, static_cast<const T*>(a.W) + s.group * a.stride_w, a.ldw, n0, a.N, 0, a.K,
+        reinterpret_cast<T*>(raw_lds), [](const auto&) {});
+  const float* bias = a.bias ? a.bias + s.group * a.ld_bias : nullptr;
+  t.each(s.begin, s.end, n0, a.N, [&](int64_t m, int64_t n, float v) __attribute__((always_inline)) {
+    if (bias) v += bias[n];
+    if (a.act == DH_ACT_RELU) v = v < 0.f ? 0.f : v;  // (a NaN passes)
+    put(m, n, v);
+  });
+}
+
+// ---- dW, db --------------------------------------------------------------------------------------------------------------------------
+// dW_g [N][K] = sum over the group's rows of dY[i, n] X[i, k]: both operands [k][row] images with the rows as the contraction.  Long groups
+// are cut into chunks of 2^shift rows; a group of one chunk is finished in place, the chunks of a longer one go to partial slots that
+// wgrad_join_kernel adds in chunk order (no atomics).  The slot of chunk j that starts at row s: 2 (s >> shift) + (j > 0): two chunks of
+// longer groups that start inside the same 2^shift rows are the last of one group (j > 0) and the first of the next (j = 0).
+struct WgradArgs {
+  Groups gr;
+  int64_t N, K;
+  const void *dY, *X;
+  int64_t ldy, ldx;
+  void* dW;
+  int64_t ldw, stride_w;
+  int dw_bf16;
+  float* db;  // [G][N] or null
+  int64_t ld_db;
+  float* part_w;  // [slots][N][K]
+  float* part_b;  // [slots][N]
+  int shift;
+  int64_t tiles_k, tiles;
+};
+
+template <class T, int MI, int NI, int WR, int WC>
+__global__ __launch_bounds__(WR* WC * 64) void grouped_wgrad_kernel(const WgradArgs a) {
+  typedef Tile<T, true, true, MI, NI, WR, WC> TileT;
+  typedef typename TileT::OpA OpA;
+  extern __shared__ __attribute__((aligned(16))) unsigned char raw_lds[];
+  const int64_t id = xcd_run(blockIdx.x, gridDim.x);
+  const Slot s = find_slot(a.gr, id / a.tiles, a.shift);
+  if (s.group < 0) return;
+  const int64_t glen = a.gr.edge(s.group + 2) - s.start;
+  if (!s.live && !(glen <= 0 && s.index == 0)) return;  // an empty group's one slot writes its zeros
+  const int64_t tile = id % a.tiles, n0 = (tile / a.tiles_k) * TileT::BM, k0 = (tile % a.tiles_k) * TileT::BN;
+  const bool alone = glen <= ((int64_t)1 << a.shift);
+  const bool sums = a.db && k0 == 0;
+  constexpr int VEC = Geo<T>::VEC;
+  float cs[OpA::PIECES > 0 ? VEC : 1];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) cs[e] = 0.f;
+  TileT t;
+  t.run(static_cast<const T*>(a.dY), a.ldy, n0, a.N, static_cast<const T*>(a.X), a.ldx, k0, a.K, s.begin, s.live ? s.end : s.begin,
+        reinterpret_cast<T*>(raw_lds), [&](const OpA& op) __attribute__((always_inline)) {
+          if (!sums) return;
+#pragma unroll
+          for (int q = 0; q < OpA::PIECES; ++q) {
+            T e[VEC];
+            __builtin_memcpy(e, &op.reg[q], 16);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+              if constexpr (sizeof(T) == 2) cs[i] += bf16_f32(e[i]);
+              else cs[i] += e[i];
+            }
+          }
+        });
+  const int64_t slot = alone ? 0 : 2 * (s.begin >> a.shift) + (s.index > 0 ? 1 : 0);
+  if (alone) {
+    char* out = static_cast<char*>(a.dW);
+    t.each(n0, a.N, k0, a.K, [&](int64_t n, int64_t k, float v) __attribute__((always_inline)) {
+      const int64_t at = s.group * a.stride_w + n * a.ldw + k;
+      if (a.dw_bf16) reinterpret_cast<uint16_t*>(out)[at] = f32_bf16(v);
+      else reinterpret_cast<float*>(out)[at] = v;
+    });
+  } else {
+    float* out = a.part_w + slot * a.N * a.K;
+    t.each(n0, a.N, k0, a.K, [&](int64_t n, int64_t k, float v) __attribute__((always_inline)) { out[n * a.K + k] = v; });
+  }
+  if (sums) {  // thread t summed columns (t % CPR) * VEC of the rows it staged
+    float* lds = reinterpret_cast<float*>(raw_lds);
+    __syncthreads();
+    constexpr int LD = TileT::BM + 4;
+    const int rg = threadIdx.x / OpA::CPR, c = (threadIdx.x % OpA::CPR) * VEC;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) lds[rg * LD + c + e] = cs[e];
+    __syncthreads();
+    for (int i = threadIdx.x; i < TileT::BM; i += TileT::THREADS) {
+      float v = 0.f;
+      for (int r = 0; r < OpA::ROWS_PER_PASS; ++r) v += lds[r * LD + i];
+      if (n0 + i < a.N) {
+        if (alone) a.db[s.group * a.ld_db + n0 + i] = v;
+        else a.part_b[slot * a.N + n0 + i] = v;
+      }
+    }
+  }
+}
+
+// The chunks of every group longer than one chunk.  blockIdx.y = b: the group that starts inside rows [b << shift, (b + 1) << shift) and
+// reaches beyond them, if there is one, contains the last of these rows.
+__global__ __launch_bounds__(256) void wgrad_join_kernel(const WgradArgs a) {
+  const int64_t b = blockIdx.y, last = ((b + 1) << a.shift) - 1;
+  if (last >= a.gr.M) return;
+  const int i = search(a.gr.G + 2, last, [&](int j) { return a.gr.edge(j); });
+  const int64_t start = a.gr.edge(i), end = a.gr.edge(i + 1);
+  if (i == 0 || i == a.gr.G + 1 || start < (b << a.shift) || start > last || end - start <= ((int64_t)1 << a.shift)) return;
+  const int group = i - 1, chunks = (int)((end - start + ((int64_t)1 << a.shift) - 1) >> a.shift);
+  const int64_t nk = a.N * a.K, total = nk + (a.db ? a.N : 0);
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (at >= total) return;
+  const bool is_b = at >= nk;
+  const float* p = is_b ? a.part_b + 2 * b * a.N + (at - nk) : a.part_w + 2 * b * nk + at;
+  const int64_t step = is_b ? a.N : nk;
+  float v = p[0];
+  int c = 1;
+  for (; c + 8 <= chunks; c += 8) {  // chunk c > 0 of the group: slot 2 (b + c) + 1
+    float t[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) t[u] = p[(2 * (int64_t)(c + u) + 1) * step];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v += t[u];
+  }
+  for (; c < chunks; ++c) v += p[(2 * (int64_t)c + 1) * step];
+  if (is_b) {
+    a.db[group * a.ld_db + (at - nk)] = v;
+  } else {
+    const int64_t o = group * a.stride_w + (at / a.K) * a.ldw + at % a.K;
+    if (a.dw_bf16) static_cast<uint16_t*>(a.dW)[o] = f32_bf16(v);
+    else static_cast<float*>(a.dW)[o] = v;
+  }
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------------------------------
+constexpr int64_t MAX_GRID = 0x7fffffff;
+
+template <class T, bool W_KM, int MI, int NI, int WR, int WC>
+int forward_launch(const char* me, const FwdArgs& a, hipStream_t st) {
+  typedef Tile<T, false, W_KM, MI, NI, WR, WC> TileT;
+  const int64_t slots = a.gr.M / TileT::BM + a.gr.G + 2, grid = slots * dh::ceil_div(a.N, TileT::BN);
+  if (grid > MAX_GRID) return dh::fail(DH_ERR_INVALID, "%s: %lld tiles in one launch", me, (long long)grid);
+  auto* kernel = grouped_forward_kernel<T, W_KM, MI, NI, WR, WC>;
+  static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, TileT::LDS_BYTES);
+  if (attr != hipSuccess) return dh::fail(DH_ERR_LAUNCH, "%s: %d bytes of LDS: %s", me, TileT::LDS_BYTES, hipGetErrorString(attr));
+  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(TileT::THREADS), TileT::LDS_BYTES, st, a);
+  return dh::check_launch(me);
+}
+
+template <class T, bool W_KM>
+int forward_pick(const char* me, const FwdArgs& a, hipStream_t st) {
+  // few rows per group: a 32-row tile wastes less of the matrix cores and of the slots
+  if (a.gr.M <= (int64_t)48 * a.gr.G) return forward_launch<T, W_KM, 1, 1, 1, 4>(me, a, st);
+  return forward_launch<T, W_KM, 2, 2, 2, 2>(me, a, st);
+}
+
+constexpr int WG_TILE = 128;
+
+// rows per chunk: enough chunks x tiles to fill the chip a few times, no chunk below 256 rows
+int wgrad_shift(int64_t M, int64_t N, int64_t K) {
+  const int64_t tiles = dh::ceil_div(N, WG_TILE) * dh::ceil_div(K, WG_TILE);
+  const int64_t want = dh::ceil_div(1024, tiles);  // chunks
+  int shift = 8;
+  while (shift < 30 && (M >> shift) > want) ++shift;
+  return shift;
+}
+
+int64_t wgrad_slots(int64_t M, int shift) { return 2 * ((M >> shift) + 1); }
+
+int check_grouped(const char* me, int64_t M, int64_t N, int64_t K, int64_t G, int dtype) {
+  if (M < 0 || N < 0 || K < 0 || G < 0) return dh::fail(DH_ERR_INVALID, "%s: negative size", me);
+  if (M > 0x7fffffff || G > 0x7fffff00) return dh::fail(DH_ERR_INVALID, "%s: more rows than an int32 bound can number", me);
+  if (dtype != DH_DTYPE_F32 && dtype != DH_DTYPE_BF16) return dh::fail(DH_ERR_INVALID, "%s: dtype %d", me, dtype);
+  return DH_OK;
+}
+
+}  // namespace
+
+extern "C" int dh_gemm_grouped(int64_t M, int64_t N, int64_t K, int64_t G, int trans_b, int dtype, const void* X, int64_t ldx, const void* W,
+                               int64_t ldw, int64_t stride_w, const int32_t* group_ptr, const float* bias, int64_t ld_bias, int act, void* Y,
+                               int64_t ldy, int y_dtype, int zero_outside, dh_stream_t stream) {
+  const char* me = "dh_gemm_grouped";
+  const int rc = check_grouped(me, M, N, K, G, dtype);
+  if (rc != DH_OK) return rc;
+  if (y_dtype != DH_DTYPE_F32 && y_dtype != DH_DTYPE_BF16) return dh::fail(DH_ERR_INVALID, "%s: output dtype %d", me, y_dtype);
+  if (act != DH_ACT_NONE && act != DH_ACT_RELU) return dh::fail(DH_ERR_INVALID, "%s: activation %d", me, act);
+  if (M == 0 || N == 0) return DH_OK;
+  if (!Y || (G > 0 && !group_ptr) || (K > 0 && (!X || (G > 0 && !W)))) return dh::fail(DH_ERR_INVALID, "%s: null tensor", me);
+  const int64_t wc = trans_b ? K : N;
+  if (ldx < K || ldw < wc || ldy < N || (bias && ld_bias < N) || (G > 1 && stride_w < 0)) return dh::fail(DH_ERR_INVALID, "%s: leading dimension below the row length", me);
+  FwdArgs a{};
+  a.gr = {group_ptr, M, (int)G};
+  a.N = N; a.K = K; a.X = X; a.W = W; a.ldx = ldx; a.ldw = ldw; a.stride_w = stride_w; a.bias = bias; a.ld_bias = ld_bias; a.Y = Y; a.ldy = ldy;
+  a.act = act; a.y_bf16 = y_dtype == DH_DTYPE_BF16; a.zero_outside = zero_outside != 0;
+  hipStream_t st = dh::as_stream(stream);
+  if (dtype == DH_DTYPE_BF16) return trans_b ? forward_pick<uint16_t, false>(me, a, st) : forward_pick<uint16_t, true>(me, a, st);
+  return trans_b ? forward_pick<float, false>(me, a, st) : forward_pick<float, true>(me, a, st);
+}
+
+extern "C" size_t dh_gemm_grouped_wgrad_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+  if (M <= 0 || N <= 0 || K < 0) return 16;
+  return 16 + (size_t)wgrad_slots(M, wgrad_shift(M, N, K)) * (size_t)N * (size_t)(K + 1) * 4;
+}
+
+extern "C" int dh_gemm_grouped_wgrad(int64_t M, int64_t N, int64_t K, int64_t G, int dtype, const void* dY, int64_t ldy, const void* X, int64_t ldx,
+                                     const int32_t* group_ptr, void* dW, int64_t ldw, int64_t stride_w, int dw_dtype, float* db, int64_t ld_db,
+                                     void* workspace, size_t workspace_bytes, dh_stream_t stream) {
+  const char* me = "dh_gemm_grouped_wgrad";
+  const int rc = check_grouped(me, M, N, K, G, dtype);
+  if (rc != DH_OK) return rc;
+  if (dw_dtype != DH_DTYPE_F32 && dw_dtype != DH_DTYPE_BF16) return dh::fail(DH_ERR_INVALID, "%s: output dtype %d", me, dw_dtype);
+  if (G == 0 || N == 0 || K == 0) return DH_OK;
+  if (!dW || !group_ptr || (M > 0 && (!dY || !X))) return dh::fail(DH_ERR_INVALID, "%s: null tensor", me);
+  if (ldy < N || ldx < K || ldw < K || (G > 1 && stride_w < (N - 1) * ldw + K) || (db && ld_db < N))
+    return dh::fail(DH_ERR_INVALID, "%s: leading dimension below the row length", me);
+  const size_t need = dh_gemm_grouped_wgrad_workspace_bytes(M, N, K);
+  if (!workspace || workspace_bytes < need) return dh::fail(DH_ERR_WORKSPACE, "%s: workspace of %zu bytes, need %zu", me, workspace_bytes, need);
+  if (!dh::aligned16(workspace)) return dh::fail(DH_ERR_INVALID, "%s: workspace must be 16-byte aligned", me);
+  WgradArgs a{};
+  a.gr = {group_ptr, M, (int)G};
+  a.N = N; a.K = K; a.dY = dY; a.X = X; a.ldy = ldy; a.ldx = ldx; a.dW = dW; a.ldw = ldw; a.stride_w = stride_w; a.dw_bf16 = dw_dtype == DH_DTYPE_BF16;
+  a.db = db; a.ld_db = ld_db; a.shift = wgrad_shift(M, N, K);
+  const int64_t slots = wgrad_slots(M, a.shift);
+  a.part_w = static_cast<float*>(workspace);
+  a.part_b = a.part_w + slots * N * K;
+  a.tiles_k = dh::ceil_div(K, WG_TILE);
+  a.tiles = dh::ceil_div(N, WG_TILE) * a.tiles_k;
+  const int64_t grid = ((M >> a.shift) + G + 2) * a.tiles;
+  if (grid > MAX_GRID) return dh::fail(DH_ERR_INVALID, "%s: %lld tiles in one launch", me, (long long)grid);
+  hipStream_t st = dh::as_stream(stream);
+  if (dtype == DH_DTYPE_BF16) {
+    typedef Tile<uint16_t, true, true, 2, 2, 2, 2> TileT;
+    auto* kernel = grouped_wgrad_kernel<uint16_t, 2, 2, 2, 2>;
+    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, TileT::LDS_BYTES);
+    if (attr != hipSuccess) return dh::fail(DH_ERR_LAUNCH, "%s: %d bytes of LDS: %s", me, TileT::LDS_BYTES, hipGetErrorString(attr));
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(TileT::THREADS), TileT::LDS_BYTES, st, a);
+  } else {
+    typedef Tile<float, true, true, 2, 2, 2, 2> TileT;
+    auto* kernel = grouped_wgrad_kernel<float, 2, 2, 2, 2>;
+    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, TileT::LDS_BYTES);
+    if (attr != hipSuccess) return dh::fail(DH_ERR_LAUNCH, "%s: %d bytes of LDS: %s", me, TileT::LDS_BYTES, hipGetErrorString(attr));
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(TileT::THREADS), TileT::LDS_BYTES, st, a);
+  }
+  if ((M >> a.shift) > 0)
+    hipLaunchKernelGGL(wgrad_join_kernel, dim3((unsigned)dh::ceil_div(N * K + N, 256), (unsigned)(M >> a.shift)), dim3(256), 0, st, a);
+  return dh::check_launch(me);
+}

@@ -1,0 +1,652 @@
+// The norms around a block, its gate and its residual in one pass each way (dance/models/nn/gnn.py:84-96: the `norm` slot of a layer and
+// the sum of a node's own and its neighbours' features are the reference's places for it):
+//
+//   n = post-norm(f)  or f          norm(v) = (v - mean) rstd w + b  (layer)  or  v rstd w + b, rstd = 1 / sqrt(mean(v^2) + eps)  (rms)
+//   r = x + scale * act(gate) * n   act = identity or sigmoid; gate per element, per row, per column, one for all, or none
+//   h = pre-norm(r)  or nothing     from the unrounded r
+//
+// Backward, with fhat / rhat the normalised f / r, u = dout w of the norm concerned and <.> the mean over a row:
+//   dr~ = dr + rstd2 (u2 - <u2> - rhat <u2 rhat>)      (rms: without <u2>);   dx = dr~
+//   dn  = scale act(gate) dr~;   dgate = scale dr~ n act'(gate);   df = rstd1 (u1 - <u1> - fhat <u1 fhat>)
+//   dw = sum_rows dout vhat,  db = sum_rows dout
+//
+// Bound: HBM.  Forward reads f and x and writes r and h; backward reads f, x, dr, dh and writes df, dx: r is recomputed from f, x and the
+// gate (the same bytes as reading it back, and unrounded in the bf16 case), only mean and rstd of each row are kept.
+// Split: a row lives in the registers of 8 .. 64 lanes of a wave (rows up to 512 columns) or of a workgroup of 256 / 512 (up to 4096),
+// 4 or 8 elements per lane (16 spill: the backward holds ten arrays of them), 16 bytes per access whatever the rows' alignment (global memory takes unaligned
+// accesses); a row length that is no multiple of the access reads its last piece from D - V and shifts it down in registers (ODD), so
+// no load is guarded.  The two-pass variance and both reductions of the backward run on registers.  Column gradients are summed in
+// registers over the rows a workgroup walks, joined in its LDS, written once per workgroup and added up by a second kernel in workgroup
+// order: no atomics, the result does not depend on timing.  All arithmetic is fp32; bf16 rounds once, at the stores.
+#include "common.h"
+
+namespace {
+
+enum { GATE_NONE = DH_GATE_NONE, GATE_SCALAR = DH_GATE_SCALAR, GATE_CHANNEL = DH_GATE_CHANNEL, GATE_ROW = DH_GATE_ROW, GATE_FULL = DH_GATE_FULL };
+constexpr int64_t MAX_D = 4096;
+constexpr int BWD_BLOCKS = 1024;  // workgroups of a backward launch at most = partial rows of the column gradients
+
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint16_t u16x8u __attribute__((ext_vector_type(8), aligned(2)));
+
+struct Args {
+  int64_t M;
+  int D, gate_kind, gate_sigmoid, rms, tpr, has_post, has_pre;
+  float scale, eps, inv_d;
+  const void *f, *x, *gate;
+  int64_t ldf, ldx, ldg;
+  const float *w1, *b1, *w2, *b2;
+  float* stats;  // [M, 4]: mean1, rstd1, mean2, rstd2
+  // forward
+  void *r, *h;
+  int64_t ldr, ldh;
+  // backward
+  const void *dr, *dh;
+  int64_t lddr, lddh;
+  void *df, *dx, *dgate;  // dgate: row and full gates
+  int64_t lddf, lddx, lddg;
+  float* partials;  // [n_arrays][gridDim.x][D]
+  int want_w1, want_b1, want_w2, want_b2, want_gate;
+};
+
+__device__ __forceinline__ float bf16_f32(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
+__device__ __forceinline__ uint16_t f32_bf16(float x) {  // nearest even; NaN stays a quiet NaN
+  const uint32_t u = __float_as_uint(x);
+  if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)((u >> 16) | 0x40u);
+  return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
+}
+
+template <class T>
+struct Elem;
+template <>
+struct Elem<float> {
+  static constexpr int VEC = 4;
+  static __device__ __forceinline__ float get(const void* p, int64_t i) { return static_cast<const float*>(p)[i]; }
+  static __device__ __forceinline__ void put(void* p, int64_t i, float v) { static_cast<float*>(p)[i] = v; }
+  template <int V>
+  static __device__ __forceinline__ void load(const void* p, int64_t i, float* v) {
+    if (V == 4) {
+      const f32x4u t = *reinterpret_cast<const f32x4u*>(static_cast<const float*>(p) + i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = t[e];
+    } else {
+      v[0] = get(p, i);
+    }
+  }
+  template <int V>
+  static __device__ __forceinline__ void store(void* p, int64_t i, const float* v) {
+    if (V == 4) {
+      f32x4u t;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) t[e] = v[e];
+      *reinterpret_cast<f32x4u*>(static_cast<float*>(p) + i) = t;
+    } else {
+      put(p, i, v[0]);
+    }
+  }
+};
+template <>
+struct Elem<uint16_t> {
+  static constexpr int VEC = 8;
+  static __device__ __forceinline__ float get(const void* p, int64_t i) { return bf16_f32(static_cast<const uint16_t*>(p)[i]); }
+  static __device__ __forceinline__ void put(void* p, int64_t i, float v) { static_cast<uint16_t*>(p)[i] = f32_bf16(v); }
+  template <int V>
+  static __device__ __forceinline__ void load(const void* p, int64_t i, float* v) {
+    if (V == 8) {
+      const u16x8u t = *reinterpret_cast<const u16x8u*>(static_cast<const uint16_t*>(p) + i);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = bf16_f32(t[e]);
+    } else {
+      v[0] = get(p, i);
+    }
+  }
+  template <int V>
+  static __device__ __forceinline__ void store(void* p, int64_t i, const float* v) {
+    if (V == 8) {
+      u16x8u t;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) t[e] = f32_bf16(v[e]);
+      *reinterpret_cast<u16x8u*>(static_cast<uint16_t*>(p) + i) = t;
+    } else {
+      put(p, i, v[0]);
+    }
+  }
+};
+
+// V consecutive fp32 parameters; they carry no alignment promise beyond their own four bytes
+template <int V>
+__device__ __forceinline__ void load_param(const float* p, int col, float* v) {
+  typedef float f32x4p __attribute__((ext_vector_type(4), aligned(4)));
+  if (V >= 4) {
+#pragma unroll
+    for (int q = 0; q < V / 4; ++q) {
+      const f32x4p t = *reinterpret_cast<const f32x4p*>(p + col + q * 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[q * 4 + e] = t[e];
+    }
+  } else {
+    v[0] = p[col];
+  }
+}
+
+__device__ __forceinline__ float sigmoid(float v) { return 1.f / (1.f + expf(-v)); }
+
+// N sums over the tpr threads of a row, the result in each of them.  BLOCK: the row is the whole workgroup.
+template <bool BLOCK, int N>
+__device__ __forceinline__ void row_sums(float (&v)[N], int tpr, float* lds) {
+  for (int o = (BLOCK ? 32 : tpr >> 1); o > 0; o >>= 1) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], o);
+  }
+  if (BLOCK) {
+    const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    __syncthreads();  // the previous reduction's values have been read
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) lds[wave * N + i] = v[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = 0.f;
+    for (int w = 0; w < waves; ++w) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] += lds[w * N + i];
+    }
+  }
+}
+
+// A lane's columns: chunk c covers (c * tpr + t) * V .. + V.  Chunks that end behind D read the last V values of the row instead; with
+// ODD their values are shifted down to the columns they belong to.  What lies at columns >= D is some value of the same row.
+template <int V>
+__device__ __forceinline__ void shift_down(int by, float* v) {
+#pragma unroll
+  for (int bit = 1; bit < V; bit *= 2)
+#pragma unroll
+    for (int e = 0; e + bit < V; ++e) v[e] = (by & bit) ? v[e + bit] : v[e];
+}
+template <class T, int V, int CH, bool ODD>
+__device__ __forceinline__ void load_row(const void* p, int64_t row_at, int t, int tpr, int D, float (&v)[V * CH]) {
+#pragma unroll
+  for (int c = 0; c < CH; ++c) Elem<T>::template load<V>(p, row_at + min((c * tpr + t) * V, D - V), v + c * V);
+  if (ODD) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) shift_down<V>(max((c * tpr + t) * V - (D - V), 0), v + c * V);
+  }
+}
+template <int V, int CH, bool ODD>
+__device__ __forceinline__ void zero_tail(int t, int tpr, int D, float (&v)[V * CH]) {
+#pragma unroll
+  for (int c = 0; c < CH; ++c)
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if ((c * tpr + t) * V + (ODD ? e : 0) >= D) v[c * V + e] = 0.f;
+}
+template <int V, int CH, bool ODD>
+__device__ __forceinline__ void load_params(const float* p, float fallback, int t, int tpr, int D, float (&v)[V * CH]) {
+  if (p) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      load_param<V>(p, min((c * tpr + t) * V, D - V), v + c * V);
+      if (ODD) shift_down<V>(max((c * tpr + t) * V - (D - V), 0), v + c * V);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V * CH; ++i) v[i] = fallback;
+  }
+}
+template <class T, int V, int CH, bool ODD>
+__device__ __forceinline__ void store_row(void* p, int64_t row_at, int t, int tpr, int D, const float (&v)[V * CH]) {
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int col = (c * tpr + t) * V;
+    if (ODD ? col + V <= D : col < D) Elem<T>::template store<V>(p, row_at + col, v + c * V);
+    else if (ODD && col < D) {
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (col + e < D) Elem<T>::put(p, row_at + col + e, v[c * V + e]);
+    }
+  }
+}
+
+// mean and rstd of a row held in registers (entries beyond D are zero)
+template <bool BLOCK, int V, int CH, bool ODD>
+__device__ __forceinline__ void row_stats(const Args& a, int t, const float (&v)[V * CH], float* lds, float& mean, float& rstd) {
+  float s[1] = {0.f};
+  mean = 0.f;
+  if (!a.rms) {
+#pragma unroll
+    for (int i = 0; i < V * CH; ++i) s[0] += v[i];
+    row_sums<BLOCK, 1>(s, a.tpr, lds);
+    mean = s[0] * a.inv_d;
+    s[0] = 0.f;
+  }
+#pragma unroll
+  for (int c = 0; c < CH; ++c)
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const float d = (c * a.tpr + t) * V + (ODD ? e : 0) < a.D ? v[c * V + e] - mean : 0.f;
+      s[0] = __builtin_fmaf(d, d, s[0]);
+    }
+  row_sums<BLOCK, 1>(s, a.tpr, lds);
+  rstd = 1.f / sqrtf(s[0] * a.inv_d + a.eps);
+}
+
+template <class T, int V, int CH, bool BLOCK, bool FULL, bool ODD>
+__global__ __launch_bounds__(BLOCK ? 512 : 256) void residual_norm_forward_kernel(const Args a) {
+  constexpr int E = V * CH;
+  __shared__ float lds[8];
+  const int tpr = a.tpr, t = BLOCK ? threadIdx.x : threadIdx.x & (tpr - 1);
+  const int rows_per_block = BLOCK ? 1 : 256 / tpr, sub = BLOCK ? 0 : threadIdx.x / tpr;
+  float ga[E];
+  if (!FULL) {
+    if (a.gate_kind == GATE_CHANNEL) load_params<V, CH, ODD>(static_cast<const float*>(a.gate), 1.f, t, tpr, a.D, ga);
+    else {
+      const float g = a.gate_kind == GATE_SCALAR ? *static_cast<const float*>(a.gate) : 1.f;
+#pragma unroll
+      for (int i = 0; i < E; ++i) ga[i] = g;
+    }
+    if (a.gate_sigmoid && (a.gate_kind == GATE_CHANNEL || a.gate_kind == GATE_SCALAR)) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) ga[i] = sigmoid(ga[i]);
+    }
+  }
+  for (int64_t base = (int64_t)blockIdx.x * rows_per_block; base < a.M; base += (int64_t)gridDim.x * rows_per_block) {
+    const int64_t row = min(base + sub, a.M - 1);
+    const bool valid = base + sub < a.M;
+    float f[E], x[E], gf[E], w[E], b[E];
+    load_row<T, V, CH, ODD>(a.f, row * a.ldf, t, tpr, a.D, f);
+    if (a.x) load_row<T, V, CH, ODD>(a.x, row * a.ldx, t, tpr, a.D, x);
+    else {
+#pragma unroll
+      for (int i = 0; i < E; ++i) x[i] = 0.f;
+    }
+    if (FULL) load_row<T, V, CH, ODD>(a.gate, row * a.ldg, t, tpr, a.D, gf);
+    float grow = 1.f;
+    if (!FULL && a.gate_kind == GATE_ROW) {
+      grow = Elem<T>::get(a.gate, row * a.ldg);
+      if (a.gate_sigmoid) grow = sigmoid(grow);
+    }
+    zero_tail<V, CH, ODD>(t, tpr, a.D, f);
+    float m1 = 0.f, s1 = 1.f, m2 = 0.f, s2 = 1.f;
+    if (a.has_post) {
+      load_params<V, CH, ODD>(a.w1, 1.f, t, tpr, a.D, w);
+      load_params<V, CH, ODD>(a.b1, 0.f, t, tpr, a.D, b);
+      row_stats<BLOCK, V, CH, ODD>(a, t, f, lds, m1, s1);
+#pragma unroll
+      for (int i = 0; i < E; ++i) f[i] = (f[i] - m1) * s1 * w[i] + b[i];
+    }
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      float g = FULL ? (a.gate_sigmoid ? sigmoid(gf[i]) : gf[i]) : ga[i];
+      if (!FULL) g *= grow;
+      f[i] = x[i] + a.scale * g * f[i];
+    }
+    if (valid && a.r) store_row<T, V, CH, ODD>(a.r, row * a.ldr, t, tpr, a.D, f);
+    if (a.has_pre) {
+      zero_tail<V, CH, ODD>(t, tpr, a.D, f);
+      load_params<V, CH, ODD>(a.w2, 1.f, t, tpr, a.D, w);
+      load_params<V, CH, ODD>(a.b2, 0.f, t, tpr, a.D, b);
+      row_stats<BLOCK, V, CH, ODD>(a, t, f, lds, m2, s2);
+#pragma unroll
+      for (int i = 0; i < E; ++i) f[i] = (f[i] - m2) * s2 * w[i] + b[i];
+      if (valid) store_row<T, V, CH, ODD>(a.h, row * a.ldh, t, tpr, a.D, f);
+    }
+    if (valid && a.stats && t == 0) *reinterpret_cast<float4*>(a.stats + row * 4) = make_float4(m1, s1, m2, s2);
+  }
+}
+
+// the workgroup's column sums of one array: joined over its row groups in LDS, written to partials[slot][blockIdx.x]
+template <int V, int CH, bool BLOCK>
+__device__ __forceinline__ void put_partials(const Args& a, int t, int sub, const float (&acc)[V * CH], int slot, float* lds) {
+  const int tpr = a.tpr;
+  float* out = a.partials + ((int64_t)slot * gridDim.x + blockIdx.x) * a.D;
+  if (BLOCK) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const int col = (c * tpr + t) * V + e;
+        if (col < a.D) out[col] = acc[c * V + e];
+      }
+  } else {
+    const int span = tpr * V * CH, groups = 256 / tpr;
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int e = 0; e < V; ++e) lds[sub * span + (c * tpr + t) * V + e] = acc[c * V + e];
+    __syncthreads();
+    for (int col = threadIdx.x; col < a.D; col += 256) {
+      float s = 0.f;
+      for (int g = 0; g < groups; ++g) s += lds[g * span + col];
+      out[col] = s;
+    }
+  }
+}
+
+template <class T, int V, int CH, bool BLOCK, bool FULL, bool ODD>
+__global__ __launch_bounds__(BLOCK ? 512 : 256) void residual_norm_backward_kernel(const Args a) {
+  constexpr int E = V * CH;
+  __shared__ float lds[BLOCK ? 32 : 256 * E];
+  const int tpr = a.tpr, t = BLOCK ? threadIdx.x : threadIdx.x & (tpr - 1);
+  const int rows_per_block = BLOCK ? 1 : 256 / tpr, sub = BLOCK ? 0 : threadIdx.x / tpr;
+  float acc_w1[E], acc_b1[E], acc_w2[E], acc_b2[E], acc_g[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) acc_w1[i] = acc_b1[i] = acc_w2[i] = acc_b2[i] = acc_g[i] = 0.f;
+  const bool col_gate = !FULL && (a.gate_kind == GATE_CHANNEL || a.gate_kind == GATE_SCALAR);
+  for (int64_t base = (int64_t)blockIdx.x * rows_per_block; base < a.M; base += (int64_t)gridDim.x * rows_per_block) {
+    const int64_t row = min(base + sub, a.M - 1);
+    const bool valid = base + sub < a.M;
+    float f[E], x[E], gf[E], dr[E], dh[E], w[E], b[E];
+    load_row<T, V, CH, ODD>(a.f, row * a.ldf, t, tpr, a.D, f);
+    if (a.x && a.has_pre) load_row<T, V, CH, ODD>(a.x, row * a.ldx, t, tpr, a.D, x);
+    else {
+#pragma unroll
+      for (int i = 0; i < E; ++i) x[i] = 0.f;
+    }
+    if (a.dr) load_row<T, V, CH, ODD>(a.dr, row * a.lddr, t, tpr, a.D, dr);
+    else {
+#pragma unroll
+      for (int i = 0; i < E; ++i) dr[i] = 0.f;
+    }
+    if (a.dh) load_row<T, V, CH, ODD>(a.dh, row * a.lddh, t, tpr, a.D, dh);
+    if (FULL) load_row<T, V, CH, ODD>(a.gate, row * a.ldg, t, tpr, a.D, gf);
+    const float4 st = *reinterpret_cast<const float4*>(a.stats + row * 4);
+    // the gate and its derivative's factor
+    if (!FULL) {
+      if (a.gate_kind == GATE_CHANNEL) load_params<V, CH, ODD>(static_cast<const float*>(a.gate), 1.f, t, tpr, a.D, gf);
+      else {
+        const float g = a.gate_kind == GATE_SCALAR ? *static_cast<const float*>(a.gate) : a.gate_kind == GATE_ROW ? Elem<T>::get(a.gate, row * a.ldg) : 1.f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) gf[i] = g;
+      }
+    }
+    const bool sig = a.gate_sigmoid && a.gate_kind != GATE_NONE;
+    if (sig) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) gf[i] = sigmoid(gf[i]);
+    }
+    if (a.has_post) {
+      load_params<V, CH, ODD>(a.w1, 1.f, t, tpr, a.D, w);
+      load_params<V, CH, ODD>(a.b1, 0.f, t, tpr, a.D, b);
+#pragma unroll
+      for (int i = 0; i < E; ++i) f[i] = (f[i] - st.x) * st.y;  // fhat from here on
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; ++i) { w[i] = 1.f; b[i] = 0.f; }
+    }
+    if (a.dh) {
+      float w2[E];
+      load_params<V, CH, ODD>(a.w2, 1.f, t, tpr, a.D, w2);
+      zero_tail<V, CH, ODD>(t, tpr, a.D, dh);
+      float s[2] = {0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        const float n = f[i] * w[i] + b[i];
+        x[i] = (x[i] + a.scale * gf[i] * n - st.z) * st.w;  // rhat
+        if (valid) {
+          acc_w2[i] = __builtin_fmaf(dh[i], x[i], acc_w2[i]);
+          acc_b2[i] += dh[i];
+        }
+        dh[i] *= w2[i];
+        s[0] = __builtin_fmaf(dh[i], x[i], s[0]);
+        s[1] += dh[i];
+      }
+      row_sums<BLOCK, 2>(s, tpr, lds);
+      const float c1 = s[0] * a.inv_d, c0 = a.rms ? 0.f : s[1] * a.inv_d;
+#pragma unroll
+      for (int i = 0; i < E; ++i) dr[i] += st.w * (dh[i] - c0 - x[i] * c1);
+    }
+    if (valid && a.dx) store_row<T, V, CH, ODD>(a.dx, row * a.lddx, t, tpr, a.D, dr);
+    zero_tail<V, CH, ODD>(t, tpr, a.D, dr);
+    float s[3] = {0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const float n = f[i] * w[i] + b[i];
+      float dg = a.scale * dr[i] * n;
+      if (sig) dg *= gf[i] * (1.f - gf[i]);
+      const float dn = a.scale * gf[i] * dr[i];
+      if (valid) {
+        acc_w1[i] = __builtin_fmaf(dn, f[i], acc_w1[i]);
+        acc_b1[i] += dn;
+        if (col_gate) acc_g[i] += dg;
+      }
+      const float u = dn * w[i];
+      s[0] = __builtin_fmaf(u, f[i], s[0]);
+      s[1] += u;
+      s[2] += dg;
+      gf[i] = dg;
+      dr[i] = u;
+    }
+    if (FULL && valid && a.dgate) store_row<T, V, CH, ODD>(a.dgate, row * a.lddg, t, tpr, a.D, gf);
+    if (a.has_post || (a.gate_kind == GATE_ROW && a.dgate)) row_sums<BLOCK, 3>(s, tpr, lds);
+    if (a.gate_kind == GATE_ROW && a.dgate && valid && t == 0) Elem<T>::put(a.dgate, row * a.lddg, s[2]);
+    if (a.df && valid) {
+      if (a.has_post) {
+        const float c1 = s[0] * a.inv_d, c0 = a.rms ? 0.f : s[1] * a.inv_d;
+#pragma unroll
+        for (int i = 0; i < E; ++i) dr[i] = st.y * (dr[i] - c0 - f[i] * c1);
+      }
+      store_row<T, V, CH, ODD>(a.df, row * a.lddf, t, tpr, a.D, dr);
+    }
+  }
+  int slot = 0;
+  if (a.want_w1) put_partials<V, CH, BLOCK>(a, t, sub, acc_w1, slot++, lds);
+  if (a.want_b1) put_partials<V, CH, BLOCK>(a, t, sub, acc_b1, slot++, lds);
+  if (a.want_w2) put_partials<V, CH, BLOCK>(a, t, sub, acc_w2, slot++, lds);
+  if (a.want_b2) put_partials<V, CH, BLOCK>(a, t, sub, acc_b2, slot++, lds);
+  if (a.want_gate) put_partials<V, CH, BLOCK>(a, t, sub, acc_g, slot++, lds);
+}
+
+struct ReduceArgs {
+  const float* partials;
+  float* out[5];
+  int n_blocks, D;
+};
+
+// out[slot][col] = sum over workgroups, 64 columns x 16 row splits per workgroup, joined in split order
+__global__ __launch_bounds__(1024) void column_reduce_kernel(const ReduceArgs a) {
+  __shared__ float part[16][64];
+  const int col = blockIdx.x * 64 + (threadIdx.x & 63), split = threadIdx.x >> 6, slot = blockIdx.y;
+  const float* p = a.partials + (int64_t)slot * a.n_blocks * a.D + min(col, a.D - 1);
+  float s = 0.f;
+  int b = split;
+  for (; b + 7 * 16 < a.n_blocks; b += 8 * 16) {
+    float v[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = p[(int64_t)(b + q * 16) * a.D];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) s += v[q];
+  }
+  for (; b < a.n_blocks; b += 16) s += p[(int64_t)b * a.D];
+  part[split][threadIdx.x & 63] = s;
+  __syncthreads();
+  if (split == 0 && col < a.D) {
+    s = part[0][threadIdx.x];
+#pragma unroll
+    for (int w = 1; w < 16; ++w) s += part[w][threadIdx.x];
+    a.out[slot][col] = s;
+  }
+}
+
+// one value: the sum of v[0 .. n) (the gate that is one for all columns)
+__global__ __launch_bounds__(256) void sum_kernel(const float* __restrict__ v, int n, float* __restrict__ out) {
+  __shared__ float part[4];
+  float s = 0.f;
+  for (int i = threadIdx.x; i < n; i += 256) s += v[i];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) *out = ((part[0] + part[1]) + part[2]) + part[3];
+}
+
+// How a row is split: V elements per access (16 bytes; rows shorter than that: 1), CH accesses per lane, tpr lanes per row.  As many
+// lanes as the row has accesses up to a wave, then up to 8 elements per lane, then a workgroup of 256 or 512 threads per row.
+struct Split {
+  int v, ch, tpr;
+  bool block, odd;
+};
+
+Split split_of(int64_t D, int vec_width) {
+  Split s;
+  s.v = D >= vec_width ? vec_width : 1;
+  s.odd = D % s.v != 0;
+  const int64_t n = dh::ceil_div(D, s.v);
+  const int64_t eight = 8 / s.v;  // accesses that hold eight elements
+  s.block = n > 64 * eight;
+  if (s.block) {
+    s.tpr = n <= 256 * eight ? 256 : 512;
+  } else {
+    s.tpr = 8;
+    while (s.tpr < 64 && s.tpr < n) s.tpr *= 2;
+  }
+  s.ch = 1;
+  while ((int64_t)s.ch * s.tpr < n) s.ch *= 2;
+  return s;
+}
+
+int64_t blocks_of(const Split& s, int64_t M, int64_t most) {
+  const int64_t per = s.block ? 1 : 256 / s.tpr, need = dh::ceil_div(M, per);
+  return need < most ? need : most;
+}
+
+template <class T, int V, int CH, bool BLOCK, bool FULL, bool ODD>
+void launch(bool backward, const Args& a, int64_t grid, hipStream_t st) {
+  const dim3 g((unsigned)grid), b(BLOCK ? a.tpr : 256);
+  if (backward) hipLaunchKernelGGL((residual_norm_backward_kernel<T, V, CH, BLOCK, FULL, ODD>), g, b, 0, st, a);
+  else hipLaunchKernelGGL((residual_norm_forward_kernel<T, V, CH, BLOCK, FULL, ODD>), g, b, 0, st, a);
+}
+
+template <class T, int V, int CH, bool BLOCK>
+void launch_gate(bool backward, const Args& a, const Split& s, int64_t grid, hipStream_t st) {
+  const bool full = a.gate_kind == GATE_FULL;
+  if constexpr (V == 1) {
+    if (full) launch<T, V, CH, BLOCK, true, false>(backward, a, grid, st);
+    else launch<T, V, CH, BLOCK, false, false>(backward, a, grid, st);
+  } else if (s.odd) {
+    if (full) launch<T, V, CH, BLOCK, true, true>(backward, a, grid, st);
+    else launch<T, V, CH, BLOCK, false, true>(backward, a, grid, st);
+  } else {
+    if (full) launch<T, V, CH, BLOCK, true, false>(backward, a, grid, st);
+    else launch<T, V, CH, BLOCK, false, false>(backward, a, grid, st);
+  }
+}
+
+template <class T>
+void launch_t(bool backward, const Args& a, const Split& s, int64_t grid, hipStream_t st) {
+  constexpr int V = Elem<T>::VEC, EIGHT = 8 / V;
+  if (s.v == 1) return launch_gate<T, 1, 1, false>(backward, a, s, grid, st);
+  if (!s.block) {
+    if (s.ch == 1) return launch_gate<T, V, 1, false>(backward, a, s, grid, st);
+    if constexpr (EIGHT == 2) launch_gate<T, V, 2, false>(backward, a, s, grid, st);
+    return;
+  }
+  launch_gate<T, V, EIGHT, true>(backward, a, s, grid, st);
+}
+
+int check_common(const char* me, int64_t M, int64_t D, int dtype, const void* f, const void* x, int64_t ldf, int64_t ldx, const void* gate,
+                 int64_t ldg, int gate_kind, int gate_sigmoid, int kind, float eps) {
+  if (M < 0 || D < 1 || D > MAX_D) return dh::fail(DH_ERR_INVALID, "%s: %lld rows of %lld columns (1 .. %lld)", me, (long long)M, (long long)D, (long long)MAX_D);
+  if (dtype != DH_DTYPE_F32 && dtype != DH_DTYPE_BF16) return dh::fail(DH_ERR_INVALID, "%s: dtype %d", me, dtype);
+  if (kind != DH_NORM_LAYER && kind != DH_NORM_RMS) return dh::fail(DH_ERR_INVALID, "%s: norm kind %d", me, kind);
+  if (gate_kind < GATE_NONE || gate_kind > GATE_FULL) return dh::fail(DH_ERR_INVALID, "%s: gate kind %d", me, gate_kind);
+  if (gate_sigmoid != 0 && gate_sigmoid != 1) return dh::fail(DH_ERR_INVALID, "%s: gate activation %d", me, gate_sigmoid);
+  if (!(eps >= 0.f)) return dh::fail(DH_ERR_INVALID, "%s: eps must not be negative", me);
+  if (M == 0) return DH_OK;
+  if (!f || (gate_kind != GATE_NONE && !gate)) return dh::fail(DH_ERR_INVALID, "%s: null tensor", me);
+  if (ldf < D || (x && ldx < D) || (gate_kind == GATE_FULL && ldg < D) || (gate_kind == GATE_ROW && ldg < 1))
+    return dh::fail(DH_ERR_INVALID, "%s: leading dimension below the row length", me);
+  return DH_OK;
+}
+
+}  // namespace
+
+extern "C" int dh_residual_norm_forward(int64_t M, int64_t D, int dtype, const void* f, int64_t ldf, const void* x, int64_t ldx, const void* gate,
+                                        int64_t ldg, int gate_kind, int gate_sigmoid, float scale, int kind, float eps, int has_post,
+                                        const float* w1, const float* b1, int has_pre, const float* w2, const float* b2, void* r, int64_t ldr,
+                                        void* h, int64_t ldh, float* stats, dh_stream_t stream) {
+  const char* me = "dh_residual_norm_forward";
+  const int rc = check_common(me, M, D, dtype, f, x, ldf, ldx, gate, ldg, gate_kind, gate_sigmoid, kind, eps);
+  if (rc != DH_OK) return rc;
+  if (M == 0) return DH_OK;
+  if ((!r && !has_pre) || (has_pre && !h)) return dh::fail(DH_ERR_INVALID, "%s: null output", me);
+  if ((r && ldr < D) || (has_pre && ldh < D)) return dh::fail(DH_ERR_INVALID, "%s: leading dimension below the row length", me);
+  if (stats && !dh::aligned16(stats)) return dh::fail(DH_ERR_INVALID, "%s: stats must be 16-byte aligned", me);
+  Args a{};
+  a.M = M; a.D = (int)D; a.gate_kind = gate_kind; a.gate_sigmoid = gate_sigmoid; a.rms = kind == DH_NORM_RMS;
+  a.has_post = has_post != 0; a.has_pre = has_pre != 0; a.scale = scale; a.eps = eps; a.inv_d = 1.f / (float)D;
+  a.f = f; a.x = x; a.gate = gate; a.ldf = ldf; a.ldx = ldx; a.ldg = ldg;
+  a.w1 = w1; a.b1 = b1; a.w2 = w2; a.b2 = b2; a.stats = stats; a.r = r; a.h = h; a.ldr = ldr; a.ldh = ldh;
+  const int vw = dtype == DH_DTYPE_BF16 ? 8 : 4;
+  const Split s = split_of(D, vw);
+  a.tpr = s.tpr;
+  const int64_t grid = blocks_of(s, M, 4096);
+  if (dtype == DH_DTYPE_BF16) launch_t<uint16_t>(false, a, s, grid, dh::as_stream(stream));
+  else launch_t<float>(false, a, s, grid, dh::as_stream(stream));
+  return dh::check_launch(me);
+}
+
+extern "C" size_t dh_residual_norm_backward_workspace_bytes(int64_t M, int64_t D) {
+  if (M <= 0 || D <= 0) return 16;
+  const int64_t rows = M < BWD_BLOCKS ? M : BWD_BLOCKS;
+  return (size_t)(5 * rows + 1) * (size_t)D * 4;  // five arrays of one partial row per workgroup, and the per-column sums of a scalar gate
+}
+
+extern "C" int dh_residual_norm_backward(int64_t M, int64_t D, int dtype, const void* f, int64_t ldf, const void* x, int64_t ldx, const void* gate,
+                                         int64_t ldg, int gate_kind, int gate_sigmoid, float scale, int kind, int has_post, const float* w1,
+                                         const float* b1, int has_pre, const float* w2, const float* stats, const void* dr, int64_t lddr,
+                                         const void* dhh, int64_t lddh, void* df, int64_t lddf, void* dx, int64_t lddx, void* dgate, int64_t lddg,
+                                         float* dw1, float* db1, float* dw2, float* db2, void* workspace, size_t workspace_bytes,
+                                         dh_stream_t stream) {
+  const char* me = "dh_residual_norm_backward";
+  const int rc = check_common(me, M, D, dtype, f, x, ldf, ldx, gate, ldg, gate_kind, gate_sigmoid, kind, 0.f);
+  if (rc != DH_OK) return rc;
+  hipStream_t st = dh::as_stream(stream);
+  const bool col_gate = gate_kind == GATE_CHANNEL || gate_kind == GATE_SCALAR;
+  if (M == 0) {  // no rows: the column gradients are empty sums
+    for (float* p : {dw1, db1, dw2, db2})
+      if (p && dh::zero_async(p, (size_t)D * 4, st) != hipSuccess) return dh::fail(DH_ERR_LAUNCH, "%s: zero fill", me);
+    if (col_gate && dgate && dh::zero_async(dgate, (gate_kind == GATE_SCALAR ? 1 : (size_t)D) * 4, st) != hipSuccess)
+      return dh::fail(DH_ERR_LAUNCH, "%s: zero fill", me);
+    return DH_OK;
+  }
+  if (!stats) return dh::fail(DH_ERR_INVALID, "%s: null stats", me);
+  if (!dh::aligned16(stats)) return dh::fail(DH_ERR_INVALID, "%s: stats must be 16-byte aligned", me);
+  if (dhh && !has_pre) return dh::fail(DH_ERR_INVALID, "%s: dh without a second norm", me);
+  if (!dr && !dhh) return dh::fail(DH_ERR_INVALID, "%s: no upstream gradient", me);
+  if ((dr && lddr < D) || (dhh && lddh < D) || (df && lddf < D) || (dx && lddx < D) || (gate_kind == GATE_FULL && dgate && lddg < D) ||
+      (gate_kind == GATE_ROW && dgate && lddg < 1))
+    return dh::fail(DH_ERR_INVALID, "%s: leading dimension below the row length", me);
+  const size_t need = dh_residual_norm_backward_workspace_bytes(M, D);
+  if (!workspace || workspace_bytes < need) return dh::fail(DH_ERR_WORKSPACE, "%s: workspace of %zu bytes, need %zu", me, workspace_bytes, need);
+  Args a{};
+  a.M = M; a.D = (int)D; a.gate_kind = gate_kind; a.gate_sigmoid = gate_sigmoid; a.rms = kind == DH_NORM_RMS;
+  a.has_post = has_post != 0; a.has_pre = has_pre != 0; a.scale = scale; a.inv_d = 1.f / (float)D;
+  a.f = f; a.x = x; a.gate = gate; a.ldf = ldf; a.ldx = ldx; a.ldg = ldg; a.w1 = w1; a.b1 = b1; a.w2 = w2;
+  a.stats = const_cast<float*>(stats); a.dr = dr; a.dh = dhh; a.lddr = lddr; a.lddh = lddh;
+  a.df = df; a.dx = dx; a.lddf = lddf; a.lddx = lddx; a.lddg = lddg;
+  a.dgate = col_gate ? nullptr : dgate;
+  a.partials = static_cast<float*>(workspace);
+  a.want_w1 = has_post && dw1; a.want_b1 = has_post && db1; a.want_w2 = dw2 != nullptr; a.want_b2 = db2 != nullptr;
+  a.want_gate = col_gate && dgate;
+  const int vw = dtype == DH_DTYPE_BF16 ? 8 : 4;
+  const Split s = split_of(D, vw);
+  a.tpr = s.tpr;
+  const int64_t grid = blocks_of(s, M, BWD_BLOCKS);
+  if (dtype == DH_DTYPE_BF16) launch_t<uint16_t>(true, a, s, grid, st);
+  else launch_t<float>(true, a, s, grid, st);
+  ReduceArgs ra{};
+  ra.partials = a.partials; ra.n_blocks = (int)grid; ra.D = (int)D;
+  int slots = 0;
+  if (a.want_w1) ra.out[slots++] = dw1;
+  if (a.want_b1) ra.out[slots++] = db1;
+  if (a.want_w2) ra.out[slots++] = dw2;
+  if (a.want_b2) ra.out[slots++] = db2;
+  float* gate_cols = a.partials + (int64_t)5 * (M < BWD_BLOCKS ? M : BWD_BLOCKS) * D;
+  if (a.want_gate) ra.out[slots++] = gate_kind == GATE_SCALAR ? gate_cols : static_cast<float*>(dgate);
+  if (slots > 0) hipLaunchKernelGGL(column_reduce_kernel, dim3((unsigned)dh::ceil_div(D, 64), (unsigned)slots), dim3(1024), 0, st, ra);
+  if (a.want_gate && gate_kind == GATE_SCALAR)
+    hipLaunchKernelGGL(sum_kernel, dim3(1), dim3(256), 0, st, gate_cols, (int)D, static_cast<float*>(dgate));
+  return dh::check_launch(me);
+}

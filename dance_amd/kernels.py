@@ -6,6 +6,7 @@ wrappers never copy to the host and never compute on the CPU.
 """
 from typing import Optional, Tuple
 
+import contextlib
 import os
 
 import torch
@@ -81,6 +82,22 @@ def _dev(t: Optional[torch.Tensor], dtype, name: str, ndim: Optional[int] = None
 def _ld(t: torch.Tensor) -> int:
     # leading dimension in elements of a row-major 2-d tensor (rows may be strided)
     return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+
+
+def _one_device(*tensors: Optional[torch.Tensor]):
+    """Context in which the tensors' own device is the current one (its current stream is the one the kernels are put on); tensors of
+    more than one device are refused."""
+    dev = None
+    for t in tensors:
+        if t is None or not t.is_cuda:  # (host tensors are refused by name in _dev)
+            continue
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise ValueError(f"tensors on more than one device: {dev} and {t.device}")
+    if dev is None or dev.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(dev)
 
 
 def _lib_ready():
@@ -685,6 +702,219 @@ def colsum_bf16(X: torch.Tensor) -> torch.Tensor:
     return out
 
 
+# ---- products grouped by row type -----------------------------------------------------------------------------
+_ELEM = {torch.float32: DTYPE_F32, _BF16: DTYPE_BF16}
+
+
+def _elem(t: torch.Tensor, name: str) -> int:
+    code = _ELEM.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{name} must be torch.float32 or torch.bfloat16, got {t.dtype}")
+    return code
+
+
+def _rows_ld(t: torch.Tensor, name: str) -> int:
+    """Row stride of a 2-d operand; overlapping rows (an expanded tensor) are refused."""
+    ld = _ld(t)
+    if t.shape[0] > 1 and ld < t.shape[1]:
+        raise ValueError(f"{name}: rows overlap (stride {ld} below the row length {t.shape[1]})")
+    return ld
+
+
+def _weight_strides(W: torch.Tensor, name: str):
+    """(row stride, group stride) of a [G, rows, cols] weight stack, rows contiguous."""
+    if W.dim() != 3:
+        raise ValueError(f"{name} must be 3-d [groups, rows, columns], got shape {tuple(W.shape)}")
+    ldw = W.stride(1) if W.shape[1] > 1 else max(W.shape[2], 1)
+    sw = W.stride(0) if W.shape[0] > 1 else 0
+    if W.numel() and (ldw < W.shape[2] or sw < 0):
+        raise ValueError(f"{name}: strides {W.stride()} of shape {tuple(W.shape)} are not supported")
+    return ldw, sw
+
+
+def gemm_grouped(X: torch.Tensor, W: torch.Tensor, group_ptr: torch.Tensor, *, trans_b: bool = True, bias: Optional[torch.Tensor] = None,
+                 act: int = ACT_NONE, out: Optional[torch.Tensor] = None, out_dtype=None) -> torch.Tensor:
+    """Y[i] = act(X[i] @ op(W[g]) + bias[g]) for the rows group_ptr[g] <= i < group_ptr[g + 1]; see dh_gemm_grouped.
+
+    X [M, K] fp32 or bf16 with its rows sorted by group; W [G, N, K] (``trans_b``, torch.nn.Linear's layout) or [G, K, N] of X's dtype;
+    ``group_ptr`` int32 [G + 1] on the device, non-decreasing; bias fp32 [G, N].  Groups may be empty, sizes are not read by the host (no
+    synchronisation, capturable).  Rows that belong to no group are zero in a fresh result and left as they are in ``out``."""
+    lib = _lib_ready()
+    dt = _elem(X, "X")
+    if X.dim() != 2:
+        raise ValueError(f"X must be 2-d, got shape {tuple(X.shape)}")
+    ldw, sw = _weight_strides(W, "W")
+    M, K = X.shape
+    G, N, Kw = (W.shape[0], W.shape[1], W.shape[2]) if trans_b else (W.shape[0], W.shape[2], W.shape[1])
+    if K != Kw:
+        raise ValueError(f"gemm_grouped: inner dimensions differ ({K} vs {Kw})")
+    if group_ptr.dim() != 1 or group_ptr.numel() != G + 1:
+        raise ValueError(f"group_ptr must hold {G + 1} bounds for {G} groups, got shape {tuple(group_ptr.shape)}")
+    if bias is not None and tuple(bias.shape) != (G, N):
+        raise ValueError(f"bias must be [{G}, {N}], got shape {tuple(bias.shape)}")
+    if act not in (ACT_NONE, ACT_RELU):
+        raise ValueError(f"gemm_grouped: unknown activation {act}")
+    fresh = out is None
+    if fresh:
+        out = torch.empty((M, N), dtype=out_dtype or X.dtype, device=X.device)
+    elif tuple(out.shape) != (M, N) or (out_dtype is not None and out.dtype != out_dtype):
+        raise ValueError(f"out must be [{M}, {N}]{'' if out_dtype is None else f' of {out_dtype}'}, got {tuple(out.shape)} of {out.dtype}")
+    with _one_device(X, W, group_ptr, bias, out):
+        _call(f"gemm_grouped_{'bf16' if dt else 'f32'}_{'nt' if trans_b else 'nn'}", lib.dh_gemm_grouped, M, N, K, G, int(trans_b), dt,
+              _dev(X, X.dtype, "X", 2), _rows_ld(X, "X"), _dev(W, X.dtype, "W", 3), ldw, sw, _dev(group_ptr, torch.int32, "group_ptr", 1),
+              _dev(bias, torch.float32, "bias", 2), 0 if bias is None else _rows_ld(bias, "bias"), act, _dev(out, out.dtype, "out", 2),
+              _rows_ld(out, "out"), _elem(out, "out"), int(fresh), _stream())
+    return out
+
+
+def gemm_grouped_wgrad(dY: torch.Tensor, X: torch.Tensor, group_ptr: torch.Tensor, *, out_dtype=None, want_bias: bool = False):
+    """dW[g] = dY_g^T @ X_g ([G, N, K]) over each group's rows and, with ``want_bias``, (dW, db) with db[g] = the column sums of dY_g (fp32
+    [G, N]); zero for an empty group.  See dh_gemm_grouped_wgrad.  The rows of a group are summed in a fixed order."""
+    lib = _lib_ready()
+    dt = _elem(X, "X")
+    if X.dim() != 2 or dY.dim() != 2 or X.shape[0] != dY.shape[0]:
+        raise ValueError(f"dY and X must be 2-d with the same rows, got shapes {tuple(dY.shape)} and {tuple(X.shape)}")
+    if group_ptr.dim() != 1 or group_ptr.numel() < 1:
+        raise ValueError(f"group_ptr must be 1-d with at least one bound, got shape {tuple(group_ptr.shape)}")
+    M, K = X.shape
+    N, G = dY.shape[1], group_ptr.numel() - 1
+    dW = torch.empty((G, N, K), dtype=out_dtype or X.dtype, device=X.device)
+    db = torch.empty((G, N), dtype=torch.float32, device=X.device) if want_bias else None
+    if K == 0 and want_bias:
+        raise ValueError("gemm_grouped_wgrad: the bias gradient needs at least one input column")
+    with _one_device(dY, X, group_ptr):
+        ws_bytes = lib.dh_gemm_grouped_wgrad_workspace_bytes(M, N, K)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=X.device)
+        _call(f"gemm_grouped_{'bf16' if dt else 'f32'}_tn", lib.dh_gemm_grouped_wgrad, M, N, K, G, dt, _dev(dY, X.dtype, "dY", 2), _rows_ld(dY, "dY"),
+              _dev(X, X.dtype, "X", 2), _rows_ld(X, "X"), _dev(group_ptr, torch.int32, "group_ptr", 1), dW.data_ptr(), max(K, 1), N * K,
+              _elem(dW, "dW"), None if db is None else db.data_ptr(), max(N, 1), ws.data_ptr(), ws_bytes, _stream())
+    return (dW, db) if want_bias else dW
+
+
+# ---- norms around a block, its gate and its residual -------------------------------------------------------------
+NORM_LAYER, NORM_RMS = 0, 1
+GATE_NONE, GATE_SCALAR, GATE_CHANNEL, GATE_ROW, GATE_FULL = 0, 1, 2, 3, 4
+RESIDUAL_NORM_MAX_COLUMNS = 4096
+
+
+def residual_norm_gate_kind(gate: Optional[torch.Tensor], M: int, D: int) -> int:
+    """Which rows and columns one gate value stands for, from the gate's shape: None, [] or [1], [D], [M, 1], [M, D]."""
+    if gate is None:
+        return GATE_NONE
+    shape = tuple(gate.shape)
+    if shape in ((), (1, )):
+        return GATE_SCALAR
+    if shape == (D, ):
+        return GATE_CHANNEL
+    if shape == (M, 1):
+        return GATE_ROW
+    if shape == (M, D):
+        return GATE_FULL
+    raise ValueError(f"gate must have shape [], [1], [{D}], [{M}, 1] or [{M}, {D}], got {shape}")
+
+
+def _norm_params(p, D: int, name: str):
+    """(has, weight pointer, bias pointer) of a norm given as None or (weight or None, bias or None)."""
+    if p is None:
+        return 0, None, None
+    w, b = p
+    for t, what in ((w, "weight"), (b, "bias")):
+        if t is not None and tuple(t.shape) != (D, ):
+            raise ValueError(f"{name} {what} must be [{D}], got shape {tuple(t.shape)}")
+    return 1, _dev(w, torch.float32, f"{name} weight", 1), _dev(b, torch.float32, f"{name} bias", 1)
+
+
+def _gate_args(gate, kind: int, dtype):
+    if kind == GATE_NONE:
+        return None, 0
+    if kind in (GATE_SCALAR, GATE_CHANNEL):
+        return _dev(gate.reshape(-1), torch.float32, "gate", 1), 0
+    return _dev(gate, dtype, "gate", 2), (gate.stride(0) if gate.shape[0] > 1 else gate.shape[1]) if kind == GATE_ROW else _rows_ld(gate, "gate")
+
+
+def _check_rows(t: Optional[torch.Tensor], like: torch.Tensor, name: str):
+    if t is not None and (t.shape != like.shape or t.dtype != like.dtype):
+        raise ValueError(f"{name} must be {tuple(like.shape)} of {like.dtype}, got {tuple(t.shape)} of {t.dtype}")
+
+
+def residual_norm_forward(f: torch.Tensor, x: Optional[torch.Tensor] = None, *, post=None, gate: Optional[torch.Tensor] = None,
+                          gate_sigmoid: bool = False, scale: float = 1.0, pre=None, kind: int = NORM_LAYER, eps: float = 1e-5,
+                          want_stats: bool = False):
+    """(r, h, stats): r = x + scale * act(gate) * post(f), h = pre(r) (None without ``pre``); see dh_residual_norm_forward.
+
+    f, x [M, D] fp32 or bf16, D <= 4096; ``post`` / ``pre``: None or (weight, bias), fp32 [D] or None each; gate: residual_norm_gate_kind
+    (scalar and channel gates fp32, the others of f's dtype).  stats [M, 4] fp32 is what residual_norm_backward needs."""
+    lib = _lib_ready()
+    dt = _elem(f, "f")
+    if f.dim() != 2:
+        raise ValueError(f"f must be 2-d, got shape {tuple(f.shape)}")
+    M, D = f.shape
+    if not 1 <= D <= RESIDUAL_NORM_MAX_COLUMNS:
+        raise ValueError(f"residual_norm: rows of 1 .. {RESIDUAL_NORM_MAX_COLUMNS} columns, got {D}")
+    if kind not in (NORM_LAYER, NORM_RMS) or not eps >= 0:
+        raise ValueError(f"residual_norm: kind {kind}, eps {eps}")
+    _check_rows(x, f, "x")
+    gk = residual_norm_gate_kind(gate, M, D)
+    has_post, w1, b1 = _norm_params(post, D, "post")
+    has_pre, w2, b2 = _norm_params(pre, D, "pre")
+    gp, ldg = _gate_args(gate, gk, f.dtype)
+    fp, xp = _dev(f, f.dtype, "f", 2), _dev(x, f.dtype, "x", 2)
+    r = torch.empty((M, D), dtype=f.dtype, device=f.device)
+    h = torch.empty_like(r) if has_pre else None
+    stats = torch.empty((M, 4), dtype=torch.float32, device=f.device) if want_stats else None
+    with _one_device(f, x, gate, *(post or ()), *(pre or ())):
+        _call("residual_norm_forward", lib.dh_residual_norm_forward, M, D, dt, fp, _rows_ld(f, "f"), xp, 0 if x is None else _rows_ld(x, "x"), gp,
+              ldg, gk, int(gate_sigmoid), float(scale), kind, float(eps), has_post, w1, b1, has_pre, w2, b2, r.data_ptr(), D,
+              None if h is None else h.data_ptr(), D, None if stats is None else stats.data_ptr(), _stream())
+    return r, h, stats
+
+
+def residual_norm_backward(dr: Optional[torch.Tensor], dh: Optional[torch.Tensor], f: torch.Tensor, x: Optional[torch.Tensor],
+                           stats: torch.Tensor, *, post=None, gate: Optional[torch.Tensor] = None, gate_sigmoid: bool = False, scale: float = 1.0,
+                           pre=None, kind: int = NORM_LAYER, want=("f", "x", "gate", "w1", "b1", "w2", "b2")):
+    """Gradients of ``residual_norm_forward`` as a dict over ``want``; see dh_residual_norm_backward.  ``dr`` / ``dh``: the upstream gradients
+    of r and h, either may be None."""
+    lib = _lib_ready()
+    dt = _elem(f, "f")
+    M, D = f.shape
+    _check_rows(x, f, "x")
+    _check_rows(dr, f, "dr")
+    _check_rows(dh, f, "dh")
+    if dr is None and dh is None:
+        raise ValueError("residual_norm_backward: neither dr nor dh")
+    if dh is not None and pre is None:
+        raise ValueError("residual_norm_backward: dh without the second norm")
+    if tuple(stats.shape) != (M, 4):
+        raise ValueError(f"stats must be [{M}, 4], got shape {tuple(stats.shape)}")
+    gk = residual_norm_gate_kind(gate, M, D)
+    has_post, w1, b1 = _norm_params(post, D, "post")
+    has_pre, w2, _ = _norm_params(pre, D, "pre")
+    gp, ldg = _gate_args(gate, gk, f.dtype)
+    new = {}
+    for key, there in (("f", True), ("x", x is not None), ("gate", gate is not None), ("w1", has_post), ("b1", has_post), ("w2", has_pre), ("b2", has_pre)):
+        if there and key in want:
+            if key in ("f", "x"):
+                new[key] = torch.empty((M, D), dtype=f.dtype, device=f.device)
+            elif key == "gate":
+                new[key] = torch.empty(gate.shape, dtype=gate.dtype, device=f.device)
+            else:
+                new[key] = torch.empty(D, dtype=torch.float32, device=f.device)
+    ptr = lambda key: new[key].data_ptr() if key in new else None
+    if dh is None:  # nothing flows through the second norm
+        for key in ("w2", "b2"):
+            if key in new:
+                new[key].zero_()
+    with _one_device(f, x, gate, stats, dr, dh, *(post or ()), *(pre or ())):
+        ws_bytes = lib.dh_residual_norm_backward_workspace_bytes(M, D)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=f.device)
+        _call("residual_norm_backward", lib.dh_residual_norm_backward, M, D, dt, _dev(f, f.dtype, "f", 2), _rows_ld(f, "f"), _dev(x, f.dtype, "x", 2),
+              0 if x is None else _rows_ld(x, "x"), gp, ldg, gk, int(gate_sigmoid), float(scale), kind, has_post, w1, b1, has_pre, w2,
+              _dev(stats, torch.float32, "stats", 2), _dev(dr, f.dtype, "dr", 2), 0 if dr is None else _rows_ld(dr, "dr"), _dev(dh, f.dtype, "dh", 2),
+              0 if dh is None else _rows_ld(dh, "dh"), ptr("f"), D, ptr("x"), D, ptr("gate"), D if gk == GATE_FULL else 1, ptr("w1"), ptr("b1"),
+              None if dh is None else ptr("w2"), None if dh is None else ptr("b2"), ws.data_ptr(), ws_bytes, _stream())
+    return new
+
+
 # ---- graph builders ----------------------------------------------------------------------------------------
 def pairwise_distance(X: torch.Tensor, metric: int = METRIC_EUCLIDEAN) -> torch.Tensor:
     """Dense [n, n] f32 distance matrix (dh_pairwise_distance_f32); spearman ranks the rows on the device first."""
@@ -971,6 +1201,149 @@ def degree_scales(rowptr: torch.Tensor, col: torch.Tensor, n_rows: int, n_cols: 
 
 def block_cells_static_workspace_bytes(n_seeds: int) -> int:
     return int(_lib_ready().dh_block_cells_static_workspace_bytes(int(n_seeds)))
+
+
+# ---- global gradient norm and clipping ---------------------------------------------------------------------------
+_NORM_TYPES = {1.0: 1, 2.0: 2, float("inf"): 0}
+
+
+def _norm_type(p) -> int:
+    try:
+        code = _NORM_TYPES.get(float(p))
+    except (TypeError, ValueError):
+        code = None
+    if code is None:
+        raise ValueError(f"norm_type must be 1, 2 or inf, got {p!r}")
+    return code
+
+
+def _is_dense(t: torch.Tensor) -> bool:
+    """The tensor's elements are consecutive in memory, in some order (a transposed parameter's gradient is; a column slice is not)."""
+    if t.is_contiguous():
+        return True
+    expect = 1
+    for size, stride in sorted(((n, s) for n, s in zip(t.shape, t.stride()) if n != 1), key=lambda v: v[1]):
+        if stride != expect:
+            return False
+        expect *= size
+    return True
+
+
+def _grad_list(tensors, name: str):
+    tensors = list(tensors)
+    for t in tensors:
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be tensors, got {type(t).__name__}")
+        if not t.is_cuda:
+            raise _lib.DanceHipError(f"{name} must be GPU tensors (got one on {t.device}); dance_amd has no CPU path")
+        if t.dtype not in _ELEM or t.layout is not torch.strided:
+            raise TypeError(f"{name} must be dense torch.float32 or torch.bfloat16 tensors, got {t.dtype} ({t.layout})")
+    return tensors
+
+
+def _refuse_overlap(spans):
+    """spans: (first byte, end byte) of memory that is written or read beside a write; two of them may not share a byte."""
+    spans = sorted(v for v in spans if v[1] > v[0])
+    for (_, end), (begin, _) in zip(spans, spans[1:]):
+        if begin < end:
+            raise ValueError("clip_grads: tensors overlap in memory (the same tensor given twice, or views of one)")
+
+
+def _norm_tables(tensors):
+    import ctypes
+    n = len(tensors)
+    return (n, (ctypes.c_void_p * n)(*[t.data_ptr() for t in tensors]), (ctypes.c_int64 * n)(*[t.numel() for t in tensors]),
+            (ctypes.c_int32 * n)(*[_ELEM[t.dtype] for t in tensors]))
+
+
+def global_norm(tensors, norm_type: float = 2.0) -> torch.Tensor:
+    """The norm of all elements of ``tensors`` (fp32 / bf16, any shapes) as one vector: an fp32 scalar on their device, summed in double
+    (dh_grad_norm).  ``norm_type`` 1, 2 or inf."""
+    lib = _lib_ready()
+    code = _norm_type(norm_type)
+    tensors = _grad_list(tensors, "global_norm: tensors")
+    if not tensors:
+        raise ValueError("global_norm: no tensors")
+    with _one_device(*tensors):
+        dense = [t if _is_dense(t) else t.contiguous() for t in tensors]
+        n, ptrs, sizes, dtypes = _norm_tables(dense)
+        norm = torch.empty((), dtype=torch.float32, device=tensors[0].device)
+        ws_bytes = lib.dh_grad_norm_workspace_bytes(n, sizes)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=norm.device)
+        _call("grad_norm", lib.dh_grad_norm, n, ptrs, sizes, dtypes, code, norm.data_ptr(), ws.data_ptr(), ws_bytes, _stream())
+    return norm
+
+
+def clip_grads(grads, max_norm: float, *, norm_type: float = 2.0, out=None) -> torch.Tensor:
+    """Scale ``grads`` (fp32 / bf16 tensors) by min(1, max_norm / (norm + 1e-6)), norm = their global norm, which is returned as an fp32 scalar
+    on the device: in place, or into the tensors of ``out`` (fp32 or bf16 each, e.g. the fp32 gradients an optimiser works on).  Nothing
+    waits for the device.  See dh_grad_clip."""
+    import ctypes
+    lib = _lib_ready()
+    code = _norm_type(norm_type)
+    max_norm = float(max_norm)
+    if not max_norm >= 0:
+        raise ValueError(f"clip_grads: max_norm must not be negative, got {max_norm}")
+    grads = _grad_list(grads, "clip_grads: gradients")
+    if not grads:
+        raise ValueError("clip_grads: no gradients")
+    targets = grads if out is None else _grad_list(out, "clip_grads: out")
+    if len(targets) != len(grads):
+        raise ValueError(f"clip_grads: {len(targets)} outputs for {len(grads)} gradients")
+    with _one_device(*grads, *(() if out is None else targets)):
+        src, dst, back, spans = [], [], [], []
+        for g, o in zip(grads, targets):
+            if g.shape != o.shape:
+                raise ValueError(f"clip_grads: an output of shape {tuple(o.shape)} for a gradient of shape {tuple(g.shape)}")
+            same = g is o or (g.data_ptr() == o.data_ptr() and g.dtype == o.dtype and g.stride() == o.stride())
+            g_flat = _is_dense(g)
+            o_flat = g_flat if same else _is_dense(o)
+            if same and not g_flat and any(s == 0 and n > 1 for n, s in zip(g.shape, g.stride())):
+                raise ValueError("clip_grads: an expanded tensor cannot be scaled in place")
+            if not g_flat or (not same and not (o_flat and g.stride() == o.stride())):
+                # not consecutive, or in another order than the output: through consecutive copies
+                g_in = g.contiguous()
+                o_in = g_in if same else torch.empty(o.shape, dtype=o.dtype, device=o.device) if not o.is_contiguous() else o
+                if o_in is not o:
+                    back.append((o, o_in))
+                src.append(g_in)
+                dst.append(o_in)
+            else:
+                src.append(g)
+                dst.append(o)
+            at, size = o.data_ptr(), o.element_size()
+            if o_flat:
+                spans.append((at, at + o.numel() * size))
+            if not same and g_flat:
+                spans.append((g.data_ptr(), g.data_ptr() + g.numel() * g.element_size()))
+        _refuse_overlap(spans)
+        n, in_ptrs, sizes, in_types = _norm_tables(src)
+        _, out_ptrs, _, out_types = _norm_tables(dst)
+        norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
+        ws_bytes = lib.dh_grad_norm_workspace_bytes(n, sizes)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=norm.device)
+        _call("grad_clip", lib.dh_grad_clip, n, in_ptrs, out_ptrs, sizes, in_types, out_types, code, max_norm, norm.data_ptr(), ws.data_ptr(), ws_bytes,
+              _stream())
+        for o, o_in in back:
+            o.copy_(o_in)
+    torch.autograd.graph.increment_version(targets)  # (written behind autograd's back)
+    return norm
+
+
+def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False, foreach: Optional[bool] = None):
+    """``torch.nn.utils.clip_grad_norm_`` on dh_grad_clip (two launches per 128 tensors; the sums in double): scales the parameters' gradients
+    in place and returns their global norm.  ``norm_type`` 1, 2 or inf; ``error_if_nonfinite`` waits for the norm and raises before
+    anything is scaled; ``foreach`` is accepted for the signature's sake."""
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    grads = [p.grad for p in parameters if p.grad is not None]
+    if not grads:
+        return torch.tensor(0.0)
+    if error_if_nonfinite:
+        norm = global_norm(grads, norm_type)
+        if not bool(torch.isfinite(norm)):
+            raise RuntimeError(f"The total norm of order {norm_type} for gradients from `parameters` is non-finite, so it cannot be clipped. To "
+                               "disable this error and scale the gradients by the non-finite norm anyway, set `error_if_nonfinite=False`")
+    return clip_grads(grads, max_norm, norm_type=norm_type)
 
 
 # ---- optimiser ---------------------------------------------------------------------------------------------

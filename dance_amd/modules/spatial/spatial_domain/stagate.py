@@ -161,13 +161,14 @@ class Stagate(nn.Module, BasePretrain, BaseClusteringMethod):
         # (:191-194), so the order in which Adam touches the aliased memory matters; the per-parameter loop is what the
         # reference's CPU run executes (the multi-tensor path would read all old values first)
         optimizer = torch.optim.Adam(self.parameters(), lr=lr, weight_decay=weight_decay, foreach=False)
+        clip = kernels.clip_grad_norm_ if x_tensor.is_cuda else torch.nn.utils.clip_grad_norm_  # dh_grad_clip: two launches for all gradients
         self.train()
         for _ in range(1, epochs + 1):
             optimizer.zero_grad()
             z, out = self(x_tensor, edge_index_tensor)
             loss = F.mse_loss(x_tensor, out)
             loss.backward()
-            torch.nn.utils.clip_grad_norm_(self.parameters(), gradient_clipping)
+            clip(self.parameters(), gradient_clipping)
             optimizer.step()
         self.eval()
         z, _ = self(x_tensor, edge_index_tensor)

@@ -50,6 +50,8 @@ enum dh_act { DH_ACT_NONE = 0, DH_ACT_RELU = 1 };
 enum dh_reduce { DH_REDUCE_SUM = 0, DH_REDUCE_MEAN = 1 };
 enum dh_knn_algo { DH_KNN_AUTO = 0, DH_KNN_SCAN = 1, DH_KNN_FILTER = 2, DH_KNN_GRID = 3 };
 enum dh_dtype { DH_DTYPE_F32 = 0, DH_DTYPE_BF16 = 1 };
+enum dh_norm { DH_NORM_LAYER = 0, DH_NORM_RMS = 1 };
+enum dh_gate { DH_GATE_NONE = 0, DH_GATE_SCALAR = 1, DH_GATE_CHANNEL = 2, DH_GATE_ROW = 3, DH_GATE_FULL = 4 };
 enum dh_metric { DH_METRIC_EUCLIDEAN = 0, DH_METRIC_PEARSON = 1, DH_METRIC_SPEARMAN = 2 };
 
 /* ---- library ---------------------------------------------------------------------------- */
@@ -853,6 +855,57 @@ DH_API int dh_dec_kl_forward_f32(int64_t n, int64_t c, const float* p, int64_t l
                           void* workspace, size_t workspace_bytes, dh_stream_t stream);
 DH_API int dh_dec_kl_backward_f32(int64_t n, int64_t c, const float* p, int64_t ldp, const float* q, int64_t ldq, float eps, double scale, const float* g,
                            float* dq, int64_t ldd, dh_stream_t stream);
+
+/* ---- global norm of many gradients and their scaling (grad_clip.hip) --------------------------------------------------------------------
+ * dance/modules/spatial/spatial_domain/stagate.py:239-242 (clip_grad_norm_ between loss.backward() and optimizer.step()).  The tables
+ * (pointers, sizes in elements, dtypes) are HOST arrays of n entries, read before the call returns; a tensor is numel consecutive elements
+ * of f32 or bf16, in any order.  norm_type: 0 = max |g|, 1 = sum |g|, 2 = sqrt(sum g^2), accumulated in double in a fixed order;
+ * *norm (device, f32) receives it.  dh_grad_clip also writes out[t] = grads[t] * min(1, max_norm / (norm + 1e-6)) in out's dtype;
+ * out[t] may be grads[t] itself (same dtype), otherwise no out may overlap any tensor of the call.  A NaN in any gradient makes the norm
+ * and every scaled value NaN, an infinity makes the factor 0.  Nothing waits for the device.                                             */
+DH_API size_t dh_grad_norm_workspace_bytes(int n, const int64_t* numel_host);
+DH_API int dh_grad_norm(int n, const void* const* grads_host, const int64_t* numel_host, const int32_t* dtype_host, int norm_type, float* norm,
+                 void* workspace, size_t workspace_bytes, dh_stream_t stream);
+DH_API int dh_grad_clip(int n, const void* const* grads_host, void* const* out_host, const int64_t* numel_host, const int32_t* dtype_host,
+                 const int32_t* out_dtype_host, int norm_type, double max_norm, float* norm, void* workspace, size_t workspace_bytes,
+                 dh_stream_t stream);
+
+/* ---- norms around a block with its gate and residual (residual_norm.hip) ------------------------------------------------------------------
+ * dance/models/nn/gnn.py:84-96 (the norm slot of a layer; a node's own features added to its block's).  Rows of D <= 4096 columns:
+ *   n = has_post ? norm(f; w1, b1) : f;   r = x + scale * act(gate) * n;   h = norm(r; w2, b2) if has_pre
+ * f, x, r, h and row / full gates have `dtype` (f32, bf16); x NULL = 0; w NULL = ones, b NULL = zeros; scalar / channel gates and the
+ * parameters are f32.  gate_kind: dh_gate; gate_sigmoid: act = sigmoid.  kind: dh_norm.  stats [M, 4] f32 (16-byte aligned; NULL: not
+ * kept): mean and rstd of both norms, what the backward needs.  r may be NULL when has_pre.
+ * Backward: dr, dh (either may be NULL) -> df, dx, dgate (row / full: dtype; scalar / channel: f32) and the column sums dw1, db1, dw2,
+ * db2 (f32), each skipped when NULL; sums over rows in a fixed order.                                                                     */
+DH_API int dh_residual_norm_forward(int64_t M, int64_t D, int dtype, const void* f, int64_t ldf, const void* x, int64_t ldx, const void* gate,
+                             int64_t ldg, int gate_kind, int gate_sigmoid, float scale, int kind, float eps, int has_post, const float* w1,
+                             const float* b1, int has_pre, const float* w2, const float* b2, void* r, int64_t ldr, void* h, int64_t ldh,
+                             float* stats, dh_stream_t stream);
+DH_API size_t dh_residual_norm_backward_workspace_bytes(int64_t M, int64_t D);
+DH_API int dh_residual_norm_backward(int64_t M, int64_t D, int dtype, const void* f, int64_t ldf, const void* x, int64_t ldx, const void* gate,
+                              int64_t ldg, int gate_kind, int gate_sigmoid, float scale, int kind, int has_post, const float* w1,
+                              const float* b1, int has_pre, const float* w2, const float* stats, const void* dr, int64_t lddr, const void* dh,
+                              int64_t lddh, void* df, int64_t lddf, void* dx, int64_t lddx, void* dgate, int64_t lddg, float* dw1, float* db1,
+                              float* dw2, float* db2, void* workspace, size_t workspace_bytes, dh_stream_t stream);
+
+/* ---- products grouped by row type with ragged sizes (gemm_grouped.hip) ---------------------------------------------------------------------
+ * dance/models/nn/gnn.py:84-96 and scdeepsort.py:26-88 apply one Linear to every node; with typed nodes (genes / cells, tissues, donors)
+ * there is one weight per type.  group_ptr [G + 1] int32 ON THE DEVICE, non-decreasing: rows ptr[g] <= i < ptr[g + 1] belong to group g
+ * (values outside [0, M] are clamped: a wrong table gives wrong rows, never an access out of bounds).
+ *   dh_gemm_grouped:       Y[i] = act(X[i] op(W_g) + bias_g), op(W_g) = W_g^T with trans_b (W [G][N][K], row stride ldw, group stride stride_w),
+ *                          W_g without (W [G][K][N]); X, W: dtype; Y: y_dtype (rounded once); bias [G][N] f32, row stride ld_bias, or NULL.
+ *                          Rows of no group (before ptr[0], from ptr[G] on) are set to zero with zero_outside, left as they are without.
+ *   dh_gemm_grouped_wgrad: dW_g = sum_i dY[i]^T X[i] ([G][N][K], dw_dtype) and, db != NULL, db_g = sum_i dY[i] (f32); an empty group's are
+ *                          zero; sums over rows in a fixed order.
+ * Accumulation in fp32 on the matrix cores; M < 2^31 rows.                                                                                 */
+DH_API int dh_gemm_grouped(int64_t M, int64_t N, int64_t K, int64_t G, int trans_b, int dtype, const void* X, int64_t ldx, const void* W, int64_t ldw,
+                    int64_t stride_w, const int32_t* group_ptr, const float* bias, int64_t ld_bias, int act, void* Y, int64_t ldy, int y_dtype,
+                    int zero_outside, dh_stream_t stream);
+DH_API size_t dh_gemm_grouped_wgrad_workspace_bytes(int64_t M, int64_t N, int64_t K);
+DH_API int dh_gemm_grouped_wgrad(int64_t M, int64_t N, int64_t K, int64_t G, int dtype, const void* dY, int64_t ldy, const void* X, int64_t ldx,
+                          const int32_t* group_ptr, void* dW, int64_t ldw, int64_t stride_w, int dw_dtype, float* db, int64_t ld_db,
+                          void* workspace, size_t workspace_bytes, dh_stream_t stream);
 
 #ifdef __cplusplus
 }
