@@ -9,6 +9,7 @@ from typing import Optional, Tuple
 import contextlib
 import os
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -60,7 +61,8 @@ def _call(tag: str, fn, *args):
 
 
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    # the raw handle without building a torch.cuda.Stream object around it: 0.1 us instead of 2.6 per launch
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def _dev(t: Optional[torch.Tensor], dtype, name: str, ndim: Optional[int] = None) -> Optional[int]:
@@ -87,17 +89,21 @@ def _ld(t: torch.Tensor) -> int:
 def _one_device(*tensors: Optional[torch.Tensor]):
     """Context in which the tensors' own device is the current one (its current stream is the one the kernels are put on); tensors of
     more than one device are refused."""
-    dev = None
+    index = None
     for t in tensors:
-        if t is None or not t.is_cuda:  # (host tensors are refused by name in _dev)
+        if t is None or not t.is_cuda:  # (host tensors are refused by name where they are used)
             continue
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise ValueError(f"tensors on more than one device: {dev} and {t.device}")
-    if dev is None or dev.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(dev)
+        i = t.get_device()
+        if index is None:
+            index = i
+        elif i != index:
+            raise ValueError(f"tensors on more than one device: cuda:{index} and cuda:{i}")
+    if index is None or index == torch._C._cuda_getDevice():
+        return _HERE
+    return torch.cuda.device(index)
+
+
+_HERE = contextlib.nullcontext()
 
 
 def _lib_ready():
@@ -704,6 +710,7 @@ def colsum_bf16(X: torch.Tensor) -> torch.Tensor:
 
 # ---- products grouped by row type -----------------------------------------------------------------------------
 _ELEM = {torch.float32: DTYPE_F32, _BF16: DTYPE_BF16}
+_GROUPED_TAGS = (("gemm_grouped_f32_nn", "gemm_grouped_f32_nt"), ("gemm_grouped_bf16_nn", "gemm_grouped_bf16_nt"))
 
 
 def _elem(t: torch.Tensor, name: str) -> int:
@@ -713,12 +720,25 @@ def _elem(t: torch.Tensor, name: str) -> int:
     return code
 
 
-def _rows_ld(t: torch.Tensor, name: str) -> int:
-    """Row stride of a 2-d operand; overlapping rows (an expanded tensor) are refused."""
-    ld = _ld(t)
-    if t.shape[0] > 1 and ld < t.shape[1]:
-        raise ValueError(f"{name}: rows overlap (stride {ld} below the row length {t.shape[1]})")
-    return ld
+def _mat(t: Optional[torch.Tensor], dtype, name: str):
+    """(address, row stride) of a 2-d operand with contiguous rows that do not overlap; (None, 0) for None."""
+    if t is None:
+        return None, 0
+    if not t.is_cuda:
+        raise _lib.DanceHipError(f"{name} must be a GPU tensor (got {t.device}); dance_amd has no CPU path")
+    if t.dtype is not dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.dim() != 2:
+        raise ValueError(f"{name} must be 2-d, got shape {tuple(t.shape)}")
+    rows, cols = t.shape
+    ld, step = t.stride()
+    if step != 1 and rows and cols:
+        raise ValueError(f"{name} must be contiguous in its last dimension")
+    if rows <= 1:
+        ld = cols or 1
+    elif ld < cols:
+        raise ValueError(f"{name}: rows overlap (stride {ld} below the row length {cols})")
+    return t.data_ptr(), ld
 
 
 def _weight_strides(W: torch.Tensor, name: str):
@@ -760,10 +780,9 @@ def gemm_grouped(X: torch.Tensor, W: torch.Tensor, group_ptr: torch.Tensor, *, t
     elif tuple(out.shape) != (M, N) or (out_dtype is not None and out.dtype != out_dtype):
         raise ValueError(f"out must be [{M}, {N}]{'' if out_dtype is None else f' of {out_dtype}'}, got {tuple(out.shape)} of {out.dtype}")
     with _one_device(X, W, group_ptr, bias, out):
-        _call(f"gemm_grouped_{'bf16' if dt else 'f32'}_{'nt' if trans_b else 'nn'}", lib.dh_gemm_grouped, M, N, K, G, int(trans_b), dt,
-              _dev(X, X.dtype, "X", 2), _rows_ld(X, "X"), _dev(W, X.dtype, "W", 3), ldw, sw, _dev(group_ptr, torch.int32, "group_ptr", 1),
-              _dev(bias, torch.float32, "bias", 2), 0 if bias is None else _rows_ld(bias, "bias"), act, _dev(out, out.dtype, "out", 2),
-              _rows_ld(out, "out"), _elem(out, "out"), int(fresh), _stream())
+        _call(_GROUPED_TAGS[dt][bool(trans_b)], lib.dh_gemm_grouped, M, N, K, G, 1 if trans_b else 0, dt, *_mat(X, X.dtype, "X"),
+              _dev(W, X.dtype, "W", 3), ldw, sw, _dev(group_ptr, torch.int32, "group_ptr", 1), *_mat(bias, torch.float32, "bias"), act,
+              *_mat(out, out.dtype, "out"), _elem(out, "out"), 1 if fresh else 0, _stream())
     return out
 
 
@@ -785,8 +804,8 @@ def gemm_grouped_wgrad(dY: torch.Tensor, X: torch.Tensor, group_ptr: torch.Tenso
     with _one_device(dY, X, group_ptr):
         ws_bytes = lib.dh_gemm_grouped_wgrad_workspace_bytes(M, N, K)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=X.device)
-        _call(f"gemm_grouped_{'bf16' if dt else 'f32'}_tn", lib.dh_gemm_grouped_wgrad, M, N, K, G, dt, _dev(dY, X.dtype, "dY", 2), _rows_ld(dY, "dY"),
-              _dev(X, X.dtype, "X", 2), _rows_ld(X, "X"), _dev(group_ptr, torch.int32, "group_ptr", 1), dW.data_ptr(), max(K, 1), N * K,
+        _call("gemm_grouped_bf16_tn" if dt else "gemm_grouped_f32_tn", lib.dh_gemm_grouped_wgrad, M, N, K, G, dt, *_mat(dY, X.dtype, "dY"),
+              *_mat(X, X.dtype, "X"), _dev(group_ptr, torch.int32, "group_ptr", 1), dW.data_ptr(), max(K, 1), N * K,
               _elem(dW, "dW"), None if db is None else db.data_ptr(), max(N, 1), ws.data_ptr(), ws_bytes, _stream())
     return (dW, db) if want_bias else dW
 
@@ -829,7 +848,7 @@ def _gate_args(gate, kind: int, dtype):
         return None, 0
     if kind in (GATE_SCALAR, GATE_CHANNEL):
         return _dev(gate.reshape(-1), torch.float32, "gate", 1), 0
-    return _dev(gate, dtype, "gate", 2), (gate.stride(0) if gate.shape[0] > 1 else gate.shape[1]) if kind == GATE_ROW else _rows_ld(gate, "gate")
+    return _mat(gate, dtype, "gate")
 
 
 def _check_rows(t: Optional[torch.Tensor], like: torch.Tensor, name: str):
@@ -858,14 +877,15 @@ def residual_norm_forward(f: torch.Tensor, x: Optional[torch.Tensor] = None, *, 
     has_post, w1, b1 = _norm_params(post, D, "post")
     has_pre, w2, b2 = _norm_params(pre, D, "pre")
     gp, ldg = _gate_args(gate, gk, f.dtype)
-    fp, xp = _dev(f, f.dtype, "f", 2), _dev(x, f.dtype, "x", 2)
-    r = torch.empty((M, D), dtype=f.dtype, device=f.device)
-    h = torch.empty_like(r) if has_pre else None
+    fp, ldf = _mat(f, f.dtype, "f")
+    xp, ldx = _mat(x, f.dtype, "x")
+    r = f.new_empty((M, D))
+    h = f.new_empty((M, D)) if has_pre else None
     stats = torch.empty((M, 4), dtype=torch.float32, device=f.device) if want_stats else None
     with _one_device(f, x, gate, *(post or ()), *(pre or ())):
-        _call("residual_norm_forward", lib.dh_residual_norm_forward, M, D, dt, fp, _rows_ld(f, "f"), xp, 0 if x is None else _rows_ld(x, "x"), gp,
-              ldg, gk, int(gate_sigmoid), float(scale), kind, float(eps), has_post, w1, b1, has_pre, w2, b2, r.data_ptr(), D,
-              None if h is None else h.data_ptr(), D, None if stats is None else stats.data_ptr(), _stream())
+        _call("residual_norm_forward", lib.dh_residual_norm_forward, M, D, dt, fp, ldf, xp, ldx, gp, ldg, gk, 1 if gate_sigmoid else 0, scale, kind, eps,
+              has_post, w1, b1, has_pre, w2, b2, r.data_ptr(), D, None if h is None else h.data_ptr(), D,
+              None if stats is None else stats.data_ptr(), _stream())
     return r, h, stats
 
 
@@ -890,29 +910,27 @@ def residual_norm_backward(dr: Optional[torch.Tensor], dh: Optional[torch.Tensor
     has_post, w1, b1 = _norm_params(post, D, "post")
     has_pre, w2, _ = _norm_params(pre, D, "pre")
     gp, ldg = _gate_args(gate, gk, f.dtype)
-    new = {}
-    for key, there in (("f", True), ("x", x is not None), ("gate", gate is not None), ("w1", has_post), ("b1", has_post), ("w2", has_pre), ("b2", has_pre)):
-        if there and key in want:
-            if key in ("f", "x"):
-                new[key] = torch.empty((M, D), dtype=f.dtype, device=f.device)
-            elif key == "gate":
-                new[key] = torch.empty(gate.shape, dtype=gate.dtype, device=f.device)
-            else:
-                new[key] = torch.empty(D, dtype=torch.float32, device=f.device)
-    ptr = lambda key: new[key].data_ptr() if key in new else None
+    df = f.new_empty((M, D)) if "f" in want else None
+    dx = f.new_empty((M, D)) if x is not None and "x" in want else None
+    dgate = torch.empty_like(gate, memory_format=torch.contiguous_format) if gate is not None and "gate" in want else None
+    # one allocation for the column gradients of the norms
+    names = [n for n, there in (("w1", has_post), ("b1", has_post), ("w2", has_pre), ("b2", has_pre)) if there and n in want]
+    cols = dict(zip(names, torch.empty((len(names), D), dtype=torch.float32, device=f.device).unbind(0))) if names else {}
     if dh is None:  # nothing flows through the second norm
-        for key in ("w2", "b2"):
-            if key in new:
-                new[key].zero_()
+        for n in ("w2", "b2"):
+            if n in cols:
+                cols[n].zero_()
+    ptr = lambda t: None if t is None else t.data_ptr()
+    pw1, pb1, pw2, pb2 = (ptr(cols.get(n)) for n in ("w1", "b1", "w2", "b2"))
     with _one_device(f, x, gate, stats, dr, dh, *(post or ()), *(pre or ())):
         ws_bytes = lib.dh_residual_norm_backward_workspace_bytes(M, D)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=f.device)
-        _call("residual_norm_backward", lib.dh_residual_norm_backward, M, D, dt, _dev(f, f.dtype, "f", 2), _rows_ld(f, "f"), _dev(x, f.dtype, "x", 2),
-              0 if x is None else _rows_ld(x, "x"), gp, ldg, gk, int(gate_sigmoid), float(scale), kind, has_post, w1, b1, has_pre, w2,
-              _dev(stats, torch.float32, "stats", 2), _dev(dr, f.dtype, "dr", 2), 0 if dr is None else _rows_ld(dr, "dr"), _dev(dh, f.dtype, "dh", 2),
-              0 if dh is None else _rows_ld(dh, "dh"), ptr("f"), D, ptr("x"), D, ptr("gate"), D if gk == GATE_FULL else 1, ptr("w1"), ptr("b1"),
-              None if dh is None else ptr("w2"), None if dh is None else ptr("b2"), ws.data_ptr(), ws_bytes, _stream())
-    return new
+        _call("residual_norm_backward", lib.dh_residual_norm_backward, M, D, dt, *_mat(f, f.dtype, "f"), *_mat(x, f.dtype, "x"), gp, ldg, gk,
+              1 if gate_sigmoid else 0, scale, kind, has_post, w1, b1, has_pre, w2, _dev(stats, torch.float32, "stats", 2), *_mat(dr, f.dtype, "dr"),
+              *_mat(dh, f.dtype, "dh"), ptr(df), D, ptr(dx), D, ptr(dgate), D if gk == GATE_FULL else 1, pw1, pb1, None if dh is None else pw2,
+              None if dh is None else pb2, ws.data_ptr(), ws_bytes, _stream())
+    new = {"f": df, "x": dx, "gate": dgate, **cols}
+    return {n: t for n, t in new.items() if t is not None}
 
 
 # ---- graph builders ----------------------------------------------------------------------------------------
@@ -1234,6 +1252,7 @@ def _grad_list(tensors, name: str):
     for t in tensors:
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name} must be tensors, got {type(t).__name__}")
+    for t in tensors:
         if not t.is_cuda:
             raise _lib.DanceHipError(f"{name} must be GPU tensors (got one on {t.device}); dance_amd has no CPU path")
         if t.dtype not in _ELEM or t.layout is not torch.strided:
@@ -1241,19 +1260,22 @@ def _grad_list(tensors, name: str):
     return tensors
 
 
-def _refuse_overlap(spans):
-    """spans: (first byte, end byte) of memory that is written or read beside a write; two of them may not share a byte."""
-    spans = sorted(v for v in spans if v[1] > v[0])
-    for (_, end), (begin, _) in zip(spans, spans[1:]):
-        if begin < end:
-            raise ValueError("clip_grads: tensors overlap in memory (the same tensor given twice, or views of one)")
+def _refuse_overlap(begins, ends):
+    """Bytes [begins[i], ends[i]) are written, or read beside a write: no two of these ranges may share one (empty ranges aside)."""
+    begins, ends = np.asarray(begins, dtype=np.int64), np.asarray(ends, dtype=np.int64)
+    some = ends > begins
+    begins, ends = begins[some], ends[some]
+    order = np.argsort(begins, kind="stable")
+    if (begins[order][1:] < ends[order][:-1]).any():
+        raise ValueError("clip_grads: tensors overlap in memory (the same tensor given twice, or views of one)")
 
 
 def _norm_tables(tensors):
-    import ctypes
-    n = len(tensors)
-    return (n, (ctypes.c_void_p * n)(*[t.data_ptr() for t in tensors]), (ctypes.c_int64 * n)(*[t.numel() for t in tensors]),
-            (ctypes.c_int32 * n)(*[_ELEM[t.dtype] for t in tensors]))
+    """Host tables of a tensor list: addresses, sizes, dtypes (one pass each through a C-level map: hundreds of tensors are usual)."""
+    ptrs = np.fromiter(map(torch.Tensor.data_ptr, tensors), dtype=np.int64, count=len(tensors))
+    sizes = np.fromiter(map(torch.Tensor.numel, tensors), dtype=np.int64, count=len(tensors))
+    dtypes = np.fromiter((_ELEM[t.dtype] for t in tensors), dtype=np.int32, count=len(tensors))
+    return ptrs, sizes, dtypes
 
 
 def global_norm(tensors, norm_type: float = 2.0) -> torch.Tensor:
@@ -1265,20 +1287,20 @@ def global_norm(tensors, norm_type: float = 2.0) -> torch.Tensor:
     if not tensors:
         raise ValueError("global_norm: no tensors")
     with _one_device(*tensors):
-        dense = [t if _is_dense(t) else t.contiguous() for t in tensors]
-        n, ptrs, sizes, dtypes = _norm_tables(dense)
+        dense = tensors if all(map(torch.Tensor.is_contiguous, tensors)) else [t if _is_dense(t) else t.contiguous() for t in tensors]
+        ptrs, sizes, dtypes = _norm_tables(dense)
         norm = torch.empty((), dtype=torch.float32, device=tensors[0].device)
-        ws_bytes = lib.dh_grad_norm_workspace_bytes(n, sizes)
+        ws_bytes = lib.dh_grad_norm_workspace_bytes(len(dense), sizes.ctypes.data)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=norm.device)
-        _call("grad_norm", lib.dh_grad_norm, n, ptrs, sizes, dtypes, code, norm.data_ptr(), ws.data_ptr(), ws_bytes, _stream())
+        _call("grad_norm", lib.dh_grad_norm, len(dense), ptrs.ctypes.data, sizes.ctypes.data, dtypes.ctypes.data, code, norm.data_ptr(), ws.data_ptr(),
+              ws_bytes, _stream())
     return norm
 
 
 def clip_grads(grads, max_norm: float, *, norm_type: float = 2.0, out=None) -> torch.Tensor:
     """Scale ``grads`` (fp32 / bf16 tensors) by min(1, max_norm / (norm + 1e-6)), norm = their global norm, which is returned as an fp32 scalar
-    on the device: in place, or into the tensors of ``out`` (fp32 or bf16 each, e.g. the fp32 gradients an optimiser works on).  Nothing
-    waits for the device.  See dh_grad_clip."""
-    import ctypes
+    on the device: in place, or into the tensors of ``out`` (fp32 or bf16 each, as many elements as their gradient: e.g. the views of the
+    flat fp32 buffer that an optimiser works on).  Nothing waits for the device.  See dh_grad_clip."""
     lib = _lib_ready()
     code = _norm_type(norm_type)
     max_norm = float(max_norm)
@@ -1291,43 +1313,56 @@ def clip_grads(grads, max_norm: float, *, norm_type: float = 2.0, out=None) -> t
     if len(targets) != len(grads):
         raise ValueError(f"clip_grads: {len(targets)} outputs for {len(grads)} gradients")
     with _one_device(*grads, *(() if out is None else targets)):
-        src, dst, back, spans = [], [], [], []
-        for g, o in zip(grads, targets):
-            if g.shape != o.shape:
-                raise ValueError(f"clip_grads: an output of shape {tuple(o.shape)} for a gradient of shape {tuple(g.shape)}")
-            same = g is o or (g.data_ptr() == o.data_ptr() and g.dtype == o.dtype and g.stride() == o.stride())
-            g_flat = _is_dense(g)
-            o_flat = g_flat if same else _is_dense(o)
-            if same and not g_flat and any(s == 0 and n > 1 for n, s in zip(g.shape, g.stride())):
-                raise ValueError("clip_grads: an expanded tensor cannot be scaled in place")
-            if not g_flat or (not same and not (o_flat and g.stride() == o.stride())):
-                # not consecutive, or in another order than the output: through consecutive copies
-                g_in = g.contiguous()
-                o_in = g_in if same else torch.empty(o.shape, dtype=o.dtype, device=o.device) if not o.is_contiguous() else o
-                if o_in is not o:
-                    back.append((o, o_in))
-                src.append(g_in)
-                dst.append(o_in)
-            else:
-                src.append(g)
-                dst.append(o)
-            at, size = o.data_ptr(), o.element_size()
-            if o_flat:
-                spans.append((at, at + o.numel() * size))
-            if not same and g_flat:
-                spans.append((g.data_ptr(), g.data_ptr() + g.numel() * g.element_size()))
-        _refuse_overlap(spans)
-        n, in_ptrs, sizes, in_types = _norm_tables(src)
-        _, out_ptrs, _, out_types = _norm_tables(dst)
+        src, dst, back = grads, targets, ()
+        if not (all(map(torch.Tensor.is_contiguous, grads)) and (out is None or all(map(torch.Tensor.is_contiguous, targets)))):
+            src, dst, back = _consecutive(grads, targets)
+        in_ptrs, sizes, in_types = _norm_tables(src)
+        if dst is src:
+            out_ptrs, out_types = in_ptrs, in_types
+        else:
+            out_ptrs, out_sizes, out_types = _norm_tables(dst)
+            if (out_sizes != sizes).any():
+                i = int((out_sizes != sizes).argmax())
+                raise ValueError(f"clip_grads: an output of shape {tuple(targets[i].shape)} for a gradient of shape {tuple(grads[i].shape)}")
+        begins, ends = out_ptrs, out_ptrs + sizes * np.where(out_types == DTYPE_BF16, 2, 4)
+        if dst is not src:
+            other = (in_ptrs != out_ptrs) | (in_types != out_types)
+            begins = np.concatenate((begins, in_ptrs[other]))
+            ends = np.concatenate((ends, (in_ptrs + sizes * np.where(in_types == DTYPE_BF16, 2, 4))[other]))
+        _refuse_overlap(begins, ends)
         norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
-        ws_bytes = lib.dh_grad_norm_workspace_bytes(n, sizes)
+        ws_bytes = lib.dh_grad_norm_workspace_bytes(len(src), sizes.ctypes.data)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=norm.device)
-        _call("grad_clip", lib.dh_grad_clip, n, in_ptrs, out_ptrs, sizes, in_types, out_types, code, max_norm, norm.data_ptr(), ws.data_ptr(), ws_bytes,
-              _stream())
+        _call("grad_clip", lib.dh_grad_clip, len(src), in_ptrs.ctypes.data, out_ptrs.ctypes.data, sizes.ctypes.data, in_types.ctypes.data,
+              out_types.ctypes.data, code, max_norm, norm.data_ptr(), ws.data_ptr(), ws_bytes, _stream())
         for o, o_in in back:
             o.copy_(o_in)
     torch.autograd.graph.increment_version(targets)  # (written behind autograd's back)
     return norm
+
+
+def _consecutive(grads, targets):
+    """(inputs, outputs, copies to make afterwards) with consecutive elements in matching order: tensors that are so are taken as they are,
+    the others (column slices, outputs in another order than their gradient) go through contiguous copies."""
+    src, dst, back = [], [], []
+    for g, o in zip(grads, targets):
+        same = g is o or (g.data_ptr() == o.data_ptr() and g.dtype == o.dtype and g.shape == o.shape and g.stride() == o.stride())
+        flat = _is_dense(g)
+        if any(n > 1 and s == 0 for n, s in zip(o.shape, o.stride())):
+            raise ValueError("clip_grads: an expanded tensor cannot be written")
+        if flat and (same or (g.is_contiguous() and o.is_contiguous()) or (g.shape == o.shape and g.stride() == o.stride())):
+            src.append(g)
+            dst.append(g if same else o)
+            continue
+        if g.shape != o.shape:
+            raise ValueError(f"clip_grads: an output of shape {tuple(o.shape)} for a gradient of shape {tuple(g.shape)}")
+        g_in = g.contiguous()
+        o_in = g_in if same else o if o.is_contiguous() else torch.empty(o.shape, dtype=o.dtype, device=o.device)
+        if o_in is not o:
+            back.append((o, o_in))
+        src.append(g_in)
+        dst.append(o_in)
+    return src, dst, back
 
 
 def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False, foreach: Optional[bool] = None):

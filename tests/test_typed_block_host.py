@@ -175,9 +175,9 @@ def test_dense_and_overlap():
     t = torch.zeros(6, 8)
     assert kernels._is_dense(t) and kernels._is_dense(t.t()) and kernels._is_dense(t[1:3]) and not kernels._is_dense(t[:, :4])
     assert not kernels._is_dense(torch.zeros(1).expand(4)) and kernels._is_dense(torch.zeros(3, 1, 2).permute(2, 1, 0))
-    kernels._refuse_overlap([(0, 4), (4, 8), (8, 8)])
+    kernels._refuse_overlap([0, 4, 8, 6], [4, 8, 8, 6])
     with pytest.raises(ValueError):
-        kernels._refuse_overlap([(4, 8), (0, 5)])
+        kernels._refuse_overlap([4, 0], [8, 5])
 
 
 def test_norm_types():
