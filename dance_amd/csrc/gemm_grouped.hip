@@ -183,6 +183,26 @@ struct Operand {
   }
 };
 
+// f(m, n, values) for the elements of a workgroup's accumulators, four consecutive n of a row at a time: the B rows are given as the
+// instruction's first operand, so a lane's 32x32 results are row m = lane & 31, n = (r & 3) + 8 (r >> 2) + 4 (lane >> 5), r = 0 .. 15
+// (with A first a lane holds 16 rows of one column: four times as many, two-byte, stores: 818 against 726 us at 200003 x 2000 -> 512 bf16)
+template <int MI, int NI, int WC, class F>
+__device__ __forceinline__ void each4(const f32x16 (&acc)[MI][NI], int64_t m0, int64_t mlim, int64_t n0, int64_t nlim, F&& f) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int i = 0; i < MI; ++i) {
+    const int64_t m = m0 + (wave / WC) * MI * 32 + i * 32 + (lane & 31);
+    if (m >= mlim) continue;
+#pragma unroll
+    for (int j = 0; j < NI; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int64_t n = n0 + (wave % WC) * NI * 32 + j * 32 + 8 * q + 4 * (lane >> 5);
+        if (n < nlim) f(m, n, f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]});
+      }
+  }
+}
+
 // ---- the tile ------------------------------------------------------------------------------------------------------------------------
 // BM x BN of C = A B^T over k in [0, K): WR x WC waves of MI x NI 32 x 32 accumulators.  Two LDS stages: while the products of one step
 // run, the next one's pieces (requested a step earlier) are written and the ones after that requested.
@@ -217,7 +237,7 @@ struct Tile {
 #pragma unroll
         for (int i = 0; i < MI; ++i)
 #pragma unroll
-          for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], b[j], acc[i][j], 0, 0, 0);
+          for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(b[j], a[i], acc[i][j], 0, 0, 0);
       }
     } else {
 #pragma unroll
@@ -232,7 +252,7 @@ struct Tile {
 #pragma unroll
           for (int i = 0; i < MI; ++i)
 #pragma unroll
-            for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i][s], b[j][s], acc[i][j], 0, 0, 0);
+            for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(b[j][s], a[i][s], acc[i][j], 0, 0, 0);
       }
     }
   }
@@ -273,22 +293,222 @@ struct Tile {
       __syncthreads();
     }
   }
-  // f(m, n, value) for the tile's elements: 32x32 accumulator layout: column lane & 31, row (r & 3) + 8 (r >> 2) + 4 (lane >> 5)
   template <class F>
   __device__ __forceinline__ void each(int64_t m0, int64_t mlim, int64_t n0, int64_t nlim, F&& f) const {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    each4<MI, NI, WC>(acc, m0, mlim, n0, nlim, f);
+  }
+};
+
+// four consecutive values of a row; n + 4 may pass the row's end
+template <bool BF16>
+__device__ __forceinline__ void put4(void* row, int64_t n, int64_t nlim, f32x4 v) {
+  typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+  typedef unsigned int u32x2u __attribute__((ext_vector_type(2), aligned(2)));
+  if (BF16) {
+    uint16_t* p = static_cast<uint16_t*>(row) + n;
+    const uint16_t h[4] = {f32_bf16(v[0]), f32_bf16(v[1]), f32_bf16(v[2]), f32_bf16(v[3])};
+    if (n + 4 <= nlim) {
+      *reinterpret_cast<u32x2u*>(p) = u32x2u{(unsigned)h[0] | (unsigned)h[1] << 16, (unsigned)h[2] | (unsigned)h[3] << 16};
+    } else {
+      for (int e = 0; e < 3; ++e)
+        if (n + e < nlim) p[e] = h[e];
+    }
+  } else {
+    float* p = static_cast<float*>(row) + n;
+    if (n + 4 <= nlim) {
+      *reinterpret_cast<f32x4u*>(p) = v;
+    } else {
+      for (int e = 0; e < 3; ++e)
+        if (n + e < nlim) p[e] = v[e];
+    }
+  }
+}
+
+// ---- the bf16 tile filled by LDS DMA ---------------------------------------------------------------------------------------------------
+// The same product with the operands going from memory to LDS without passing registers (global_load_lds, 16 bytes a lane): what the big
+// products run on.  The DMA writes a wave's 64 pieces to 1 KB of LDS in lane order, so images cannot be padded; bank conflicts are avoided by
+// choosing WHICH piece a lane fetches: piece c of an image row lies at position c ^ x,
+//   [row][k] images (128-byte rows):  x = (row >> 1) & 7: the 16 rows that a 16-byte fragment read takes at a time cover all 16 slots of
+//                                     two rows;
+//   [k][row] images (2 R-byte rows):  x = (k & 3) << 2: the four k rows that a transposing read takes from lie 64 bytes apart.
+// Needs 16-byte aligned rows (address and stride) and, for a [k][row] operand, a row count that is a multiple of 8 (a piece is whole or
+// absent).  The last, partial step of k goes through registers with zeros beyond the end, requested one step ahead like every other.
+typedef const __attribute__((address_space(1))) void* global_ptr;
+typedef __attribute__((address_space(3))) void* lds_ptr;
+
+template <bool KM, int R, int THREADS>
+struct DmaOperand {
+  static constexpr int BK = 64, CPR = KM ? R / 8 : 8, PIECES = R * 8 / THREADS, ELEMS = R * BK;
+  static_assert(PIECES * THREADS == R * 8 && (!KM || R >= 128), "tile does not divide among the threads");
+
+  const uint16_t* p[PIECES];
+
+  static __device__ __forceinline__ int image_row(int q) { return (q * THREADS + (int)threadIdx.x) / CPR; }
+  static __device__ __forceinline__ int piece(int q) {
+    const int row = image_row(q), c = (q * THREADS + (int)threadIdx.x) % CPR;
+    return KM ? c ^ ((row & 3) << 2) : c ^ ((row >> 1) & 7);
+  }
+  __device__ __forceinline__ void start(const uint16_t* base, int64_t ld, int64_t r0, int64_t rlim, int64_t k0) {
+#pragma unroll
+    for (int q = 0; q < PIECES; ++q) {
+      if (KM) p[q] = base + (k0 + image_row(q)) * ld + min(r0 + piece(q) * 8, rlim - 8);
+      else p[q] = base + min(r0 + image_row(q), rlim - 1) * ld + k0 + piece(q) * 8;
+    }
+  }
+  // the next BK of k into an image
+  __device__ __forceinline__ void issue(uint16_t* img, int64_t ld) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+    for (int q = 0; q < PIECES; ++q) {
+      __builtin_amdgcn_global_load_lds((global_ptr)p[q], (lds_ptr)(img + (q * THREADS + wave * 64) * 8), 16, 0, 0);
+      p[q] += KM ? BK * ld : BK;
+    }
+  }
+  // the last `left` < BK of k
+  __device__ __forceinline__ void fetch_tail(u32x4 (&v)[PIECES], int left, int64_t ld) const {
+#pragma unroll
+    for (int q = 0; q < PIECES; ++q) {
+      const int k = KM ? image_row(q) : piece(q) * 8;
+      const int back = max(k - (KM ? left - 1 : left - 8), 0);  // pieces beyond the end read the last one again
+      v[q] = *reinterpret_cast<const u32x4*>(p[q] - (KM ? back * ld : back));
+    }
+  }
+  static __device__ __forceinline__ void store_tail(uint16_t* img, const u32x4 (&v)[PIECES], int left) {
+#pragma unroll
+    for (int q = 0; q < PIECES; ++q) {
+      const int k = KM ? image_row(q) : piece(q) * 8;
+      *reinterpret_cast<u32x4*>(img + (q * THREADS + (int)threadIdx.x) * 8) = k < left ? v[q] : u32x4(0u);
+    }
+  }
+  // the fragment of rows [32 tile, 32 tile + 32), k [kk, kk + 16): lane l holds row l & 31, k (l >> 5) * 8 .. + 8
+  static __device__ __forceinline__ bf16x8 frag(const uint16_t* img, int tile, int kk) {
+    const int lane = threadIdx.x & 63;
+    if (!KM) {
+      const int c = (kk >> 3) + (lane >> 5);
+      return *reinterpret_cast<const bf16x8*>(img + (tile * 32 + (lane & 31)) * BK + ((c ^ ((lane >> 1) & 7)) << 3));
+    }
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef s16x4 __attribute__((address_space(3))) * lds_s16x4;
+    const int b = lane >> 4, i = lane & 15, x = i >> 2;  // x = k & 3 of the lane's row
+    const uint16_t* at = img + (kk + (b >> 1) * 8 + x) * R + (tile ^ x) * 32 + (b & 1) * 16 + (i & 3) * 4;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)at);
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + 4 * R));
+    bf16x8 f;
+    __builtin_memcpy(&f, &lo, 8);
+    __builtin_memcpy(reinterpret_cast<char*>(&f) + 8, &hi, 8);
+    return f;
+  }
+};
+
+// every wave's DMA has landed and its image reads are done: what the barrier by itself does not wait for is the DMA (vmcnt)
+__device__ __forceinline__ void images_ready() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __syncthreads();
+}
+
+template <bool A_KM, bool B_KM, int MI, int NI, int WR, int WC>
+struct DmaTile {
+  static constexpr int BM = MI * WR * 32, BN = NI * WC * 32, THREADS = WR * WC * 64, BK = 64;
+  typedef DmaOperand<A_KM, BM, THREADS> OpA;
+  typedef DmaOperand<B_KM, BN, THREADS> OpB;
+  static constexpr int STAGE = OpA::ELEMS + OpB::ELEMS, LDS_BYTES = 2 * STAGE * 2;
+
+  f32x16 acc[MI][NI];
+  float row_sum[MI];  // with SUMS: sum over k of the A rows, over the k that this lane's fragments hold
+
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      row_sum[i] = 0.f;
+#pragma unroll
+      for (int j = 0; j < NI; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+    }
+  }
+  template <bool SUMS>
+  __device__ __forceinline__ void product(const uint16_t* st, int kk) {
+    const int wave = threadIdx.x >> 6, tm = (wave / WC) * MI, tn = (wave % WC) * NI;
+    bf16x8 a[MI], b[NI];
+#pragma unroll
+    for (int i = 0; i < MI; ++i) a[i] = OpA::frag(st, tm + i, kk);
+#pragma unroll
+    for (int j = 0; j < NI; ++j) b[j] = OpB::frag(st + OpA::ELEMS, tn + j, kk);
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
-      for (int j = 0; j < NI; ++j) {
-        const int64_t n = n0 + (wave % WC) * NI * 32 + j * 32 + (lane & 31);
-        if (n >= nlim) continue;
+      for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(b[j], a[i], acc[i][j], 0, 0, 0);
+    if (SUMS) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int64_t m = m0 + (wave / WC) * MI * 32 + i * 32 + (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5);
-          if (m < mlim) f(m, n, acc[i][j][r]);
-        }
+      for (int i = 0; i < MI; ++i) {
+        u32x4 v;
+        __builtin_memcpy(&v, &a[i], 16);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) row_sum[i] += __uint_as_float(v[e] << 16) + __uint_as_float(v[e] & 0xffff0000u);
       }
+    }
+  }
+  template <bool SUMS>
+  __device__ __forceinline__ void run(const uint16_t* A, int64_t lda, int64_t m0, int64_t mlim, const uint16_t* B, int64_t ldb, int64_t n0,
+                                      int64_t nlim, int64_t k_begin, int64_t k_end, uint16_t* lds) {
+    zero();
+    if (k_end <= k_begin) return;
+    OpA a;
+    OpB b;
+    a.start(A, lda, m0, mlim, k_begin);
+    b.start(B, ldb, n0, nlim, k_begin);
+    const int64_t full = (k_end - k_begin) / BK;
+    const int left = (int)((k_end - k_begin) % BK);
+    const int64_t steps = full + (left > 0);
+    u32x4 ta[OpA::PIECES], tb[OpB::PIECES];
+    if (full > 0) {
+      a.issue(lds, lda);
+      b.issue(lds + OpA::ELEMS, ldb);
+    } else {
+      a.fetch_tail(ta, left, lda);
+      b.fetch_tail(tb, left, ldb);
+      OpA::store_tail(lds, ta, left);
+      OpB::store_tail(lds + OpA::ELEMS, tb, left);
+    }
+    images_ready();
+    for (int64_t t = 0; t + 1 < full; ++t) {
+      uint16_t *st = lds + (t & 1) * STAGE, *next = lds + ((t + 1) & 1) * STAGE;
+      a.issue(next, lda);
+      b.issue(next + OpA::ELEMS, ldb);
+#pragma unroll
+      for (int kk = 0; kk < BK; kk += 16) product<SUMS>(st, kk);
+      images_ready();
+    }
+    if (full > 0) {
+      uint16_t *st = lds + ((full - 1) & 1) * STAGE, *next = lds + (full & 1) * STAGE;
+      if (left > 0) {
+        a.fetch_tail(ta, left, lda);
+        b.fetch_tail(tb, left, ldb);
+      }
+#pragma unroll
+      for (int kk = 0; kk < BK; kk += 16) product<SUMS>(st, kk);
+      if (left > 0) {
+        OpA::store_tail(next, ta, left);
+        OpB::store_tail(next + OpA::ELEMS, tb, left);
+        images_ready();
+      }
+    }
+    if (left > 0)
+      for (int kk = 0; kk < left; kk += 16) product<SUMS>(lds + ((steps - 1) & 1) * STAGE, kk);
+  }
+  template <class F>
+  __device__ __forceinline__ void each(int64_t m0, int64_t mlim, int64_t n0, int64_t nlim, F&& f) const {
+    each4<MI, NI, WC>(acc, m0, mlim, n0, nlim, f);
+  }
+  // put(row of the tile, its sum): the waves of the first tile column hold every row, the two half waves half of its k each
+  template <class Put>
+  __device__ __forceinline__ void row_sums(Put&& put) const {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      const float v = row_sum[i] + __shfl_xor(row_sum[i], 32);
+      if (wave % WC == 0 && lane < 32) put((wave / WC) * MI * 32 + i * 32 + lane, v);
+    }
   }
 };
 
@@ -305,18 +525,34 @@ struct FwdArgs {
   int act, y_bf16, zero_outside;
 };
 
-template <class T, bool W_KM, int MI, int NI, int WR, int WC>
-__global__ __launch_bounds__(WR* WC * 64) void grouped_forward_kernel(const FwdArgs a) {
-  typedef Tile<T, false, W_KM, MI, NI, WR, WC> TileT;
+// bias and activation of a tile, then its stores
+template <class TileT, class Put>
+__device__ __forceinline__ void finish(const FwdArgs& a, const Slot& s, int64_t n0, const TileT& t, Put&& put) {
+  const float* bias = a.bias ? a.bias + s.group * a.ld_bias : nullptr;
+  t.each(s.begin, s.end, n0, a.N, [&](int64_t m, int64_t n, f32x4 v) __attribute__((always_inline)) {
+    if (bias) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += bias[min(n + e, a.N - 1)];
+    }
+    if (a.act == DH_ACT_RELU) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = v[e] < 0.f ? 0.f : v[e];  // (a NaN passes)
+    }
+    put(m, n, v);
+  });
+}
+
+template <class T, class TileT, bool DMA>
+__global__ __launch_bounds__(TileT::THREADS) void grouped_forward_kernel(const FwdArgs a) {
   extern __shared__ __attribute__((aligned(16))) unsigned char raw_lds[];
   const int64_t tiles_n = (a.N + TileT::BN - 1) / TileT::BN;
   const int64_t id = xcd_run(blockIdx.x, gridDim.x);
   const Slot s = find_slot(a.gr, id / tiles_n, __builtin_ctz(TileT::BM));
   if (!s.live) return;
   const int64_t n0 = (id % tiles_n) * TileT::BN;
-  auto put = [&](int64_t m, int64_t n, float v) __attribute__((always_inline)) {
-    if (a.y_bf16) static_cast<uint16_t*>(a.Y)[m * a.ldy + n] = f32_bf16(v);
-    else static_cast<float*>(a.Y)[m * a.ldy + n] = v;
+  auto put = [&](int64_t m, int64_t n, f32x4 v) __attribute__((always_inline)) {
+    if (a.y_bf16) put4<true>(static_cast<uint16_t*>(a.Y) + m * a.ldy, n, a.N, v);
+    else put4<false>(static_cast<float*>(a.Y) + m * a.ldy, n, a.N, v);
   };
   TileT t;
   if (s.group < 0) {
@@ -325,14 +561,11 @@ __global__ __launch_bounds__(WR* WC * 64) void grouped_forward_kernel(const FwdA
     t.each(s.begin, s.end, n0, a.N, put);
     return;
   }
-  t.run(static_cast<const T*>(a.X), a.ldx, s.begin, s.end, static_cast<const T*>(a.W) + s.group * a.stride_w, a.ldw, n0, a.N, 0, a.K,
-        reinterpret_cast<T*>(raw_lds), [](const auto&) {});
-  const float* bias = a.bias ? a.bias + s.group * a.ld_bias : nullptr;
-  t.each(s.begin, s.end, n0, a.N, [&](int64_t m, int64_t n, float v) __attribute__((always_inline)) {
-    if (bias) v += bias[n];
-    if (a.act == DH_ACT_RELU) v = v < 0.f ? 0.f : v;  // (a NaN passes)
-    put(m, n, v);
-  });
+  const T *X = static_cast<const T*>(a.X), *W = static_cast<const T*>(a.W) + s.group * a.stride_w;
+  T* lds = reinterpret_cast<T*>(raw_lds);
+  if constexpr (DMA) t.template run<false>(X, a.ldx, s.begin, s.end, W, a.ldw, n0, a.N, 0, a.K, lds);
+  else t.run(X, a.ldx, s.begin, s.end, W, a.ldw, n0, a.N, 0, a.K, lds, [](const auto&) {});
+  finish(a, s, n0, t, put);
 }
 
 // ---- dW, db --------------------------------------------------------------------------------------------------------------------------
@@ -356,9 +589,8 @@ struct WgradArgs {
   int64_t tiles_k, tiles;
 };
 
-template <class T, int MI, int NI, int WR, int WC>
-__global__ __launch_bounds__(WR* WC * 64) void grouped_wgrad_kernel(const WgradArgs a) {
-  typedef Tile<T, true, true, MI, NI, WR, WC> TileT;
+template <class T, class TileT, bool DMA>
+__global__ __launch_bounds__(TileT::THREADS) void grouped_wgrad_kernel(const WgradArgs a) {
   typedef typename TileT::OpA OpA;
   extern __shared__ __attribute__((aligned(16))) unsigned char raw_lds[];
   const int64_t id = xcd_run(blockIdx.x, gridDim.x);
@@ -369,51 +601,62 @@ __global__ __launch_bounds__(WR* WC * 64) void grouped_wgrad_kernel(const WgradA
   const int64_t tile = id % a.tiles, n0 = (tile / a.tiles_k) * TileT::BM, k0 = (tile % a.tiles_k) * TileT::BN;
   const bool alone = glen <= ((int64_t)1 << a.shift);
   const bool sums = a.db && k0 == 0;
-  constexpr int VEC = Geo<T>::VEC;
-  float cs[OpA::PIECES > 0 ? VEC : 1];
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) cs[e] = 0.f;
+  const int64_t end = s.live ? s.end : s.begin;
+  const T *dY = static_cast<const T*>(a.dY), *X = static_cast<const T*>(a.X);
+  T* stages = reinterpret_cast<T*>(raw_lds);
   TileT t;
-  t.run(static_cast<const T*>(a.dY), a.ldy, n0, a.N, static_cast<const T*>(a.X), a.ldx, k0, a.K, s.begin, s.live ? s.end : s.begin,
-        reinterpret_cast<T*>(raw_lds), [&](const OpA& op) __attribute__((always_inline)) {
-          if (!sums) return;
+  constexpr int VEC = Geo<T>::VEC;
+  float cs[VEC];
+  if constexpr (DMA) {
+    if (sums) t.template run<true>(dY, a.ldy, n0, a.N, X, a.ldx, k0, a.K, s.begin, end, stages);
+    else t.template run<false>(dY, a.ldy, n0, a.N, X, a.ldx, k0, a.K, s.begin, end, stages);
+  } else {
 #pragma unroll
-          for (int q = 0; q < OpA::PIECES; ++q) {
-            T e[VEC];
-            __builtin_memcpy(e, &op.reg[q], 16);
+    for (int e = 0; e < VEC; ++e) cs[e] = 0.f;
+    t.run(dY, a.ldy, n0, a.N, X, a.ldx, k0, a.K, s.begin, end, stages, [&](const OpA& op) __attribute__((always_inline)) {
+      if (!sums) return;
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-              if constexpr (sizeof(T) == 2) cs[i] += bf16_f32(e[i]);
-              else cs[i] += e[i];
-            }
-          }
-        });
+      for (int q = 0; q < OpA::PIECES; ++q) {
+        T e[VEC];
+        __builtin_memcpy(e, &op.reg[q], 16);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          if constexpr (sizeof(T) == 2) cs[i] += bf16_f32(e[i]);
+          else cs[i] += e[i];
+        }
+      }
+    });
+  }
   const int64_t slot = alone ? 0 : 2 * (s.begin >> a.shift) + (s.index > 0 ? 1 : 0);
   if (alone) {
-    char* out = static_cast<char*>(a.dW);
-    t.each(n0, a.N, k0, a.K, [&](int64_t n, int64_t k, float v) __attribute__((always_inline)) {
-      const int64_t at = s.group * a.stride_w + n * a.ldw + k;
-      if (a.dw_bf16) reinterpret_cast<uint16_t*>(out)[at] = f32_bf16(v);
-      else reinterpret_cast<float*>(out)[at] = v;
+    const int64_t at = s.group * a.stride_w;
+    t.each(n0, a.N, k0, a.K, [&](int64_t n, int64_t k, f32x4 v) __attribute__((always_inline)) {
+      if (a.dw_bf16) put4<true>(static_cast<uint16_t*>(a.dW) + at + n * a.ldw, k, a.K, v);
+      else put4<false>(static_cast<float*>(a.dW) + at + n * a.ldw, k, a.K, v);
     });
   } else {
     float* out = a.part_w + slot * a.N * a.K;
-    t.each(n0, a.N, k0, a.K, [&](int64_t n, int64_t k, float v) __attribute__((always_inline)) { out[n * a.K + k] = v; });
+    t.each(n0, a.N, k0, a.K, [&](int64_t n, int64_t k, f32x4 v) __attribute__((always_inline)) { put4<false>(out + n * a.K, k, a.K, v); });
   }
-  if (sums) {  // thread t summed columns (t % CPR) * VEC of the rows it staged
-    float* lds = reinterpret_cast<float*>(raw_lds);
-    __syncthreads();
-    constexpr int LD = TileT::BM + 4;
-    const int rg = threadIdx.x / OpA::CPR, c = (threadIdx.x % OpA::CPR) * VEC;
+  if (sums) {
+    auto put = [&](int i, float v) __attribute__((always_inline)) {
+      if (n0 + i >= a.N) return;
+      if (alone) a.db[s.group * a.ld_db + n0 + i] = v;
+      else a.part_b[slot * a.N + n0 + i] = v;
+    };
+    if constexpr (DMA) t.row_sums(put);
+    else {  // thread t summed columns (t % CPR) * VEC of the rows it staged
+      float* lds = reinterpret_cast<float*>(raw_lds);
+      __syncthreads();
+      constexpr int LD = TileT::BM + 4;
+      const int rg = threadIdx.x / OpA::CPR, c = (threadIdx.x % OpA::CPR) * VEC;
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) lds[rg * LD + c + e] = cs[e];
-    __syncthreads();
-    for (int i = threadIdx.x; i < TileT::BM; i += TileT::THREADS) {
-      float v = 0.f;
-      for (int r = 0; r < OpA::ROWS_PER_PASS; ++r) v += lds[r * LD + i];
-      if (n0 + i < a.N) {
-        if (alone) a.db[s.group * a.ld_db + n0 + i] = v;
-        else a.part_b[slot * a.N + n0 + i] = v;
+      for (int e = 0; e < VEC; ++e) lds[rg * LD + c + e] = cs[e];
+      __syncthreads();
+      for (int i = threadIdx.x; i < TileT::BM; i += TileT::THREADS) {
+        float v = 0.f;
+        for (int r = 0; r < OpA::ROWS_PER_PASS; ++r) v += lds[r * LD + i];
+        put(i, v);
       }
     }
   }
@@ -456,23 +699,29 @@ __global__ __launch_bounds__(256) void wgrad_join_kernel(const WgradArgs a) {
 // ---- host ----------------------------------------------------------------------------------------------------------------------------
 constexpr int64_t MAX_GRID = 0x7fffffff;
 
-template <class T, bool W_KM, int MI, int NI, int WR, int WC>
+template <class T, class TileT, bool DMA>
 int forward_launch(const char* me, const FwdArgs& a, hipStream_t st) {
-  typedef Tile<T, false, W_KM, MI, NI, WR, WC> TileT;
   const int64_t slots = a.gr.M / TileT::BM + a.gr.G + 2, grid = slots * dh::ceil_div(a.N, TileT::BN);
   if (grid > MAX_GRID) return dh::fail(DH_ERR_INVALID, "%s: %lld tiles in one launch", me, (long long)grid);
-  auto* kernel = grouped_forward_kernel<T, W_KM, MI, NI, WR, WC>;
+  auto* kernel = grouped_forward_kernel<T, TileT, DMA>;
   static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, TileT::LDS_BYTES);
   if (attr != hipSuccess) return dh::fail(DH_ERR_LAUNCH, "%s: %d bytes of LDS: %s", me, TileT::LDS_BYTES, hipGetErrorString(attr));
   hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(TileT::THREADS), TileT::LDS_BYTES, st, a);
   return dh::check_launch(me);
 }
 
+bool dma_rows(const void* p, int64_t ld) { return dh::aligned16(p) && ld % 8 == 0; }
+
 template <class T, bool W_KM>
 int forward_pick(const char* me, const FwdArgs& a, hipStream_t st) {
   // few rows per group: a 32-row tile wastes less of the matrix cores and of the slots
-  if (a.gr.M <= (int64_t)48 * a.gr.G) return forward_launch<T, W_KM, 1, 1, 1, 4>(me, a, st);
-  return forward_launch<T, W_KM, 2, 2, 2, 2>(me, a, st);
+  if (a.gr.M <= (int64_t)48 * a.gr.G) return forward_launch<T, Tile<T, false, W_KM, 1, 1, 1, 4>, false>(me, a, st);
+  if constexpr (sizeof(T) == 2) {
+    const bool dma = dma_rows(a.X, a.ldx) && dma_rows(a.W, a.ldw) && a.stride_w % 8 == 0 && a.K % 8 == 0 && (!W_KM || a.N % 8 == 0);
+    if (dma && a.gr.M >= (int64_t)1024 * a.gr.G) return forward_launch<T, DmaTile<false, W_KM, 4, 2, 2, 4>, true>(me, a, st);
+    if (dma) return forward_launch<T, DmaTile<false, W_KM, 2, 2, 2, 2>, true>(me, a, st);
+  }
+  return forward_launch<T, Tile<T, false, W_KM, 2, 2, 2, 2>, false>(me, a, st);
 }
 
 constexpr int WG_TILE = 128;
@@ -487,6 +736,19 @@ int wgrad_shift(int64_t M, int64_t N, int64_t K) {
 }
 
 int64_t wgrad_slots(int64_t M, int shift) { return 2 * ((M >> shift) + 1); }
+
+template <class T, class TileT, bool DMA>
+int wgrad_launch(const char* me, WgradArgs a, hipStream_t st) {
+  a.tiles_k = dh::ceil_div(a.K, TileT::BN);
+  a.tiles = dh::ceil_div(a.N, TileT::BM) * a.tiles_k;
+  const int64_t grid = ((a.gr.M >> a.shift) + a.gr.G + 2) * a.tiles;
+  if (grid > MAX_GRID) return dh::fail(DH_ERR_INVALID, "%s: %lld tiles in one launch", me, (long long)grid);
+  auto* kernel = grouped_wgrad_kernel<T, TileT, DMA>;
+  static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, TileT::LDS_BYTES);
+  if (attr != hipSuccess) return dh::fail(DH_ERR_LAUNCH, "%s: %d bytes of LDS: %s", me, TileT::LDS_BYTES, hipGetErrorString(attr));
+  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(TileT::THREADS), TileT::LDS_BYTES, st, a);
+  return dh::check_launch(me);
+}
 
 int check_grouped(const char* me, int64_t M, int64_t N, int64_t K, int64_t G, int dtype) {
   if (M < 0 || N < 0 || K < 0 || G < 0) return dh::fail(DH_ERR_INVALID, "%s: negative size", me);
@@ -544,24 +806,12 @@ extern "C" int dh_gemm_grouped_wgrad(int64_t M, int64_t N, int64_t K, int64_t G,
   const int64_t slots = wgrad_slots(M, a.shift);
   a.part_w = static_cast<float*>(workspace);
   a.part_b = a.part_w + slots * N * K;
-  a.tiles_k = dh::ceil_div(K, WG_TILE);
-  a.tiles = dh::ceil_div(N, WG_TILE) * a.tiles_k;
-  const int64_t grid = ((M >> a.shift) + G + 2) * a.tiles;
-  if (grid > MAX_GRID) return dh::fail(DH_ERR_INVALID, "%s: %lld tiles in one launch", me, (long long)grid);
   hipStream_t st = dh::as_stream(stream);
-  if (dtype == DH_DTYPE_BF16) {
-    typedef Tile<uint16_t, true, true, 2, 2, 2, 2> TileT;
-    auto* kernel = grouped_wgrad_kernel<uint16_t, 2, 2, 2, 2>;
-    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, TileT::LDS_BYTES);
-    if (attr != hipSuccess) return dh::fail(DH_ERR_LAUNCH, "%s: %d bytes of LDS: %s", me, TileT::LDS_BYTES, hipGetErrorString(attr));
-    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(TileT::THREADS), TileT::LDS_BYTES, st, a);
-  } else {
-    typedef Tile<float, true, true, 2, 2, 2, 2> TileT;
-    auto* kernel = grouped_wgrad_kernel<float, 2, 2, 2, 2>;
-    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, TileT::LDS_BYTES);
-    if (attr != hipSuccess) return dh::fail(DH_ERR_LAUNCH, "%s: %d bytes of LDS: %s", me, TileT::LDS_BYTES, hipGetErrorString(attr));
-    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(TileT::THREADS), TileT::LDS_BYTES, st, a);
-  }
+  int launched;
+  if (dtype != DH_DTYPE_BF16) launched = wgrad_launch<float, Tile<float, true, true, 2, 2, 2, 2>, false>(me, a, st);
+  else if (dma_rows(dY, ldy) && dma_rows(X, ldx) && N % 8 == 0 && K % 8 == 0) launched = wgrad_launch<uint16_t, DmaTile<true, true, 2, 2, 2, 2>, true>(me, a, st);
+  else launched = wgrad_launch<uint16_t, Tile<uint16_t, true, true, 2, 2, 2, 2>, false>(me, a, st);
+  if (launched != DH_OK) return launched;
   if ((M >> a.shift) > 0)
     hipLaunchKernelGGL(wgrad_join_kernel, dim3((unsigned)dh::ceil_div(N * K + N, 256), (unsigned)(M >> a.shift)), dim3(256), 0, st, a);
   return dh::check_launch(me);
