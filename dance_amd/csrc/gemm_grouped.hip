@@ -332,9 +332,11 @@ __device__ __forceinline__ void put4(void* row, int64_t n, int64_t nlim, f32x4 v
 //                                     two rows;
 //   [k][row] images (2 R-byte rows):  x = (k & 3) << 2: the four k rows that a transposing read takes from lie 64 bytes apart.
 // Needs 16-byte aligned rows (address and stride) and, for a [k][row] operand, a row count that is a multiple of 8 (a piece is whole or
-// absent).  The last, partial step of k goes through registers with zeros beyond the end, requested one step ahead like every other.
+// absent).  In the last, partial step of k the lanes whose pieces lie behind the end fetch a piece of zeros instead.
 typedef const __attribute__((address_space(1))) void* global_ptr;
 typedef __attribute__((address_space(3))) void* lds_ptr;
+
+__device__ __attribute__((aligned(16))) const uint32_t zero_piece[4] = {0, 0, 0, 0};
 
 template <bool KM, int R, int THREADS>
 struct DmaOperand {
@@ -364,20 +366,14 @@ struct DmaOperand {
       p[q] += KM ? BK * ld : BK;
     }
   }
-  // the last `left` < BK of k
-  __device__ __forceinline__ void fetch_tail(u32x4 (&v)[PIECES], int left, int64_t ld) const {
+  // the last `left` < BK of k, zeros behind them
+  __device__ __forceinline__ void issue_last(uint16_t* img, int left) const {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
     for (int q = 0; q < PIECES; ++q) {
       const int k = KM ? image_row(q) : piece(q) * 8;
-      const int back = max(k - (KM ? left - 1 : left - 8), 0);  // pieces beyond the end read the last one again
-      v[q] = *reinterpret_cast<const u32x4*>(p[q] - (KM ? back * ld : back));
-    }
-  }
-  static __device__ __forceinline__ void store_tail(uint16_t* img, const u32x4 (&v)[PIECES], int left) {
-#pragma unroll
-    for (int q = 0; q < PIECES; ++q) {
-      const int k = KM ? image_row(q) : piece(q) * 8;
-      *reinterpret_cast<u32x4*>(img + (q * THREADS + (int)threadIdx.x) * 8) = k < left ? v[q] : u32x4(0u);
+      const void* from = k < left ? static_cast<const void*>(p[q]) : static_cast<const void*>(zero_piece);
+      __builtin_amdgcn_global_load_lds((global_ptr)from, (lds_ptr)(img + (q * THREADS + wave * 64) * 8), 16, 0, 0);
     }
   }
   // the fragment of rows [32 tile, 32 tile + 32), k [kk, kk + 16): lane l holds row l & 31, k (l >> 5) * 8 .. + 8
@@ -401,17 +397,17 @@ struct DmaOperand {
 };
 
 // every wave's DMA has landed and its image reads are done: what the barrier by itself does not wait for is the DMA (vmcnt)
-__device__ __forceinline__ void images_ready() {
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-  __syncthreads();
-}
+__device__ __forceinline__ void images_ready() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+// Schedule of a step: its first fragments are in registers when it begins; the fragments of k group kk + 1 are read while the products of
+// group kk run, the barrier that hands over the next image stands in front of the LAST group, and behind it the next step's first fragments
+// are read and the step after that is requested: a wave never waits for LDS with nothing to multiply, and the DMA has a whole step to land.
 template <bool A_KM, bool B_KM, int MI, int NI, int WR, int WC>
 struct DmaTile {
   static constexpr int BM = MI * WR * 32, BN = NI * WC * 32, THREADS = WR * WC * 64, BK = 64;
   typedef DmaOperand<A_KM, BM, THREADS> OpA;
   typedef DmaOperand<B_KM, BN, THREADS> OpB;
-  static constexpr int STAGE = OpA::ELEMS + OpB::ELEMS, LDS_BYTES = 2 * STAGE * 2;
+  static constexpr int STAGE = OpA::ELEMS + OpB::ELEMS, OUT = 4096, LDS_BYTES = 2 * STAGE * 2 + WR * WC * OUT;
 
   f32x16 acc[MI][NI];
   float row_sum[MI];  // with SUMS: sum over k of the A rows, over the k that this lane's fragments hold
@@ -426,26 +422,39 @@ struct DmaTile {
         for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
     }
   }
-  template <bool SUMS>
-  __device__ __forceinline__ void product(const uint16_t* st, int kk) {
-    const int wave = threadIdx.x >> 6, tm = (wave / WC) * MI, tn = (wave % WC) * NI;
+  struct Frags {
     bf16x8 a[MI], b[NI];
+    __device__ __forceinline__ void read(const uint16_t* st, int kk) {
+      const int wave = threadIdx.x >> 6, tm = (wave / WC) * MI, tn = (wave % WC) * NI;
 #pragma unroll
-    for (int i = 0; i < MI; ++i) a[i] = OpA::frag(st, tm + i, kk);
+      for (int i = 0; i < MI; ++i) a[i] = OpA::frag(st, tm + i, kk);
 #pragma unroll
-    for (int j = 0; j < NI; ++j) b[j] = OpB::frag(st + OpA::ELEMS, tn + j, kk);
+      for (int j = 0; j < NI; ++j) b[j] = OpB::frag(st + OpA::ELEMS, tn + j, kk);
+    }
+  };
+  template <bool SUMS>
+  __device__ __forceinline__ void multiply(const Frags& f) {
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
-      for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(b[j], a[i], acc[i][j], 0, 0, 0);
+      for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.b[j], f.a[i], acc[i][j], 0, 0, 0);
     if (SUMS) {
 #pragma unroll
       for (int i = 0; i < MI; ++i) {
         u32x4 v;
-        __builtin_memcpy(&v, &a[i], 16);
+        __builtin_memcpy(&v, &f.a[i], 16);
 #pragma unroll
         for (int e = 0; e < 4; ++e) row_sum[i] += __uint_as_float(v[e] << 16) + __uint_as_float(v[e] & 0xffff0000u);
       }
+    }
+  }
+  // LDS reads of one fragment set per group of MI x NI products: spread one behind each product
+  static constexpr int READS = (A_KM ? 2 : 1) * MI + (B_KM ? 2 : 1) * NI, PER = (READS + MI * NI - 1) / (MI * NI);
+  static __device__ __forceinline__ void interleave() {
+#pragma unroll
+    for (int i = 0; i < MI * NI; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
     }
   }
   template <bool SUMS>
@@ -460,45 +469,92 @@ struct DmaTile {
     const int64_t full = (k_end - k_begin) / BK;
     const int left = (int)((k_end - k_begin) % BK);
     const int64_t steps = full + (left > 0);
-    u32x4 ta[OpA::PIECES], tb[OpB::PIECES];
-    if (full > 0) {
-      a.issue(lds, lda);
-      b.issue(lds + OpA::ELEMS, ldb);
-    } else {
-      a.fetch_tail(ta, left, lda);
-      b.fetch_tail(tb, left, ldb);
-      OpA::store_tail(lds, ta, left);
-      OpB::store_tail(lds + OpA::ELEMS, tb, left);
-    }
+    auto image = [&](int64_t t) __attribute__((always_inline)) { return lds + (t & 1) * STAGE; };
+    auto issue = [&](int64_t t) __attribute__((always_inline)) {
+      if (t < full) {
+        a.issue(image(t), lda);
+        b.issue(image(t) + OpA::ELEMS, ldb);
+      } else {
+        a.issue_last(image(t), left);
+        b.issue_last(image(t) + OpA::ELEMS, left);
+      }
+    };
+    Frags f[2];
+    issue(0);
+    if (steps > 1) issue(1);
     images_ready();
-    for (int64_t t = 0; t + 1 < full; ++t) {
-      uint16_t *st = lds + (t & 1) * STAGE, *next = lds + ((t + 1) & 1) * STAGE;
-      a.issue(next, lda);
-      b.issue(next + OpA::ELEMS, ldb);
+    f[0].read(image(0), 0);
+    int64_t t = 0;
+    for (; t + 1 < steps; ++t) {
+      const uint16_t* st = image(t);
 #pragma unroll
-      for (int kk = 0; kk < BK; kk += 16) product<SUMS>(st, kk);
+      for (int g = 0; g < 3; ++g) {
+        f[(g + 1) & 1].read(st, (g + 1) * 16);
+        multiply<SUMS>(f[g & 1]);
+        interleave();
+      }
       images_ready();
+      if (t + 2 < steps) issue(t + 2);
+      f[0].read(image(t + 1), 0);
+      multiply<SUMS>(f[1]);
+      interleave();
     }
-    if (full > 0) {
-      uint16_t *st = lds + ((full - 1) & 1) * STAGE, *next = lds + (full & 1) * STAGE;
-      if (left > 0) {
-        a.fetch_tail(ta, left, lda);
-        b.fetch_tail(tb, left, ldb);
-      }
-#pragma unroll
-      for (int kk = 0; kk < BK; kk += 16) product<SUMS>(st, kk);
-      if (left > 0) {
-        OpA::store_tail(next, ta, left);
-        OpB::store_tail(next + OpA::ELEMS, tb, left);
-        images_ready();
-      }
+    const int groups = left > 0 ? (left + 15) / 16 : 4;
+    for (int g = 0; g < groups; ++g) {
+      if (g + 1 < groups) f[1].read(image(t), (g + 1) * 16);
+      multiply<SUMS>(f[0]);
+      f[0] = f[1];
     }
-    if (left > 0)
-      for (int kk = 0; kk < left; kk += 16) product<SUMS>(lds + ((steps - 1) & 1) * STAGE, kk);
   }
-  template <class F>
-  __device__ __forceinline__ void each(int64_t m0, int64_t mlim, int64_t n0, int64_t nlim, F&& f) const {
-    each4<MI, NI, WC>(acc, m0, mlim, n0, nlim, f);
+  // The tile to memory: base[m * ld + n] = value(n, four accumulators) for m < mlim, n < nlim.  A lane holds four-runs of one row each 8
+  // columns apart; written like that, every store instruction scatters 16-byte bits over 32 rows.  Each wave turns 32 rows x 128 bytes at
+  // a time in its own 4 KB of LDS (16-byte piece c of row r at c ^ (r >> 1) & 7, as in the images) and stores whole 128-byte row pieces.
+  template <bool BF16, class V>
+  __device__ __forceinline__ void store(void* base, int64_t ld, int64_t m0, int64_t mlim, int64_t n0, int64_t nlim, uint16_t* lds, V&& value) const {
+    constexpr int SIZE = BF16 ? 2 : 4, COLS = 128 / SIZE, PER = COLS / 32;  // columns and accumulator tiles of a 128-byte row piece
+    static_assert(NI % PER == 0, "a wave's columns do not divide into row pieces");
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    unsigned char* out = reinterpret_cast<unsigned char*>(lds + 2 * STAGE) + wave * OUT;
+    const int r = lane & 31, x = (r >> 1) & 7;
+    const int64_t wm = m0 + (wave / WC) * MI * 32, wn = n0 + (wave % WC) * NI * 32;
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int jj = 0; jj < NI; jj += PER) {
+        if (wm + i * 32 >= mlim || wn + jj * 32 >= nlim) continue;  // (uniform)
+#pragma unroll
+        for (int j = jj; j < jj + PER; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const f32x4 v = value(wn + j * 32 + 8 * q + 4 * (lane >> 5),
+                                  f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]});
+            const int col = (j - jj) * 32 + 8 * q + 4 * (lane >> 5);
+            if (BF16) {
+              *reinterpret_cast<u32x2*>(out + r * 128 + (((col >> 3) ^ x) << 4) + (col & 4) * 2) =
+                  u32x2{(unsigned)f32_bf16(v[0]) | (unsigned)f32_bf16(v[1]) << 16, (unsigned)f32_bf16(v[2]) | (unsigned)f32_bf16(v[3]) << 16};
+            } else {
+              *reinterpret_cast<f32x4*>(out + r * 128 + (((col >> 2) ^ x) << 4)) = v;
+            }
+          }
+#pragma unroll
+        for (int it = 0; it < 4; ++it) {
+          const int row = it * 8 + (lane >> 3), c = lane & 7;
+          const u32x4 v = *reinterpret_cast<const u32x4*>(out + row * 128 + ((c ^ ((row >> 1) & 7)) << 4));
+          const int64_t m = wm + i * 32 + row, n = wn + jj * 32 + c * (16 / SIZE);
+          if (m < mlim && n < nlim) {
+            unsigned char* to = static_cast<unsigned char*>(base) + (m * ld + n) * SIZE;
+            if (n + 16 / SIZE <= nlim) {
+              *reinterpret_cast<u32x4u*>(to) = v;
+            } else {
+              for (int e = 0; e < 16 / SIZE - 1; ++e) {
+                if (n + e >= nlim) break;
+                if (BF16) reinterpret_cast<uint16_t*>(to)[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
+                else reinterpret_cast<uint32_t*>(to)[e] = v[e];
+              }
+            }
+          }
+        }
+      }
   }
   // put(row of the tile, its sum): the waves of the first tile column hold every row, the two half waves half of its k each
   template <class Put>
@@ -525,11 +581,26 @@ struct FwdArgs {
   int act, y_bf16, zero_outside;
 };
 
-// bias and activation of a tile, then its stores
-template <class TileT, class Put>
-__device__ __forceinline__ void finish(const FwdArgs& a, const Slot& s, int64_t n0, const TileT& t, Put&& put) {
-  const float* bias = a.bias ? a.bias + s.group * a.ld_bias : nullptr;
-  t.each(s.begin, s.end, n0, a.N, [&](int64_t m, int64_t n, f32x4 v) __attribute__((always_inline)) {
+template <class T, class TileT, bool DMA>
+__global__ __launch_bounds__(TileT::THREADS) void grouped_forward_kernel(const FwdArgs a) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char raw_lds[];
+  const int64_t tiles_n = (a.N + TileT::BN - 1) / TileT::BN;
+  const int64_t id = xcd_run(blockIdx.x, gridDim.x);
+  const Slot s = find_slot(a.gr, id / tiles_n, __builtin_ctz(TileT::BM));
+  if (!s.live || (s.group < 0 && !a.zero_outside)) return;
+  const int64_t n0 = (id % tiles_n) * TileT::BN;
+  T* lds = reinterpret_cast<T*>(raw_lds);
+  TileT t;
+  const float* bias = nullptr;
+  if (s.group < 0) {
+    t.zero();
+  } else {
+    const T *X = static_cast<const T*>(a.X), *W = static_cast<const T*>(a.W) + s.group * a.stride_w;
+    if constexpr (DMA) t.template run<false>(X, a.ldx, s.begin, s.end, W, a.ldw, n0, a.N, 0, a.K, lds);
+    else t.run(X, a.ldx, s.begin, s.end, W, a.ldw, n0, a.N, 0, a.K, lds, [](const auto&) {});
+    if (a.bias) bias = a.bias + s.group * a.ld_bias;
+  }
+  auto value = [&](int64_t n, f32x4 v) __attribute__((always_inline)) {
     if (bias) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] += bias[min(n + e, a.N - 1)];
@@ -538,34 +609,18 @@ __device__ __forceinline__ void finish(const FwdArgs& a, const Slot& s, int64_t 
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = v[e] < 0.f ? 0.f : v[e];  // (a NaN passes)
     }
-    put(m, n, v);
-  });
-}
-
-template <class T, class TileT, bool DMA>
-__global__ __launch_bounds__(TileT::THREADS) void grouped_forward_kernel(const FwdArgs a) {
-  extern __shared__ __attribute__((aligned(16))) unsigned char raw_lds[];
-  const int64_t tiles_n = (a.N + TileT::BN - 1) / TileT::BN;
-  const int64_t id = xcd_run(blockIdx.x, gridDim.x);
-  const Slot s = find_slot(a.gr, id / tiles_n, __builtin_ctz(TileT::BM));
-  if (!s.live) return;
-  const int64_t n0 = (id % tiles_n) * TileT::BN;
-  auto put = [&](int64_t m, int64_t n, f32x4 v) __attribute__((always_inline)) {
-    if (a.y_bf16) put4<true>(static_cast<uint16_t*>(a.Y) + m * a.ldy, n, a.N, v);
-    else put4<false>(static_cast<float*>(a.Y) + m * a.ldy, n, a.N, v);
+    return v;
   };
-  TileT t;
-  if (s.group < 0) {
-    if (!a.zero_outside) return;
-    t.zero();
-    t.each(s.begin, s.end, n0, a.N, put);
-    return;
+  if constexpr (DMA) {
+    if (a.y_bf16) t.template store<true>(a.Y, a.ldy, s.begin, s.end, n0, a.N, lds, value);
+    else t.template store<false>(a.Y, a.ldy, s.begin, s.end, n0, a.N, lds, value);
+  } else {
+    t.each(s.begin, s.end, n0, a.N, [&](int64_t m, int64_t n, f32x4 v) __attribute__((always_inline)) {
+      v = value(n, v);
+      if (a.y_bf16) put4<true>(static_cast<uint16_t*>(a.Y) + m * a.ldy, n, a.N, v);
+      else put4<false>(static_cast<float*>(a.Y) + m * a.ldy, n, a.N, v);
+    });
   }
-  const T *X = static_cast<const T*>(a.X), *W = static_cast<const T*>(a.W) + s.group * a.stride_w;
-  T* lds = reinterpret_cast<T*>(raw_lds);
-  if constexpr (DMA) t.template run<false>(X, a.ldx, s.begin, s.end, W, a.ldw, n0, a.N, 0, a.K, lds);
-  else t.run(X, a.ldx, s.begin, s.end, W, a.ldw, n0, a.N, 0, a.K, lds, [](const auto&) {});
-  finish(a, s, n0, t, put);
 }
 
 // ---- dW, db --------------------------------------------------------------------------------------------------------------------------
@@ -628,15 +683,23 @@ __global__ __launch_bounds__(TileT::THREADS) void grouped_wgrad_kernel(const Wgr
     });
   }
   const int64_t slot = alone ? 0 : 2 * (s.begin >> a.shift) + (s.index > 0 ? 1 : 0);
+  void* out = a.part_w + slot * a.N * a.K;
+  int64_t ld = a.K;
+  bool bf16 = false;
   if (alone) {
-    const int64_t at = s.group * a.stride_w;
-    t.each(n0, a.N, k0, a.K, [&](int64_t n, int64_t k, f32x4 v) __attribute__((always_inline)) {
-      if (a.dw_bf16) put4<true>(static_cast<uint16_t*>(a.dW) + at + n * a.ldw, k, a.K, v);
-      else put4<false>(static_cast<float*>(a.dW) + at + n * a.ldw, k, a.K, v);
-    });
+    bf16 = a.dw_bf16;
+    ld = a.ldw;
+    out = static_cast<char*>(a.dW) + s.group * a.stride_w * (bf16 ? 2 : 4);
+  }
+  if constexpr (DMA) {
+    auto value = [](int64_t, f32x4 v) __attribute__((always_inline)) { return v; };
+    if (bf16) t.template store<true>(out, ld, n0, a.N, k0, a.K, stages, value);
+    else t.template store<false>(out, ld, n0, a.N, k0, a.K, stages, value);
   } else {
-    float* out = a.part_w + slot * a.N * a.K;
-    t.each(n0, a.N, k0, a.K, [&](int64_t n, int64_t k, f32x4 v) __attribute__((always_inline)) { put4<false>(out + n * a.K, k, a.K, v); });
+    t.each(n0, a.N, k0, a.K, [&](int64_t n, int64_t k, f32x4 v) __attribute__((always_inline)) {
+      if (bf16) put4<true>(static_cast<uint16_t*>(out) + n * ld, k, a.K, v);
+      else put4<false>(static_cast<float*>(out) + n * ld, k, a.K, v);
+    });
   }
   if (sums) {
     auto put = [&](int i, float v) __attribute__((always_inline)) {

@@ -20,6 +20,7 @@ LAYOUTS = {
     "all_empty": (9, [0, 0, 0], 4),
     "ragged": (611, [1, 128, 129, 127, 3, 0, 200, 23], 0),
     "many": (700, [i % 5 for i in range(350)], 0),    # more groups than one 64-wide probe
+    "long": (3700, [2500, 1100], 60),                 # the large tile
     "chunks": (1900, [700, 0, 256, 257, 1, 686], 0),  # groups of several weight-gradient chunks beside groups of one
 }
 
@@ -60,7 +61,7 @@ def _check(got, ref, mag, n, out_bf16=False):
 
 @pytest.mark.parametrize("layout", sorted(LAYOUTS))
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("K,N", [(40, 24), (33, 17), (1, 1), (200, 136)])
+@pytest.mark.parametrize("K,N", [(40, 24), (33, 17), (1, 1), (200, 136), (64, 256), (136, 264), (320, 40)])
 @pytest.mark.parametrize("trans_b", [True, False])
 def test_forward(cuda_device, layout, dtype, K, N, trans_b):
     from dance_amd import kernels
@@ -77,7 +78,7 @@ def test_forward(cuda_device, layout, dtype, K, N, trans_b):
 
 @pytest.mark.parametrize("layout", sorted(LAYOUTS))
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("K,N", [(40, 24), (33, 17), (1, 1), (136, 200)])
+@pytest.mark.parametrize("K,N", [(40, 24), (33, 17), (1, 1), (136, 200), (264, 520)])
 def test_weight_gradient(cuda_device, layout, dtype, K, N):
     from dance_amd import kernels
     x, w, b, dy, ptr = _operands(layout, K, N, dtype)
