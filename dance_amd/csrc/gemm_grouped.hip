@@ -22,10 +22,12 @@ typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned int u32x4u __attribute__((ext_vector_type(4), aligned(2)));  // 16 bytes at an element's own alignment
 
 __device__ __forceinline__ float bf16_f32(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
-__device__ __forceinline__ uint16_t f32_bf16(float x) {  // nearest even; NaN stays a quiet NaN
-  const uint32_t u = __float_as_uint(x);
-  if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)((u >> 16) | 0x40u);
-  return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
+// two values rounded to bf16 (v_cvt_pk_bf16_f32: nearest even, a NaN stays one); the rounding in integer arithmetic, eight instructions a
+// value, cost a third of a tile's time at K = 512
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
 }
 
 // ---- groups --------------------------------------------------------------------------------------------------------------------------
@@ -306,12 +308,12 @@ __device__ __forceinline__ void put4(void* row, int64_t n, int64_t nlim, f32x4 v
   typedef unsigned int u32x2u __attribute__((ext_vector_type(2), aligned(2)));
   if (BF16) {
     uint16_t* p = static_cast<uint16_t*>(row) + n;
-    const uint16_t h[4] = {f32_bf16(v[0]), f32_bf16(v[1]), f32_bf16(v[2]), f32_bf16(v[3])};
+    const u32x2 h = {pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
     if (n + 4 <= nlim) {
-      *reinterpret_cast<u32x2u*>(p) = u32x2u{(unsigned)h[0] | (unsigned)h[1] << 16, (unsigned)h[2] | (unsigned)h[3] << 16};
+      *reinterpret_cast<u32x2u*>(p) = h;
     } else {
       for (int e = 0; e < 3; ++e)
-        if (n + e < nlim) p[e] = h[e];
+        if (n + e < nlim) p[e] = (uint16_t)(h[e >> 1] >> (16 * (e & 1)));
     }
   } else {
     float* p = static_cast<float*>(row) + n;
@@ -328,8 +330,8 @@ __device__ __forceinline__ void put4(void* row, int64_t n, int64_t nlim, f32x4 v
 // The same product with the operands going from memory to LDS without passing registers (global_load_lds, 16 bytes a lane): what the big
 // products run on.  The DMA writes a wave's 64 pieces to 1 KB of LDS in lane order, so images cannot be padded; bank conflicts are avoided by
 // choosing WHICH piece a lane fetches: piece c of an image row lies at position c ^ x,
-//   [row][k] images (128-byte rows):  x = (row >> 1) & 7: the 16 rows that a 16-byte fragment read takes at a time cover all 16 slots of
-//                                     two rows;
+//   [row][k] images (64- or 128-byte rows):  x = (row >> 2) & 3 or (row >> 1) & 7: the 16 rows that a 16-byte fragment read takes at a
+//                                     time cover all 16 slots of 256 bytes;
 //   [k][row] images (2 R-byte rows):  x = (k & 3) << 2: the four k rows that a transposing read takes from lie 64 bytes apart.
 // Needs 16-byte aligned rows (address and stride) and, for a [k][row] operand, a row count that is a multiple of 8 (a piece is whole or
 // absent).  In the last, partial step of k the lanes whose pieces lie behind the end fetch a piece of zeros instead.
@@ -338,50 +340,59 @@ typedef __attribute__((address_space(3))) void* lds_ptr;
 
 __device__ __attribute__((aligned(16))) const uint32_t zero_piece[4] = {0, 0, 0, 0};
 
-template <bool KM, int R, int THREADS>
+// The value again, unknown to the compiler: what is computed from it is not kept in registers across the loop over tiles (hoisted, the
+// lane-dependent addresses of all phases together spilled 180 registers).
+__device__ __forceinline__ int anew(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
+template <bool KM, int R, int BK, int THREADS>
 struct DmaOperand {
-  static constexpr int BK = 64, CPR = KM ? R / 8 : 8, PIECES = R * 8 / THREADS, ELEMS = R * BK;
-  static_assert(PIECES * THREADS == R * 8 && (!KM || R >= 128), "tile does not divide among the threads");
+  static constexpr int CPR = KM ? R / 8 : BK / 8, PIECES = R * BK / 8 / THREADS, ELEMS = R * BK;
+  static_assert((BK == 32 || BK == 64) && PIECES * THREADS == R * BK / 8 && (!KM || R >= 128), "tile does not divide among the threads");
 
-  const uint16_t* p[PIECES];
+  const char* base;         // uniform: advances with k
+  uint32_t offset[PIECES];  // the lane's pieces, in bytes (a tile spans less than 4 GB: dma_rows)
 
-  static __device__ __forceinline__ int image_row(int q) { return (q * THREADS + (int)threadIdx.x) / CPR; }
-  static __device__ __forceinline__ int piece(int q) {
-    const int row = image_row(q), c = (q * THREADS + (int)threadIdx.x) % CPR;
-    return KM ? c ^ ((row & 3) << 2) : c ^ ((row >> 1) & 7);
+  static __device__ __forceinline__ int swizzle(int row) { return BK == 64 ? (row >> 1) & 7 : (row >> 2) & 3; }
+  static __device__ __forceinline__ int image_row(int q, int tid) { return (q * THREADS + tid) / CPR; }
+  static __device__ __forceinline__ int piece(int q, int tid) {
+    const int row = image_row(q, tid), c = (q * THREADS + tid) % CPR;
+    return KM ? c ^ ((row & 3) << 2) : c ^ swizzle(row);
   }
-  __device__ __forceinline__ void start(const uint16_t* base, int64_t ld, int64_t r0, int64_t rlim, int64_t k0) {
+  __device__ __forceinline__ void start(const uint16_t* op, int64_t ld, int64_t r0, int64_t rlim, int64_t k0) {
+    const int tid = anew(threadIdx.x), most = (int)min(rlim - r0, (int64_t)R);
+    base = reinterpret_cast<const char*>(op + (KM ? k0 * ld + r0 : r0 * ld + k0));
 #pragma unroll
     for (int q = 0; q < PIECES; ++q) {
-      if (KM) p[q] = base + (k0 + image_row(q)) * ld + min(r0 + piece(q) * 8, rlim - 8);
-      else p[q] = base + min(r0 + image_row(q), rlim - 1) * ld + k0 + piece(q) * 8;
+      if (KM) offset[q] = ((uint32_t)image_row(q, tid) * (uint32_t)ld + (uint32_t)min(piece(q, tid) * 8, most - 8)) * 2u;
+      else offset[q] = ((uint32_t)min(image_row(q, tid), most - 1) * (uint32_t)ld + (uint32_t)piece(q, tid) * 8u) * 2u;
     }
   }
   // the next BK of k into an image
   __device__ __forceinline__ void issue(uint16_t* img, int64_t ld) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
-    for (int q = 0; q < PIECES; ++q) {
-      __builtin_amdgcn_global_load_lds((global_ptr)p[q], (lds_ptr)(img + (q * THREADS + wave * 64) * 8), 16, 0, 0);
-      p[q] += KM ? BK * ld : BK;
-    }
+    for (int q = 0; q < PIECES; ++q)
+      __builtin_amdgcn_global_load_lds((global_ptr)(base + offset[q]), (lds_ptr)(img + (q * THREADS + wave * 64) * 8), 16, 0, 0);
+    base += KM ? BK * ld * 2 : BK * 2;
   }
   // the last `left` < BK of k, zeros behind them
   __device__ __forceinline__ void issue_last(uint16_t* img, int left) const {
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), tid = anew(threadIdx.x);
 #pragma unroll
     for (int q = 0; q < PIECES; ++q) {
-      const int k = KM ? image_row(q) : piece(q) * 8;
-      const void* from = k < left ? static_cast<const void*>(p[q]) : static_cast<const void*>(zero_piece);
+      const int k = KM ? image_row(q, tid) : piece(q, tid) * 8;
+      const void* from = k < left ? static_cast<const void*>(base + offset[q]) : static_cast<const void*>(zero_piece);
       __builtin_amdgcn_global_load_lds((global_ptr)from, (lds_ptr)(img + (q * THREADS + wave * 64) * 8), 16, 0, 0);
     }
   }
   // the fragment of rows [32 tile, 32 tile + 32), k [kk, kk + 16): lane l holds row l & 31, k (l >> 5) * 8 .. + 8
-  static __device__ __forceinline__ bf16x8 frag(const uint16_t* img, int tile, int kk) {
-    const int lane = threadIdx.x & 63;
+  static __device__ __forceinline__ bf16x8 frag(const uint16_t* img, int tile, int kk, int lane) {
     if (!KM) {
       const int c = (kk >> 3) + (lane >> 5);
-      return *reinterpret_cast<const bf16x8*>(img + (tile * 32 + (lane & 31)) * BK + ((c ^ ((lane >> 1) & 7)) << 3));
+      return *reinterpret_cast<const bf16x8*>(img + (tile * 32 + (lane & 31)) * BK + ((c ^ swizzle(lane)) << 3));
     }
     typedef short s16x4 __attribute__((ext_vector_type(4)));
     typedef s16x4 __attribute__((address_space(3))) * lds_s16x4;
@@ -396,19 +407,37 @@ struct DmaOperand {
   }
 };
 
-// every wave's DMA has landed and its image reads are done: what the barrier by itself does not wait for is the DMA (vmcnt)
-__device__ __forceinline__ void images_ready() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+// Every wave's DMA but its last LATER instructions has landed and its image reads are done: the barrier by itself waits for neither.
+template <int LATER>
+__device__ __forceinline__ void images_ready() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LATER) : "memory");
+}
 
 // Schedule of a step: its first fragments are in registers when it begins; the fragments of k group kk + 1 are read while the products of
 // group kk run, the barrier that hands over the next image stands in front of the LAST group, and behind it the next step's first fragments
-// are read and the step after that is requested: a wave never waits for LDS with nothing to multiply, and the DMA has a whole step to land.
-template <bool A_KM, bool B_KM, int MI, int NI, int WR, int WC>
+// are read and the image just emptied is requested again, STAGES steps ahead: a wave never waits for LDS with nothing to multiply.
+// begin() requests a tile's first steps, main() multiplies, store() writes the result out of an LDS region of its own, so that the next
+// tile's begin() runs before this one's store(): with one workgroup on a CU nothing else would fill these gaps (measured in cycles at
+// 200003 rows, 2000 -> 512, per tile: first request to first product 8500, 32 steps 107000, stores 16000 before they were made cheap).
+template <bool A_KM, bool B_KM, int MI, int NI, int WR, int WC, int K_STEP, int STAGES>
 struct DmaTile {
-  static constexpr int BM = MI * WR * 32, BN = NI * WC * 32, THREADS = WR * WC * 64, BK = 64;
-  typedef DmaOperand<A_KM, BM, THREADS> OpA;
-  typedef DmaOperand<B_KM, BN, THREADS> OpB;
-  static constexpr int STAGE = OpA::ELEMS + OpB::ELEMS, OUT = 4096, LDS_BYTES = 2 * STAGE * 2 + WR * WC * OUT;
+  static constexpr int BM = MI * WR * 32, BN = NI * WC * 32, THREADS = WR * WC * 64, BK = K_STEP, GROUPS = BK / 16;
+  typedef DmaOperand<A_KM, BM, BK, THREADS> OpA;
+  typedef DmaOperand<B_KM, BN, BK, THREADS> OpB;
+  static constexpr int STAGE = OpA::ELEMS + OpB::ELEMS, OUT = 4096, LDS_BYTES = STAGES * STAGE * 2 + WR * WC * OUT;
+  static constexpr int INSTRS = OpA::PIECES + OpB::PIECES;  // DMA instructions of a wave per step
+  static_assert((STAGES - 1) * INSTRS < 64 && GROUPS % 2 == 0, "");
 
+  struct Source {  // a tile's operands: rows [m0, mlim) of A and [n0, nlim) of B, k in [k_begin, k_end)
+    const uint16_t *A, *B;
+    int64_t lda, ldb, m0, mlim, n0, nlim, k_begin, k_end;
+  };
+
+  OpA a;
+  OpB b;
+  uint16_t* lds;
+  int64_t lda, ldb, full, steps;
+  int left;
   f32x16 acc[MI][NI];
   float row_sum[MI];  // with SUMS: sum over k of the A rows, over the k that this lane's fragments hold
 
@@ -424,12 +453,12 @@ struct DmaTile {
   }
   struct Frags {
     bf16x8 a[MI], b[NI];
-    __device__ __forceinline__ void read(const uint16_t* st, int kk) {
-      const int wave = threadIdx.x >> 6, tm = (wave / WC) * MI, tn = (wave % WC) * NI;
+    __device__ __forceinline__ void read(const uint16_t* st, int kk, int lane) {
+      const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), tm = (wave / WC) * MI, tn = (wave % WC) * NI;
 #pragma unroll
-      for (int i = 0; i < MI; ++i) a[i] = OpA::frag(st, tm + i, kk);
+      for (int i = 0; i < MI; ++i) a[i] = OpA::frag(st, tm + i, kk, lane);
 #pragma unroll
-      for (int j = 0; j < NI; ++j) b[j] = OpB::frag(st + OpA::ELEMS, tn + j, kk);
+      for (int j = 0; j < NI; ++j) b[j] = OpB::frag(st + OpA::ELEMS, tn + j, kk, lane);
     }
   };
   template <bool SUMS>
@@ -457,97 +486,122 @@ struct DmaTile {
       __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
     }
   }
+  __device__ __forceinline__ void issue(int64_t t, uint16_t* image) {
+    if (t < full) {
+      a.issue(image, lda);
+      b.issue(image + OpA::ELEMS, ldb);
+    } else {
+      a.issue_last(image, left);
+      b.issue_last(image + OpA::ELEMS, left);
+    }
+  }
+  __device__ __forceinline__ void begin(const Source& s) {
+    const int64_t k = s.k_end > s.k_begin ? s.k_end - s.k_begin : 0;
+    full = k / BK;
+    left = (int)(k % BK);
+    steps = full + (left > 0);
+    lda = s.lda;
+    ldb = s.ldb;
+    if (steps == 0) return;
+    a.start(s.A, lda, s.m0, s.mlim, s.k_begin);
+    b.start(s.B, ldb, s.n0, s.nlim, s.k_begin);
+#pragma unroll
+    for (int t = 0; t < STAGES; ++t)
+      if (t < steps) issue(t, lds + t * STAGE);
+  }
   template <bool SUMS>
-  __device__ __forceinline__ void run(const uint16_t* A, int64_t lda, int64_t m0, int64_t mlim, const uint16_t* B, int64_t ldb, int64_t n0,
-                                      int64_t nlim, int64_t k_begin, int64_t k_end, uint16_t* lds) {
+  __device__ __forceinline__ void main() {
     zero();
-    if (k_end <= k_begin) return;
-    OpA a;
-    OpB b;
-    a.start(A, lda, m0, mlim, k_begin);
-    b.start(B, ldb, n0, nlim, k_begin);
-    const int64_t full = (k_end - k_begin) / BK;
-    const int left = (int)((k_end - k_begin) % BK);
-    const int64_t steps = full + (left > 0);
-    auto image = [&](int64_t t) __attribute__((always_inline)) { return lds + (t & 1) * STAGE; };
-    auto issue = [&](int64_t t) __attribute__((always_inline)) {
-      if (t < full) {
-        a.issue(image(t), lda);
-        b.issue(image(t) + OpA::ELEMS, ldb);
-      } else {
-        a.issue_last(image(t), left);
-        b.issue_last(image(t) + OpA::ELEMS, left);
-      }
-    };
+    if (steps == 0) return;
+    const int lane = anew(threadIdx.x & 63);
     Frags f[2];
-    issue(0);
-    if (steps > 1) issue(1);
-    images_ready();
-    f[0].read(image(0), 0);
+    uint16_t* image = lds;
+    // (whatever was issued after begin() only makes this wait longer)
+    if (steps >= STAGES) images_ready<(STAGES - 1) * INSTRS>();
+    else images_ready<0>();
+    f[0].read(image, 0, lane);
     int64_t t = 0;
     for (; t + 1 < steps; ++t) {
-      const uint16_t* st = image(t);
+      uint16_t* next = image == lds + (STAGES - 1) * STAGE ? lds : image + STAGE;
 #pragma unroll
-      for (int g = 0; g < 3; ++g) {
-        f[(g + 1) & 1].read(st, (g + 1) * 16);
+      for (int g = 0; g + 1 < GROUPS; ++g) {
+        f[(g + 1) & 1].read(image, (g + 1) * 16, lane);
         multiply<SUMS>(f[g & 1]);
         interleave();
       }
-      images_ready();
-      if (t + 2 < steps) issue(t + 2);
-      f[0].read(image(t + 1), 0);
+      // step t + 1 has landed when only the STAGES - 2 steps behind it are outstanding; near the end fewer were requested: wait for all
+      if (t + STAGES - 1 < steps) images_ready<(STAGES - 2) * INSTRS>();
+      else images_ready<0>();
+      if (t + STAGES < steps) issue(t + STAGES, image);
+      f[0].read(next, 0, lane);
       multiply<SUMS>(f[1]);
       interleave();
+      image = next;
     }
-    const int groups = left > 0 ? (left + 15) / 16 : 4;
+    const int groups = left > 0 ? (left + 15) / 16 : GROUPS;
     for (int g = 0; g < groups; ++g) {
-      if (g + 1 < groups) f[1].read(image(t), (g + 1) * 16);
+      if (g + 1 < groups) f[1].read(image, (g + 1) * 16, lane);
       multiply<SUMS>(f[0]);
       f[0] = f[1];
     }
+    images_ready<0>();  // nobody reads the images any more: the next begin() may overwrite them
   }
-  // The tile to memory: base[m * ld + n] = value(n, four accumulators) for m < mlim, n < nlim.  A lane holds four-runs of one row each 8
+  // The tile to memory: base[m * ld + n] = act(accumulator + bias[n]) for m < mlim, n < nlim.  A lane holds four-runs of one row each 8
   // columns apart; written like that, every store instruction scatters 16-byte bits over 32 rows.  Each wave turns 32 rows x 128 bytes at
   // a time in its own 4 KB of LDS (16-byte piece c of row r at c ^ (r >> 1) & 7, as in the images) and stores whole 128-byte row pieces.
-  template <bool BF16, class V>
-  __device__ __forceinline__ void store(void* base, int64_t ld, int64_t m0, int64_t mlim, int64_t n0, int64_t nlim, uint16_t* lds, V&& value) const {
+  template <bool BF16>
+  __device__ __forceinline__ void store(void* base, int64_t ld, int64_t m0, int64_t mlim, int64_t n0, int64_t nlim, const float* bias, bool relu) const {
     constexpr int SIZE = BF16 ? 2 : 4, COLS = 128 / SIZE, PER = COLS / 32;  // columns and accumulator tiles of a 128-byte row piece
     static_assert(NI % PER == 0, "a wave's columns do not divide into row pieces");
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    unsigned char* out = reinterpret_cast<unsigned char*>(lds + 2 * STAGE) + wave * OUT;
-    const int r = lane & 31, x = (r >> 1) & 7;
+    const int lane = anew(threadIdx.x & 63), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    unsigned char* out = reinterpret_cast<unsigned char*>(lds + STAGES * STAGE) + wave * OUT;
+    const int r = lane & 31, x = (r >> 1) & 7, h = lane >> 5;
     const int64_t wm = m0 + (wave / WC) * MI * 32, wn = n0 + (wave % WC) * NI * 32;
+    const int rows = (int)min((int64_t)(MI * 32), mlim - wm), cols = (int)min((int64_t)(NI * 32), nlim - wn);  // of the wave's part; <= 0: none
+    unsigned char* const origin = static_cast<unsigned char*>(base) + (wm * ld + wn) * SIZE;
+    if (rows <= 0 || cols <= 0) return;
 #pragma unroll
-    for (int i = 0; i < MI; ++i)
+    for (int jj = 0; jj < NI; jj += PER) {
+      if (jj * 32 >= cols) continue;
+      f32x4 add[PER][4];
+      if (bias) {
 #pragma unroll
-      for (int jj = 0; jj < NI; jj += PER) {
-        if (wm + i * 32 >= mlim || wn + jj * 32 >= nlim) continue;  // (uniform)
-#pragma unroll
-        for (int j = jj; j < jj + PER; ++j)
+        for (int j = 0; j < PER; ++j)
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            const f32x4 v = value(wn + j * 32 + 8 * q + 4 * (lane >> 5),
-                                  f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]});
-            const int col = (j - jj) * 32 + 8 * q + 4 * (lane >> 5);
-            if (BF16) {
-              *reinterpret_cast<u32x2*>(out + r * 128 + (((col >> 3) ^ x) << 4) + (col & 4) * 2) =
-                  u32x2{(unsigned)f32_bf16(v[0]) | (unsigned)f32_bf16(v[1]) << 16, (unsigned)f32_bf16(v[2]) | (unsigned)f32_bf16(v[3]) << 16};
-            } else {
-              *reinterpret_cast<f32x4*>(out + r * 128 + (((col >> 2) ^ x) << 4)) = v;
+            const int n = (jj + j) * 32 + 8 * q + 4 * h;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) add[j][q][e] = bias[wn + min(n + e, cols - 1)];
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < MI; ++i) {
+        if (i * 32 >= rows) continue;
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            f32x4 v = {acc[i][jj + j][4 * q], acc[i][jj + j][4 * q + 1], acc[i][jj + j][4 * q + 2], acc[i][jj + j][4 * q + 3]};
+            if (bias) v += add[j][q];
+            if (relu) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) v[e] = v[e] < 0.f ? 0.f : v[e];  // (a NaN passes)
             }
+            const int col = j * 32 + 8 * q + 4 * h;
+            if (BF16) *reinterpret_cast<u32x2*>(out + r * 128 + (((col >> 3) ^ x) << 4) + (col & 4) * 2) = u32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+            else *reinterpret_cast<f32x4*>(out + r * 128 + (((col >> 2) ^ x) << 4)) = v;
           }
 #pragma unroll
         for (int it = 0; it < 4; ++it) {
-          const int row = it * 8 + (lane >> 3), c = lane & 7;
+          const int row = it * 8 + (lane >> 3), c = lane & 7, m = i * 32 + row, n = jj * 32 + c * (16 / SIZE);
           const u32x4 v = *reinterpret_cast<const u32x4*>(out + row * 128 + ((c ^ ((row >> 1) & 7)) << 4));
-          const int64_t m = wm + i * 32 + row, n = wn + jj * 32 + c * (16 / SIZE);
-          if (m < mlim && n < nlim) {
-            unsigned char* to = static_cast<unsigned char*>(base) + (m * ld + n) * SIZE;
-            if (n + 16 / SIZE <= nlim) {
+          if (m < rows && n < cols) {
+            unsigned char* to = origin + (int64_t)m * ld * SIZE + n * SIZE;
+            if (n + 16 / SIZE <= cols) {
               *reinterpret_cast<u32x4u*>(to) = v;
             } else {
               for (int e = 0; e < 16 / SIZE - 1; ++e) {
-                if (n + e >= nlim) break;
+                if (n + e >= cols) break;
                 if (BF16) reinterpret_cast<uint16_t*>(to)[e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
                 else reinterpret_cast<uint32_t*>(to)[e] = v[e];
               }
@@ -555,6 +609,7 @@ struct DmaTile {
           }
         }
       }
+    }
   }
   // put(row of the tile, its sum): the waves of the first tile column hold every row, the two half waves half of its k each
   template <class Put>
@@ -581,53 +636,92 @@ struct FwdArgs {
   int act, y_bf16, zero_outside;
 };
 
-template <class T, class TileT, bool DMA>
-__global__ __launch_bounds__(TileT::THREADS) void grouped_forward_kernel(const FwdArgs a) {
+// tile `id` of the launch: its row slot and first column; false where there is nothing to write
+template <class TileT>
+__device__ __forceinline__ bool forward_tile(const FwdArgs& a, int64_t id, int64_t tiles_n, Slot& s, int64_t& n0) {
+  s = find_slot(a.gr, id / tiles_n, __builtin_ctz(TileT::BM));
+  n0 = (id % tiles_n) * TileT::BN;
+  return s.live && (s.group >= 0 || a.zero_outside);
+}
+
+template <class T, class TileT>
+__global__ __launch_bounds__(TileT::THREADS, 2) void grouped_forward_kernel(const FwdArgs a) {
   extern __shared__ __attribute__((aligned(16))) unsigned char raw_lds[];
   const int64_t tiles_n = (a.N + TileT::BN - 1) / TileT::BN;
-  const int64_t id = xcd_run(blockIdx.x, gridDim.x);
-  const Slot s = find_slot(a.gr, id / tiles_n, __builtin_ctz(TileT::BM));
-  if (!s.live || (s.group < 0 && !a.zero_outside)) return;
-  const int64_t n0 = (id % tiles_n) * TileT::BN;
-  T* lds = reinterpret_cast<T*>(raw_lds);
+  Slot s;
+  int64_t n0;
+  if (!forward_tile<TileT>(a, xcd_run(blockIdx.x, gridDim.x), tiles_n, s, n0)) return;
   TileT t;
   const float* bias = nullptr;
   if (s.group < 0) {
     t.zero();
   } else {
-    const T *X = static_cast<const T*>(a.X), *W = static_cast<const T*>(a.W) + s.group * a.stride_w;
-    if constexpr (DMA) t.template run<false>(X, a.ldx, s.begin, s.end, W, a.ldw, n0, a.N, 0, a.K, lds);
-    else t.run(X, a.ldx, s.begin, s.end, W, a.ldw, n0, a.N, 0, a.K, lds, [](const auto&) {});
+    t.run(static_cast<const T*>(a.X), a.ldx, s.begin, s.end, static_cast<const T*>(a.W) + s.group * a.stride_w, a.ldw, n0, a.N, 0, a.K,
+          reinterpret_cast<T*>(raw_lds), [](const auto&) {});
     if (a.bias) bias = a.bias + s.group * a.ld_bias;
   }
-  auto value = [&](int64_t n, f32x4 v) __attribute__((always_inline)) {
+  const bool relu = s.group >= 0 && a.act == DH_ACT_RELU;
+  t.each(s.begin, s.end, n0, a.N, [&](int64_t m, int64_t n, f32x4 v) __attribute__((always_inline)) {
     if (bias) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] += bias[min(n + e, a.N - 1)];
     }
-    if (a.act == DH_ACT_RELU) {
+    if (relu) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = v[e] < 0.f ? 0.f : v[e];  // (a NaN passes)
     }
-    return v;
+    if (a.y_bf16) put4<true>(static_cast<uint16_t*>(a.Y) + m * a.ldy, n, a.N, v);
+    else put4<false>(static_cast<float*>(a.Y) + m * a.ldy, n, a.N, v);
+  });
+}
+
+// As many workgroups as the chip holds; each walks the tiles l, l + L, l + 2 L ... of its XCD's contiguous run, L workgroups on that XCD.
+template <class TileT>
+__global__ __launch_bounds__(TileT::THREADS, 2) void grouped_forward_dma_kernel(const FwdArgs a, int64_t n_tiles) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char raw_lds[];
+  const int64_t tiles_n = (a.N + TileT::BN - 1) / TileT::BN;
+  const int64_t xcd = blockIdx.x % 8, q = n_tiles / 8, rest = n_tiles % 8;
+  const int64_t stop = (xcd < rest ? (xcd + 1) * (q + 1) : rest * (q + 1) + (xcd + 1 - rest) * q), step = (gridDim.x + 7 - xcd) / 8;
+  int64_t id = (xcd < rest ? xcd * (q + 1) : rest * (q + 1) + (xcd - rest) * q) + blockIdx.x / 8;
+  TileT t;
+  t.lds = reinterpret_cast<uint16_t*>(raw_lds);
+  auto advance = [&](Slot& s, int64_t& n0) __attribute__((always_inline)) {  // the next tile with something to write
+    for (; id < stop; id += step)
+      if (forward_tile<TileT>(a, id, tiles_n, s, n0)) {
+        id += step;
+        return true;
+      }
+    return false;
   };
-  if constexpr (DMA) {
-    if (a.y_bf16) t.template store<true>(a.Y, a.ldy, s.begin, s.end, n0, a.N, lds, value);
-    else t.template store<false>(a.Y, a.ldy, s.begin, s.end, n0, a.N, lds, value);
-  } else {
-    t.each(s.begin, s.end, n0, a.N, [&](int64_t m, int64_t n, f32x4 v) __attribute__((always_inline)) {
-      v = value(n, v);
-      if (a.y_bf16) put4<true>(static_cast<uint16_t*>(a.Y) + m * a.ldy, n, a.N, v);
-      else put4<false>(static_cast<float*>(a.Y) + m * a.ldy, n, a.N, v);
-    });
+  auto begin = [&](const Slot& s, int64_t n0) __attribute__((always_inline)) {
+    t.begin({static_cast<const uint16_t*>(a.X), static_cast<const uint16_t*>(a.W) + (s.group < 0 ? 0 : s.group * a.stride_w), a.ldx, a.ldw, s.begin,
+             s.end, n0, a.N, 0, s.group < 0 ? 0 : a.K});
+  };
+  Slot s, ns;
+  int64_t n0, nn0 = 0;
+  if (!advance(s, n0)) return;
+  begin(s, n0);
+  bool more = advance(ns, nn0);
+  while (true) {
+    t.template main<false>();
+    if (more) begin(ns, nn0);
+    const float* bias = a.bias && s.group >= 0 ? a.bias + s.group * a.ld_bias : nullptr;
+    const bool relu = s.group >= 0 && a.act == DH_ACT_RELU;
+    if (a.y_bf16) t.template store<true>(a.Y, a.ldy, s.begin, s.end, n0, a.N, bias, relu);
+    else t.template store<false>(a.Y, a.ldy, s.begin, s.end, n0, a.N, bias, relu);
+    if (!more) return;
+    s = ns;
+    n0 = nn0;
+    more = advance(ns, nn0);
   }
 }
 
 // ---- dW, db --------------------------------------------------------------------------------------------------------------------------
-// dW_g [N][K] = sum over the group's rows of dY[i, n] X[i, k]: both operands [k][row] images with the rows as the contraction.  Long groups
-// are cut into chunks of 2^shift rows; a group of one chunk is finished in place, the chunks of a longer one go to partial slots that
-// wgrad_join_kernel adds in chunk order (no atomics).  The slot of chunk j that starts at row s: 2 (s >> shift) + (j > 0): two chunks of
-// longer groups that start inside the same 2^shift rows are the last of one group (j > 0) and the first of the next (j = 0).
+// dW_g [N][K] = sum over the group's rows of dY[i, n] X[i, k]: both operands [k][row] images with the rows as the contraction.  The rows are
+// cut into equal chunks whatever the groups: a workgroup takes one tile of dW through one chunk, group by group, so every workgroup has the
+// same number of rows to multiply however ragged the groups are.  A group that lies inside a chunk is finished in place; of one that spans
+// several, chunk c holds either its beginning (partial slot 2 c) or a later part that starts with the chunk (slot 2 c + 1; never two of a
+// kind), which wgrad_join_kernel adds in chunk order (no atomics).  An empty group's zeros are written by the chunk of its position.
 struct WgradArgs {
   Groups gr;
   int64_t N, K;
@@ -638,77 +732,100 @@ struct WgradArgs {
   int dw_bf16;
   float* db;  // [G][N] or null
   int64_t ld_db;
-  float* part_w;  // [slots][N][K]
-  float* part_b;  // [slots][N]
-  int shift;
-  int64_t tiles_k, tiles;
+  float* part_w;  // [2 chunks][N][K]
+  float* part_b;  // [2 chunks][N]
+  int64_t chunk, chunks, tiles_k, tiles;
 };
 
-template <class T, class TileT, bool DMA>
-__global__ __launch_bounds__(TileT::THREADS) void grouped_wgrad_kernel(const WgradArgs a) {
+struct Segment {  // the rows [begin, end) of a group inside a chunk
+  int group;
+  int64_t begin, end;
+  int64_t slot;  // partial slot, -1: the whole group
+};
+
+// Walks the groups of chunk c.
+struct Segments {
+  const WgradArgs& a;
+  int64_t c, first, last;  // rows [first, last)
+  int i;                   // next edge index: group i - 1
+
+  __device__ __forceinline__ Segments(const WgradArgs& args, int64_t chunk_id) : a(args), c(chunk_id) {
+    first = c * a.chunk;
+    last = min(first + a.chunk, a.gr.M);
+    // the first group that touches the chunk: the one that holds its first row, or earlier empty ones at that very position
+    if (c == 0) {
+      i = 1;
+    } else {
+      i = search(a.gr.G + 2, first - 1, [&](int j) { return a.gr.edge(j); });  // holds row first - 1
+      if (a.gr.edge(i + 1) <= first) ++i;                                      // and ends there: nothing of it is left
+      if (i < 1) i = 1;
+    }
+  }
+  __device__ __forceinline__ bool next(Segment& s) {
+    while (i <= a.gr.G) {
+      const int64_t b = a.gr.edge(i), e = a.gr.edge(i + 1);
+      const bool final_chunk = c + 1 == a.chunks;
+      if (b > last || (b == last && !(final_chunk && e <= b))) return false;
+      ++i;
+      if (e <= b) {  // empty: at position b of this chunk (at its end only in the last chunk)
+        s = {i - 2, 0, 0, -1};
+        return true;
+      }
+      const int64_t from = max(b, first), to = min(e, last);
+      if (from >= to) continue;
+      s = {i - 2, from, to, b >= first && e <= last ? -1 : b >= first ? 2 * c : 2 * c + 1};
+      return true;
+    }
+    return false;
+  }
+};
+
+// where a segment's result goes
+struct WgradOut {
+  void* to;
+  int64_t ld;
+  float* sums;
+  bool bf16;
+};
+__device__ __forceinline__ WgradOut wgrad_out(const WgradArgs& a, const Segment& s) {
+  if (s.slot >= 0) return {a.part_w + s.slot * a.N * a.K, a.K, a.part_b + s.slot * a.N, false};
+  return {static_cast<char*>(a.dW) + s.group * a.stride_w * (a.dw_bf16 ? 2 : 4), a.ldw, a.db ? a.db + s.group * a.ld_db : nullptr, a.dw_bf16 != 0};
+}
+
+template <class T, class TileT>
+__global__ __launch_bounds__(TileT::THREADS, 2) void grouped_wgrad_kernel(const WgradArgs a) {
   typedef typename TileT::OpA OpA;
   extern __shared__ __attribute__((aligned(16))) unsigned char raw_lds[];
-  const int64_t id = xcd_run(blockIdx.x, gridDim.x);
-  const Slot s = find_slot(a.gr, id / a.tiles, a.shift);
-  if (s.group < 0) return;
-  const int64_t glen = a.gr.edge(s.group + 2) - s.start;
-  if (!s.live && !(glen <= 0 && s.index == 0)) return;  // an empty group's one slot writes its zeros
-  const int64_t tile = id % a.tiles, n0 = (tile / a.tiles_k) * TileT::BM, k0 = (tile % a.tiles_k) * TileT::BN;
-  const bool alone = glen <= ((int64_t)1 << a.shift);
+  const int64_t id = xcd_run(blockIdx.x, gridDim.x), tile = id % a.tiles, n0 = (tile / a.tiles_k) * TileT::BM, k0 = (tile % a.tiles_k) * TileT::BN;
   const bool sums = a.db && k0 == 0;
-  const int64_t end = s.live ? s.end : s.begin;
-  const T *dY = static_cast<const T*>(a.dY), *X = static_cast<const T*>(a.X);
-  T* stages = reinterpret_cast<T*>(raw_lds);
-  TileT t;
   constexpr int VEC = Geo<T>::VEC;
-  float cs[VEC];
-  if constexpr (DMA) {
-    if (sums) t.template run<true>(dY, a.ldy, n0, a.N, X, a.ldx, k0, a.K, s.begin, end, stages);
-    else t.template run<false>(dY, a.ldy, n0, a.N, X, a.ldx, k0, a.K, s.begin, end, stages);
-  } else {
+  Segments walk(a, id / a.tiles);
+  Segment s;
+  while (walk.next(s)) {
+    TileT t;
+    float cs[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) cs[e] = 0.f;
-    t.run(dY, a.ldy, n0, a.N, X, a.ldx, k0, a.K, s.begin, end, stages, [&](const OpA& op) __attribute__((always_inline)) {
-      if (!sums) return;
+    t.run(static_cast<const T*>(a.dY), a.ldy, n0, a.N, static_cast<const T*>(a.X), a.ldx, k0, a.K, s.begin, s.end, reinterpret_cast<T*>(raw_lds),
+          [&](const OpA& op) __attribute__((always_inline)) {
+            if (!sums) return;
 #pragma unroll
-      for (int q = 0; q < OpA::PIECES; ++q) {
-        T e[VEC];
-        __builtin_memcpy(e, &op.reg[q], 16);
+            for (int q = 0; q < OpA::PIECES; ++q) {
+              T e[VEC];
+              __builtin_memcpy(e, &op.reg[q], 16);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          if constexpr (sizeof(T) == 2) cs[i] += bf16_f32(e[i]);
-          else cs[i] += e[i];
-        }
-      }
-    });
-  }
-  const int64_t slot = alone ? 0 : 2 * (s.begin >> a.shift) + (s.index > 0 ? 1 : 0);
-  void* out = a.part_w + slot * a.N * a.K;
-  int64_t ld = a.K;
-  bool bf16 = false;
-  if (alone) {
-    bf16 = a.dw_bf16;
-    ld = a.ldw;
-    out = static_cast<char*>(a.dW) + s.group * a.stride_w * (bf16 ? 2 : 4);
-  }
-  if constexpr (DMA) {
-    auto value = [](int64_t, f32x4 v) __attribute__((always_inline)) { return v; };
-    if (bf16) t.template store<true>(out, ld, n0, a.N, k0, a.K, stages, value);
-    else t.template store<false>(out, ld, n0, a.N, k0, a.K, stages, value);
-  } else {
+              for (int i = 0; i < VEC; ++i) {
+                if constexpr (sizeof(T) == 2) cs[i] += bf16_f32(e[i]);
+                else cs[i] += e[i];
+              }
+            }
+          });
+    const WgradOut o = wgrad_out(a, s);
     t.each(n0, a.N, k0, a.K, [&](int64_t n, int64_t k, f32x4 v) __attribute__((always_inline)) {
-      if (bf16) put4<true>(static_cast<uint16_t*>(out) + n * ld, k, a.K, v);
-      else put4<false>(static_cast<float*>(out) + n * ld, k, a.K, v);
+      if (o.bf16) put4<true>(static_cast<uint16_t*>(o.to) + n * o.ld, k, a.K, v);
+      else put4<false>(static_cast<float*>(o.to) + n * o.ld, k, a.K, v);
     });
-  }
-  if (sums) {
-    auto put = [&](int i, float v) __attribute__((always_inline)) {
-      if (n0 + i >= a.N) return;
-      if (alone) a.db[s.group * a.ld_db + n0 + i] = v;
-      else a.part_b[slot * a.N + n0 + i] = v;
-    };
-    if constexpr (DMA) t.row_sums(put);
-    else {  // thread t summed columns (t % CPR) * VEC of the rows it staged
+    if (sums) {  // thread t summed columns (t % CPR) * VEC of the rows it staged
       float* lds = reinterpret_cast<float*>(raw_lds);
       __syncthreads();
       constexpr int LD = TileT::BM + 4;
@@ -719,42 +836,78 @@ __global__ __launch_bounds__(TileT::THREADS) void grouped_wgrad_kernel(const Wgr
       for (int i = threadIdx.x; i < TileT::BM; i += TileT::THREADS) {
         float v = 0.f;
         for (int r = 0; r < OpA::ROWS_PER_PASS; ++r) v += lds[r * LD + i];
-        put(i, v);
+        if (n0 + i < a.N) o.sums[n0 + i] = v;
       }
     }
+    __syncthreads();  // the next segment's images
   }
 }
 
-// The chunks of every group longer than one chunk.  blockIdx.y = b: the group that starts inside rows [b << shift, (b + 1) << shift) and
-// reaches beyond them, if there is one, contains the last of these rows.
+template <class TileT, bool SUMS>
+__device__ __forceinline__ void wgrad_dma(const WgradArgs& a, int64_t c, int64_t n0, int64_t k0, uint16_t* lds) {
+  TileT t;
+  t.lds = lds;
+  auto begin = [&](const Segment& s) __attribute__((always_inline)) {
+    t.begin({static_cast<const uint16_t*>(a.dY), static_cast<const uint16_t*>(a.X), a.ldy, a.ldx, n0, a.N, k0, a.K, s.begin, s.end});
+  };
+  Segments walk(a, c);
+  Segment s, ns;
+  if (!walk.next(s)) return;
+  begin(s);
+  bool more = walk.next(ns);
+  while (true) {
+    t.template main<SUMS>();
+    if (more) begin(ns);
+    const WgradOut o = wgrad_out(a, s);
+    if (o.bf16) t.template store<true>(o.to, o.ld, n0, a.N, k0, a.K, nullptr, false);
+    else t.template store<false>(o.to, o.ld, n0, a.N, k0, a.K, nullptr, false);
+    if (SUMS)
+      t.row_sums([&](int i, float v) __attribute__((always_inline)) {
+        if (n0 + i < a.N) o.sums[n0 + i] = v;
+      });
+    if (!more) return;
+    s = ns;
+    more = walk.next(ns);
+  }
+}
+
+template <class TileT>
+__global__ __launch_bounds__(TileT::THREADS, 2) void grouped_wgrad_dma_kernel(const WgradArgs a) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char raw_lds[];
+  const int64_t id = xcd_run(blockIdx.x, gridDim.x), tile = id % a.tiles, n0 = (tile / a.tiles_k) * TileT::BM, k0 = (tile % a.tiles_k) * TileT::BN;
+  if (a.db && k0 == 0) wgrad_dma<TileT, true>(a, id / a.tiles, n0, k0, reinterpret_cast<uint16_t*>(raw_lds));
+  else wgrad_dma<TileT, false>(a, id / a.tiles, n0, k0, reinterpret_cast<uint16_t*>(raw_lds));
+}
+
+// The parts of every group that spans chunks.  blockIdx.y = c: the group that begins in chunk c and reaches beyond it, if there is one,
+// contains the chunk's last row.
 __global__ __launch_bounds__(256) void wgrad_join_kernel(const WgradArgs a) {
-  const int64_t b = blockIdx.y, last = ((b + 1) << a.shift) - 1;
-  if (last >= a.gr.M) return;
+  const int64_t c0 = blockIdx.y, last = (c0 + 1) * a.chunk - 1;
   const int i = search(a.gr.G + 2, last, [&](int j) { return a.gr.edge(j); });
   const int64_t start = a.gr.edge(i), end = a.gr.edge(i + 1);
-  if (i == 0 || i == a.gr.G + 1 || start < (b << a.shift) || start > last || end - start <= ((int64_t)1 << a.shift)) return;
-  const int group = i - 1, chunks = (int)((end - start + ((int64_t)1 << a.shift) - 1) >> a.shift);
+  if (i == 0 || i == a.gr.G + 1 || start < c0 * a.chunk || start > last || end <= last + 1) return;
+  const int group = i - 1, parts = (int)((end - 1) / a.chunk - c0);  // later ones
   const int64_t nk = a.N * a.K, total = nk + (a.db ? a.N : 0);
   const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (at >= total) return;
   const bool is_b = at >= nk;
-  const float* p = is_b ? a.part_b + 2 * b * a.N + (at - nk) : a.part_w + 2 * b * nk + at;
   const int64_t step = is_b ? a.N : nk;
+  const float* p = (is_b ? a.part_b + (at - nk) : a.part_w + at) + 2 * c0 * step;
   float v = p[0];
   int c = 1;
-  for (; c + 8 <= chunks; c += 8) {  // chunk c > 0 of the group: slot 2 (b + c) + 1
+  for (; c + 7 <= parts; c += 8) {  // part c: slot 2 (c0 + c) + 1
     float t[8];
 #pragma unroll
     for (int u = 0; u < 8; ++u) t[u] = p[(2 * (int64_t)(c + u) + 1) * step];
 #pragma unroll
     for (int u = 0; u < 8; ++u) v += t[u];
   }
-  for (; c < chunks; ++c) v += p[(2 * (int64_t)c + 1) * step];
+  for (; c <= parts; ++c) v += p[(2 * (int64_t)c + 1) * step];
   if (is_b) {
     a.db[group * a.ld_db + (at - nk)] = v;
   } else {
     const int64_t o = group * a.stride_w + (at / a.K) * a.ldw + at % a.K;
-    if (a.dw_bf16) static_cast<uint16_t*>(a.dW)[o] = f32_bf16(v);
+    if (a.dw_bf16) static_cast<uint16_t*>(a.dW)[o] = (uint16_t)pack_bf16(v, 0.f);
     else static_cast<float*>(a.dW)[o] = v;
   }
 }
@@ -762,53 +915,72 @@ __global__ __launch_bounds__(256) void wgrad_join_kernel(const WgradArgs a) {
 // ---- host ----------------------------------------------------------------------------------------------------------------------------
 constexpr int64_t MAX_GRID = 0x7fffffff;
 
-template <class T, class TileT, bool DMA>
+constexpr int CUS = 256;
+
+// raises a kernel's dynamic LDS limit once
+template <class Kernel>
+int allow_lds(const char* me, Kernel* kernel, int bytes) {
+  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  return e == hipSuccess ? DH_OK : dh::fail(DH_ERR_LAUNCH, "%s: %d bytes of LDS: %s", me, bytes, hipGetErrorString(e));
+}
+
+template <class T, class TileT>
 int forward_launch(const char* me, const FwdArgs& a, hipStream_t st) {
-  const int64_t slots = a.gr.M / TileT::BM + a.gr.G + 2, grid = slots * dh::ceil_div(a.N, TileT::BN);
+  const int64_t grid = (a.gr.M / TileT::BM + a.gr.G + 2) * dh::ceil_div(a.N, TileT::BN);
   if (grid > MAX_GRID) return dh::fail(DH_ERR_INVALID, "%s: %lld tiles in one launch", me, (long long)grid);
-  auto* kernel = grouped_forward_kernel<T, TileT, DMA>;
-  static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, TileT::LDS_BYTES);
-  if (attr != hipSuccess) return dh::fail(DH_ERR_LAUNCH, "%s: %d bytes of LDS: %s", me, TileT::LDS_BYTES, hipGetErrorString(attr));
-  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(TileT::THREADS), TileT::LDS_BYTES, st, a);
+  static const int allowed = allow_lds(me, grouped_forward_kernel<T, TileT>, TileT::LDS_BYTES);
+  if (allowed != DH_OK) return allowed;
+  hipLaunchKernelGGL((grouped_forward_kernel<T, TileT>), dim3((unsigned)grid), dim3(TileT::THREADS), TileT::LDS_BYTES, st, a);
   return dh::check_launch(me);
 }
 
-bool dma_rows(const void* p, int64_t ld) { return dh::aligned16(p) && ld % 8 == 0; }
+template <class TileT>
+int forward_dma_launch(const char* me, const FwdArgs& a, hipStream_t st) {
+  const int64_t tiles = (a.gr.M / TileT::BM + a.gr.G + 2) * dh::ceil_div(a.N, TileT::BN);
+  const int64_t resident = (int64_t)CUS * (160 * 1024 / TileT::LDS_BYTES);
+  static const int allowed = allow_lds(me, grouped_forward_dma_kernel<TileT>, TileT::LDS_BYTES);
+  if (allowed != DH_OK) return allowed;
+  hipLaunchKernelGGL((grouped_forward_dma_kernel<TileT>), dim3((unsigned)(tiles < resident ? tiles : resident)), dim3(TileT::THREADS), TileT::LDS_BYTES, st,
+                     a, tiles);
+  return dh::check_launch(me);
+}
+
+// 16-byte aligned rows, and a tile (256 rows) within the 32-bit byte offsets of its lanes
+bool dma_rows(const void* p, int64_t ld) { return dh::aligned16(p) && ld % 8 == 0 && ld < (1 << 22); }
 
 template <class T, bool W_KM>
 int forward_pick(const char* me, const FwdArgs& a, hipStream_t st) {
   // few rows per group: a 32-row tile wastes less of the matrix cores and of the slots
-  if (a.gr.M <= (int64_t)48 * a.gr.G) return forward_launch<T, Tile<T, false, W_KM, 1, 1, 1, 4>, false>(me, a, st);
+  if (a.gr.M <= (int64_t)48 * a.gr.G) return forward_launch<T, Tile<T, false, W_KM, 1, 1, 1, 4>>(me, a, st);
   if constexpr (sizeof(T) == 2) {
     const bool dma = dma_rows(a.X, a.ldx) && dma_rows(a.W, a.ldw) && a.stride_w % 8 == 0 && a.K % 8 == 0 && (!W_KM || a.N % 8 == 0);
-    if (dma && a.gr.M >= (int64_t)1024 * a.gr.G) return forward_launch<T, DmaTile<false, W_KM, 4, 2, 2, 4>, true>(me, a, st);
-    if (dma) return forward_launch<T, DmaTile<false, W_KM, 2, 2, 2, 2>, true>(me, a, st);
+    if (dma && a.gr.M >= (int64_t)1024 * a.gr.G) return forward_dma_launch<DmaTile<false, W_KM, 4, 2, 2, 4, 64, 2>>(me, a, st);
+    if (dma) return forward_dma_launch<DmaTile<false, W_KM, 2, 2, 2, 2, 64, 2>>(me, a, st);
   }
-  return forward_launch<T, Tile<T, false, W_KM, 2, 2, 2, 2>, false>(me, a, st);
+  return forward_launch<T, Tile<T, false, W_KM, 2, 2, 2, 2>>(me, a, st);
 }
 
-constexpr int WG_TILE = 128;
+// the three tiles of the weight gradient
+typedef Tile<float, true, true, 2, 2, 2, 2> WgradF32;
+typedef Tile<uint16_t, true, true, 2, 2, 2, 2> WgradBf16;
+typedef DmaTile<true, true, 4, 2, 2, 4, 64, 2> WgradDma;
 
-// rows per chunk: enough chunks x tiles to fill the chip a few times, no chunk below 256 rows
-int wgrad_shift(int64_t M, int64_t N, int64_t K) {
-  const int64_t tiles = dh::ceil_div(N, WG_TILE) * dh::ceil_div(K, WG_TILE);
-  const int64_t want = dh::ceil_div(1024, tiles);  // chunks
-  int shift = 8;
-  while (shift < 30 && (M >> shift) > want) ++shift;
-  return shift;
+// Rows per chunk: as many chunks x tiles as workgroups run at a time (2 per CU, 1 of the 256 x 256 tile), so that all end together; no chunk
+// below 32 rows, which a step of k would not fill.
+int64_t wgrad_chunk(int64_t M, int64_t N, int64_t K, int dtype) {
+  const int64_t edge = dtype == DH_DTYPE_BF16 ? 256 : 128, tiles = dh::ceil_div(N, edge) * dh::ceil_div(K, edge);
+  const int64_t want = dtype == DH_DTYPE_BF16 ? CUS : 2 * CUS, chunks = want / tiles > 1 ? want / tiles : 1;
+  const int64_t rows = dh::ceil_div(dh::ceil_div(M, chunks), 32) * 32;
+  return rows < 32 ? 32 : rows;
 }
 
-int64_t wgrad_slots(int64_t M, int shift) { return 2 * ((M >> shift) + 1); }
-
-template <class T, class TileT, bool DMA>
-int wgrad_launch(const char* me, WgradArgs a, hipStream_t st) {
+template <class TileT, class Kernel>
+int wgrad_launch(const char* me, WgradArgs a, Kernel* kernel, int allowed, hipStream_t st) {
+  if (allowed != DH_OK) return allowed;
   a.tiles_k = dh::ceil_div(a.K, TileT::BN);
   a.tiles = dh::ceil_div(a.N, TileT::BM) * a.tiles_k;
-  const int64_t grid = ((a.gr.M >> a.shift) + a.gr.G + 2) * a.tiles;
+  const int64_t grid = a.chunks * a.tiles;
   if (grid > MAX_GRID) return dh::fail(DH_ERR_INVALID, "%s: %lld tiles in one launch", me, (long long)grid);
-  auto* kernel = grouped_wgrad_kernel<T, TileT, DMA>;
-  static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, TileT::LDS_BYTES);
-  if (attr != hipSuccess) return dh::fail(DH_ERR_LAUNCH, "%s: %d bytes of LDS: %s", me, TileT::LDS_BYTES, hipGetErrorString(attr));
   hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(TileT::THREADS), TileT::LDS_BYTES, st, a);
   return dh::check_launch(me);
 }
@@ -843,9 +1015,10 @@ extern "C" int dh_gemm_grouped(int64_t M, int64_t N, int64_t K, int64_t G, int t
   return trans_b ? forward_pick<float, false>(me, a, st) : forward_pick<float, true>(me, a, st);
 }
 
-extern "C" size_t dh_gemm_grouped_wgrad_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-  if (M <= 0 || N <= 0 || K < 0) return 16;
-  return 16 + (size_t)wgrad_slots(M, wgrad_shift(M, N, K)) * (size_t)N * (size_t)(K + 1) * 4;
+extern "C" size_t dh_gemm_grouped_wgrad_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype) {
+  if (M <= 0 || N <= 0 || K <= 0) return 16;
+  const int64_t chunks = dh::ceil_div(M, wgrad_chunk(M, N, K, dtype));
+  return chunks < 2 ? 16 : 16 + (size_t)(2 * chunks) * (size_t)N * (size_t)(K + 1) * 4;
 }
 
 extern "C" int dh_gemm_grouped_wgrad(int64_t M, int64_t N, int64_t K, int64_t G, int dtype, const void* dY, int64_t ldy, const void* X, int64_t ldx,
@@ -859,23 +1032,31 @@ extern "C" int dh_gemm_grouped_wgrad(int64_t M, int64_t N, int64_t K, int64_t G,
   if (!dW || !group_ptr || (M > 0 && (!dY || !X))) return dh::fail(DH_ERR_INVALID, "%s: null tensor", me);
   if (ldy < N || ldx < K || ldw < K || (G > 1 && stride_w < (N - 1) * ldw + K) || (db && ld_db < N))
     return dh::fail(DH_ERR_INVALID, "%s: leading dimension below the row length", me);
-  const size_t need = dh_gemm_grouped_wgrad_workspace_bytes(M, N, K);
+  const size_t need = dh_gemm_grouped_wgrad_workspace_bytes(M, N, K, dtype);
   if (!workspace || workspace_bytes < need) return dh::fail(DH_ERR_WORKSPACE, "%s: workspace of %zu bytes, need %zu", me, workspace_bytes, need);
   if (!dh::aligned16(workspace)) return dh::fail(DH_ERR_INVALID, "%s: workspace must be 16-byte aligned", me);
   WgradArgs a{};
   a.gr = {group_ptr, M, (int)G};
   a.N = N; a.K = K; a.dY = dY; a.X = X; a.ldy = ldy; a.ldx = ldx; a.dW = dW; a.ldw = ldw; a.stride_w = stride_w; a.dw_bf16 = dw_dtype == DH_DTYPE_BF16;
-  a.db = db; a.ld_db = ld_db; a.shift = wgrad_shift(M, N, K);
-  const int64_t slots = wgrad_slots(M, a.shift);
+  a.db = db; a.ld_db = ld_db;
+  a.chunk = wgrad_chunk(M, N, K, dtype);
+  a.chunks = M > 0 ? dh::ceil_div(M, a.chunk) : 1;
   a.part_w = static_cast<float*>(workspace);
-  a.part_b = a.part_w + slots * N * K;
+  a.part_b = a.part_w + 2 * a.chunks * N * K;
   hipStream_t st = dh::as_stream(stream);
   int launched;
-  if (dtype != DH_DTYPE_BF16) launched = wgrad_launch<float, Tile<float, true, true, 2, 2, 2, 2>, false>(me, a, st);
-  else if (dma_rows(dY, ldy) && dma_rows(X, ldx) && N % 8 == 0 && K % 8 == 0) launched = wgrad_launch<uint16_t, DmaTile<true, true, 2, 2, 2, 2>, true>(me, a, st);
-  else launched = wgrad_launch<uint16_t, Tile<uint16_t, true, true, 2, 2, 2, 2>, false>(me, a, st);
+  if (dtype != DH_DTYPE_BF16) {
+    static const int allowed = allow_lds(me, grouped_wgrad_kernel<float, WgradF32>, WgradF32::LDS_BYTES);
+    launched = wgrad_launch<WgradF32>(me, a, grouped_wgrad_kernel<float, WgradF32>, allowed, st);
+  } else if (dma_rows(dY, ldy) && dma_rows(X, ldx) && N % 8 == 0 && K % 8 == 0) {
+    static const int allowed = allow_lds(me, grouped_wgrad_dma_kernel<WgradDma>, WgradDma::LDS_BYTES);
+    launched = wgrad_launch<WgradDma>(me, a, grouped_wgrad_dma_kernel<WgradDma>, allowed, st);
+  } else {
+    static const int allowed = allow_lds(me, grouped_wgrad_kernel<uint16_t, WgradBf16>, WgradBf16::LDS_BYTES);
+    launched = wgrad_launch<WgradBf16>(me, a, grouped_wgrad_kernel<uint16_t, WgradBf16>, allowed, st);
+  }
   if (launched != DH_OK) return launched;
-  if ((M >> a.shift) > 0)
-    hipLaunchKernelGGL(wgrad_join_kernel, dim3((unsigned)dh::ceil_div(N * K + N, 256), (unsigned)(M >> a.shift)), dim3(256), 0, st, a);
+  if (a.chunks > 1)
+    hipLaunchKernelGGL(wgrad_join_kernel, dim3((unsigned)dh::ceil_div(N * K + N, 256), (unsigned)(a.chunks - 1)), dim3(256), 0, st, a);
   return dh::check_launch(me);
 }

@@ -802,7 +802,7 @@ def gemm_grouped_wgrad(dY: torch.Tensor, X: torch.Tensor, group_ptr: torch.Tenso
     if K == 0 and want_bias:
         raise ValueError("gemm_grouped_wgrad: the bias gradient needs at least one input column")
     with _one_device(dY, X, group_ptr):
-        ws_bytes = lib.dh_gemm_grouped_wgrad_workspace_bytes(M, N, K)
+        ws_bytes = lib.dh_gemm_grouped_wgrad_workspace_bytes(M, N, K, dt)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=X.device)
         _call("gemm_grouped_bf16_tn" if dt else "gemm_grouped_f32_tn", lib.dh_gemm_grouped_wgrad, M, N, K, G, dt, *_mat(dY, X.dtype, "dY"),
               *_mat(X, X.dtype, "X"), _dev(group_ptr, torch.int32, "group_ptr", 1), dW.data_ptr(), max(K, 1), N * K,

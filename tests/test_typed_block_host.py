@@ -50,10 +50,11 @@ def test_grouped_wgrad_refusals(lib, bad):
 
 
 def test_grouped_wgrad_workspace(lib):
-    need = lib.dh_gemm_grouped_wgrad_workspace_bytes(8, 4, 4)
+    need = lib.dh_gemm_grouped_wgrad_workspace_bytes(8, 4, 4, 0)
     assert _wgrad(lib, ws_bytes=need - 1) == WORKSPACE and _wgrad(lib, ws=None) == WORKSPACE
-    for m in (1, 255, 256, 257, 5000, 200003):  # every partial slot 2 (s >> shift) + 1 of a row s < m fits
-        assert lib.dh_gemm_grouped_wgrad_workspace_bytes(m, 512, 2000) >= 2 * 512 * 2001 * 4
+    for dtype in (0, 1):
+        assert lib.dh_gemm_grouped_wgrad_workspace_bytes(31, 512, 2000, dtype) == 16        # one chunk of rows: no partial results
+        assert lib.dh_gemm_grouped_wgrad_workspace_bytes(200003, 512, 2000, dtype) >= 2 * 2 * 512 * 2001 * 4
 
 
 def _norm_fwd(lib, **kw):
@@ -132,19 +133,73 @@ def test_row_slots_cover_every_row_once(seed):
     M, G, shift = int(rng.integers(0, 900)), int(rng.integers(0, 90)), int(rng.integers(3, 8))
     ptr = np.sort(rng.integers(0, M + 1, G + 1)) if seed % 3 else np.sort(rng.choice([0, M // 3, M], G + 1))
     owner = np.full(M, -2)
-    parts = {}
-    for group, begin, end, start, index in _slots(ptr, M, shift):
+    for group, begin, end, _, _ in _slots(ptr, M, shift):
         assert (owner[begin:end] == -2).all()
         owner[begin:end] = group
-        if group >= 0 and ptr[group + 1] - ptr[group] > (1 << shift):  # a chunk of a longer group: its partial slot is its own
-            slot = 2 * (begin >> shift) + (index > 0)
-            assert slot not in parts and slot < 2 * ((M >> shift) + 1)
-            assert slot == (2 * (start >> shift) if index == 0 else 2 * ((start >> shift) + index) + 1)
-            parts[slot] = group
     want = np.full(M, -1)
     for g in range(G):
         want[ptr[g]:ptr[g + 1]] = g
     assert (owner == want).all()
+
+
+def _segments(ptr, M, chunk, chunks, c):
+    """(group, begin, end, partial slot) of a chunk of rows, as Segments walks them."""
+    e, G = _edges(ptr, M), len(ptr) - 1
+    first, last = c * chunk, min(c * chunk + chunk, M)
+    if c == 0:
+        i = 1
+    else:
+        i = max(j for j in range(G + 2) if e[j] <= first - 1)
+        if e[i + 1] <= first:
+            i += 1
+        i = max(i, 1)
+    out = []
+    while i <= G:
+        b, t = e[i], e[i + 1]
+        if b > last or (b == last and not (c + 1 == chunks and t <= b)):
+            break
+        i += 1
+        if t <= b:
+            out.append((i - 2, 0, 0, -1))
+            continue
+        lo, hi = max(b, first), min(t, last)
+        if lo < hi:
+            out.append((i - 2, lo, hi, -1 if b >= first and t <= last else 2 * c if b >= first else 2 * c + 1))
+    return out
+
+
+@pytest.mark.parametrize("seed", range(60))
+def test_weight_gradient_segments(seed):
+    """Every row of a group is in one segment, every group is finished once (in place, as zeros, or by the join of its parts, which reads
+    exactly the slots that were written), and no slot is written twice."""
+    rng = np.random.default_rng(seed)
+    M, G, chunk = int(rng.integers(0, 700)), int(rng.integers(1, 60)), int(rng.choice([32, 64, 96, 1000]))
+    ptr = np.sort(rng.integers(0, M + 1, G + 1)) if seed % 3 else np.sort(rng.choice([0, M // 3, M // 2, M], G + 1))
+    chunks = max(1, -(-M // chunk))
+    owner, done, slots = np.full(M, -1), np.zeros(G, int), {}
+    for c in range(chunks):
+        for group, lo, hi, slot in _segments(ptr, M, chunk, chunks, c):
+            assert (owner[lo:hi] == -1).all() and ptr[group] <= lo <= hi <= ptr[group + 1] or lo == hi == 0
+            owner[lo:hi] = group
+            if slot < 0:
+                done[group] += 1
+                assert hi - lo == ptr[group + 1] - ptr[group]
+            else:
+                assert slot not in slots and slot < 2 * chunks
+                slots[slot] = group
+    e = _edges(ptr, M)
+    for c0 in range(chunks - 1):  # wgrad_join_kernel
+        last = (c0 + 1) * chunk - 1
+        i = max(j for j in range(G + 2) if e[j] <= last)
+        start, end = e[i], e[i + 1]
+        if i in (0, G + 1) or start < c0 * chunk or start > last or end <= last + 1:
+            continue
+        done[i - 1] += 1
+        for c in range((end - 1) // chunk - c0 + 1):
+            assert slots.pop(2 * (c0 + c) + (c > 0)) == i - 1
+    assert not slots and (done == 1).all()
+    for g in range(G):
+        assert (owner[ptr[g]:ptr[g + 1]] == g).all()
 
 
 @pytest.mark.parametrize("seed", range(10))
