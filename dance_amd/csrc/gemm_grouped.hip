@@ -19,6 +19,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef unsigned int u32x4u __attribute__((ext_vector_type(4), aligned(2)));  // 16 bytes at an element's own alignment
 
 __device__ __forceinline__ float bf16_f32(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
@@ -119,6 +120,8 @@ struct Operand {
   static_assert(PIECES >= 1 && PIECES * THREADS == (KM ? BK : R) * CPR, "tile does not divide among the threads");
 
   u32x4 reg[PIECES];
+  const T* p[PIECES];  // the lane's pieces of the next step
+  int valid[PIECES];   // [k][row] images: values of the piece below rlim
 
   static __device__ __forceinline__ u32x4 guarded(const T* p, int64_t n_valid) {
     if (n_valid >= VEC) return *reinterpret_cast<const u32x4u*>(p);
@@ -129,25 +132,30 @@ struct Operand {
     __builtin_memcpy(&v, e, 16);
     return v;
   }
-  // rows [r0, rlim) of the operand, k in [k0, klim).  Rows beyond rlim read some row below it (their products are never stored);
-  // k beyond klim reads as zero.  FULL: the whole BK lies below klim (and for KM all R rows below rlim).
-  template <bool FULL>
-  __device__ __forceinline__ void load(const T* base, int64_t ld, int64_t r0, int64_t rlim, int64_t k0, int64_t klim) {
+  // rows [r0, rlim) of the operand from k0 on.  Rows beyond rlim read some row below it (their products are never stored).
+  __device__ __forceinline__ void start(const T* base, int64_t ld, int64_t r0, int64_t rlim, int64_t k0) {
     const int tid = threadIdx.x;
 #pragma unroll
     for (int q = 0; q < PIECES; ++q) {
       const int ir = tid / CPR + q * ROWS_PER_PASS, ic = (tid % CPR) * VEC;
       if (!KM) {
-        const int64_t row = min(r0 + ir, rlim - 1), k = k0 + ic;
-        const T* p = base + row * ld + k;
-        if (FULL) reg[q] = *reinterpret_cast<const u32x4u*>(p);
-        else reg[q] = guarded(p, klim - k);
+        p[q] = base + min(r0 + ir, rlim - 1) * ld + k0 + ic;
       } else {
-        const int64_t k = k0 + ir, row = r0 + ic;
-        const T* p = base + k * ld + row;
-        if (FULL) reg[q] = *reinterpret_cast<const u32x4u*>(p);
-        else reg[q] = guarded(p, k < klim ? rlim - row : 0);
+        p[q] = base + (k0 + ir) * ld + r0 + ic;
+        valid[q] = (int)max((int64_t)0, min((int64_t)VEC, rlim - r0 - ic));
       }
+    }
+  }
+  // the next BK of k, of which `left` exist (the others read as zero).  FULL: all of them (and for KM all R rows).
+  template <bool FULL>
+  __device__ __forceinline__ void load(int64_t ld, int64_t left) {
+    const int tid = threadIdx.x;
+#pragma unroll
+    for (int q = 0; q < PIECES; ++q) {
+      if (FULL) reg[q] = *reinterpret_cast<const u32x4u*>(p[q]);
+      else if (!KM) reg[q] = guarded(p[q], left - (tid % CPR) * VEC);
+      else reg[q] = guarded(p[q], tid / CPR + q * ROWS_PER_PASS < left ? valid[q] : 0);
+      p[q] += KM ? BK * ld : BK;
     }
   }
   __device__ __forceinline__ void store(T* img) const {
@@ -267,13 +275,15 @@ struct Tile {
     const bool whole = (!A_KM || m0 + BM <= mlim) && (!B_KM || n0 + BN <= nlim);
     OpA a;
     OpB b;
+    a.start(A, lda, m0, mlim, k_begin);
+    b.start(B, ldb, n0, nlim, k_begin);
     auto fetch = [&](int64_t k0) __attribute__((always_inline)) {
       if (whole && k0 + BK <= k_end) {
-        a.template load<true>(A, lda, m0, mlim, k0, k_end);
-        b.template load<true>(B, ldb, n0, nlim, k0, k_end);
+        a.template load<true>(lda, BK);
+        b.template load<true>(ldb, BK);
       } else {
-        a.template load<false>(A, lda, m0, mlim, k0, k_end);
-        b.template load<false>(B, ldb, n0, nlim, k0, k_end);
+        a.template load<false>(lda, k_end - k0);
+        b.template load<false>(ldb, k_end - k0);
       }
     };
     auto put = [&](int stage) __attribute__((always_inline)) {
@@ -304,7 +314,6 @@ struct Tile {
 // four consecutive values of a row; n + 4 may pass the row's end
 template <bool BF16>
 __device__ __forceinline__ void put4(void* row, int64_t n, int64_t nlim, f32x4 v) {
-  typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
   typedef unsigned int u32x2u __attribute__((ext_vector_type(2), aligned(2)));
   if (BF16) {
     uint16_t* p = static_cast<uint16_t*>(row) + n;
@@ -716,6 +725,111 @@ __global__ __launch_bounds__(TileT::THREADS, 2) void grouped_forward_dma_kernel(
   }
 }
 
+// ---- few rows: K split over the waves -------------------------------------------------------------------------------------------------
+// A 32 x 32 tile per workgroup, its K cut into one contiguous piece per wave: every wave requests the fragments of up to BATCH k groups
+// straight into registers before it multiplies the first, so a whole product of K <= 8 waves x BATCH groups costs one round trip to memory
+// where the staged tile pays one per step (16 rows of 8 types, 400 -> 200 fp32: 14.7 us staged).  The waves' partial tiles are added in LDS
+// in wave order.  Bound: latency, then the L1 (every 2 KB of fragments feeds one or four matrix instructions).
+template <class T, bool W_KM>
+struct SmallFrags {
+  static constexpr int KG = sizeof(T) == 2 ? 16 : 8, PER = KG / 2, BATCH = 4;  // k per group, per lane, groups in flight
+  T a[BATCH][PER], b[BATCH][PER];
+
+  static __device__ __forceinline__ void vec(T (&to)[PER], const T* p) {
+    const u32x4 v = *reinterpret_cast<const u32x4u*>(p);
+    __builtin_memcpy(to, &v, 16);
+  }
+  // groups [g, g + BATCH) below g_end; xr: the lane's row of X, w: its row (or, W_KM, column) of W
+  __device__ __forceinline__ void load(const T* xr, const T* w, int64_t ldw, int g, int g_end, int64_t K, int half) {
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) {
+      const int64_t k = (int64_t)min(g + u, g_end - 1) * KG + half * PER;
+      const int64_t whole = (int64_t)min(g + u, g_end - 1) * KG + KG;
+      if (whole <= K) {  // uniform
+        vec(a[u], xr + k);
+        if (!W_KM) vec(b[u], w + k);
+        else {
+#pragma unroll
+          for (int e = 0; e < PER; ++e) b[u][e] = w[(k + e) * ldw];
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+          const int64_t c = min(k + e, K - 1);
+          const T av = xr[c], bv = W_KM ? w[c * ldw] : w[c];
+          a[u][e] = k + e < K ? av : T(0);
+          b[u][e] = k + e < K ? bv : T(0);
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void multiply(f32x16& acc, int g, int g_end) const {
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) {
+      if (g + u >= g_end) continue;  // uniform
+      if constexpr (sizeof(T) == 2) {
+        bf16x8 fa, fb;
+        __builtin_memcpy(&fa, a[u], 16);
+        __builtin_memcpy(&fb, b[u], 16);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fb, fa, acc, 0, 0, 0);
+      } else {
+#pragma unroll
+        for (int e = 0; e < PER; ++e) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(b[u][e], a[u][e], acc, 0, 0, 0);
+      }
+    }
+  }
+};
+
+template <class T, bool W_KM>
+__global__ __launch_bounds__(512) void grouped_small_kernel(const FwdArgs a) {
+  typedef SmallFrags<T, W_KM> Frags;
+  __shared__ __attribute__((aligned(16))) float part[8][32][36];
+  const int64_t tiles_n = (a.N + 31) / 32, id = xcd_run(blockIdx.x, gridDim.x);
+  const Slot s = find_slot(a.gr, id / tiles_n, 5);
+  const int64_t n0 = (id % tiles_n) * 32;
+  if (!s.live || (s.group < 0 && !a.zero_outside)) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, half = lane >> 5;
+  f32x16 acc;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) acc[r] = 0.f;
+  if (s.group >= 0 && a.K > 0) {
+    const int groups = (int)((a.K + Frags::KG - 1) / Frags::KG), per = (groups + waves - 1) / waves, g_end = min(groups, (wave + 1) * per);
+    const T* xr = static_cast<const T*>(a.X) + min(s.begin + (lane & 31), s.end - 1) * a.ldx;
+    const int64_t n = min(n0 + (lane & 31), a.N - 1);
+    const T* w = static_cast<const T*>(a.W) + s.group * a.stride_w + (W_KM ? n : n * a.ldw);
+    int g = wave * per;
+    if (g < g_end) {
+      Frags f[2];
+      f[0].load(xr, w, a.ldw, g, g_end, a.K, half);
+      for (; g < g_end; g += 2 * Frags::BATCH) {  // two batches in flight
+        if (g + Frags::BATCH < g_end) f[1].load(xr, w, a.ldw, g + Frags::BATCH, g_end, a.K, half);
+        f[0].multiply(acc, g, g_end);
+        if (g + 2 * Frags::BATCH < g_end) f[0].load(xr, w, a.ldw, g + 2 * Frags::BATCH, g_end, a.K, half);
+        if (g + Frags::BATCH < g_end) f[1].multiply(acc, g + Frags::BATCH, g_end);
+      }
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q)  // the lane's row, columns 8 q + 4 half .. + 4
+    *reinterpret_cast<f32x4*>(&part[wave][lane & 31][8 * q + 4 * half]) = f32x4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
+  __syncthreads();
+  const float* bias = a.bias && s.group >= 0 ? a.bias + s.group * a.ld_bias : nullptr;
+  const bool relu = s.group >= 0 && a.act == DH_ACT_RELU;
+  for (int i = threadIdx.x; i < 32 * 8; i += blockDim.x) {
+    const int64_t m = s.begin + (i >> 3), n = n0 + (i & 7) * 4;
+    if (m >= s.end || n >= a.N) continue;
+    f32x4 v = *reinterpret_cast<const f32x4*>(&part[0][i >> 3][(i & 7) * 4]);
+    for (int w = 1; w < waves; ++w) v += *reinterpret_cast<const f32x4*>(&part[w][i >> 3][(i & 7) * 4]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (bias) v[e] += bias[min(n + e, a.N - 1)];
+      if (relu) v[e] = v[e] < 0.f ? 0.f : v[e];  // (a NaN passes)
+    }
+    if (a.y_bf16) put4<true>(static_cast<uint16_t*>(a.Y) + m * a.ldy, n, a.N, v);
+    else put4<false>(static_cast<float*>(a.Y) + m * a.ldy, n, a.N, v);
+  }
+}
+
 // ---- dW, db --------------------------------------------------------------------------------------------------------------------------
 // dW_g [N][K] = sum over the group's rows of dY[i, n] X[i, k]: both operands [k][row] images with the rows as the contraction.  The rows are
 // cut into equal chunks whatever the groups: a workgroup takes one tile of dW through one chunk, group by group, so every workgroup has the
@@ -887,29 +1001,50 @@ __global__ __launch_bounds__(256) void wgrad_join_kernel(const WgradArgs a) {
   const int64_t start = a.gr.edge(i), end = a.gr.edge(i + 1);
   if (i == 0 || i == a.gr.G + 1 || start < c0 * a.chunk || start > last || end <= last + 1) return;
   const int group = i - 1, parts = (int)((end - 1) / a.chunk - c0);  // later ones
-  const int64_t nk = a.N * a.K, total = nk + (a.db ? a.N : 0);
-  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (at >= total) return;
-  const bool is_b = at >= nk;
-  const int64_t step = is_b ? a.N : nk;
-  const float* p = (is_b ? a.part_b + (at - nk) : a.part_w + at) + 2 * c0 * step;
-  float v = p[0];
-  int c = 1;
-  for (; c + 7 <= parts; c += 8) {  // part c: slot 2 (c0 + c) + 1
-    float t[8];
+  const int64_t nk = a.N * a.K, at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  // four consecutive values of the parts' sum; part c > 0: slot 2 (c0 + c) + 1; eight in flight, past the last one it is read again and not added
+  auto joined = [&](const float* p, int64_t step, int64_t count) __attribute__((always_inline)) {
+    p += 2 * c0 * step;
+    f32x4 v;
 #pragma unroll
-    for (int u = 0; u < 8; ++u) t[u] = p[(2 * (int64_t)(c + u) + 1) * step];
+    for (int e = 0; e < 4; ++e) v[e] = p[min((int64_t)e, count - 1)];
+    for (int c = 1; c <= parts; c += 8) {
+      f32x4 t[8];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) v += t[u];
+      for (int u = 0; u < 8; ++u) {
+        const float* from = p + (2 * (int64_t)min(c + u, parts) + 1) * step;
+        if (count >= 4) {
+          t[u] = *reinterpret_cast<const f32x4u*>(from);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) t[u][e] = from[min((int64_t)e, count - 1)];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (c + u <= parts) v += t[u];
+    }
+    return v;
+  };
+  if (at < nk) {
+    const f32x4 v = joined(a.part_w + at, nk, nk - at);
+    void* to = static_cast<char*>(a.dW) + group * a.stride_w * (a.dw_bf16 ? 2 : 4);
+    int64_t n = nk <= 0xffffffffll ? (int64_t)((uint32_t)at / (uint32_t)a.K) : at / a.K, k = at - n * a.K;
+    if (k + 4 <= a.K || n + 1 == a.N) {
+      if (a.dw_bf16) put4<true>(static_cast<uint16_t*>(to) + n * a.ldw, k, a.K, v);
+      else put4<false>(static_cast<float*>(to) + n * a.ldw, k, a.K, v);
+    } else {  // the four pass the end of a row
+      for (int e = 0; e < 4 && n < a.N; ++e) {
+        if (a.dw_bf16) static_cast<uint16_t*>(to)[n * a.ldw + k] = (uint16_t)pack_bf16(v[e], 0.f);
+        else static_cast<float*>(to)[n * a.ldw + k] = v[e];
+        if (++k == a.K) {
+          k = 0;
+          ++n;
+        }
+      }
+    }
   }
-  for (; c <= parts; ++c) v += p[(2 * (int64_t)c + 1) * step];
-  if (is_b) {
-    a.db[group * a.ld_db + (at - nk)] = v;
-  } else {
-    const int64_t o = group * a.stride_w + (at / a.K) * a.ldw + at % a.K;
-    if (a.dw_bf16) static_cast<uint16_t*>(a.dW)[o] = (uint16_t)pack_bf16(v, 0.f);
-    else static_cast<float*>(a.dW)[o] = v;
-  }
+  if (a.db && at < a.N) put4<false>(a.db + group * a.ld_db, at, a.N, joined(a.part_b + at, a.N, a.N - at));
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------------------------
@@ -949,39 +1084,74 @@ int forward_dma_launch(const char* me, const FwdArgs& a, hipStream_t st) {
 bool dma_rows(const void* p, int64_t ld) { return dh::aligned16(p) && ld % 8 == 0 && ld < (1 << 22); }
 
 template <class T, bool W_KM>
+int small_launch(const char* me, const FwdArgs& a, hipStream_t st) {
+  const int64_t grid = (a.gr.M / 32 + a.gr.G + 2) * dh::ceil_div(a.N, 32);
+  if (grid > MAX_GRID) return dh::fail(DH_ERR_INVALID, "%s: %lld tiles in one launch", me, (long long)grid);
+  const int64_t groups = dh::ceil_div(a.K, SmallFrags<T, W_KM>::KG), waves = dh::ceil_div(groups, SmallFrags<T, W_KM>::BATCH);
+  hipLaunchKernelGGL((grouped_small_kernel<T, W_KM>), dim3((unsigned)grid), dim3(64 * (unsigned)(waves < 1 ? 1 : waves > 8 ? 8 : waves)), 0, st, a);
+  return dh::check_launch(me);
+}
+
+template <class T, bool W_KM>
 int forward_pick(const char* me, const FwdArgs& a, hipStream_t st) {
-  // few rows per group: a 32-row tile wastes less of the matrix cores and of the slots
-  if (a.gr.M <= (int64_t)48 * a.gr.G) return forward_launch<T, Tile<T, false, W_KM, 1, 1, 1, 4>>(me, a, st);
+  const int64_t tiles = (a.gr.M / 128 + a.gr.G) * dh::ceil_div(a.N, 128);  // of 128 x 128
+  // few rows per group, or too few tiles to occupy half of the CUs
+  if (a.gr.M <= (int64_t)48 * a.gr.G || tiles <= CUS / 2) return small_launch<T, W_KM>(me, a, st);
   if constexpr (sizeof(T) == 2) {
     const bool dma = dma_rows(a.X, a.ldx) && dma_rows(a.W, a.ldw) && a.stride_w % 8 == 0 && a.K % 8 == 0 && (!W_KM || a.N % 8 == 0);
     if (dma && a.gr.M >= (int64_t)1024 * a.gr.G) return forward_dma_launch<DmaTile<false, W_KM, 4, 2, 2, 4, 64, 2>>(me, a, st);
     if (dma) return forward_dma_launch<DmaTile<false, W_KM, 2, 2, 2, 2, 64, 2>>(me, a, st);
+  } else {
+    // fp32: below four rounds of workgroups the last, partly filled one costs more than the smaller tile's extra operand traffic
+    if (tiles < 4 * CUS) return forward_launch<T, Tile<T, false, W_KM, 1, 2, 2, 2>>(me, a, st);
   }
   return forward_launch<T, Tile<T, false, W_KM, 2, 2, 2, 2>>(me, a, st);
 }
 
-// the three tiles of the weight gradient
-typedef Tile<float, true, true, 2, 2, 2, 2> WgradF32;
-typedef Tile<uint16_t, true, true, 2, 2, 2, 2> WgradBf16;
-typedef DmaTile<true, true, 4, 2, 2, 4, 64, 2> WgradDma;
-
-// Rows per chunk: as many chunks x tiles as workgroups run at a time (2 per CU, 1 of the 256 x 256 tile), so that all end together; no chunk
-// below 32 rows, which a step of k would not fill.
-int64_t wgrad_chunk(int64_t M, int64_t N, int64_t K, int dtype) {
-  const int64_t edge = dtype == DH_DTYPE_BF16 ? 256 : 128, tiles = dh::ceil_div(N, edge) * dh::ceil_div(K, edge);
-  const int64_t want = dtype == DH_DTYPE_BF16 ? CUS : 2 * CUS, chunks = want / tiles > 1 ? want / tiles : 1;
-  const int64_t rows = dh::ceil_div(dh::ceil_div(M, chunks), 32) * 32;
-  return rows < 32 ? 32 : rows;
+// The tile of the weight gradient and its chunks: as many chunks x tiles as workgroups run at a time, so that all end together; no chunk below
+// 32 rows, which a step of k would not fill.  The large tile reads its operands least often; where it would leave a chunk short (few rows,
+// or a small dW) the smaller one has more workgroups to share the groups among.
+struct WgradPlan {
+  int edge;  // rows and columns of the tile
+  int64_t chunk;
+};
+WgradPlan wgrad_plan(int64_t M, int64_t N, int64_t K, int dtype) {
+  const int large = dtype == DH_DTYPE_BF16 ? 256 : 128;
+  WgradPlan p{};
+  for (int edge : {large, large / 2}) {
+    const int64_t tiles = dh::ceil_div(N, edge) * dh::ceil_div(K, edge), resident = edge == 256 ? CUS : 2 * CUS;
+    const int64_t chunks = resident / tiles > 1 ? resident / tiles : 1;
+    int64_t rows = dh::ceil_div(dh::ceil_div(M, chunks), 32) * 32;
+    if (rows < 32) rows = 32;
+    p = {edge, rows};
+    if (rows >= 1024) break;
+  }
+  return p;
 }
 
-template <class TileT, class Kernel>
-int wgrad_launch(const char* me, WgradArgs a, Kernel* kernel, int allowed, hipStream_t st) {
-  if (allowed != DH_OK) return allowed;
+template <class TileT>
+int wgrad_grid(const char* me, WgradArgs& a) {
   a.tiles_k = dh::ceil_div(a.K, TileT::BN);
   a.tiles = dh::ceil_div(a.N, TileT::BM) * a.tiles_k;
-  const int64_t grid = a.chunks * a.tiles;
-  if (grid > MAX_GRID) return dh::fail(DH_ERR_INVALID, "%s: %lld tiles in one launch", me, (long long)grid);
-  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(TileT::THREADS), TileT::LDS_BYTES, st, a);
+  if (a.chunks * a.tiles > MAX_GRID) return dh::fail(DH_ERR_INVALID, "%s: %lld tiles in one launch", me, (long long)(a.chunks * a.tiles));
+  return DH_OK;
+}
+
+template <class T, class TileT>
+int wgrad_launch(const char* me, WgradArgs a, hipStream_t st) {
+  static const int allowed = allow_lds(me, grouped_wgrad_kernel<T, TileT>, TileT::LDS_BYTES);
+  const int rc = allowed == DH_OK ? wgrad_grid<TileT>(me, a) : allowed;
+  if (rc != DH_OK) return rc;
+  hipLaunchKernelGGL((grouped_wgrad_kernel<T, TileT>), dim3((unsigned)(a.chunks * a.tiles)), dim3(TileT::THREADS), TileT::LDS_BYTES, st, a);
+  return dh::check_launch(me);
+}
+
+template <class TileT>
+int wgrad_dma_launch(const char* me, WgradArgs a, hipStream_t st) {
+  static const int allowed = allow_lds(me, grouped_wgrad_dma_kernel<TileT>, TileT::LDS_BYTES);
+  const int rc = allowed == DH_OK ? wgrad_grid<TileT>(me, a) : allowed;
+  if (rc != DH_OK) return rc;
+  hipLaunchKernelGGL((grouped_wgrad_dma_kernel<TileT>), dim3((unsigned)(a.chunks * a.tiles)), dim3(TileT::THREADS), TileT::LDS_BYTES, st, a);
   return dh::check_launch(me);
 }
 
@@ -1017,7 +1187,7 @@ extern "C" int dh_gemm_grouped(int64_t M, int64_t N, int64_t K, int64_t G, int t
 
 extern "C" size_t dh_gemm_grouped_wgrad_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype) {
   if (M <= 0 || N <= 0 || K <= 0) return 16;
-  const int64_t chunks = dh::ceil_div(M, wgrad_chunk(M, N, K, dtype));
+  const int64_t chunks = dh::ceil_div(M, wgrad_plan(M, N, K, dtype).chunk);
   return chunks < 2 ? 16 : 16 + (size_t)(2 * chunks) * (size_t)N * (size_t)(K + 1) * 4;
 }
 
@@ -1039,24 +1209,22 @@ extern "C" int dh_gemm_grouped_wgrad(int64_t M, int64_t N, int64_t K, int64_t G,
   a.gr = {group_ptr, M, (int)G};
   a.N = N; a.K = K; a.dY = dY; a.X = X; a.ldy = ldy; a.ldx = ldx; a.dW = dW; a.ldw = ldw; a.stride_w = stride_w; a.dw_bf16 = dw_dtype == DH_DTYPE_BF16;
   a.db = db; a.ld_db = ld_db;
-  a.chunk = wgrad_chunk(M, N, K, dtype);
+  const WgradPlan plan = wgrad_plan(M, N, K, dtype);
+  a.chunk = plan.chunk;
   a.chunks = M > 0 ? dh::ceil_div(M, a.chunk) : 1;
   a.part_w = static_cast<float*>(workspace);
   a.part_b = a.part_w + 2 * a.chunks * N * K;
   hipStream_t st = dh::as_stream(stream);
+  const bool dma = dtype == DH_DTYPE_BF16 && dma_rows(dY, ldy) && dma_rows(X, ldx) && N % 8 == 0 && K % 8 == 0;
   int launched;
-  if (dtype != DH_DTYPE_BF16) {
-    static const int allowed = allow_lds(me, grouped_wgrad_kernel<float, WgradF32>, WgradF32::LDS_BYTES);
-    launched = wgrad_launch<WgradF32>(me, a, grouped_wgrad_kernel<float, WgradF32>, allowed, st);
-  } else if (dma_rows(dY, ldy) && dma_rows(X, ldx) && N % 8 == 0 && K % 8 == 0) {
-    static const int allowed = allow_lds(me, grouped_wgrad_dma_kernel<WgradDma>, WgradDma::LDS_BYTES);
-    launched = wgrad_launch<WgradDma>(me, a, grouped_wgrad_dma_kernel<WgradDma>, allowed, st);
-  } else {
-    static const int allowed = allow_lds(me, grouped_wgrad_kernel<uint16_t, WgradBf16>, WgradBf16::LDS_BYTES);
-    launched = wgrad_launch<WgradBf16>(me, a, grouped_wgrad_kernel<uint16_t, WgradBf16>, allowed, st);
-  }
+  if (dtype != DH_DTYPE_BF16)
+    launched = plan.edge == 128 ? wgrad_launch<float, Tile<float, true, true, 2, 2, 2, 2>>(me, a, st) : wgrad_launch<float, Tile<float, true, true, 1, 1, 2, 2>>(me, a, st);
+  else if (dma)
+    launched = plan.edge == 256 ? wgrad_dma_launch<DmaTile<true, true, 4, 2, 2, 4, 64, 2>>(me, a, st) : wgrad_dma_launch<DmaTile<true, true, 2, 2, 2, 2, 64, 2>>(me, a, st);
+  else
+    launched = wgrad_launch<uint16_t, Tile<uint16_t, true, true, 2, 2, 2, 2>>(me, a, st);
   if (launched != DH_OK) return launched;
   if (a.chunks > 1)
-    hipLaunchKernelGGL(wgrad_join_kernel, dim3((unsigned)dh::ceil_div(N * K + N, 256), (unsigned)(a.chunks - 1)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(wgrad_join_kernel, dim3((unsigned)dh::ceil_div(N * K, 1024), (unsigned)(a.chunks - 1)), dim3(256), 0, st, a);
   return dh::check_launch(me);
 }
