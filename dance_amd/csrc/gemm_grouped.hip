@@ -119,7 +119,7 @@ struct Operand {
   static constexpr int ROWS_PER_PASS = THREADS / CPR;
   static_assert(PIECES >= 1 && PIECES * THREADS == (KM ? BK : R) * CPR, "tile does not divide among the threads");
 
-  u32x4 reg[PIECES];
+  u32x4 reg[2][PIECES];  // two steps in flight
   const T* p[PIECES];  // the lane's pieces of the next step
   int valid[PIECES];   // [k][row] images: values of the piece below rlim
 
@@ -147,23 +147,24 @@ struct Operand {
     }
   }
   // the next BK of k, of which `left` exist (the others read as zero).  FULL: all of them (and for KM all R rows).
-  template <bool FULL>
+  template <bool FULL, int U>
   __device__ __forceinline__ void load(int64_t ld, int64_t left) {
     const int tid = threadIdx.x;
 #pragma unroll
     for (int q = 0; q < PIECES; ++q) {
-      if (FULL) reg[q] = *reinterpret_cast<const u32x4u*>(p[q]);
-      else if (!KM) reg[q] = guarded(p[q], left - (tid % CPR) * VEC);
-      else reg[q] = guarded(p[q], tid / CPR + q * ROWS_PER_PASS < left ? valid[q] : 0);
+      if (FULL) reg[U][q] = *reinterpret_cast<const u32x4u*>(p[q]);
+      else if (!KM) reg[U][q] = guarded(p[q], left - (tid % CPR) * VEC);
+      else reg[U][q] = guarded(p[q], tid / CPR + q * ROWS_PER_PASS < left ? valid[q] : 0);
       p[q] += KM ? BK * ld : BK;
     }
   }
+  template <int U>
   __device__ __forceinline__ void store(T* img) const {
     const int tid = threadIdx.x;
 #pragma unroll
     for (int q = 0; q < PIECES; ++q) {
       const int ir = tid / CPR + q * ROWS_PER_PASS, ic = (tid % CPR) * VEC;
-      *reinterpret_cast<u32x4*>(img + ir * LD + ic) = reg[q];
+      *reinterpret_cast<u32x4*>(img + ir * LD + ic) = reg[U][q];
     }
   }
   // bf16: the 32x32x16 fragment of rows [row, row + 32), k [kk, kk + 16): lane l holds row l & 31, k (l >> 5) * 8 .. + 8
@@ -214,8 +215,8 @@ __device__ __forceinline__ void each4(const f32x16 (&acc)[MI][NI], int64_t m0, i
 }
 
 // ---- the tile ------------------------------------------------------------------------------------------------------------------------
-// BM x BN of C = A B^T over k in [0, K): WR x WC waves of MI x NI 32 x 32 accumulators.  Two LDS stages: while the products of one step
-// run, the next one's pieces (requested a step earlier) are written and the ones after that requested.
+// BM x BN of C = A B^T over k: WR x WC waves of MI x NI 32 x 32 accumulators.  Two LDS stages and two register buffers: while the products
+// of one step run, the next one's pieces are written and those of the step two behind it are requested.
 template <class T, bool A_KM, bool B_KM, int MI, int NI, int WR, int WC>
 struct Tile {
   static constexpr int BM = MI * WR * 32, BN = NI * WC * 32, THREADS = WR * WC * 64, BK = Geo<T>::BK;
@@ -266,7 +267,7 @@ struct Tile {
       }
     }
   }
-  // seen(opB or opA): called with the A operand's registers of every step (the bias gradient's column sums)
+  // seen(pieces): called with the A operand's pieces of every step (the bias gradient's column sums)
   template <class Seen>
   __device__ __forceinline__ void run(const T* A, int64_t lda, int64_t m0, int64_t mlim, const T* B, int64_t ldb, int64_t n0, int64_t nlim,
                                       int64_t k_begin, int64_t k_end, T* lds, Seen&& seen) {
@@ -277,32 +278,42 @@ struct Tile {
     OpB b;
     a.start(A, lda, m0, mlim, k_begin);
     b.start(B, ldb, n0, nlim, k_begin);
-    auto fetch = [&](int64_t k0) __attribute__((always_inline)) {
-      if (whole && k0 + BK <= k_end) {
-        a.template load<true>(lda, BK);
-        b.template load<true>(ldb, BK);
+    auto fetch = [&](int64_t t, auto buf) __attribute__((always_inline)) {
+      constexpr int U = decltype(buf)::value;
+      const int64_t left = k_end - k_begin - t * BK;
+      if (whole && left >= BK) {
+        a.template load<true, U>(lda, BK);
+        b.template load<true, U>(ldb, BK);
       } else {
-        a.template load<false>(lda, k_end - k0);
-        b.template load<false>(ldb, k_end - k0);
+        a.template load<false, U>(lda, left);
+        b.template load<false, U>(ldb, left);
       }
     };
-    auto put = [&](int stage) __attribute__((always_inline)) {
-      a.store(lds + stage * STAGE);
-      b.store(lds + stage * STAGE + OpA::ELEMS);
-      seen(a);
+    auto put = [&](auto buf) __attribute__((always_inline)) {  // the buffer's step into the stage of the same parity
+      constexpr int U = decltype(buf)::value;
+      a.template store<U>(lds + U * STAGE);
+      b.template store<U>(lds + U * STAGE + OpA::ELEMS);
+      seen(a.reg[U]);
     };
+    typedef std::integral_constant<int, 0> Even;
+    typedef std::integral_constant<int, 1> Odd;
     const int64_t steps = (k_end - k_begin + BK - 1) / BK;
-    fetch(k_begin);
-    put(0);
-    if (steps > 1) fetch(k_begin + BK);
+    fetch(0, Even{});
+    if (steps > 1) fetch(1, Odd{});
+    put(Even{});
+    if (steps > 2) fetch(2, Even{});
     __syncthreads();
-    for (int64_t t = 0; t < steps; ++t) {
+    auto step = [&](int64_t t, auto mine, auto other) __attribute__((always_inline)) {
       if (t + 1 < steps) {
-        put((t + 1) & 1);
-        if (t + 2 < steps) fetch(k_begin + (t + 2) * BK);
+        put(other);
+        if (t + 3 < steps) fetch(t + 3, other);
       }
-      products(lds + (t & 1) * STAGE);
+      products(lds + decltype(mine)::value * STAGE);
       __syncthreads();
+    };
+    for (int64_t t = 0; t < steps; t += 2) {
+      step(t, Even{}, Odd{});
+      if (t + 1 < steps) step(t + 1, Odd{}, Even{});
     }
   }
   template <class F>
@@ -921,12 +932,12 @@ __global__ __launch_bounds__(TileT::THREADS, 2) void grouped_wgrad_kernel(const 
 #pragma unroll
     for (int e = 0; e < VEC; ++e) cs[e] = 0.f;
     t.run(static_cast<const T*>(a.dY), a.ldy, n0, a.N, static_cast<const T*>(a.X), a.ldx, k0, a.K, s.begin, s.end, reinterpret_cast<T*>(raw_lds),
-          [&](const OpA& op) __attribute__((always_inline)) {
+          [&](const u32x4(&reg)[OpA::PIECES]) __attribute__((always_inline)) {
             if (!sums) return;
 #pragma unroll
             for (int q = 0; q < OpA::PIECES; ++q) {
               T e[VEC];
-              __builtin_memcpy(e, &op.reg[q], 16);
+              __builtin_memcpy(e, &reg[q], 16);
 #pragma unroll
               for (int i = 0; i < VEC; ++i) {
                 if constexpr (sizeof(T) == 2) cs[i] += bf16_f32(e[i]);
@@ -1103,7 +1114,7 @@ int forward_pick(const char* me, const FwdArgs& a, hipStream_t st) {
     if (dma) return forward_dma_launch<DmaTile<false, W_KM, 2, 2, 2, 2, 64, 2>>(me, a, st);
   } else {
     // fp32: below four rounds of workgroups the last, partly filled one costs more than the smaller tile's extra operand traffic
-    if (tiles < 4 * CUS) return forward_launch<T, Tile<T, false, W_KM, 1, 2, 2, 2>>(me, a, st);
+    if (tiles < 4 * CUS) return forward_launch<T, Tile<T, false, W_KM, 1, 1, 2, 2>>(me, a, st);
   }
   return forward_launch<T, Tile<T, false, W_KM, 2, 2, 2, 2>>(me, a, st);
 }
