@@ -346,15 +346,16 @@ __device__ __forceinline__ void put4(void* row, int64_t n, int64_t nlim, f32x4 v
   }
 }
 
-// ---- the bf16 tile filled by LDS DMA ---------------------------------------------------------------------------------------------------
+// ---- the tile filled by LDS DMA --------------------------------------------------------------------------------------------------------
 // The same product with the operands going from memory to LDS without passing registers (global_load_lds, 16 bytes a lane): what the big
 // products run on.  The DMA writes a wave's 64 pieces to 1 KB of LDS in lane order, so images cannot be padded; bank conflicts are avoided by
 // choosing WHICH piece a lane fetches: piece c of an image row lies at position c ^ x,
-//   [row][k] images (64- or 128-byte rows):  x = (row >> 2) & 3 or (row >> 1) & 7: the 16 rows that a 16-byte fragment read takes at a
-//                                     time cover all 16 slots of 256 bytes;
-//   [k][row] images (2 R-byte rows):  x = (k & 3) << 2: the four k rows that a transposing read takes from lie 64 bytes apart.
-// Needs 16-byte aligned rows (address and stride) and, for a [k][row] operand, a row count that is a multiple of 8 (a piece is whole or
-// absent).  In the last, partial step of k the lanes whose pieces lie behind the end fetch a piece of zeros instead.
+//   [row][k] images (128-byte rows):  x = (row >> 1) & 7: the 16 rows that a 16-byte fragment read takes at a time cover all 16 slots of 256
+//                                     bytes;
+//   [k][row] images, bf16:            x = (k & 3) << 2: the four k rows that a transposing read takes from lie 64 bytes apart;
+//   [k][row] images, fp32:            x = ((k >> 2) & 1) << 3: the half waves read rows 4 apart, in opposite halves of 256 bytes.
+// Needs 16-byte aligned rows (address and stride), k counts that are whole pieces where k is contiguous, and for a [k][row] operand whole
+// pieces of rows.  In the last, partial step of k the lanes whose pieces lie behind the end fetch a piece of zeros instead.
 typedef const __attribute__((address_space(1))) void* global_ptr;
 typedef __attribute__((address_space(3))) void* lds_ptr;
 
@@ -367,63 +368,80 @@ __device__ __forceinline__ int anew(int v) {
   return v;
 }
 
-template <bool KM, int R, int BK, int THREADS>
+// a lane's share of a 32-row fragment: 16 bytes, 8 bf16 or 4 fp32 of k
+template <class T>
+struct Fragment;
+template <>
+struct Fragment<uint16_t> {
+  typedef bf16x8 Type;
+};
+template <>
+struct Fragment<float> {
+  typedef f32x4 Type;
+};
+
+template <class T, bool KM, int R, int THREADS>
 struct DmaOperand {
-  static constexpr int CPR = KM ? R / 8 : BK / 8, PIECES = R * BK / 8 / THREADS, ELEMS = R * BK;
-  static_assert((BK == 32 || BK == 64) && PIECES * THREADS == R * BK / 8 && (!KM || R >= 128), "tile does not divide among the threads");
+  static constexpr int VEC = 16 / sizeof(T), BK = 128 / sizeof(T);  // a step of k is 128 bytes of a [row][k] operand
+  static constexpr int CPR = KM ? R / VEC : 8, PIECES = R * 8 / THREADS, ELEMS = R * BK;
+  static_assert(PIECES * THREADS == R * 8 && (!KM || R >= (sizeof(T) == 2 ? 128 : 64)), "tile does not divide among the threads");
+  typedef typename Fragment<T>::Type Frag;
 
   const char* base;         // uniform: advances with k
   uint32_t offset[PIECES];  // the lane's pieces, in bytes (a tile spans less than 4 GB: dma_rows)
 
-  static __device__ __forceinline__ int swizzle(int row) { return BK == 64 ? (row >> 1) & 7 : (row >> 2) & 3; }
   static __device__ __forceinline__ int image_row(int q, int tid) { return (q * THREADS + tid) / CPR; }
   static __device__ __forceinline__ int piece(int q, int tid) {
     const int row = image_row(q, tid), c = (q * THREADS + tid) % CPR;
-    return KM ? c ^ ((row & 3) << 2) : c ^ swizzle(row);
+    return c ^ (!KM ? (row >> 1) & 7 : sizeof(T) == 2 ? (row & 3) << 2 : ((row >> 2) & 1) << 3);
   }
-  __device__ __forceinline__ void start(const uint16_t* op, int64_t ld, int64_t r0, int64_t rlim, int64_t k0) {
+  __device__ __forceinline__ void start(const T* op, int64_t ld, int64_t r0, int64_t rlim, int64_t k0) {
     const int tid = anew(threadIdx.x), most = (int)min(rlim - r0, (int64_t)R);
     base = reinterpret_cast<const char*>(op + (KM ? k0 * ld + r0 : r0 * ld + k0));
 #pragma unroll
     for (int q = 0; q < PIECES; ++q) {
-      if (KM) offset[q] = ((uint32_t)image_row(q, tid) * (uint32_t)ld + (uint32_t)min(piece(q, tid) * 8, most - 8)) * 2u;
-      else offset[q] = ((uint32_t)min(image_row(q, tid), most - 1) * (uint32_t)ld + (uint32_t)piece(q, tid) * 8u) * 2u;
+      if (KM) offset[q] = ((uint32_t)image_row(q, tid) * (uint32_t)ld + (uint32_t)min(piece(q, tid) * VEC, most - VEC)) * (uint32_t)sizeof(T);
+      else offset[q] = ((uint32_t)min(image_row(q, tid), most - 1) * (uint32_t)ld + (uint32_t)(piece(q, tid) * VEC)) * (uint32_t)sizeof(T);
     }
   }
   // the next BK of k into an image
-  __device__ __forceinline__ void issue(uint16_t* img, int64_t ld) {
+  __device__ __forceinline__ void issue(T* img, int64_t ld) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
     for (int q = 0; q < PIECES; ++q)
-      __builtin_amdgcn_global_load_lds((global_ptr)(base + offset[q]), (lds_ptr)(img + (q * THREADS + wave * 64) * 8), 16, 0, 0);
-    base += KM ? BK * ld * 2 : BK * 2;
+      __builtin_amdgcn_global_load_lds((global_ptr)(base + offset[q]), (lds_ptr)(img + (q * THREADS + wave * 64) * VEC), 16, 0, 0);
+    base += (KM ? BK * ld : BK) * (int64_t)sizeof(T);
   }
   // the last `left` < BK of k, zeros behind them
-  __device__ __forceinline__ void issue_last(uint16_t* img, int left) const {
+  __device__ __forceinline__ void issue_last(T* img, int left) const {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), tid = anew(threadIdx.x);
 #pragma unroll
     for (int q = 0; q < PIECES; ++q) {
-      const int k = KM ? image_row(q, tid) : piece(q, tid) * 8;
+      const int k = KM ? image_row(q, tid) : piece(q, tid) * VEC;
       const void* from = k < left ? static_cast<const void*>(base + offset[q]) : static_cast<const void*>(zero_piece);
-      __builtin_amdgcn_global_load_lds((global_ptr)from, (lds_ptr)(img + (q * THREADS + wave * 64) * 8), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((global_ptr)from, (lds_ptr)(img + (q * THREADS + wave * 64) * VEC), 16, 0, 0);
     }
   }
-  // the fragment of rows [32 tile, 32 tile + 32), k [kk, kk + 16): lane l holds row l & 31, k (l >> 5) * 8 .. + 8
-  static __device__ __forceinline__ bf16x8 frag(const uint16_t* img, int tile, int kk, int lane) {
-    if (!KM) {
-      const int c = (kk >> 3) + (lane >> 5);
-      return *reinterpret_cast<const bf16x8*>(img + (tile * 32 + (lane & 31)) * BK + ((c ^ swizzle(lane)) << 3));
+  // the fragment of rows [32 tile, 32 tile + 32), k group g (16 bf16 or 8 fp32): lane l holds row l & 31, the half l >> 5 of the group's k
+  static __device__ __forceinline__ Frag frag(const T* img, int tile, int g, int lane) {
+    if constexpr (!KM) {
+      return *reinterpret_cast<const Frag*>(img + (tile * 32 + (lane & 31)) * BK + (((2 * g + (lane >> 5)) ^ ((lane >> 1) & 7)) * VEC));
+    } else if constexpr (sizeof(T) == 2) {
+      typedef short s16x4 __attribute__((ext_vector_type(4)));
+      typedef s16x4 __attribute__((address_space(3))) * lds_s16x4;
+      const int b = lane >> 4, i = lane & 15, x = i >> 2;  // x = k & 3 of the lane's row
+      const T* at = img + (g * 16 + (b >> 1) * 8 + x) * R + (tile ^ x) * 32 + (b & 1) * 16 + (i & 3) * 4;
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)at);
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + 4 * R));
+      Frag f;
+      __builtin_memcpy(&f, &lo, 8);
+      __builtin_memcpy(reinterpret_cast<char*>(&f) + 8, &hi, 8);
+      return f;
+    } else {
+      const int h = lane >> 5;
+      const T* at = img + (g * 8 + 4 * h) * R + (tile ^ h) * 32 + (lane & 31);
+      return Frag{at[0], at[R], at[2 * R], at[3 * R]};
     }
-    typedef short s16x4 __attribute__((ext_vector_type(4)));
-    typedef s16x4 __attribute__((address_space(3))) * lds_s16x4;
-    const int b = lane >> 4, i = lane & 15, x = i >> 2;  // x = k & 3 of the lane's row
-    const uint16_t* at = img + (kk + (b >> 1) * 8 + x) * R + (tile ^ x) * 32 + (b & 1) * 16 + (i & 3) * 4;
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)at);
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + 4 * R));
-    bf16x8 f;
-    __builtin_memcpy(&f, &lo, 8);
-    __builtin_memcpy(reinterpret_cast<char*>(&f) + 8, &hi, 8);
-    return f;
   }
 };
 
@@ -439,23 +457,25 @@ __device__ __forceinline__ void images_ready() {
 // begin() requests a tile's first steps, main() multiplies, store() writes the result out of an LDS region of its own, so that the next
 // tile's begin() runs before this one's store(): with one workgroup on a CU nothing else would fill these gaps (measured in cycles at
 // 200003 rows, 2000 -> 512, per tile: first request to first product 8500, 32 steps 107000, stores 16000 before they were made cheap).
-template <bool A_KM, bool B_KM, int MI, int NI, int WR, int WC, int K_STEP, int STAGES>
+template <class T, bool A_KM, bool B_KM, int MI, int NI, int WR, int WC>
 struct DmaTile {
-  static constexpr int BM = MI * WR * 32, BN = NI * WC * 32, THREADS = WR * WC * 64, BK = K_STEP, GROUPS = BK / 16;
-  typedef DmaOperand<A_KM, BM, BK, THREADS> OpA;
-  typedef DmaOperand<B_KM, BN, BK, THREADS> OpB;
-  static constexpr int STAGE = OpA::ELEMS + OpB::ELEMS, OUT = 4096, LDS_BYTES = STAGES * STAGE * 2 + WR * WC * OUT;
+  static constexpr int STAGES = 2, BM = MI * WR * 32, BN = NI * WC * 32, THREADS = WR * WC * 64, BK = 128 / sizeof(T);
+  static constexpr int GROUPS = 4, GK = BK / GROUPS, STEPS_PER_GROUP = sizeof(T) == 2 ? 1 : 4;  // matrix instructions per fragment pair
+  typedef DmaOperand<T, A_KM, BM, THREADS> OpA;
+  typedef DmaOperand<T, B_KM, BN, THREADS> OpB;
+  static constexpr int STAGE = OpA::ELEMS + OpB::ELEMS, OUT = 4096, LDS_BYTES = STAGES * STAGE * (int)sizeof(T) + WR * WC * OUT;
   static constexpr int INSTRS = OpA::PIECES + OpB::PIECES;  // DMA instructions of a wave per step
   static_assert((STAGES - 1) * INSTRS < 64 && GROUPS % 2 == 0, "");
+  typedef T Elem;
 
   struct Source {  // a tile's operands: rows [m0, mlim) of A and [n0, nlim) of B, k in [k_begin, k_end)
-    const uint16_t *A, *B;
+    const T *A, *B;
     int64_t lda, ldb, m0, mlim, n0, nlim, k_begin, k_end;
   };
 
   OpA a;
   OpB b;
-  uint16_t* lds;
+  T* lds;
   int64_t lda, ldb, full, steps;
   int left;
   f32x16 acc[MI][NI];
@@ -472,41 +492,54 @@ struct DmaTile {
     }
   }
   struct Frags {
-    bf16x8 a[MI], b[NI];
-    __device__ __forceinline__ void read(const uint16_t* st, int kk, int lane) {
+    typename Fragment<T>::Type a[MI], b[NI];
+    __device__ __forceinline__ void read(const T* st, int g, int lane) {
       const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), tm = (wave / WC) * MI, tn = (wave % WC) * NI;
 #pragma unroll
-      for (int i = 0; i < MI; ++i) a[i] = OpA::frag(st, tm + i, kk, lane);
+      for (int i = 0; i < MI; ++i) a[i] = OpA::frag(st, tm + i, g, lane);
 #pragma unroll
-      for (int j = 0; j < NI; ++j) b[j] = OpB::frag(st + OpA::ELEMS, tn + j, kk, lane);
+      for (int j = 0; j < NI; ++j) b[j] = OpB::frag(st + OpA::ELEMS, tn + j, g, lane);
     }
   };
   template <bool SUMS>
   __device__ __forceinline__ void multiply(const Frags& f) {
+    if constexpr (sizeof(T) == 2) {
 #pragma unroll
-    for (int i = 0; i < MI; ++i)
+      for (int i = 0; i < MI; ++i)
 #pragma unroll
-      for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.b[j], f.a[i], acc[i][j], 0, 0, 0);
+        for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.b[j], f.a[i], acc[i][j], 0, 0, 0);
+    } else {
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+          for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(f.b[j][s], f.a[i][s], acc[i][j], 0, 0, 0);
+    }
     if (SUMS) {
 #pragma unroll
       for (int i = 0; i < MI; ++i) {
         u32x4 v;
         __builtin_memcpy(&v, &f.a[i], 16);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) row_sum[i] += __uint_as_float(v[e] << 16) + __uint_as_float(v[e] & 0xffff0000u);
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (sizeof(T) == 2) row_sum[i] += __uint_as_float(v[e] << 16) + __uint_as_float(v[e] & 0xffff0000u);
+          else row_sum[i] += __uint_as_float(v[e]);
+        }
       }
     }
   }
-  // LDS reads of one fragment set per group of MI x NI products: spread one behind each product
-  static constexpr int READS = (A_KM ? 2 : 1) * MI + (B_KM ? 2 : 1) * NI, PER = (READS + MI * NI - 1) / (MI * NI);
+  // the LDS reads of one fragment set spread behind the products of a group
+  static constexpr int KM_READS = sizeof(T) == 2 ? 2 : 4, READS = (A_KM ? KM_READS : 1) * MI + (B_KM ? KM_READS : 1) * NI;
+  static constexpr int PRODUCTS = MI * NI * STEPS_PER_GROUP, PER = (READS + PRODUCTS - 1) / PRODUCTS;
   static __device__ __forceinline__ void interleave() {
 #pragma unroll
-    for (int i = 0; i < MI * NI; ++i) {
+    for (int i = 0; i < PRODUCTS; ++i) {
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
       __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
     }
   }
-  __device__ __forceinline__ void issue(int64_t t, uint16_t* image) {
+  __device__ __forceinline__ void issue(int64_t t, T* image) {
     if (t < full) {
       a.issue(image, lda);
       b.issue(image + OpA::ELEMS, ldb);
@@ -535,17 +568,17 @@ struct DmaTile {
     if (steps == 0) return;
     const int lane = anew(threadIdx.x & 63);
     Frags f[2];
-    uint16_t* image = lds;
+    T* image = lds;
     // (whatever was issued after begin() only makes this wait longer)
     if (steps >= STAGES) images_ready<(STAGES - 1) * INSTRS>();
     else images_ready<0>();
     f[0].read(image, 0, lane);
     int64_t t = 0;
     for (; t + 1 < steps; ++t) {
-      uint16_t* next = image == lds + (STAGES - 1) * STAGE ? lds : image + STAGE;
+      T* next = image == lds + (STAGES - 1) * STAGE ? lds : image + STAGE;
 #pragma unroll
       for (int g = 0; g + 1 < GROUPS; ++g) {
-        f[(g + 1) & 1].read(image, (g + 1) * 16, lane);
+        f[(g + 1) & 1].read(image, g + 1, lane);
         multiply<SUMS>(f[g & 1]);
         interleave();
       }
@@ -558,9 +591,9 @@ struct DmaTile {
       interleave();
       image = next;
     }
-    const int groups = left > 0 ? (left + 15) / 16 : GROUPS;
+    const int groups = left > 0 ? (left + GK - 1) / GK : GROUPS;
     for (int g = 0; g < groups; ++g) {
-      if (g + 1 < groups) f[1].read(image, (g + 1) * 16, lane);
+      if (g + 1 < groups) f[1].read(image, g + 1, lane);
       multiply<SUMS>(f[0]);
       f[0] = f[1];
     }
@@ -571,7 +604,7 @@ struct DmaTile {
   // a time in its own 4 KB of LDS (16-byte piece c of row r at c ^ (r >> 1) & 7, as in the images) and stores whole 128-byte row pieces.
   template <bool BF16>
   __device__ __forceinline__ void store(void* base, int64_t ld, int64_t m0, int64_t mlim, int64_t n0, int64_t nlim, const float* bias, bool relu) const {
-    constexpr int SIZE = BF16 ? 2 : 4, COLS = 128 / SIZE, PER = COLS / 32;  // columns and accumulator tiles of a 128-byte row piece
+    constexpr int SIZE = BF16 ? 2 : 4, PER = BF16 && NI > 1 ? 2 : 1;  // accumulator tiles of a 128-byte (one bf16 tile: 64-byte) row piece
     static_assert(NI % PER == 0, "a wave's columns do not divide into row pieces");
     const int lane = anew(threadIdx.x & 63), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     unsigned char* out = reinterpret_cast<unsigned char*>(lds + STAGES * STAGE) + wave * OUT;
@@ -698,13 +731,14 @@ __global__ __launch_bounds__(TileT::THREADS, 2) void grouped_forward_kernel(cons
 // As many workgroups as the chip holds; each walks the tiles l, l + L, l + 2 L ... of its XCD's contiguous run, L workgroups on that XCD.
 template <class TileT>
 __global__ __launch_bounds__(TileT::THREADS, 2) void grouped_forward_dma_kernel(const FwdArgs a, int64_t n_tiles) {
+  typedef typename TileT::Elem T;
   extern __shared__ __attribute__((aligned(16))) unsigned char raw_lds[];
   const int64_t tiles_n = (a.N + TileT::BN - 1) / TileT::BN;
   const int64_t xcd = blockIdx.x % 8, q = n_tiles / 8, rest = n_tiles % 8;
   const int64_t stop = (xcd < rest ? (xcd + 1) * (q + 1) : rest * (q + 1) + (xcd + 1 - rest) * q), step = (gridDim.x + 7 - xcd) / 8;
   int64_t id = (xcd < rest ? xcd * (q + 1) : rest * (q + 1) + (xcd - rest) * q) + blockIdx.x / 8;
   TileT t;
-  t.lds = reinterpret_cast<uint16_t*>(raw_lds);
+  t.lds = reinterpret_cast<T*>(raw_lds);
   auto advance = [&](Slot& s, int64_t& n0) __attribute__((always_inline)) {  // the next tile with something to write
     for (; id < stop; id += step)
       if (forward_tile<TileT>(a, id, tiles_n, s, n0)) {
@@ -714,7 +748,7 @@ __global__ __launch_bounds__(TileT::THREADS, 2) void grouped_forward_dma_kernel(
     return false;
   };
   auto begin = [&](const Slot& s, int64_t n0) __attribute__((always_inline)) {
-    t.begin({static_cast<const uint16_t*>(a.X), static_cast<const uint16_t*>(a.W) + (s.group < 0 ? 0 : s.group * a.stride_w), a.ldx, a.ldw, s.begin,
+    t.begin({static_cast<const T*>(a.X), static_cast<const T*>(a.W) + (s.group < 0 ? 0 : s.group * a.stride_w), a.ldx, a.ldw, s.begin,
              s.end, n0, a.N, 0, s.group < 0 ? 0 : a.K});
   };
   Slot s, ns;
@@ -969,11 +1003,12 @@ __global__ __launch_bounds__(TileT::THREADS, 2) void grouped_wgrad_kernel(const 
 }
 
 template <class TileT, bool SUMS>
-__device__ __forceinline__ void wgrad_dma(const WgradArgs& a, int64_t c, int64_t n0, int64_t k0, uint16_t* lds) {
+__device__ __forceinline__ void wgrad_dma(const WgradArgs& a, int64_t c, int64_t n0, int64_t k0, typename TileT::Elem* lds) {
+  typedef typename TileT::Elem T;
   TileT t;
   t.lds = lds;
   auto begin = [&](const Segment& s) __attribute__((always_inline)) {
-    t.begin({static_cast<const uint16_t*>(a.dY), static_cast<const uint16_t*>(a.X), a.ldy, a.ldx, n0, a.N, k0, a.K, s.begin, s.end});
+    t.begin({static_cast<const T*>(a.dY), static_cast<const T*>(a.X), a.ldy, a.ldx, n0, a.N, k0, a.K, s.begin, s.end});
   };
   Segments walk(a, c);
   Segment s, ns;
@@ -1000,8 +1035,8 @@ template <class TileT>
 __global__ __launch_bounds__(TileT::THREADS, 2) void grouped_wgrad_dma_kernel(const WgradArgs a) {
   extern __shared__ __attribute__((aligned(16))) unsigned char raw_lds[];
   const int64_t id = xcd_run(blockIdx.x, gridDim.x), tile = id % a.tiles, n0 = (tile / a.tiles_k) * TileT::BM, k0 = (tile % a.tiles_k) * TileT::BN;
-  if (a.db && k0 == 0) wgrad_dma<TileT, true>(a, id / a.tiles, n0, k0, reinterpret_cast<uint16_t*>(raw_lds));
-  else wgrad_dma<TileT, false>(a, id / a.tiles, n0, k0, reinterpret_cast<uint16_t*>(raw_lds));
+  if (a.db && k0 == 0) wgrad_dma<TileT, true>(a, id / a.tiles, n0, k0, reinterpret_cast<typename TileT::Elem*>(raw_lds));
+  else wgrad_dma<TileT, false>(a, id / a.tiles, n0, k0, reinterpret_cast<typename TileT::Elem*>(raw_lds));
 }
 
 // The parts of every group that spans chunks.  blockIdx.y = c: the group that begins in chunk c and reaches beyond it, if there is one,
@@ -1091,8 +1126,8 @@ int forward_dma_launch(const char* me, const FwdArgs& a, hipStream_t st) {
   return dh::check_launch(me);
 }
 
-// 16-byte aligned rows, and a tile (256 rows) within the 32-bit byte offsets of its lanes
-bool dma_rows(const void* p, int64_t ld) { return dh::aligned16(p) && ld % 8 == 0 && ld < (1 << 22); }
+// whole 16-byte pieces: address, row stride; and a tile (256 rows) within the 32-bit byte offsets of its lanes
+bool dma_rows(const void* p, int64_t ld, int vec) { return dh::aligned16(p) && ld % vec == 0 && ld < (1 << 21); }
 
 template <class T, bool W_KM>
 int small_launch(const char* me, const FwdArgs& a, hipStream_t st) {
@@ -1108,13 +1143,15 @@ int forward_pick(const char* me, const FwdArgs& a, hipStream_t st) {
   const int64_t tiles = (a.gr.M / 128 + a.gr.G) * dh::ceil_div(a.N, 128);  // of 128 x 128
   // few rows per group, or too few tiles to occupy half of the CUs
   if (a.gr.M <= (int64_t)48 * a.gr.G || tiles <= CUS / 2) return small_launch<T, W_KM>(me, a, st);
-  if constexpr (sizeof(T) == 2) {
-    const bool dma = dma_rows(a.X, a.ldx) && dma_rows(a.W, a.ldw) && a.stride_w % 8 == 0 && a.K % 8 == 0 && (!W_KM || a.N % 8 == 0);
-    if (dma && a.gr.M >= (int64_t)1024 * a.gr.G) return forward_dma_launch<DmaTile<false, W_KM, 4, 2, 2, 4, 64, 2>>(me, a, st);
-    if (dma) return forward_dma_launch<DmaTile<false, W_KM, 2, 2, 2, 2, 64, 2>>(me, a, st);
-  } else {
-    // fp32: below four rounds of workgroups the last, partly filled one costs more than the smaller tile's extra operand traffic
-    if (tiles < 4 * CUS) return forward_launch<T, Tile<T, false, W_KM, 1, 1, 2, 2>>(me, a, st);
+  constexpr int VEC = 16 / sizeof(T);
+  if (dma_rows(a.X, a.ldx, VEC) && dma_rows(a.W, a.ldw, VEC) && a.stride_w % VEC == 0 && a.K % VEC == 0 && (!W_KM || a.N % VEC == 0)) {
+    if constexpr (sizeof(T) == 2) {
+      if (a.gr.M >= (int64_t)1024 * a.gr.G) return forward_dma_launch<DmaTile<T, false, W_KM, 4, 2, 2, 4>>(me, a, st);
+    } else {
+      // fp32: below four rounds of workgroups the last, partly filled one costs more than the smaller tile's extra operand traffic
+      if (tiles < 4 * CUS) return forward_dma_launch<DmaTile<T, false, W_KM, 1, 1, 2, 2>>(me, a, st);
+    }
+    return forward_dma_launch<DmaTile<T, false, W_KM, 2, 2, 2, 2>>(me, a, st);
   }
   return forward_launch<T, Tile<T, false, W_KM, 2, 2, 2, 2>>(me, a, st);
 }
@@ -1226,14 +1263,16 @@ extern "C" int dh_gemm_grouped_wgrad(int64_t M, int64_t N, int64_t K, int64_t G,
   a.part_w = static_cast<float*>(workspace);
   a.part_b = a.part_w + 2 * a.chunks * N * K;
   hipStream_t st = dh::as_stream(stream);
-  const bool dma = dtype == DH_DTYPE_BF16 && dma_rows(dY, ldy) && dma_rows(X, ldx) && N % 8 == 0 && K % 8 == 0;
+  const int vec = dtype == DH_DTYPE_BF16 ? 8 : 4;
+  const bool dma = dma_rows(dY, ldy, vec) && dma_rows(X, ldx, vec) && N % vec == 0 && K % vec == 0;
   int launched;
-  if (dtype != DH_DTYPE_BF16)
-    launched = plan.edge == 128 ? wgrad_launch<float, Tile<float, true, true, 2, 2, 2, 2>>(me, a, st) : wgrad_launch<float, Tile<float, true, true, 1, 1, 2, 2>>(me, a, st);
-  else if (dma)
-    launched = plan.edge == 256 ? wgrad_dma_launch<DmaTile<true, true, 4, 2, 2, 4, 64, 2>>(me, a, st) : wgrad_dma_launch<DmaTile<true, true, 2, 2, 2, 2, 64, 2>>(me, a, st);
-  else
-    launched = wgrad_launch<uint16_t, Tile<uint16_t, true, true, 2, 2, 2, 2>>(me, a, st);
+  if (dtype != DH_DTYPE_BF16) {
+    if (!dma) launched = plan.edge == 128 ? wgrad_launch<float, Tile<float, true, true, 2, 2, 2, 2>>(me, a, st) : wgrad_launch<float, Tile<float, true, true, 1, 1, 2, 2>>(me, a, st);
+    else launched = plan.edge == 128 ? wgrad_dma_launch<DmaTile<float, true, true, 2, 2, 2, 2>>(me, a, st) : wgrad_dma_launch<DmaTile<float, true, true, 1, 1, 2, 2>>(me, a, st);
+  } else {
+    if (!dma) launched = wgrad_launch<uint16_t, Tile<uint16_t, true, true, 2, 2, 2, 2>>(me, a, st);
+    else launched = plan.edge == 256 ? wgrad_dma_launch<DmaTile<uint16_t, true, true, 4, 2, 2, 4>>(me, a, st) : wgrad_dma_launch<DmaTile<uint16_t, true, true, 2, 2, 2, 2>>(me, a, st);
+  }
   if (launched != DH_OK) return launched;
   if (a.chunks > 1)
     hipLaunchKernelGGL(wgrad_join_kernel, dim3((unsigned)dh::ceil_div(N * K, 1024), (unsigned)(a.chunks - 1)), dim3(256), 0, st, a);
