@@ -1141,15 +1141,23 @@ int small_launch(const char* me, const FwdArgs& a, hipStream_t st) {
 template <class T, bool W_KM>
 int forward_pick(const char* me, const FwdArgs& a, hipStream_t st) {
   const int64_t tiles = (a.gr.M / 128 + a.gr.G) * dh::ceil_div(a.N, 128);  // of 128 x 128
-  // few rows per group, or too few tiles to occupy half of the CUs
-  if (a.gr.M <= (int64_t)48 * a.gr.G || tiles <= CUS / 2) return small_launch<T, W_KM>(me, a, st);
   constexpr int VEC = 16 / sizeof(T);
-  if (dma_rows(a.X, a.ldx, VEC) && dma_rows(a.W, a.ldw, VEC) && a.stride_w % VEC == 0 && a.K % VEC == 0 && (!W_KM || a.N % VEC == 0)) {
+  constexpr bool BF16 = sizeof(T) == 2;
+  const bool dma = dma_rows(a.X, a.ldx, VEC) && dma_rows(a.W, a.ldw, VEC) && a.stride_w % VEC == 0 && a.K % VEC == 0 && (!W_KM || a.N % VEC == 0);
+  // A handful of tiles (bf16 1000 x 400 -> 200, 18 tiles: 5.9 us against 12.4 of the DMA tile; 3000 x 512 -> 512, 100 tiles: 24.6 against
+  // 14.7; fp32 the same shapes: 8.7 against 15.5 and 44 against 27; 1000 x 2000 -> 512, 32 tiles: 61 against 49), or few rows per group: fp32
+  // 4000 rows of 100 types, 2000 -> 512: 302 us against 383.  (bf16 the same: 148 against 107: there the DMA tile stays ahead.)
+  if (tiles <= (BF16 ? 64 : 24) || (a.gr.M <= (int64_t)48 * a.gr.G && !(BF16 && dma))) return small_launch<T, W_KM>(me, a, st);
+  if (dma) {
     if constexpr (sizeof(T) == 2) {
-      if (a.gr.M >= (int64_t)1024 * a.gr.G) return forward_dma_launch<DmaTile<T, false, W_KM, 4, 2, 2, 4>>(me, a, st);
+      // three rounds of 256 x 256 tiles: 200003 x 400 -> 200 (791 tiles) 90 us against 96 of the 128 x 128 one, which has two workgroups on a CU
+      // to fill each other's gaps and half the waste at ragged ends: 50000 x 1000 -> 304 (402 tiles) 64 against 70, 8000 x 2000 -> 512 37
+      // against 53
+      if (a.N > 128 && (a.gr.M / 256 + a.gr.G) * dh::ceil_div(a.N, 256) >= 3 * CUS) return forward_dma_launch<DmaTile<T, false, W_KM, 4, 2, 2, 4>>(me, a, st);
     } else {
-      // fp32: below four rounds of workgroups the last, partly filled one costs more than the smaller tile's extra operand traffic
-      if (tiles < 4 * CUS) return forward_dma_launch<DmaTile<T, false, W_KM, 1, 1, 2, 2>>(me, a, st);
+      // fp32 with less than a round of workgroups: 64 x 64 (20011 x 512 -> 256, 336 tiles of 128: 68 / 67 us against 78 / 65; 60000 x 400 ->
+      // 200, 996 tiles: 141 against 128)
+      if (tiles < 2 * CUS) return forward_dma_launch<DmaTile<T, false, W_KM, 1, 1, 2, 2>>(me, a, st);
     }
     return forward_dma_launch<DmaTile<T, false, W_KM, 2, 2, 2, 2>>(me, a, st);
   }
@@ -1172,7 +1180,7 @@ WgradPlan wgrad_plan(int64_t M, int64_t N, int64_t K, int dtype) {
     int64_t rows = dh::ceil_div(dh::ceil_div(M, chunks), 32) * 32;
     if (rows < 32) rows = 32;
     p = {edge, rows};
-    if (rows >= 1024) break;
+    if (rows >= 4096) break;  // (1563 rows a chunk: 50000 x 1000 -> 304 76 us with the 256 tile, 62 with 128)
   }
   return p;
 }
