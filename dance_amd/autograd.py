@@ -705,12 +705,13 @@ class _GroupedLinearFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, group_ptr, bias, relu):
-        x = _rows(x)
-        w = weight.detach()
+        x, w, b = _rows(x), weight, bias
         if x.dtype == torch.bfloat16 and w.dtype == torch.float32:
             w = w.to(torch.bfloat16)
-        w = w if w.dim() == 3 and (w.numel() == 0 or w.stride(-1) == 1) else w.contiguous()
-        b = None if bias is None else bias.detach().float().contiguous()
+        if w.dim() == 3 and w.stride(2) != 1:
+            w = w.contiguous()
+        if b is not None and (b.dtype != torch.float32 or not b.is_contiguous()):
+            b = b.float().contiguous()
         y = kernels.gemm_grouped(x, w, group_ptr, trans_b=True, bias=b, act=kernels.ACT_RELU if relu else kernels.ACT_NONE)
         ctx.relu, ctx.w_dtype, ctx.b_dtype = relu, weight.dtype, None if bias is None else bias.dtype
         ctx.save_for_backward(x, w, group_ptr, y if relu else None)
@@ -724,20 +725,22 @@ class _GroupedLinearFn(torch.autograd.Function):
         if ctx.relu:
             dy = kernels.relu_backward_bf16(y, dy) if dy.dtype == torch.bfloat16 else kernels.relu_backward(y, dy)
         dx = dw = db = None
-        if ctx.needs_input_grad[0]:
+        need_x, need_w, _, need_b, _ = ctx.needs_input_grad
+        if need_x:
             dx = kernels.gemm_grouped(dy, w, group_ptr, trans_b=False)
-        want_b = ctx.b_dtype is not None and ctx.needs_input_grad[3]
-        if ctx.needs_input_grad[1] or want_b:
+        want_b = ctx.b_dtype is not None and need_b
+        if need_w or want_b:
             dw = kernels.gemm_grouped_wgrad(dy, x, group_ptr, out_dtype=ctx.w_dtype, want_bias=want_b)
             if want_b:
                 dw, db = dw
-                db = db.to(ctx.b_dtype)
-        return dx, dw if ctx.needs_input_grad[1] else None, None, db, None
+                if ctx.b_dtype != torch.float32:
+                    db = db.to(ctx.b_dtype)
+        return dx, dw if need_w else None, None, db, None
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """t itself where its rows are contiguous and do not overlap, else a contiguous copy (expanded and transposed tensors)."""
-    if t.dim() == 2 and (t.numel() == 0 or (t.stride(1) == 1 and (t.shape[0] == 1 or t.stride(0) >= t.shape[1]))):
+    if t.is_contiguous() or (t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= t.shape[1]):
         return t
     return t.contiguous()
 
@@ -768,7 +771,7 @@ class _ResidualNormFn(torch.autograd.Function):
         r, h, stats = kernels.residual_norm_forward(f, x, post=post, gate=gate, gate_sigmoid=gate_sigmoid, scale=scale, pre=pre, kind=kind, eps=eps,
                                                     want_stats=any(ctx.needs_input_grad))
         ctx.opts = opts
-        ctx.save_for_backward(f, x, gate, *params, stats)
+        ctx.save_for_backward(f, x if has_pre else None, gate, *params, stats)  # (without the second norm the backward does not need r)
         return (r, h) if has_pre else r
 
     @staticmethod
@@ -779,11 +782,13 @@ class _ResidualNormFn(torch.autograd.Function):
         names = ("f", "x", "gate", "w1", "b1", "w2", "b2")
         if dr is None and dh is None:
             return (None, ) * 8
-        want = [n for n, need in zip(names, ctx.needs_input_grad) if need]
+        want = [n for n, need in zip(names, ctx.needs_input_grad) if need and (has_pre or n != "x")]
         g = kernels.residual_norm_backward(None if dr is None else _rows(dr), None if dh is None else _rows(dh), f, x, stats,
                                            post=(w1, b1) if has_post else None, gate=gate, gate_sigmoid=gate_sigmoid, scale=scale,
                                            pre=(w2, b2) if has_pre else None, kind=kind, want=want)
-        return tuple(g.get(n) for n in names) + (None, )
+        if not has_pre and ctx.needs_input_grad[1]:
+            g["x"] = dr  # r = x + ...
+        return (*(g.get(n) for n in names), None)
 
 
 def residual_norm(f: torch.Tensor, x: Optional[torch.Tensor] = None, *, post=None, gate: Optional[torch.Tensor] = None, gate_act: str = "none",

@@ -27,7 +27,7 @@ constexpr int64_t MAX_D = 4096;
 constexpr int BWD_BLOCKS = 1024;  // workgroups of a backward launch at most = partial rows of the column gradients
 
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
-typedef uint16_t u16x8u __attribute__((ext_vector_type(8), aligned(2)));
+typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(2)));
 
 struct Args {
   int64_t M;
@@ -50,10 +50,11 @@ struct Args {
 };
 
 __device__ __forceinline__ float bf16_f32(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
-__device__ __forceinline__ uint16_t f32_bf16(float x) {  // nearest even; NaN stays a quiet NaN
-  const uint32_t u = __float_as_uint(x);
-  if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)((u >> 16) | 0x40u);
-  return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
+// two values rounded to bf16 (v_cvt_pk_bf16_f32: nearest even, a NaN stays one)
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
 }
 
 template <class T>
@@ -89,13 +90,16 @@ template <>
 struct Elem<uint16_t> {
   static constexpr int VEC = 8;
   static __device__ __forceinline__ float get(const void* p, int64_t i) { return bf16_f32(static_cast<const uint16_t*>(p)[i]); }
-  static __device__ __forceinline__ void put(void* p, int64_t i, float v) { static_cast<uint16_t*>(p)[i] = f32_bf16(v); }
+  static __device__ __forceinline__ void put(void* p, int64_t i, float v) { static_cast<uint16_t*>(p)[i] = (uint16_t)pack_bf16(v, 0.f); }
   template <int V>
   static __device__ __forceinline__ void load(const void* p, int64_t i, float* v) {
     if (V == 8) {
-      const u16x8u t = *reinterpret_cast<const u16x8u*>(static_cast<const uint16_t*>(p) + i);
+      const u32x4u t = *reinterpret_cast<const u32x4u*>(static_cast<const uint16_t*>(p) + i);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = bf16_f32(t[e]);
+      for (int e = 0; e < 4; ++e) {
+        v[2 * e] = __uint_as_float(t[e] << 16);
+        v[2 * e + 1] = __uint_as_float(t[e] & 0xffff0000u);
+      }
     } else {
       v[0] = get(p, i);
     }
@@ -103,10 +107,10 @@ struct Elem<uint16_t> {
   template <int V>
   static __device__ __forceinline__ void store(void* p, int64_t i, const float* v) {
     if (V == 8) {
-      u16x8u t;
+      u32x4u t;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) t[e] = f32_bf16(v[e]);
-      *reinterpret_cast<u16x8u*>(static_cast<uint16_t*>(p) + i) = t;
+      for (int e = 0; e < 4; ++e) t[e] = pack_bf16(v[2 * e], v[2 * e + 1]);
+      *reinterpret_cast<u32x4u*>(static_cast<uint16_t*>(p) + i) = t;
     } else {
       put(p, i, v[0]);
     }
@@ -506,43 +510,55 @@ Split split_of(int64_t D, int vec_width) {
   return s;
 }
 
-int64_t blocks_of(const Split& s, int64_t M, int64_t most) {
-  const int64_t per = s.block ? 1 : 256 / s.tpr, need = dh::ceil_div(M, per);
-  return need < most ? need : most;
+int64_t rows_per_block(const Split& s) { return s.block ? 1 : 256 / s.tpr; }
+
+// Workgroups of a launch: what the chip holds at a time, so that no second, partly filled round follows (1024 workgroups where 768 fit took
+// 534 us instead of 400 at 200003 x 512 bf16), and the rows shared out evenly among them.
+int64_t even_grid(int64_t M, int64_t per_block, int64_t resident) {
+  const int64_t need = dh::ceil_div(M, per_block);
+  return need <= resident ? need : dh::ceil_div(need, dh::ceil_div(need, resident));
 }
 
 template <class T, int V, int CH, bool BLOCK, bool FULL, bool ODD>
-void launch(bool backward, const Args& a, int64_t grid, hipStream_t st) {
-  const dim3 g((unsigned)grid), b(BLOCK ? a.tpr : 256);
+int64_t launch(bool backward, const Args& a, const Split& s, hipStream_t st) {
+  const dim3 b(BLOCK ? a.tpr : 256);
+  const void* kernel = backward ? reinterpret_cast<const void*>(residual_norm_backward_kernel<T, V, CH, BLOCK, FULL, ODD>)
+                                : reinterpret_cast<const void*>(residual_norm_forward_kernel<T, V, CH, BLOCK, FULL, ODD>);
+  // (a row of 257 .. 512 threads is asked for separately: static per direction and width)
+  static int per_cu[2][2] = {{0, 0}, {0, 0}};
+  int& fit = per_cu[backward][b.x > 256];
+  if (fit == 0 && (hipOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kernel, (int)b.x, 0) != hipSuccess || fit < 1)) fit = 2;
+  int64_t resident = (int64_t)256 * fit;
+  if (backward && resident > BWD_BLOCKS) resident = BWD_BLOCKS;
+  const int64_t grid = even_grid(a.M, rows_per_block(s), resident);
+  const dim3 g((unsigned)grid);
   if (backward) hipLaunchKernelGGL((residual_norm_backward_kernel<T, V, CH, BLOCK, FULL, ODD>), g, b, 0, st, a);
   else hipLaunchKernelGGL((residual_norm_forward_kernel<T, V, CH, BLOCK, FULL, ODD>), g, b, 0, st, a);
+  return grid;
 }
 
 template <class T, int V, int CH, bool BLOCK>
-void launch_gate(bool backward, const Args& a, const Split& s, int64_t grid, hipStream_t st) {
+int64_t launch_gate(bool backward, const Args& a, const Split& s, hipStream_t st) {
   const bool full = a.gate_kind == GATE_FULL;
   if constexpr (V == 1) {
-    if (full) launch<T, V, CH, BLOCK, true, false>(backward, a, grid, st);
-    else launch<T, V, CH, BLOCK, false, false>(backward, a, grid, st);
+    return full ? launch<T, V, CH, BLOCK, true, false>(backward, a, s, st) : launch<T, V, CH, BLOCK, false, false>(backward, a, s, st);
   } else if (s.odd) {
-    if (full) launch<T, V, CH, BLOCK, true, true>(backward, a, grid, st);
-    else launch<T, V, CH, BLOCK, false, true>(backward, a, grid, st);
+    return full ? launch<T, V, CH, BLOCK, true, true>(backward, a, s, st) : launch<T, V, CH, BLOCK, false, true>(backward, a, s, st);
   } else {
-    if (full) launch<T, V, CH, BLOCK, true, false>(backward, a, grid, st);
-    else launch<T, V, CH, BLOCK, false, false>(backward, a, grid, st);
+    return full ? launch<T, V, CH, BLOCK, true, false>(backward, a, s, st) : launch<T, V, CH, BLOCK, false, false>(backward, a, s, st);
   }
 }
 
+// returns the number of workgroups
 template <class T>
-void launch_t(bool backward, const Args& a, const Split& s, int64_t grid, hipStream_t st) {
+int64_t launch_t(bool backward, const Args& a, const Split& s, hipStream_t st) {
   constexpr int V = Elem<T>::VEC, EIGHT = 8 / V;
-  if (s.v == 1) return launch_gate<T, 1, 1, false>(backward, a, s, grid, st);
-  if (!s.block) {
-    if (s.ch == 1) return launch_gate<T, V, 1, false>(backward, a, s, grid, st);
-    if constexpr (EIGHT == 2) launch_gate<T, V, 2, false>(backward, a, s, grid, st);
-    return;
+  if (s.v == 1) return launch_gate<T, 1, 1, false>(backward, a, s, st);
+  if (s.block) return launch_gate<T, V, EIGHT, true>(backward, a, s, st);
+  if constexpr (EIGHT == 2) {
+    if (s.ch == 2) return launch_gate<T, V, 2, false>(backward, a, s, st);
   }
-  launch_gate<T, V, EIGHT, true>(backward, a, s, grid, st);
+  return launch_gate<T, V, 1, false>(backward, a, s, st);
 }
 
 int check_common(const char* me, int64_t M, int64_t D, int dtype, const void* f, const void* x, int64_t ldf, int64_t ldx, const void* gate,
@@ -581,9 +597,8 @@ extern "C" int dh_residual_norm_forward(int64_t M, int64_t D, int dtype, const v
   const int vw = dtype == DH_DTYPE_BF16 ? 8 : 4;
   const Split s = split_of(D, vw);
   a.tpr = s.tpr;
-  const int64_t grid = blocks_of(s, M, 4096);
-  if (dtype == DH_DTYPE_BF16) launch_t<uint16_t>(false, a, s, grid, dh::as_stream(stream));
-  else launch_t<float>(false, a, s, grid, dh::as_stream(stream));
+  if (dtype == DH_DTYPE_BF16) launch_t<uint16_t>(false, a, s, dh::as_stream(stream));
+  else launch_t<float>(false, a, s, dh::as_stream(stream));
   return dh::check_launch(me);
 }
 
@@ -633,9 +648,7 @@ extern "C" int dh_residual_norm_backward(int64_t M, int64_t D, int dtype, const 
   const int vw = dtype == DH_DTYPE_BF16 ? 8 : 4;
   const Split s = split_of(D, vw);
   a.tpr = s.tpr;
-  const int64_t grid = blocks_of(s, M, BWD_BLOCKS);
-  if (dtype == DH_DTYPE_BF16) launch_t<uint16_t>(true, a, s, grid, st);
-  else launch_t<float>(true, a, s, grid, st);
+  const int64_t grid = dtype == DH_DTYPE_BF16 ? launch_t<uint16_t>(true, a, s, st) : launch_t<float>(true, a, s, st);
   ReduceArgs ra{};
   ra.partials = a.partials; ra.n_blocks = (int)grid; ra.D = (int)D;
   int slots = 0;

@@ -91,14 +91,13 @@ def _one_device(*tensors: Optional[torch.Tensor]):
     more than one device are refused."""
     index = None
     for t in tensors:
-        if t is None or not t.is_cuda:  # (host tensors are refused by name where they are used)
-            continue
-        i = t.get_device()
-        if index is None:
-            index = i
-        elif i != index:
-            raise ValueError(f"tensors on more than one device: cuda:{index} and cuda:{i}")
-    if index is None or index == torch._C._cuda_getDevice():
+        if t is not None:
+            i = t.get_device()
+            if index is None:
+                index = i
+            elif i != index:
+                raise ValueError(f"tensors on more than one device: {index} and {i}")
+    if index is None or index < 0 or index == torch._C._cuda_getDevice():  # (host tensors are refused by name where they are used)
         return _HERE
     return torch.cuda.device(index)
 
@@ -741,15 +740,30 @@ def _mat(t: Optional[torch.Tensor], dtype, name: str):
     return t.data_ptr(), ld
 
 
-def _weight_strides(W: torch.Tensor, name: str):
-    """(row stride, group stride) of a [G, rows, cols] weight stack, rows contiguous."""
-    if W.dim() != 3:
-        raise ValueError(f"{name} must be 3-d [groups, rows, columns], got shape {tuple(W.shape)}")
-    ldw = W.stride(1) if W.shape[1] > 1 else max(W.shape[2], 1)
-    sw = W.stride(0) if W.shape[0] > 1 else 0
-    if W.numel() and (ldw < W.shape[2] or sw < 0):
-        raise ValueError(f"{name}: strides {W.stride()} of shape {tuple(W.shape)} are not supported")
-    return ldw, sw
+def _stack(W: torch.Tensor, dtype, name: str):
+    """(address, row stride, group stride, shape) of a [G, rows, cols] stack of matrices with contiguous rows."""
+    if not W.is_cuda:
+        raise _lib.DanceHipError(f"{name} must be a GPU tensor (got {W.device}); dance_amd has no CPU path")
+    if W.dtype is not dtype:
+        raise TypeError(f"{name} must be {dtype}, got {W.dtype}")
+    shape = W.shape
+    if len(shape) != 3:
+        raise ValueError(f"{name} must be 3-d [groups, rows, columns], got shape {tuple(shape)}")
+    groups, rows, cols = shape
+    sw, ldw, step = W.stride()
+    if rows <= 1:
+        ldw = cols or 1
+    if groups <= 1:
+        sw = 0
+    if groups and rows and cols and (step != 1 or ldw < cols or sw < 0):
+        raise ValueError(f"{name}: strides {W.stride()} of shape {tuple(shape)} are not supported")
+    return W.data_ptr(), ldw, sw, shape
+
+
+def _bounds(group_ptr: torch.Tensor, groups: int) -> int:
+    if group_ptr.dim() != 1 or (groups >= 0 and group_ptr.numel() != groups + 1) or group_ptr.numel() < 1:
+        raise ValueError(f"group_ptr must hold one bound more than there are groups{'' if groups < 0 else f' ({groups})'}, got shape {tuple(group_ptr.shape)}")
+    return _dev(group_ptr, torch.int32, "group_ptr", 1)
 
 
 def gemm_grouped(X: torch.Tensor, W: torch.Tensor, group_ptr: torch.Tensor, *, trans_b: bool = True, bias: Optional[torch.Tensor] = None,
@@ -760,53 +774,59 @@ def gemm_grouped(X: torch.Tensor, W: torch.Tensor, group_ptr: torch.Tensor, *, t
     ``group_ptr`` int32 [G + 1] on the device, non-decreasing; bias fp32 [G, N].  Groups may be empty, sizes are not read by the host (no
     synchronisation, capturable).  Rows that belong to no group are zero in a fresh result and left as they are in ``out``."""
     lib = _lib_ready()
+    xt = X.dtype
     dt = _elem(X, "X")
-    if X.dim() != 2:
-        raise ValueError(f"X must be 2-d, got shape {tuple(X.shape)}")
-    ldw, sw = _weight_strides(W, "W")
+    xp, ldx = _mat(X, xt, "X")
+    wp, ldw, sw, (G, N, Kw) = _stack(W, xt, "W")
+    if not trans_b:
+        N, Kw = Kw, N
     M, K = X.shape
-    G, N, Kw = (W.shape[0], W.shape[1], W.shape[2]) if trans_b else (W.shape[0], W.shape[2], W.shape[1])
     if K != Kw:
         raise ValueError(f"gemm_grouped: inner dimensions differ ({K} vs {Kw})")
-    if group_ptr.dim() != 1 or group_ptr.numel() != G + 1:
-        raise ValueError(f"group_ptr must hold {G + 1} bounds for {G} groups, got shape {tuple(group_ptr.shape)}")
-    if bias is not None and tuple(bias.shape) != (G, N):
+    gp = _bounds(group_ptr, G)
+    bp, ldb = _mat(bias, torch.float32, "bias")
+    if bias is not None and bias.shape != (G, N):
         raise ValueError(f"bias must be [{G}, {N}], got shape {tuple(bias.shape)}")
-    if act not in (ACT_NONE, ACT_RELU):
+    if act != ACT_NONE and act != ACT_RELU:
         raise ValueError(f"gemm_grouped: unknown activation {act}")
-    fresh = out is None
-    if fresh:
-        out = torch.empty((M, N), dtype=out_dtype or X.dtype, device=X.device)
-    elif tuple(out.shape) != (M, N) or (out_dtype is not None and out.dtype != out_dtype):
-        raise ValueError(f"out must be [{M}, {N}]{'' if out_dtype is None else f' of {out_dtype}'}, got {tuple(out.shape)} of {out.dtype}")
+    if out is None:
+        yt = out_dtype or xt
+        y = X.new_empty((M, N)) if yt is xt else torch.empty((M, N), dtype=yt, device=X.device)
+        yp, ldy = y.data_ptr(), N or 1
+    else:
+        y, yt = out, out.dtype
+        if out.shape != (M, N) or (out_dtype is not None and yt != out_dtype):
+            raise ValueError(f"out must be [{M}, {N}]{'' if out_dtype is None else f' of {out_dtype}'}, got {tuple(out.shape)} of {out.dtype}")
+        yp, ldy = _mat(out, yt, "out")
     with _one_device(X, W, group_ptr, bias, out):
-        _call(_GROUPED_TAGS[dt][bool(trans_b)], lib.dh_gemm_grouped, M, N, K, G, 1 if trans_b else 0, dt, *_mat(X, X.dtype, "X"),
-              _dev(W, X.dtype, "W", 3), ldw, sw, _dev(group_ptr, torch.int32, "group_ptr", 1), *_mat(bias, torch.float32, "bias"), act,
-              *_mat(out, out.dtype, "out"), _elem(out, "out"), 1 if fresh else 0, _stream())
-    return out
+        _call(_GROUPED_TAGS[dt][bool(trans_b)], lib.dh_gemm_grouped, M, N, K, G, 1 if trans_b else 0, dt, xp, ldx, wp, ldw, sw, gp, bp, ldb, act, yp, ldy,
+              _elem(y, "out"), 1 if out is None else 0, _stream())
+    return y
 
 
 def gemm_grouped_wgrad(dY: torch.Tensor, X: torch.Tensor, group_ptr: torch.Tensor, *, out_dtype=None, want_bias: bool = False):
     """dW[g] = dY_g^T @ X_g ([G, N, K]) over each group's rows and, with ``want_bias``, (dW, db) with db[g] = the column sums of dY_g (fp32
     [G, N]); zero for an empty group.  See dh_gemm_grouped_wgrad.  The rows of a group are summed in a fixed order."""
     lib = _lib_ready()
+    xt = X.dtype
     dt = _elem(X, "X")
-    if X.dim() != 2 or dY.dim() != 2 or X.shape[0] != dY.shape[0]:
-        raise ValueError(f"dY and X must be 2-d with the same rows, got shapes {tuple(dY.shape)} and {tuple(X.shape)}")
-    if group_ptr.dim() != 1 or group_ptr.numel() < 1:
-        raise ValueError(f"group_ptr must be 1-d with at least one bound, got shape {tuple(group_ptr.shape)}")
+    xp, ldx = _mat(X, xt, "X")
+    yp, ldy = _mat(dY, xt, "dY")
+    gp = _bounds(group_ptr, -1)
     M, K = X.shape
-    N, G = dY.shape[1], group_ptr.numel() - 1
-    dW = torch.empty((G, N, K), dtype=out_dtype or X.dtype, device=X.device)
-    db = torch.empty((G, N), dtype=torch.float32, device=X.device) if want_bias else None
+    My, N = dY.shape
+    G = group_ptr.numel() - 1
+    if M != My:
+        raise ValueError(f"dY and X must have the same rows, got shapes {tuple(dY.shape)} and {tuple(X.shape)}")
     if K == 0 and want_bias:
         raise ValueError("gemm_grouped_wgrad: the bias gradient needs at least one input column")
+    dW = X.new_empty((G, N, K)) if out_dtype is None or out_dtype is xt else torch.empty((G, N, K), dtype=out_dtype, device=X.device)
+    db = torch.empty((G, N), dtype=torch.float32, device=X.device) if want_bias else None
     with _one_device(dY, X, group_ptr):
         ws_bytes = lib.dh_gemm_grouped_wgrad_workspace_bytes(M, N, K, dt)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=X.device)
-        _call("gemm_grouped_bf16_tn" if dt else "gemm_grouped_f32_tn", lib.dh_gemm_grouped_wgrad, M, N, K, G, dt, *_mat(dY, X.dtype, "dY"),
-              *_mat(X, X.dtype, "X"), _dev(group_ptr, torch.int32, "group_ptr", 1), dW.data_ptr(), max(K, 1), N * K,
-              _elem(dW, "dW"), None if db is None else db.data_ptr(), max(N, 1), ws.data_ptr(), ws_bytes, _stream())
+        _call("gemm_grouped_bf16_tn" if dt else "gemm_grouped_f32_tn", lib.dh_gemm_grouped_wgrad, M, N, K, G, dt, yp, ldy, xp, ldx, gp, dW.data_ptr(),
+              K or 1, N * K, _elem(dW, "dW"), None if db is None else db.data_ptr(), N or 1, ws.data_ptr(), ws_bytes, _stream())
     return (dW, db) if want_bias else dW
 
 
@@ -821,7 +841,7 @@ def residual_norm_gate_kind(gate: Optional[torch.Tensor], M: int, D: int) -> int
     if gate is None:
         return GATE_NONE
     shape = tuple(gate.shape)
-    if shape in ((), (1, )):
+    if shape == () or shape == (1, ):
         return GATE_SCALAR
     if shape == (D, ):
         return GATE_CHANNEL
@@ -837,10 +857,10 @@ def _norm_params(p, D: int, name: str):
     if p is None:
         return 0, None, None
     w, b = p
-    for t, what in ((w, "weight"), (b, "bias")):
-        if t is not None and tuple(t.shape) != (D, ):
-            raise ValueError(f"{name} {what} must be [{D}], got shape {tuple(t.shape)}")
-    return 1, _dev(w, torch.float32, f"{name} weight", 1), _dev(b, torch.float32, f"{name} bias", 1)
+    for t in (w, b):
+        if t is not None and t.shape != (D, ):
+            raise ValueError(f"{name} weight and bias must be [{D}], got shape {tuple(t.shape)}")
+    return 1, _dev(w, torch.float32, name, 1), _dev(b, torch.float32, name, 1)
 
 
 def _gate_args(gate, kind: int, dtype):
