@@ -18,12 +18,17 @@
 // no load is guarded.  The two-pass variance and both reductions of the backward run on registers.  Column gradients are summed in
 // registers over the rows a workgroup walks, joined in its LDS, written once per workgroup and added up by a second kernel in workgroup
 // order: no atomics, the result does not depend on timing.  All arithmetic is fp32; bf16 rounds once, at the stores.
+#include <type_traits>
+
 #include "common.h"
 
 namespace {
 
 enum { GATE_NONE = DH_GATE_NONE, GATE_SCALAR = DH_GATE_SCALAR, GATE_CHANNEL = DH_GATE_CHANNEL, GATE_ROW = DH_GATE_ROW, GATE_FULL = DH_GATE_FULL };
 constexpr int64_t MAX_D = 4096;
+// who holds a row: part of a wave, a wave, a workgroup;  how the row ends: with the lanes' last access, with an access before, inside one
+enum { SUB = 0, WAVE = 1, GROUP = 2 };
+enum { WHOLE = 0, SHORT = 1, ODD = 2 };
 constexpr int BWD_BLOCKS = 1024;  // workgroups of a backward launch at most = partial rows of the column gradients
 
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
@@ -112,14 +117,33 @@ __device__ __forceinline__ void load_param(const float* p, int col, float* v) {
 
 __device__ __forceinline__ float sigmoid(float v) { return 1.f / (1.f + expf(-v)); }
 
-// N sums over the tpr threads of a row, the result in each of them.  BLOCK: the row is the whole workgroup.
-template <bool BLOCK, int N>
+// the sum over a wave in every lane, by DPP adds: 6 instructions where a butterfly through LDS takes 18 and its latencies
+__device__ __forceinline__ float wave_sum(float v) {
+  auto add = [&](auto ctrl, auto rows) __attribute__((always_inline)) {
+    v += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), decltype(ctrl)::value, decltype(rows)::value, 0xf, false));
+  };
+  add(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xf>{});  // row_shr 1, 2, 4, 8: lane 15 of a row of 16 has its sum
+  add(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xf>{});
+  add(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xf>{});
+  add(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xf>{});
+  add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});  // row_bcast 15 into rows 1 and 3
+  add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});  // row_bcast 31 into rows 2 and 3
+  return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), 63));
+}
+
+// N sums over the threads of a row, the result in each of them
+template <int MODE, int N>
 __device__ __forceinline__ void row_sums(float (&v)[N], int tpr, float* lds) {
-  for (int o = (BLOCK ? 32 : tpr >> 1); o > 0; o >>= 1) {
+  if (MODE == SUB) {
+    for (int o = tpr >> 1; o > 0; o >>= 1) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], o);
+      for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], o);
+    }
+    return;
   }
-  if (BLOCK) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = wave_sum(v[i]);
+  if (MODE == GROUP) {
     const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
     __syncthreads();  // the previous reduction's values have been read
     if ((threadIdx.x & 63) == 0) {
@@ -165,7 +189,7 @@ struct RawRow {
       }
     }
   }
-  template <bool ODD>
+  template <int TAIL>
   __device__ __forceinline__ void unpack(int t, int tpr, int D, float (&v)[V * CH]) const {
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
@@ -179,38 +203,39 @@ struct RawRow {
 #pragma unroll
         for (int e = 0; e < WORDS; ++e) v[c * V + e] = __uint_as_float(w[c][e]);
       }
-      if (ODD) shift_down<V>(max((c * tpr + t) * V - (D - V), 0), v + c * V);
+      if (TAIL == ODD) shift_down<V>(max((c * tpr + t) * V - (D - V), 0), v + c * V);
     }
   }
 };
-template <int V, int CH, bool ODD>
+template <int V, int CH, int TAIL>
 __device__ __forceinline__ void zero_tail(int t, int tpr, int D, float (&v)[V * CH]) {
+  if (TAIL == WHOLE) return;
 #pragma unroll
   for (int c = 0; c < CH; ++c)
 #pragma unroll
     for (int e = 0; e < V; ++e)
-      if ((c * tpr + t) * V + (ODD ? e : 0) >= D) v[c * V + e] = 0.f;
+      if ((c * tpr + t) * V + (TAIL == ODD ? e : 0) >= D) v[c * V + e] = 0.f;
 }
-template <int V, int CH, bool ODD>
+template <int V, int CH, int TAIL>
 __device__ __forceinline__ void load_params(const float* p, float fallback, int t, int tpr, int D, float (&v)[V * CH]) {
   if (p) {
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       load_param<V>(p, min((c * tpr + t) * V, D - V), v + c * V);
-      if (ODD) shift_down<V>(max((c * tpr + t) * V - (D - V), 0), v + c * V);
+      if (TAIL == ODD) shift_down<V>(max((c * tpr + t) * V - (D - V), 0), v + c * V);
     }
   } else {
 #pragma unroll
     for (int i = 0; i < V * CH; ++i) v[i] = fallback;
   }
 }
-template <class T, int V, int CH, bool ODD>
+template <class T, int V, int CH, int TAIL>
 __device__ __forceinline__ void store_row(void* p, int64_t row_at, int t, int tpr, int D, const float (&v)[V * CH]) {
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
     const int col = (c * tpr + t) * V;
-    if (ODD ? col + V <= D : col < D) Elem<T>::template store<V>(p, row_at + col, v + c * V);
-    else if (ODD && col < D) {
+    if (TAIL == WHOLE || (TAIL == ODD ? col + V <= D : col < D)) Elem<T>::template store<V>(p, row_at + col, v + c * V);
+    else if (TAIL == ODD && col < D) {
 #pragma unroll
       for (int e = 0; e < V; ++e)
         if (col + e < D) Elem<T>::put(p, row_at + col + e, v[c * V + e]);
@@ -219,14 +244,14 @@ __device__ __forceinline__ void store_row(void* p, int64_t row_at, int t, int tp
 }
 
 // mean and rstd of a row held in registers (entries beyond D are zero)
-template <bool BLOCK, int V, int CH, bool ODD>
+template <int MODE, int V, int CH, int TAIL>
 __device__ __forceinline__ void row_stats(const Args& a, int t, const float (&v)[V * CH], float* lds, float& mean, float& rstd) {
   float s[1] = {0.f};
   mean = 0.f;
   if (!a.rms) {
 #pragma unroll
     for (int i = 0; i < V * CH; ++i) s[0] += v[i];
-    row_sums<BLOCK, 1>(s, a.tpr, lds);
+    row_sums<MODE, 1>(s, a.tpr, lds);
     mean = s[0] * a.inv_d;
     s[0] = 0.f;
   }
@@ -234,22 +259,32 @@ __device__ __forceinline__ void row_stats(const Args& a, int t, const float (&v)
   for (int c = 0; c < CH; ++c)
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      const float d = (c * a.tpr + t) * V + (ODD ? e : 0) < a.D ? v[c * V + e] - mean : 0.f;
+      const float d = TAIL == WHOLE || (c * a.tpr + t) * V + (TAIL == ODD ? e : 0) < a.D ? v[c * V + e] - mean : 0.f;
       s[0] = __builtin_fmaf(d, d, s[0]);
     }
-  row_sums<BLOCK, 1>(s, a.tpr, lds);
+  row_sums<MODE, 1>(s, a.tpr, lds);
   rstd = 1.f / sqrtf(s[0] * a.inv_d + a.eps);
 }
 
-template <class T, int V, int CH, bool BLOCK, bool FULL, bool ODD>
-__global__ __launch_bounds__(BLOCK ? 512 : 256) void residual_norm_forward_kernel(const Args a) {
+// v = (v - mean) rstd w + b as two fused steps: v rstd - mean rstd, then w, b
+template <int E>
+__device__ __forceinline__ void normalise(float (&v)[E], float mean, float rstd, const float (&w)[E], const float (&b)[E]) {
+  const float shift = -mean * rstd;
+#pragma unroll
+  for (int i = 0; i < E; ++i) v[i] = __builtin_fmaf(__builtin_fmaf(v[i], rstd, shift), w[i], b[i]);
+}
+
+template <class T, int V, int CH, int MODE, bool FULL, int TAIL>
+__global__ __launch_bounds__(MODE == GROUP ? 512 : 256) void residual_norm_forward_kernel(const Args a) {
   constexpr int E = V * CH;
   __shared__ float lds[8];
-  const int tpr = a.tpr, t = BLOCK ? threadIdx.x : threadIdx.x & (tpr - 1);
-  const int rows_per_block = BLOCK ? 1 : 256 / tpr, sub = BLOCK ? 0 : threadIdx.x / tpr;
+  const int tpr = MODE == WAVE ? 64 : a.tpr, t = MODE == GROUP ? threadIdx.x : threadIdx.x & (tpr - 1);
+  const int rows_per_block = MODE == GROUP ? 1 : 256 / tpr;
+  // the row within the workgroup's pass; uniform (a scalar, and with it the rows' addresses) where a wave holds one row
+  const int sub = MODE == GROUP ? 0 : MODE == WAVE ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : threadIdx.x / tpr;
   float ga[E];
   if (!FULL) {
-    if (a.gate_kind == GATE_CHANNEL) load_params<V, CH, ODD>(static_cast<const float*>(a.gate), 1.f, t, tpr, a.D, ga);
+    if (a.gate_kind == GATE_CHANNEL) load_params<V, CH, TAIL>(static_cast<const float*>(a.gate), 1.f, t, tpr, a.D, ga);
     else {
       const float g = a.gate_kind == GATE_SCALAR ? *static_cast<const float*>(a.gate) : 1.f;
 #pragma unroll
@@ -259,6 +294,8 @@ __global__ __launch_bounds__(BLOCK ? 512 : 256) void residual_norm_forward_kerne
 #pragma unroll
       for (int i = 0; i < E; ++i) ga[i] = sigmoid(ga[i]);
     }
+#pragma unroll
+    for (int i = 0; i < E; ++i) ga[i] *= a.scale;
   }
   for (int64_t base = (int64_t)blockIdx.x * rows_per_block; base < a.M; base += (int64_t)gridDim.x * rows_per_block) {
     const int64_t row = min(base + sub, a.M - 1);
@@ -269,49 +306,56 @@ __global__ __launch_bounds__(BLOCK ? 512 : 256) void residual_norm_forward_kerne
     if (a.x) rx.load(a.x, row * a.ldx, t, tpr, a.D);
     if (FULL) rg.load(a.gate, row * a.ldg, t, tpr, a.D);
     else if (a.gate_kind == GATE_ROW) grow = Elem<T>::get(a.gate, row * a.ldg);
-    rf.template unpack<ODD>(t, tpr, a.D, f);
-    if (a.x) rx.template unpack<ODD>(t, tpr, a.D, x);
+    rf.template unpack<TAIL>(t, tpr, a.D, f);
+    if (a.x) rx.template unpack<TAIL>(t, tpr, a.D, x);
     else {
 #pragma unroll
       for (int i = 0; i < E; ++i) x[i] = 0.f;
     }
-    if (FULL) rg.template unpack<ODD>(t, tpr, a.D, gf);
+    if (FULL) rg.template unpack<TAIL>(t, tpr, a.D, gf);
     if (!FULL && a.gate_kind == GATE_ROW && a.gate_sigmoid) grow = sigmoid(grow);
-    zero_tail<V, CH, ODD>(t, tpr, a.D, f);
+    zero_tail<V, CH, TAIL>(t, tpr, a.D, f);
     float m1 = 0.f, s1 = 1.f, m2 = 0.f, s2 = 1.f;
     if (a.has_post) {
-      load_params<V, CH, ODD>(a.w1, 1.f, t, tpr, a.D, w);
-      load_params<V, CH, ODD>(a.b1, 0.f, t, tpr, a.D, b);
-      row_stats<BLOCK, V, CH, ODD>(a, t, f, lds, m1, s1);
-#pragma unroll
-      for (int i = 0; i < E; ++i) f[i] = (f[i] - m1) * s1 * w[i] + b[i];
+      load_params<V, CH, TAIL>(a.w1, 1.f, t, tpr, a.D, w);
+      load_params<V, CH, TAIL>(a.b1, 0.f, t, tpr, a.D, b);
+      row_stats<MODE, V, CH, TAIL>(a, t, f, lds, m1, s1);
+      normalise<E>(f, m1, s1, w, b);
     }
+    if (FULL) {
+      if (a.gate_sigmoid) {
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      float g = FULL ? (a.gate_sigmoid ? sigmoid(gf[i]) : gf[i]) : ga[i];
-      if (!FULL) g *= grow;
-      f[i] = x[i] + a.scale * g * f[i];
+        for (int i = 0; i < E; ++i) gf[i] = sigmoid(gf[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < E; ++i) f[i] = __builtin_fmaf(a.scale * gf[i], f[i], x[i]);
+    } else if (a.gate_kind == GATE_ROW) {
+      const float g = a.scale * grow;
+#pragma unroll
+      for (int i = 0; i < E; ++i) f[i] = __builtin_fmaf(g, f[i], x[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; ++i) f[i] = __builtin_fmaf(ga[i], f[i], x[i]);
     }
-    if (valid && a.r) store_row<T, V, CH, ODD>(a.r, row * a.ldr, t, tpr, a.D, f);
+    if (valid && a.r) store_row<T, V, CH, TAIL>(a.r, row * a.ldr, t, tpr, a.D, f);
     if (a.has_pre) {
-      zero_tail<V, CH, ODD>(t, tpr, a.D, f);
-      load_params<V, CH, ODD>(a.w2, 1.f, t, tpr, a.D, w);
-      load_params<V, CH, ODD>(a.b2, 0.f, t, tpr, a.D, b);
-      row_stats<BLOCK, V, CH, ODD>(a, t, f, lds, m2, s2);
-#pragma unroll
-      for (int i = 0; i < E; ++i) f[i] = (f[i] - m2) * s2 * w[i] + b[i];
-      if (valid) store_row<T, V, CH, ODD>(a.h, row * a.ldh, t, tpr, a.D, f);
+      zero_tail<V, CH, TAIL>(t, tpr, a.D, f);
+      load_params<V, CH, TAIL>(a.w2, 1.f, t, tpr, a.D, w);
+      load_params<V, CH, TAIL>(a.b2, 0.f, t, tpr, a.D, b);
+      row_stats<MODE, V, CH, TAIL>(a, t, f, lds, m2, s2);
+      normalise<E>(f, m2, s2, w, b);
+      if (valid) store_row<T, V, CH, TAIL>(a.h, row * a.ldh, t, tpr, a.D, f);
     }
     if (valid && a.stats && t == 0) *reinterpret_cast<float4*>(a.stats + row * 4) = make_float4(m1, s1, m2, s2);
   }
 }
 
 // the workgroup's column sums of one array: joined over its row groups in LDS, written to partials[slot][blockIdx.x]
-template <int V, int CH, bool BLOCK>
+template <int V, int CH, int MODE>
 __device__ __forceinline__ void put_partials(const Args& a, int t, int sub, const float (&acc)[V * CH], int slot, float* lds) {
-  const int tpr = a.tpr;
+  const int tpr = MODE == WAVE ? 64 : a.tpr;
   float* out = a.partials + ((int64_t)slot * gridDim.x + blockIdx.x) * a.D;
-  if (BLOCK) {
+  if (MODE == GROUP) {
 #pragma unroll
     for (int c = 0; c < CH; ++c)
 #pragma unroll
@@ -335,19 +379,21 @@ __device__ __forceinline__ void put_partials(const Args& a, int t, int sub, cons
   }
 }
 
-template <class T, int V, int CH, bool BLOCK, bool FULL, bool ODD>
-__global__ __launch_bounds__(BLOCK ? 512 : 256) void residual_norm_backward_kernel(const Args a) {
+template <class T, int V, int CH, int MODE, bool FULL, int TAIL>
+__global__ __launch_bounds__(MODE == GROUP ? 512 : 256) void residual_norm_backward_kernel(const Args a) {
   constexpr int E = V * CH;
-  __shared__ float lds[BLOCK ? 32 : 256 * E];
-  const int tpr = a.tpr, t = BLOCK ? threadIdx.x : threadIdx.x & (tpr - 1);
-  const int rows_per_block = BLOCK ? 1 : 256 / tpr, sub = BLOCK ? 0 : threadIdx.x / tpr;
+  __shared__ float lds[MODE == GROUP ? 32 : 256 * E];
+  const int tpr = MODE == WAVE ? 64 : a.tpr, t = MODE == GROUP ? threadIdx.x : threadIdx.x & (tpr - 1);
+  const int rows_per_block = MODE == GROUP ? 1 : 256 / tpr;
+  // the row within the workgroup's pass; uniform (a scalar, and with it the rows' addresses) where a wave holds one row
+  const int sub = MODE == GROUP ? 0 : MODE == WAVE ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : threadIdx.x / tpr;
   float acc_w1[E], acc_b1[E], acc_w2[E], acc_b2[E], acc_g[E];
 #pragma unroll
   for (int i = 0; i < E; ++i) acc_w1[i] = acc_b1[i] = acc_w2[i] = acc_b2[i] = acc_g[i] = 0.f;
   const bool col_gate = !FULL && (a.gate_kind == GATE_CHANNEL || a.gate_kind == GATE_SCALAR);
   // A wave's rows: the next one is requested while the present one is worked on (200003 x 512 bf16: 371 -> 332 us).  Not where a workgroup
   // holds a row: there the registers for it cost a wave per SIMD (4099 x 2000 bf16: 38.6 -> 42.0 us), nor in the forward (193 -> 202).
-  constexpr bool AHEAD = !BLOCK;
+  constexpr bool AHEAD = MODE != GROUP;
   const bool use_x = a.x && a.dh;  // r enters through the second norm only
   RawRow<T, V, CH> rf, rx, rr, rh, rg;
   float4 st_next;
@@ -369,25 +415,25 @@ __global__ __launch_bounds__(BLOCK ? 512 : 256) void residual_norm_backward_kern
     const bool valid = base + sub < a.M;
     float f[E], x[E], gf[E], dr[E], dh[E], w[E], b[E];
     if (!AHEAD) request(base);
-    rf.template unpack<ODD>(t, tpr, a.D, f);
-    if (use_x) rx.template unpack<ODD>(t, tpr, a.D, x);
+    rf.template unpack<TAIL>(t, tpr, a.D, f);
+    if (use_x) rx.template unpack<TAIL>(t, tpr, a.D, x);
     else {
 #pragma unroll
       for (int i = 0; i < E; ++i) x[i] = 0.f;
     }
-    if (a.dr) rr.template unpack<ODD>(t, tpr, a.D, dr);
+    if (a.dr) rr.template unpack<TAIL>(t, tpr, a.D, dr);
     else {
 #pragma unroll
       for (int i = 0; i < E; ++i) dr[i] = 0.f;
     }
-    if (a.dh) rh.template unpack<ODD>(t, tpr, a.D, dh);
-    if (FULL) rg.template unpack<ODD>(t, tpr, a.D, gf);
+    if (a.dh) rh.template unpack<TAIL>(t, tpr, a.D, dh);
+    if (FULL) rg.template unpack<TAIL>(t, tpr, a.D, gf);
     const float4 st = st_next;
     const float grow = grow_next;
     if (AHEAD && base + stride < a.M) request(base + stride);
     // the gate and its derivative's factor
     if (!FULL) {
-      if (a.gate_kind == GATE_CHANNEL) load_params<V, CH, ODD>(static_cast<const float*>(a.gate), 1.f, t, tpr, a.D, gf);
+      if (a.gate_kind == GATE_CHANNEL) load_params<V, CH, TAIL>(static_cast<const float*>(a.gate), 1.f, t, tpr, a.D, gf);
       else {
         const float g = a.gate_kind == GATE_SCALAR ? *static_cast<const float*>(a.gate) : a.gate_kind == GATE_ROW ? grow : 1.f;
 #pragma unroll
@@ -400,23 +446,25 @@ __global__ __launch_bounds__(BLOCK ? 512 : 256) void residual_norm_backward_kern
       for (int i = 0; i < E; ++i) gf[i] = sigmoid(gf[i]);
     }
     if (a.has_post) {
-      load_params<V, CH, ODD>(a.w1, 1.f, t, tpr, a.D, w);
-      load_params<V, CH, ODD>(a.b1, 0.f, t, tpr, a.D, b);
+      load_params<V, CH, TAIL>(a.w1, 1.f, t, tpr, a.D, w);
+      load_params<V, CH, TAIL>(a.b1, 0.f, t, tpr, a.D, b);
+      const float shift = -st.x * st.y;
 #pragma unroll
-      for (int i = 0; i < E; ++i) f[i] = (f[i] - st.x) * st.y;  // fhat from here on
+      for (int i = 0; i < E; ++i) f[i] = __builtin_fmaf(f[i], st.y, shift);  // fhat from here on
     } else {
 #pragma unroll
       for (int i = 0; i < E; ++i) { w[i] = 1.f; b[i] = 0.f; }
     }
     if (a.dh) {
       float w2[E];
-      load_params<V, CH, ODD>(a.w2, 1.f, t, tpr, a.D, w2);
-      zero_tail<V, CH, ODD>(t, tpr, a.D, dh);
+      load_params<V, CH, TAIL>(a.w2, 1.f, t, tpr, a.D, w2);
+      zero_tail<V, CH, TAIL>(t, tpr, a.D, dh);
       float s[2] = {0.f, 0.f};
+      const float shift2 = -st.z * st.w;
 #pragma unroll
       for (int i = 0; i < E; ++i) {
-        const float n = f[i] * w[i] + b[i];
-        x[i] = (x[i] + a.scale * gf[i] * n - st.z) * st.w;  // rhat
+        const float n = __builtin_fmaf(f[i], w[i], b[i]);
+        x[i] = __builtin_fmaf(__builtin_fmaf(a.scale * gf[i], n, x[i]), st.w, shift2);  // rhat
         if (valid) {
           acc_w2[i] = __builtin_fmaf(dh[i], x[i], acc_w2[i]);
           acc_b2[i] += dh[i];
@@ -425,20 +473,20 @@ __global__ __launch_bounds__(BLOCK ? 512 : 256) void residual_norm_backward_kern
         s[0] = __builtin_fmaf(dh[i], x[i], s[0]);
         s[1] += dh[i];
       }
-      row_sums<BLOCK, 2>(s, tpr, lds);
+      row_sums<MODE, 2>(s, tpr, lds);
       const float c1 = s[0] * a.inv_d, c0 = a.rms ? 0.f : s[1] * a.inv_d;
 #pragma unroll
-      for (int i = 0; i < E; ++i) dr[i] += st.w * (dh[i] - c0 - x[i] * c1);
+      for (int i = 0; i < E; ++i) dr[i] = __builtin_fmaf(st.w, __builtin_fmaf(-x[i], c1, dh[i] - c0), dr[i]);
     }
-    if (valid && a.dx) store_row<T, V, CH, ODD>(a.dx, row * a.lddx, t, tpr, a.D, dr);
-    zero_tail<V, CH, ODD>(t, tpr, a.D, dr);
+    if (valid && a.dx) store_row<T, V, CH, TAIL>(a.dx, row * a.lddx, t, tpr, a.D, dr);
+    zero_tail<V, CH, TAIL>(t, tpr, a.D, dr);
     float s[3] = {0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      const float n = f[i] * w[i] + b[i];
-      float dg = a.scale * dr[i] * n;
+      const float n = __builtin_fmaf(f[i], w[i], b[i]), sd = a.scale * dr[i];
+      float dg = sd * n;
       if (sig) dg *= gf[i] * (1.f - gf[i]);
-      const float dn = a.scale * gf[i] * dr[i];
+      const float dn = sd * gf[i];
       if (valid) {
         acc_w1[i] = __builtin_fmaf(dn, f[i], acc_w1[i]);
         acc_b1[i] += dn;
@@ -451,24 +499,24 @@ __global__ __launch_bounds__(BLOCK ? 512 : 256) void residual_norm_backward_kern
       gf[i] = dg;
       dr[i] = u;
     }
-    if (FULL && valid && a.dgate) store_row<T, V, CH, ODD>(a.dgate, row * a.lddg, t, tpr, a.D, gf);
-    if (a.has_post || (a.gate_kind == GATE_ROW && a.dgate)) row_sums<BLOCK, 3>(s, tpr, lds);
+    if (FULL && valid && a.dgate) store_row<T, V, CH, TAIL>(a.dgate, row * a.lddg, t, tpr, a.D, gf);
+    if (a.has_post || (a.gate_kind == GATE_ROW && a.dgate)) row_sums<MODE, 3>(s, tpr, lds);
     if (a.gate_kind == GATE_ROW && a.dgate && valid && t == 0) Elem<T>::put(a.dgate, row * a.lddg, s[2]);
     if (a.df && valid) {
       if (a.has_post) {
         const float c1 = s[0] * a.inv_d, c0 = a.rms ? 0.f : s[1] * a.inv_d;
 #pragma unroll
-        for (int i = 0; i < E; ++i) dr[i] = st.y * (dr[i] - c0 - f[i] * c1);
+        for (int i = 0; i < E; ++i) dr[i] = st.y * __builtin_fmaf(-f[i], c1, dr[i] - c0);
       }
-      store_row<T, V, CH, ODD>(a.df, row * a.lddf, t, tpr, a.D, dr);
+      store_row<T, V, CH, TAIL>(a.df, row * a.lddf, t, tpr, a.D, dr);
     }
   }
   int slot = 0;
-  if (a.want_w1) put_partials<V, CH, BLOCK>(a, t, sub, acc_w1, slot++, lds);
-  if (a.want_b1) put_partials<V, CH, BLOCK>(a, t, sub, acc_b1, slot++, lds);
-  if (a.want_w2) put_partials<V, CH, BLOCK>(a, t, sub, acc_w2, slot++, lds);
-  if (a.want_b2) put_partials<V, CH, BLOCK>(a, t, sub, acc_b2, slot++, lds);
-  if (a.want_gate) put_partials<V, CH, BLOCK>(a, t, sub, acc_g, slot++, lds);
+  if (a.want_w1) put_partials<V, CH, MODE>(a, t, sub, acc_w1, slot++, lds);
+  if (a.want_b1) put_partials<V, CH, MODE>(a, t, sub, acc_b1, slot++, lds);
+  if (a.want_w2) put_partials<V, CH, MODE>(a, t, sub, acc_w2, slot++, lds);
+  if (a.want_b2) put_partials<V, CH, MODE>(a, t, sub, acc_b2, slot++, lds);
+  if (a.want_gate) put_partials<V, CH, MODE>(a, t, sub, acc_g, slot++, lds);
 }
 
 struct ReduceArgs {
@@ -518,28 +566,30 @@ __global__ __launch_bounds__(256) void sum_kernel(const float* __restrict__ v, i
 // lanes as the row has accesses up to a wave, then up to 8 elements per lane, then a workgroup of 256 or 512 threads per row.
 struct Split {
   int v, ch, tpr;
-  bool block, odd;
+  int mode, tail;
 };
 
 Split split_of(int64_t D, int vec_width) {
   Split s;
   s.v = D >= vec_width ? vec_width : 1;
-  s.odd = D % s.v != 0;
   const int64_t n = dh::ceil_div(D, s.v);
   const int64_t eight = 8 / s.v;  // accesses that hold eight elements
-  s.block = n > 64 * eight;
-  if (s.block) {
+  if (n > 64 * eight) {
+    s.mode = GROUP;
     s.tpr = n <= 256 * eight ? 256 : 512;
   } else {
     s.tpr = 8;
     while (s.tpr < 64 && s.tpr < n) s.tpr *= 2;
+    s.mode = s.tpr == 64 ? WAVE : SUB;
   }
   s.ch = 1;
   while ((int64_t)s.ch * s.tpr < n) s.ch *= 2;
+  if (s.mode == GROUP) s.ch = (int)eight;
+  s.tail = D % s.v != 0 ? ODD : (int64_t)s.tpr * s.ch == n ? WHOLE : SHORT;
   return s;
 }
 
-int64_t rows_per_block(const Split& s) { return s.block ? 1 : 256 / s.tpr; }
+int64_t rows_per_block(const Split& s) { return s.mode == GROUP ? 1 : 256 / s.tpr; }
 
 // Workgroups of a launch: what the chip holds at a time, so that no second, partly filled round follows (1024 workgroups where 768 fit took
 // 534 us instead of 400 at 200003 x 512 bf16), and the rows shared out evenly among them.
@@ -548,11 +598,11 @@ int64_t even_grid(int64_t M, int64_t per_block, int64_t resident) {
   return need <= resident ? need : dh::ceil_div(need, dh::ceil_div(need, resident));
 }
 
-template <class T, int V, int CH, bool BLOCK, bool FULL, bool ODD>
+template <class T, int V, int CH, int MODE, bool FULL, int TAIL>
 int64_t launch(bool backward, const Args& a, const Split& s, hipStream_t st) {
-  const dim3 b(BLOCK ? a.tpr : 256);
-  const void* kernel = backward ? reinterpret_cast<const void*>(residual_norm_backward_kernel<T, V, CH, BLOCK, FULL, ODD>)
-                                : reinterpret_cast<const void*>(residual_norm_forward_kernel<T, V, CH, BLOCK, FULL, ODD>);
+  const dim3 b(MODE == GROUP ? a.tpr : 256);
+  const void* kernel = backward ? reinterpret_cast<const void*>(residual_norm_backward_kernel<T, V, CH, MODE, FULL, TAIL>)
+                                : reinterpret_cast<const void*>(residual_norm_forward_kernel<T, V, CH, MODE, FULL, TAIL>);
   // (a row of 257 .. 512 threads is asked for separately: static per direction and width)
   static int per_cu[2][2] = {{0, 0}, {0, 0}};
   int& fit = per_cu[backward][b.x > 256];
@@ -561,33 +611,35 @@ int64_t launch(bool backward, const Args& a, const Split& s, hipStream_t st) {
   if (backward && resident > BWD_BLOCKS) resident = BWD_BLOCKS;
   const int64_t grid = even_grid(a.M, rows_per_block(s), resident);
   const dim3 g((unsigned)grid);
-  if (backward) hipLaunchKernelGGL((residual_norm_backward_kernel<T, V, CH, BLOCK, FULL, ODD>), g, b, 0, st, a);
-  else hipLaunchKernelGGL((residual_norm_forward_kernel<T, V, CH, BLOCK, FULL, ODD>), g, b, 0, st, a);
+  if (backward) hipLaunchKernelGGL((residual_norm_backward_kernel<T, V, CH, MODE, FULL, TAIL>), g, b, 0, st, a);
+  else hipLaunchKernelGGL((residual_norm_forward_kernel<T, V, CH, MODE, FULL, TAIL>), g, b, 0, st, a);
   return grid;
 }
 
-template <class T, int V, int CH, bool BLOCK>
+template <class T, int V, int CH, int MODE, int TAIL>
 int64_t launch_gate(bool backward, const Args& a, const Split& s, hipStream_t st) {
-  const bool full = a.gate_kind == GATE_FULL;
-  if constexpr (V == 1) {
-    return full ? launch<T, V, CH, BLOCK, true, false>(backward, a, s, st) : launch<T, V, CH, BLOCK, false, false>(backward, a, s, st);
-  } else if (s.odd) {
-    return full ? launch<T, V, CH, BLOCK, true, true>(backward, a, s, st) : launch<T, V, CH, BLOCK, false, true>(backward, a, s, st);
-  } else {
-    return full ? launch<T, V, CH, BLOCK, true, false>(backward, a, s, st) : launch<T, V, CH, BLOCK, false, false>(backward, a, s, st);
+  return a.gate_kind == GATE_FULL ? launch<T, V, CH, MODE, true, TAIL>(backward, a, s, st) : launch<T, V, CH, MODE, false, TAIL>(backward, a, s, st);
+}
+template <class T, int V, int CH, int MODE>
+int64_t launch_tail(bool backward, const Args& a, const Split& s, hipStream_t st) {
+  if constexpr (V > 1) {
+    if (s.tail == ODD) return launch_gate<T, V, CH, MODE, ODD>(backward, a, s, st);
+    if (s.tail == WHOLE) return launch_gate<T, V, CH, MODE, WHOLE>(backward, a, s, st);
   }
+  return launch_gate<T, V, CH, MODE, SHORT>(backward, a, s, st);
 }
 
 // returns the number of workgroups
 template <class T>
 int64_t launch_t(bool backward, const Args& a, const Split& s, hipStream_t st) {
   constexpr int V = Elem<T>::VEC, EIGHT = 8 / V;
-  if (s.v == 1) return launch_gate<T, 1, 1, false>(backward, a, s, st);
-  if (s.block) return launch_gate<T, V, EIGHT, true>(backward, a, s, st);
+  if (s.v == 1) return launch_tail<T, 1, 1, SUB>(backward, a, s, st);
+  if (s.mode == GROUP) return launch_tail<T, V, EIGHT, GROUP>(backward, a, s, st);
+  if (s.mode == SUB) return launch_tail<T, V, 1, SUB>(backward, a, s, st);
   if constexpr (EIGHT == 2) {
-    if (s.ch == 2) return launch_gate<T, V, 2, false>(backward, a, s, st);
+    if (s.ch == 2) return launch_tail<T, V, 2, WAVE>(backward, a, s, st);
   }
-  return launch_gate<T, V, 1, false>(backward, a, s, st);
+  return launch_tail<T, V, 1, WAVE>(backward, a, s, st);
 }
 
 int check_common(const char* me, int64_t M, int64_t D, int dtype, const void* f, const void* x, int64_t ldf, int64_t ldx, const void* gate,
