@@ -1268,16 +1268,30 @@ def _is_dense(t: torch.Tensor) -> bool:
 
 
 def _grad_list(tensors, name: str):
+    """The tensors as a list, and their device: one C-level pass each, hundreds of tensors are usual; the messages come from a second look."""
     tensors = list(tensors)
+    try:
+        devices = set(map(torch.Tensor.get_device, tensors))
+        fine = len(devices) <= 1 and -1 not in devices
+    except TypeError:
+        fine = False
+    if not fine:
+        for t in tensors:
+            if not isinstance(t, torch.Tensor):
+                raise TypeError(f"{name} must be tensors, got {type(t).__name__}")
+            if not t.is_cuda:
+                raise _lib.DanceHipError(f"{name} must be GPU tensors (got one on {t.device}); dance_amd has no CPU path")
+        raise ValueError(f"{name}: tensors on more than one device: {sorted(devices)}")
+    return tensors, (devices.pop() if devices else None)
+
+
+def _all_contiguous(tensors, name: str) -> bool:
+    if all(map(torch.Tensor.is_contiguous, tensors)):
+        return True
     for t in tensors:
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{name} must be tensors, got {type(t).__name__}")
-    for t in tensors:
-        if not t.is_cuda:
-            raise _lib.DanceHipError(f"{name} must be GPU tensors (got one on {t.device}); dance_amd has no CPU path")
-        if t.dtype not in _ELEM or t.layout is not torch.strided:
-            raise TypeError(f"{name} must be dense torch.float32 or torch.bfloat16 tensors, got {t.dtype} ({t.layout})")
-    return tensors
+        if t.layout is not torch.strided:
+            raise TypeError(f"{name} must be dense torch.float32 or torch.bfloat16 tensors, got {t.layout}")
+    return False
 
 
 def _refuse_overlap(begins, ends):
@@ -1290,12 +1304,18 @@ def _refuse_overlap(begins, ends):
         raise ValueError("clip_grads: tensors overlap in memory (the same tensor given twice, or views of one)")
 
 
-def _norm_tables(tensors):
-    """Host tables of a tensor list: addresses, sizes, dtypes (one pass each through a C-level map: hundreds of tensors are usual)."""
-    ptrs = np.fromiter(map(torch.Tensor.data_ptr, tensors), dtype=np.int64, count=len(tensors))
-    sizes = np.fromiter(map(torch.Tensor.numel, tensors), dtype=np.int64, count=len(tensors))
-    dtypes = np.fromiter((_ELEM[t.dtype] for t in tensors), dtype=np.int32, count=len(tensors))
-    return ptrs, sizes, dtypes
+def _norm_tables(tensors, name: str):
+    """Host tables of a tensor list: addresses, sizes, dtypes."""
+    n = len(tensors)
+    dtypes = [_ELEM.get(t.dtype) for t in tensors]
+    if None in dtypes:
+        raise TypeError(f"{name} must be dense torch.float32 or torch.bfloat16 tensors, got {tensors[dtypes.index(None)].dtype}")
+    return (np.fromiter(map(torch.Tensor.data_ptr, tensors), dtype=np.int64, count=n), np.fromiter(map(torch.Tensor.numel, tensors), dtype=np.int64, count=n),
+            np.array(dtypes, dtype=np.int32))
+
+
+def _device_of(index):
+    return _HERE if index is None or index == torch._C._cuda_getDevice() else torch.cuda.device(index)
 
 
 def global_norm(tensors, norm_type: float = 2.0) -> torch.Tensor:
@@ -1303,12 +1323,13 @@ def global_norm(tensors, norm_type: float = 2.0) -> torch.Tensor:
     (dh_grad_norm).  ``norm_type`` 1, 2 or inf."""
     lib = _lib_ready()
     code = _norm_type(norm_type)
-    tensors = _grad_list(tensors, "global_norm: tensors")
+    name = "global_norm: tensors"
+    tensors, device = _grad_list(tensors, name)
     if not tensors:
         raise ValueError("global_norm: no tensors")
-    with _one_device(*tensors):
-        dense = tensors if all(map(torch.Tensor.is_contiguous, tensors)) else [t if _is_dense(t) else t.contiguous() for t in tensors]
-        ptrs, sizes, dtypes = _norm_tables(dense)
+    with _device_of(device):
+        dense = tensors if _all_contiguous(tensors, name) else [t if _is_dense(t) else t.contiguous() for t in tensors]
+        ptrs, sizes, dtypes = _norm_tables(dense, name)
         norm = torch.empty((), dtype=torch.float32, device=tensors[0].device)
         ws_bytes = lib.dh_grad_norm_workspace_bytes(len(dense), sizes.ctypes.data)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=norm.device)
@@ -1326,29 +1347,30 @@ def clip_grads(grads, max_norm: float, *, norm_type: float = 2.0, out=None) -> t
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise ValueError(f"clip_grads: max_norm must not be negative, got {max_norm}")
-    grads = _grad_list(grads, "clip_grads: gradients")
+    grads, device = _grad_list(grads, "clip_grads: gradients")
     if not grads:
         raise ValueError("clip_grads: no gradients")
-    targets = grads if out is None else _grad_list(out, "clip_grads: out")
+    targets, target_device = (grads, device) if out is None else _grad_list(out, "clip_grads: out")
     if len(targets) != len(grads):
         raise ValueError(f"clip_grads: {len(targets)} outputs for {len(grads)} gradients")
-    with _one_device(*grads, *(() if out is None else targets)):
+    if device != target_device:
+        raise ValueError(f"clip_grads: gradients on cuda:{device}, outputs on cuda:{target_device}")
+    with _device_of(device):
         src, dst, back = grads, targets, ()
-        if not (all(map(torch.Tensor.is_contiguous, grads)) and (out is None or all(map(torch.Tensor.is_contiguous, targets)))):
+        if not (_all_contiguous(grads, "clip_grads: gradients") and (out is None or _all_contiguous(targets, "clip_grads: out"))):
             src, dst, back = _consecutive(grads, targets)
-        in_ptrs, sizes, in_types = _norm_tables(src)
+        in_ptrs, sizes, in_types = _norm_tables(src, "clip_grads: gradients")
+        ends = in_ptrs + (sizes << (2 - in_types))  # DTYPE_F32 = 0: four bytes, DTYPE_BF16 = 1: two
         if dst is src:
-            out_ptrs, out_types = in_ptrs, in_types
+            out_ptrs, out_types, begins = in_ptrs, in_types, in_ptrs
         else:
-            out_ptrs, out_sizes, out_types = _norm_tables(dst)
+            out_ptrs, out_sizes, out_types = _norm_tables(dst, "clip_grads: out")
             if (out_sizes != sizes).any():
                 i = int((out_sizes != sizes).argmax())
                 raise ValueError(f"clip_grads: an output of shape {tuple(targets[i].shape)} for a gradient of shape {tuple(grads[i].shape)}")
-        begins, ends = out_ptrs, out_ptrs + sizes * np.where(out_types == DTYPE_BF16, 2, 4)
-        if dst is not src:
-            other = (in_ptrs != out_ptrs) | (in_types != out_types)
-            begins = np.concatenate((begins, in_ptrs[other]))
-            ends = np.concatenate((ends, (in_ptrs + sizes * np.where(in_types == DTYPE_BF16, 2, 4))[other]))
+            other = (in_ptrs != out_ptrs) | (in_types != out_types)  # read beside the write
+            begins = np.concatenate((out_ptrs, in_ptrs[other]))
+            ends = np.concatenate((out_ptrs + (sizes << (2 - out_types)), ends[other]))
         _refuse_overlap(begins, ends)
         norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
         ws_bytes = lib.dh_grad_norm_workspace_bytes(len(src), sizes.ctypes.data)

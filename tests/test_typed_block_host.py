@@ -26,7 +26,7 @@ def _grouped(lib, **kw):
 
 @pytest.mark.parametrize("bad", [dict(M=-1), dict(N=-1), dict(K=-1), dict(G=-1), dict(M=2**31), dict(dtype=2), dict(y_dtype=-1), dict(act=7), dict(X=None),
                                  dict(W=None), dict(ptr=None), dict(Y=None), dict(ldx=3), dict(ldw=3), dict(ldy=3), dict(bias=P, ld_bias=3),
-                                 dict(stride_w=-1), dict(N=2**28, ldy=2**28, M=2**20)])
+                                 dict(stride_w=-1)])
 def test_grouped_refusals(lib, bad):
     assert _grouped(lib, **bad) == INVALID
     assert b"dh_gemm_grouped" in lib.dh_last_error_string()
