@@ -8,6 +8,7 @@
 // them: group g owns the row slots [floor(ptr[g] / R) + g, floor(ptr[g + 1] / R) + g + 1), R rows each, always enough for its
 // ceil(len / R) tiles and monotone in g, so a workgroup finds its group with one 64-wide search per 64 groups instead of a prefix sum;
 // at most one slot per group and none of the work is wasted on it.
+#include <atomic>
 #include <type_traits>
 
 #include "common.h"
@@ -880,7 +881,8 @@ __global__ __launch_bounds__(512) void grouped_small_kernel(const FwdArgs a) {
 // cut into equal chunks whatever the groups: a workgroup takes one tile of dW through one chunk, group by group, so every workgroup has the
 // same number of rows to multiply however ragged the groups are.  A group that lies inside a chunk is finished in place; of one that spans
 // several, chunk c holds either its beginning (partial slot 2 c) or a later part that starts with the chunk (slot 2 c + 1; never two of a
-// kind), which wgrad_join_kernel adds in chunk order (no atomics).  An empty group's zeros are written by the chunk of its position.
+// kind), which wgrad_join_kernel adds in chunk order (no atomics).  The zeros of empty groups are written by workgroups of their own, the
+// first ZEROERS of the launch.
 struct WgradArgs {
   Groups gr;
   int64_t N, K;
@@ -911,33 +913,48 @@ struct Segments {
   __device__ __forceinline__ Segments(const WgradArgs& args, int64_t chunk_id) : a(args), c(chunk_id) {
     first = c * a.chunk;
     last = min(first + a.chunk, a.gr.M);
-    // the first group that touches the chunk: the one that holds its first row, or earlier empty ones at that very position
-    if (c == 0) {
-      i = 1;
-    } else {
-      i = search(a.gr.G + 2, first - 1, [&](int j) { return a.gr.edge(j); });  // holds row first - 1
-      if (a.gr.edge(i + 1) <= first) ++i;                                      // and ends there: nothing of it is left
-      if (i < 1) i = 1;
-    }
+    // the group that holds the chunk's first row, or an earlier one that ends at or before it
+    i = c == 0 ? 1 : max(1, search(a.gr.G + 2, first, [&](int j) { return a.gr.edge(j); }));
   }
   __device__ __forceinline__ bool next(Segment& s) {
     while (i <= a.gr.G) {
       const int64_t b = a.gr.edge(i), e = a.gr.edge(i + 1);
-      const bool final_chunk = c + 1 == a.chunks;
-      if (b > last || (b == last && !(final_chunk && e <= b))) return false;
+      if (b >= last) return false;
       ++i;
-      if (e <= b) {  // empty: at position b of this chunk (at its end only in the last chunk)
-        s = {i - 2, 0, 0, -1};
-        return true;
-      }
       const int64_t from = max(b, first), to = min(e, last);
-      if (from >= to) continue;
+      if (from >= to) continue;  // empty, or before the chunk
       s = {i - 2, from, to, b >= first && e <= last ? -1 : b >= first ? 2 * c : 2 * c + 1};
       return true;
     }
     return false;
   }
 };
+
+constexpr int ZEROERS = 8;  // (a multiple of the XCDs: the other workgroups keep their places)
+
+// dW, db of the empty groups among every ZEROERS-th 64
+__device__ void write_empty_groups(const WgradArgs& a, int part) {
+  const int lane = threadIdx.x & 63;
+  for (int64_t base = (int64_t)part * 64; base < a.gr.G; base += ZEROERS * 64) {
+    const int g = (int)base + lane;
+    unsigned long long empty = __ballot(g < a.gr.G && a.gr.edge(g + 2) <= a.gr.edge(g + 1));
+    while (empty) {
+      const int64_t group = base + __builtin_ctzll(empty);
+      empty &= empty - 1;
+      char* to = static_cast<char*>(a.dW) + group * a.stride_w * (a.dw_bf16 ? 2 : 4);
+      const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+      const int pieces = (int)((a.K + 3) / 4), rows = blockDim.x / min(pieces, (int)blockDim.x);  // rows at a time
+      const int r = threadIdx.x / min(pieces, (int)blockDim.x), c = threadIdx.x % min(pieces, (int)blockDim.x);
+      for (int64_t n = r; r < rows && n < a.N; n += rows)
+        for (int64_t k = (int64_t)c * 4; k < a.K; k += (int64_t)blockDim.x * 4) {
+          if (a.dw_bf16) put4<true>(reinterpret_cast<uint16_t*>(to) + n * a.ldw, k, a.K, zero);
+          else put4<false>(reinterpret_cast<float*>(to) + n * a.ldw, k, a.K, zero);
+        }
+      if (a.db)
+        for (int64_t n = threadIdx.x; n < a.N; n += blockDim.x) a.db[group * a.ld_db + n] = 0.f;
+    }
+  }
+}
 
 // where a segment's result goes
 struct WgradOut {
@@ -955,7 +972,8 @@ template <class T, class TileT>
 __global__ __launch_bounds__(TileT::THREADS, 2) void grouped_wgrad_kernel(const WgradArgs a) {
   typedef typename TileT::OpA OpA;
   extern __shared__ __attribute__((aligned(16))) unsigned char raw_lds[];
-  const int64_t id = xcd_run(blockIdx.x, gridDim.x), tile = id % a.tiles, n0 = (tile / a.tiles_k) * TileT::BM, k0 = (tile % a.tiles_k) * TileT::BN;
+  if (blockIdx.x < ZEROERS) return write_empty_groups(a, blockIdx.x);
+  const int64_t id = xcd_run(blockIdx.x - ZEROERS, gridDim.x - ZEROERS), tile = id % a.tiles, n0 = (tile / a.tiles_k) * TileT::BM, k0 = (tile % a.tiles_k) * TileT::BN;
   const bool sums = a.db && k0 == 0;
   constexpr int VEC = Geo<T>::VEC;
   Segments walk(a, id / a.tiles);
@@ -1034,7 +1052,9 @@ __device__ __forceinline__ void wgrad_dma(const WgradArgs& a, int64_t c, int64_t
 template <class TileT>
 __global__ __launch_bounds__(TileT::THREADS, 2) void grouped_wgrad_dma_kernel(const WgradArgs a) {
   extern __shared__ __attribute__((aligned(16))) unsigned char raw_lds[];
-  const int64_t id = xcd_run(blockIdx.x, gridDim.x), tile = id % a.tiles, n0 = (tile / a.tiles_k) * TileT::BM, k0 = (tile % a.tiles_k) * TileT::BN;
+  if (blockIdx.x < ZEROERS) return write_empty_groups(a, blockIdx.x);
+  const int64_t id = xcd_run(blockIdx.x - ZEROERS, gridDim.x - ZEROERS), tile = id % a.tiles, n0 = (tile / a.tiles_k) * TileT::BM;
+  const int64_t k0 = (tile % a.tiles_k) * TileT::BN;
   if (a.db && k0 == 0) wgrad_dma<TileT, true>(a, id / a.tiles, n0, k0, reinterpret_cast<typename TileT::Elem*>(raw_lds));
   else wgrad_dma<TileT, false>(a, id / a.tiles, n0, k0, reinterpret_cast<typename TileT::Elem*>(raw_lds));
 }
@@ -1098,18 +1118,24 @@ constexpr int64_t MAX_GRID = 0x7fffffff;
 
 constexpr int CUS = 256;
 
-// raises a kernel's dynamic LDS limit once
-template <class Kernel>
-int allow_lds(const char* me, Kernel* kernel, int bytes) {
-  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  return e == hipSuccess ? DH_OK : dh::fail(DH_ERR_LAUNCH, "%s: %d bytes of LDS: %s", me, bytes, hipGetErrorString(e));
+// Raises a kernel's dynamic LDS limit, once per device: `done` is the kernel's own mask of devices.
+int allow_lds(const char* me, const void* kernel, int bytes, std::atomic<uint64_t>& done) {
+  int device = 0;
+  if (hipGetDevice(&device) != hipSuccess) return dh::fail(DH_ERR_NO_DEVICE, "%s: no device", me);
+  const uint64_t bit = 1ull << (device & 63);
+  if (done.load(std::memory_order_relaxed) & bit) return DH_OK;
+  const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != hipSuccess) return dh::fail(DH_ERR_LAUNCH, "%s: %d bytes of LDS: %s", me, bytes, hipGetErrorString(e));
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return DH_OK;
 }
 
 template <class T, class TileT>
 int forward_launch(const char* me, const FwdArgs& a, hipStream_t st) {
   const int64_t grid = (a.gr.M / TileT::BM + a.gr.G + 2) * dh::ceil_div(a.N, TileT::BN);
   if (grid > MAX_GRID) return dh::fail(DH_ERR_INVALID, "%s: %lld tiles in one launch", me, (long long)grid);
-  static const int allowed = allow_lds(me, grouped_forward_kernel<T, TileT>, TileT::LDS_BYTES);
+  static std::atomic<uint64_t> done{0};
+  const int allowed = allow_lds(me, reinterpret_cast<const void*>(grouped_forward_kernel<T, TileT>), TileT::LDS_BYTES, done);
   if (allowed != DH_OK) return allowed;
   hipLaunchKernelGGL((grouped_forward_kernel<T, TileT>), dim3((unsigned)grid), dim3(TileT::THREADS), TileT::LDS_BYTES, st, a);
   return dh::check_launch(me);
@@ -1119,7 +1145,8 @@ template <class TileT>
 int forward_dma_launch(const char* me, const FwdArgs& a, hipStream_t st) {
   const int64_t tiles = (a.gr.M / TileT::BM + a.gr.G + 2) * dh::ceil_div(a.N, TileT::BN);
   const int64_t resident = (int64_t)CUS * (160 * 1024 / TileT::LDS_BYTES);
-  static const int allowed = allow_lds(me, grouped_forward_dma_kernel<TileT>, TileT::LDS_BYTES);
+  static std::atomic<uint64_t> done{0};
+  const int allowed = allow_lds(me, reinterpret_cast<const void*>(grouped_forward_dma_kernel<TileT>), TileT::LDS_BYTES, done);
   if (allowed != DH_OK) return allowed;
   hipLaunchKernelGGL((grouped_forward_dma_kernel<TileT>), dim3((unsigned)(tiles < resident ? tiles : resident)), dim3(TileT::THREADS), TileT::LDS_BYTES, st,
                      a, tiles);
@@ -1189,25 +1216,27 @@ template <class TileT>
 int wgrad_grid(const char* me, WgradArgs& a) {
   a.tiles_k = dh::ceil_div(a.K, TileT::BN);
   a.tiles = dh::ceil_div(a.N, TileT::BM) * a.tiles_k;
-  if (a.chunks * a.tiles > MAX_GRID) return dh::fail(DH_ERR_INVALID, "%s: %lld tiles in one launch", me, (long long)(a.chunks * a.tiles));
+  if (a.chunks * a.tiles > MAX_GRID - ZEROERS) return dh::fail(DH_ERR_INVALID, "%s: %lld tiles in one launch", me, (long long)(a.chunks * a.tiles));
   return DH_OK;
 }
 
 template <class T, class TileT>
 int wgrad_launch(const char* me, WgradArgs a, hipStream_t st) {
-  static const int allowed = allow_lds(me, grouped_wgrad_kernel<T, TileT>, TileT::LDS_BYTES);
+  static std::atomic<uint64_t> done{0};
+  const int allowed = allow_lds(me, reinterpret_cast<const void*>(grouped_wgrad_kernel<T, TileT>), TileT::LDS_BYTES, done);
   const int rc = allowed == DH_OK ? wgrad_grid<TileT>(me, a) : allowed;
   if (rc != DH_OK) return rc;
-  hipLaunchKernelGGL((grouped_wgrad_kernel<T, TileT>), dim3((unsigned)(a.chunks * a.tiles)), dim3(TileT::THREADS), TileT::LDS_BYTES, st, a);
+  hipLaunchKernelGGL((grouped_wgrad_kernel<T, TileT>), dim3((unsigned)(a.chunks * a.tiles + ZEROERS)), dim3(TileT::THREADS), TileT::LDS_BYTES, st, a);
   return dh::check_launch(me);
 }
 
 template <class TileT>
 int wgrad_dma_launch(const char* me, WgradArgs a, hipStream_t st) {
-  static const int allowed = allow_lds(me, grouped_wgrad_dma_kernel<TileT>, TileT::LDS_BYTES);
+  static std::atomic<uint64_t> done{0};
+  const int allowed = allow_lds(me, reinterpret_cast<const void*>(grouped_wgrad_dma_kernel<TileT>), TileT::LDS_BYTES, done);
   const int rc = allowed == DH_OK ? wgrad_grid<TileT>(me, a) : allowed;
   if (rc != DH_OK) return rc;
-  hipLaunchKernelGGL((grouped_wgrad_dma_kernel<TileT>), dim3((unsigned)(a.chunks * a.tiles)), dim3(TileT::THREADS), TileT::LDS_BYTES, st, a);
+  hipLaunchKernelGGL((grouped_wgrad_dma_kernel<TileT>), dim3((unsigned)(a.chunks * a.tiles + ZEROERS)), dim3(TileT::THREADS), TileT::LDS_BYTES, st, a);
   return dh::check_launch(me);
 }
 

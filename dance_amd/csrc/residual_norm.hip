@@ -18,6 +18,7 @@
 // no load is guarded.  The two-pass variance and both reductions of the backward run on registers.  Column gradients are summed in
 // registers over the rows a workgroup walks, joined in its LDS, written once per workgroup and added up by a second kernel in workgroup
 // order: no atomics, the result does not depend on timing.  All arithmetic is fp32; bf16 rounds once, at the stores.
+#include <atomic>
 #include <type_traits>
 
 #include "common.h"
@@ -243,35 +244,34 @@ __device__ __forceinline__ void store_row(void* p, int64_t row_at, int t, int tp
   }
 }
 
-// mean and rstd of a row held in registers (entries beyond D are zero)
+// mean and rstd of a row held in registers (entries beyond D are zero); v becomes v - mean: the subtraction comes first everywhere, so a row
+// that is nearly constant keeps the digits its differences have
 template <int MODE, int V, int CH, int TAIL>
-__device__ __forceinline__ void row_stats(const Args& a, int t, const float (&v)[V * CH], float* lds, float& mean, float& rstd) {
+__device__ __forceinline__ void row_stats(const Args& a, int t, float (&v)[V * CH], float* lds, float& mean, float& rstd) {
+  const int tpr = MODE == WAVE ? 64 : a.tpr;
   float s[1] = {0.f};
   mean = 0.f;
   if (!a.rms) {
 #pragma unroll
     for (int i = 0; i < V * CH; ++i) s[0] += v[i];
-    row_sums<MODE, 1>(s, a.tpr, lds);
+    row_sums<MODE, 1>(s, tpr, lds);
     mean = s[0] * a.inv_d;
+#pragma unroll
+    for (int i = 0; i < V * CH; ++i) v[i] -= mean;
+    zero_tail<V, CH, TAIL>(t, tpr, a.D, v);
     s[0] = 0.f;
   }
 #pragma unroll
-  for (int c = 0; c < CH; ++c)
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const float d = TAIL == WHOLE || (c * a.tpr + t) * V + (TAIL == ODD ? e : 0) < a.D ? v[c * V + e] - mean : 0.f;
-      s[0] = __builtin_fmaf(d, d, s[0]);
-    }
-  row_sums<MODE, 1>(s, a.tpr, lds);
+  for (int i = 0; i < V * CH; ++i) s[0] = __builtin_fmaf(v[i], v[i], s[0]);
+  row_sums<MODE, 1>(s, tpr, lds);
   rstd = 1.f / sqrtf(s[0] * a.inv_d + a.eps);
 }
 
-// v = (v - mean) rstd w + b as two fused steps: v rstd - mean rstd, then w, b
+// v = v rstd w + b
 template <int E>
-__device__ __forceinline__ void normalise(float (&v)[E], float mean, float rstd, const float (&w)[E], const float (&b)[E]) {
-  const float shift = -mean * rstd;
+__device__ __forceinline__ void scale_shift(float (&v)[E], float rstd, const float (&w)[E], const float (&b)[E]) {
 #pragma unroll
-  for (int i = 0; i < E; ++i) v[i] = __builtin_fmaf(__builtin_fmaf(v[i], rstd, shift), w[i], b[i]);
+  for (int i = 0; i < E; ++i) v[i] = __builtin_fmaf(v[i] * rstd, w[i], b[i]);
 }
 
 template <class T, int V, int CH, int MODE, bool FULL, int TAIL>
@@ -320,7 +320,7 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256) void residual_norm_forwa
       load_params<V, CH, TAIL>(a.w1, 1.f, t, tpr, a.D, w);
       load_params<V, CH, TAIL>(a.b1, 0.f, t, tpr, a.D, b);
       row_stats<MODE, V, CH, TAIL>(a, t, f, lds, m1, s1);
-      normalise<E>(f, m1, s1, w, b);
+      scale_shift<E>(f, s1, w, b);
     }
     if (FULL) {
       if (a.gate_sigmoid) {
@@ -343,7 +343,7 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256) void residual_norm_forwa
       load_params<V, CH, TAIL>(a.w2, 1.f, t, tpr, a.D, w);
       load_params<V, CH, TAIL>(a.b2, 0.f, t, tpr, a.D, b);
       row_stats<MODE, V, CH, TAIL>(a, t, f, lds, m2, s2);
-      normalise<E>(f, m2, s2, w, b);
+      scale_shift<E>(f, s2, w, b);
       if (valid) store_row<T, V, CH, TAIL>(a.h, row * a.ldh, t, tpr, a.D, f);
     }
     if (valid && a.stats && t == 0) *reinterpret_cast<float4*>(a.stats + row * 4) = make_float4(m1, s1, m2, s2);
@@ -448,9 +448,8 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256) void residual_norm_backw
     if (a.has_post) {
       load_params<V, CH, TAIL>(a.w1, 1.f, t, tpr, a.D, w);
       load_params<V, CH, TAIL>(a.b1, 0.f, t, tpr, a.D, b);
-      const float shift = -st.x * st.y;
 #pragma unroll
-      for (int i = 0; i < E; ++i) f[i] = __builtin_fmaf(f[i], st.y, shift);  // fhat from here on
+      for (int i = 0; i < E; ++i) f[i] = (f[i] - st.x) * st.y;  // fhat from here on
     } else {
 #pragma unroll
       for (int i = 0; i < E; ++i) { w[i] = 1.f; b[i] = 0.f; }
@@ -460,11 +459,10 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256) void residual_norm_backw
       load_params<V, CH, TAIL>(a.w2, 1.f, t, tpr, a.D, w2);
       zero_tail<V, CH, TAIL>(t, tpr, a.D, dh);
       float s[2] = {0.f, 0.f};
-      const float shift2 = -st.z * st.w;
 #pragma unroll
       for (int i = 0; i < E; ++i) {
         const float n = __builtin_fmaf(f[i], w[i], b[i]);
-        x[i] = __builtin_fmaf(__builtin_fmaf(a.scale * gf[i], n, x[i]), st.w, shift2);  // rhat
+        x[i] = (__builtin_fmaf(a.scale * gf[i], n, x[i]) - st.z) * st.w;  // rhat
         if (valid) {
           acc_w2[i] = __builtin_fmaf(dh[i], x[i], acc_w2[i]);
           acc_b2[i] += dh[i];
@@ -604,9 +602,15 @@ int64_t launch(bool backward, const Args& a, const Split& s, hipStream_t st) {
   const void* kernel = backward ? reinterpret_cast<const void*>(residual_norm_backward_kernel<T, V, CH, MODE, FULL, TAIL>)
                                 : reinterpret_cast<const void*>(residual_norm_forward_kernel<T, V, CH, MODE, FULL, TAIL>);
   // (a row of 257 .. 512 threads is asked for separately: static per direction and width)
-  static int per_cu[2][2] = {{0, 0}, {0, 0}};
-  int& fit = per_cu[backward][b.x > 256];
-  if (fit == 0 && (hipOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kernel, (int)b.x, 0) != hipSuccess || fit < 1)) fit = 2;
+  static std::atomic<int> per_cu[2][2];
+  int fit = per_cu[backward][b.x > 256].load(std::memory_order_relaxed);
+  if (fit == 0) {
+    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kernel, (int)b.x, 0) != hipSuccess || fit < 1) {
+      (void)hipGetLastError();
+      fit = 2;
+    }
+    per_cu[backward][b.x > 256].store(fit, std::memory_order_relaxed);
+  }
   int64_t resident = (int64_t)256 * fit;
   if (backward && resident > BWD_BLOCKS) resident = BWD_BLOCKS;
   const int64_t grid = even_grid(a.M, rows_per_block(s), resident);

@@ -7,6 +7,7 @@ wrappers never copy to the host and never compute on the CPU.
 from typing import Optional, Tuple
 
 import contextlib
+import operator
 import os
 
 import numpy as np
@@ -766,6 +767,23 @@ def _bounds(group_ptr: torch.Tensor, groups: int) -> int:
     return _dev(group_ptr, torch.int32, "group_ptr", 1)
 
 
+def _span(t: torch.Tensor):
+    """First byte and end byte of the memory between a tensor's first and last element."""
+    if t.numel() == 0:
+        return 0, 0
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _refuse_shared_output(out: torch.Tensor, *inputs):
+    begin, end = _span(out)
+    for t in inputs:
+        if t is not None:
+            b, e = _span(t)
+            if b < end and begin < e:
+                raise ValueError("out overlaps an operand in memory")
+
+
 def gemm_grouped(X: torch.Tensor, W: torch.Tensor, group_ptr: torch.Tensor, *, trans_b: bool = True, bias: Optional[torch.Tensor] = None,
                  act: int = ACT_NONE, out: Optional[torch.Tensor] = None, out_dtype=None) -> torch.Tensor:
     """Y[i] = act(X[i] @ op(W[g]) + bias[g]) for the rows group_ptr[g] <= i < group_ptr[g + 1]; see dh_gemm_grouped.
@@ -798,6 +816,7 @@ def gemm_grouped(X: torch.Tensor, W: torch.Tensor, group_ptr: torch.Tensor, *, t
         if out.shape != (M, N) or (out_dtype is not None and yt != out_dtype):
             raise ValueError(f"out must be [{M}, {N}]{'' if out_dtype is None else f' of {out_dtype}'}, got {tuple(out.shape)} of {out.dtype}")
         yp, ldy = _mat(out, yt, "out")
+        _refuse_shared_output(out, X, W, bias, group_ptr)
     with _one_device(X, W, group_ptr, bias, out):
         _call(_GROUPED_TAGS[dt][bool(trans_b)], lib.dh_gemm_grouped, M, N, K, G, 1 if trans_b else 0, dt, xp, ldx, wp, ldw, sw, gp, bp, ldb, act, yp, ldy,
               _elem(y, "out"), 1 if out is None else 0, _stream())
@@ -1242,6 +1261,7 @@ def block_cells_static_workspace_bytes(n_seeds: int) -> int:
 
 
 # ---- global gradient norm and clipping ---------------------------------------------------------------------------
+_DTYPE_OF = operator.attrgetter("dtype")
 _NORM_TYPES = {1.0: 1, 2.0: 2, float("inf"): 0}
 
 
@@ -1307,7 +1327,7 @@ def _refuse_overlap(begins, ends):
 def _norm_tables(tensors, name: str):
     """Host tables of a tensor list: addresses, sizes, dtypes."""
     n = len(tensors)
-    dtypes = [_ELEM.get(t.dtype) for t in tensors]
+    dtypes = list(map(_ELEM.get, map(_DTYPE_OF, tensors)))
     if None in dtypes:
         raise TypeError(f"{name} must be dense torch.float32 or torch.bfloat16 tensors, got {tensors[dtypes.index(None)].dtype}")
     return (np.fromiter(map(torch.Tensor.data_ptr, tensors), dtype=np.int64, count=n), np.fromiter(map(torch.Tensor.numel, tensors), dtype=np.int64, count=n),

@@ -18,6 +18,7 @@ LAYOUTS = {
     "empty_groups": (70, [0, 33, 0, 0, 37, 0], 0),
     "gaps": (90, [5, 0, 40], 13),                     # 13 rows in front and 32 behind belong to no group
     "all_empty": (9, [0, 0, 0], 4),
+    "mostly_empty": (7, [0] * 300 + [3] + [0] * 700 + [4] + [0] * 100, 0),
     "ragged": (611, [1, 128, 129, 127, 3, 0, 200, 23], 0),
     "many": (700, [i % 5 for i in range(350)], 0),    # more groups than one 64-wide probe
     "long": (3700, [2500, 1100], 60),                 # the large tile
@@ -262,12 +263,15 @@ def test_refusals(cuda_device):
         ok(out_dtype=torch.float16)
     with pytest.raises(_lib.DanceHipError):
         ok(ptr=ptr.cpu())
-    for kw in (dict(ptr=ptr[:-1]), dict(x=x[:, :39]), dict(bias=b[:, :5]), dict(w=w[0]), dict(x=x[0]), dict(act=5), dict(x=x.t()), dict(out=x),
+    for kw in (dict(ptr=ptr[:-1]), dict(x=x[:, :39]), dict(bias=b[:, :5]), dict(w=w[0]), dict(x=x[0]), dict(act=5), dict(x=x.t()), dict(out=x), dict(out=torch.zeros(90, 64, device=DEV)[:, :24], x=torch.zeros(90, 40, device=DEV).t()),
                dict(x=x[:1].expand(90, 40)), dict(ptr=ptr[None])):
         with pytest.raises(ValueError):
             ok(**kw)
     with pytest.raises(ValueError):
         kernels.gemm_grouped_wgrad(dy[:5], x, ptr)
+    shared = torch.zeros(90, 64, device=DEV)
+    with pytest.raises(ValueError, match="overlaps"):
+        kernels.gemm_grouped(shared[:, :40], w, ptr, out=shared[:, 40:])
     with pytest.raises(ValueError):
         kernels.gemm_grouped_wgrad(dy.t(), x, ptr)
 

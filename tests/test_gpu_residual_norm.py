@@ -231,6 +231,20 @@ def test_rows_do_not_touch_each_other(cuda_device, dtype):
     assert not bool(r.any()) and not bool(h.any())
 
 
+@pytest.mark.parametrize("D", [40, 512, 2000])
+def test_offset_rows(cuda_device, D):
+    """Rows of a large common offset and small differences: the differences are what the norm sees.  mean carries 22 roundings of the row's
+    magnitude, the subtraction is exact to a rounding: |error| <= 32 2^-24 |offset| rstd + 120 2^-24 |value|."""
+    from dance_amd import kernels
+    gen = torch.Generator().manual_seed(0)
+    f = (1000.0 + torch.randn(30, D, generator=gen)).to(DEV)
+    f[7] = 1234.5678                                              # constant: nothing but the bias may come out
+    r, _, _ = kernels.residual_norm_forward(f, post=(None, None))
+    ref = torch.nn.functional.layer_norm(f.double(), (D, ))
+    rstd = (f.double().var(1, unbiased=False, keepdim=True) + 1e-5).rsqrt()
+    assert bool(((r.double() - ref).abs() <= 32 * U * f.double().abs() * rstd + 120 * U * ref.abs()).all())
+
+
 def test_gradient_against_differences(cuda_device):
     """<grad, d> against the central difference of L = <r, dr> + <h, dh> along d, L evaluated by the float64 reference (which the forward is
     held to above): the truncation error is O(step^2) = 1e-8 of a third derivative of order one."""

@@ -146,22 +146,13 @@ def _segments(ptr, M, chunk, chunks, c):
     """(group, begin, end, partial slot) of a chunk of rows, as Segments walks them."""
     e, G = _edges(ptr, M), len(ptr) - 1
     first, last = c * chunk, min(c * chunk + chunk, M)
-    if c == 0:
-        i = 1
-    else:
-        i = max(j for j in range(G + 2) if e[j] <= first - 1)
-        if e[i + 1] <= first:
-            i += 1
-        i = max(i, 1)
+    i = 1 if c == 0 else max(1, max(j for j in range(G + 2) if e[j] <= first))
     out = []
     while i <= G:
         b, t = e[i], e[i + 1]
-        if b > last or (b == last and not (c + 1 == chunks and t <= b)):
+        if b >= last:
             break
         i += 1
-        if t <= b:
-            out.append((i - 2, 0, 0, -1))
-            continue
         lo, hi = max(b, first), min(t, last)
         if lo < hi:
             out.append((i - 2, lo, hi, -1 if b >= first and t <= last else 2 * c if b >= first else 2 * c + 1))
@@ -170,7 +161,7 @@ def _segments(ptr, M, chunk, chunks, c):
 
 @pytest.mark.parametrize("seed", range(60))
 def test_weight_gradient_segments(seed):
-    """Every row of a group is in one segment, every group is finished once (in place, as zeros, or by the join of its parts, which reads
+    """Every row of a group is in one segment, every group with rows is finished once (in place, or by the join of its parts, which reads
     exactly the slots that were written), and no slot is written twice."""
     rng = np.random.default_rng(seed)
     M, G, chunk = int(rng.integers(0, 700)), int(rng.integers(1, 60)), int(rng.choice([32, 64, 96, 1000]))
@@ -179,7 +170,7 @@ def test_weight_gradient_segments(seed):
     owner, done, slots = np.full(M, -1), np.zeros(G, int), {}
     for c in range(chunks):
         for group, lo, hi, slot in _segments(ptr, M, chunk, chunks, c):
-            assert (owner[lo:hi] == -1).all() and ptr[group] <= lo <= hi <= ptr[group + 1] or lo == hi == 0
+            assert (owner[lo:hi] == -1).all() and ptr[group] <= lo < hi <= ptr[group + 1]
             owner[lo:hi] = group
             if slot < 0:
                 done[group] += 1
@@ -197,7 +188,7 @@ def test_weight_gradient_segments(seed):
         done[i - 1] += 1
         for c in range((end - 1) // chunk - c0 + 1):
             assert slots.pop(2 * (c0 + c) + (c > 0)) == i - 1
-    assert not slots and (done == 1).all()
+    assert not slots and (done == (ptr[1:] > ptr[:-1])).all()
     for g in range(G):
         assert (owner[ptr[g]:ptr[g + 1]] == g).all()
 
