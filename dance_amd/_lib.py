@@ -160,7 +160,7 @@ def _declare(lib):
         "dh_residual_norm_backward": (c_int, [i64, i64, i32, P, i64, P, i64, P, i64, i32, i32, c_float, i32, i32, P, P, i32, P, P, P, i64, P, i64, P, i64,
                                               P, i64, P, i64, P, P, P, P, P, c_size_t, P]),
         "dh_gemm_grouped": (c_int, [i64, i64, i64, i64, i32, i32, P, i64, P, i64, i64, P, P, i64, i32, P, i64, i32, i32, P]),
-        "dh_gemm_grouped_wgrad_workspace_bytes": (c_size_t, [i64, i64, i64, i32]),
+        "dh_gemm_grouped_wgrad_workspace_bytes": (c_size_t, [i64, i64, i64, i64, i32]),
         "dh_gemm_grouped_wgrad": (c_int, [i64, i64, i64, i64, i32, P, i64, P, i64, P, P, i64, i64, i32, P, i64, P, c_size_t, P]),
         "dh_sage_alpha_grad_f32": (c_int, [i64, i64, i64, i64, P, P, P, P, P, P, i64, P, i64, P, P]),
         "dh_dec_target_f32": (c_int, [i64, i64, P, i64, P, P, i64, P]),

@@ -45,6 +45,13 @@ struct Groups {
     const int64_t v = ptr[i - 1];
     return v < 0 ? 0 : v > M ? M : v;
   }
+  // of an index that all lanes share: a scalar
+  __device__ __forceinline__ int64_t shared_edge(int i) const {
+    if (i <= 0) return 0;
+    if (i >= G + 2) return M;
+    const int64_t v = __builtin_amdgcn_readfirstlane(ptr[i - 1]);
+    return v < 0 ? 0 : v > M ? M : v;
+  }
 };
 
 // the last i in [0, n) with key(i) <= s, key non-decreasing and key(0) <= s: 64 probes at a time
@@ -75,7 +82,7 @@ struct Slot {
 __device__ __forceinline__ Slot find_slot(const Groups& gr, int64_t s, int shift) {
   const int n = gr.G + 2;
   const int i = search(n, s, [&](int j) { return (gr.edge(j) >> shift) + j; });
-  const int64_t a = gr.edge(i), b = gr.edge(i + 1);
+  const int64_t a = gr.shared_edge(i), b = gr.shared_edge(i + 1);
   const int64_t first = (a >> shift) + i;
   Slot r;
   r.group = i == 0 || i == n - 1 ? -1 : i - 1;
@@ -89,8 +96,8 @@ __device__ __forceinline__ Slot find_slot(const Groups& gr, int64_t s, int shift
 
 // the logical number of a workgroup: the dispatcher deals workgroups round robin to the 8 XCDs; handing each XCD a contiguous run keeps
 // the tiles that share an operand panel on one L2
-__device__ __forceinline__ int64_t xcd_run(int64_t bid, int64_t n) {
-  const int64_t q = n / 8, r = n % 8, xcd = bid % 8;
+__device__ __forceinline__ int xcd_run(int bid, int n) {
+  const int q = n / 8, r = n % 8, xcd = bid % 8;
   return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + bid / 8;
 }
 
@@ -692,16 +699,17 @@ struct FwdArgs {
 
 // tile `id` of the launch: its row slot and first column; false where there is nothing to write
 template <class TileT>
-__device__ __forceinline__ bool forward_tile(const FwdArgs& a, int64_t id, int64_t tiles_n, Slot& s, int64_t& n0) {
-  s = find_slot(a.gr, id / tiles_n, __builtin_ctz(TileT::BM));
-  n0 = (id % tiles_n) * TileT::BN;
+__device__ __forceinline__ bool forward_tile(const FwdArgs& a, int id, int tiles_n, Slot& s, int64_t& n0) {
+  const int slot = __builtin_amdgcn_readfirstlane(id / tiles_n);
+  s = find_slot(a.gr, slot, __builtin_ctz(TileT::BM));
+  n0 = (int64_t)(id - slot * tiles_n) * TileT::BN;
   return s.live && (s.group >= 0 || a.zero_outside);
 }
 
 template <class T, class TileT>
 __global__ __launch_bounds__(TileT::THREADS, 2) void grouped_forward_kernel(const FwdArgs a) {
   extern __shared__ __attribute__((aligned(16))) unsigned char raw_lds[];
-  const int64_t tiles_n = (a.N + TileT::BN - 1) / TileT::BN;
+  const int tiles_n = (int)((a.N + TileT::BN - 1) / TileT::BN);
   Slot s;
   int64_t n0;
   if (!forward_tile<TileT>(a, xcd_run(blockIdx.x, gridDim.x), tiles_n, s, n0)) return;
@@ -731,13 +739,13 @@ __global__ __launch_bounds__(TileT::THREADS, 2) void grouped_forward_kernel(cons
 
 // As many workgroups as the chip holds; each walks the tiles l, l + L, l + 2 L ... of its XCD's contiguous run, L workgroups on that XCD.
 template <class TileT>
-__global__ __launch_bounds__(TileT::THREADS, 2) void grouped_forward_dma_kernel(const FwdArgs a, int64_t n_tiles) {
+__global__ __launch_bounds__(TileT::THREADS, 2) void grouped_forward_dma_kernel(const FwdArgs a, int n_tiles) {
   typedef typename TileT::Elem T;
   extern __shared__ __attribute__((aligned(16))) unsigned char raw_lds[];
-  const int64_t tiles_n = (a.N + TileT::BN - 1) / TileT::BN;
-  const int64_t xcd = blockIdx.x % 8, q = n_tiles / 8, rest = n_tiles % 8;
-  const int64_t stop = (xcd < rest ? (xcd + 1) * (q + 1) : rest * (q + 1) + (xcd + 1 - rest) * q), step = (gridDim.x + 7 - xcd) / 8;
-  int64_t id = (xcd < rest ? xcd * (q + 1) : rest * (q + 1) + (xcd - rest) * q) + blockIdx.x / 8;
+  const int tiles_n = (int)((a.N + TileT::BN - 1) / TileT::BN);
+  const int xcd = blockIdx.x % 8, q = n_tiles / 8, rest = n_tiles % 8;
+  const int run = xcd < rest ? xcd * (q + 1) : rest * (q + 1) + (xcd - rest) * q, stop = run + (xcd < rest ? q + 1 : q), step = (gridDim.x + 7 - xcd) / 8;
+  int id = run + blockIdx.x / 8;
   TileT t;
   t.lds = reinterpret_cast<T*>(raw_lds);
   auto advance = [&](Slot& s, int64_t& n0) __attribute__((always_inline)) {  // the next tile with something to write
@@ -830,9 +838,9 @@ template <class T, bool W_KM>
 __global__ __launch_bounds__(512) void grouped_small_kernel(const FwdArgs a) {
   typedef SmallFrags<T, W_KM> Frags;
   __shared__ __attribute__((aligned(16))) float part[8][32][36];
-  const int64_t tiles_n = (a.N + 31) / 32, id = xcd_run(blockIdx.x, gridDim.x);
-  const Slot s = find_slot(a.gr, id / tiles_n, 5);
-  const int64_t n0 = (id % tiles_n) * 32;
+  const int tiles_n = (int)((a.N + 31) / 32), id = xcd_run(blockIdx.x, gridDim.x), slot = __builtin_amdgcn_readfirstlane(id / tiles_n);
+  const Slot s = find_slot(a.gr, slot, 5);
+  const int64_t n0 = (int64_t)(id - slot * tiles_n) * 32;
   if (!s.live || (s.group < 0 && !a.zero_outside)) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, half = lane >> 5;
   f32x16 acc;
@@ -882,7 +890,7 @@ __global__ __launch_bounds__(512) void grouped_small_kernel(const FwdArgs a) {
 // same number of rows to multiply however ragged the groups are.  A group that lies inside a chunk is finished in place; of one that spans
 // several, chunk c holds either its beginning (partial slot 2 c) or a later part that starts with the chunk (slot 2 c + 1; never two of a
 // kind), which wgrad_join_kernel adds in chunk order (no atomics).  The zeros of empty groups are written by workgroups of their own, the
-// first ZEROERS of the launch.
+// first `zeroers` of the launch.
 struct WgradArgs {
   Groups gr;
   int64_t N, K;
@@ -895,8 +903,19 @@ struct WgradArgs {
   int64_t ld_db;
   float* part_w;  // [2 chunks][N][K]
   float* part_b;  // [2 chunks][N]
-  int64_t chunk, chunks, tiles_k, tiles;
+  int64_t chunk, chunks;
+  int tiles_k, tiles;
+  int zeroers;  // a multiple of the XCDs: the other workgroups keep their places
 };
+
+struct WgradTile {
+  int chunk, n, k;
+};
+__device__ __forceinline__ WgradTile wgrad_tile(const WgradArgs& a) {  // of this workgroup, scalars
+  const int id = xcd_run(blockIdx.x - a.zeroers, gridDim.x - a.zeroers), chunk = __builtin_amdgcn_readfirstlane(id / a.tiles), tile = id - chunk * a.tiles;
+  const int n = __builtin_amdgcn_readfirstlane(tile / a.tiles_k);
+  return {chunk, n, tile - n * a.tiles_k};
+}
 
 struct Segment {  // the rows [begin, end) of a group inside a chunk
   int group;
@@ -904,40 +923,38 @@ struct Segment {  // the rows [begin, end) of a group inside a chunk
   int64_t slot;  // partial slot, -1: the whole group
 };
 
-// Walks the groups of chunk c.
+// Walks the groups of chunk c, from row to row: empty ones cost nothing.
 struct Segments {
   const WgradArgs& a;
   int64_t c, first, last;  // rows [first, last)
-  int i;                   // next edge index: group i - 1
+  int64_t at;              // the next row
 
   __device__ __forceinline__ Segments(const WgradArgs& args, int64_t chunk_id) : a(args), c(chunk_id) {
-    first = c * a.chunk;
+    first = at = c * a.chunk;
     last = min(first + a.chunk, a.gr.M);
-    // the group that holds the chunk's first row, or an earlier one that ends at or before it
-    i = c == 0 ? 1 : max(1, search(a.gr.G + 2, first, [&](int j) { return a.gr.edge(j); }));
   }
   __device__ __forceinline__ bool next(Segment& s) {
-    while (i <= a.gr.G) {
-      const int64_t b = a.gr.edge(i), e = a.gr.edge(i + 1);
-      if (b >= last) return false;
-      ++i;
-      const int64_t from = max(b, first), to = min(e, last);
-      if (from >= to) continue;  // empty, or before the chunk
-      s = {i - 2, from, to, b >= first && e <= last ? -1 : b >= first ? 2 * c : 2 * c + 1};
+    while (at < last) {
+      const int64_t from = at;
+      const int i = search(a.gr.G + 2, from, [&](int j) { return a.gr.edge(j); });  // holds row `from`
+      const int64_t b = a.gr.shared_edge(i), e = a.gr.shared_edge(i + 1);
+      if (e <= from) return false;  // (bounds that decrease)
+      at = min(e, last);
+      if (i == 0) continue;  // rows before the first group
+      if (i == a.gr.G + 1) return false;
+      s = {i - 1, from, at, b >= first && e <= last ? -1 : b >= first ? 2 * c : 2 * c + 1};
       return true;
     }
     return false;
   }
 };
 
-constexpr int ZEROERS = 8;  // (a multiple of the XCDs: the other workgroups keep their places)
-
-// dW, db of the empty groups among every ZEROERS-th 64
+// dW, db of the empty groups among every zeroers-th eight
 __device__ void write_empty_groups(const WgradArgs& a, int part) {
   const int lane = threadIdx.x & 63;
-  for (int64_t base = (int64_t)part * 64; base < a.gr.G; base += ZEROERS * 64) {
+  for (int64_t base = (int64_t)part * 8; base < a.gr.G; base += (int64_t)a.zeroers * 8) {
     const int g = (int)base + lane;
-    unsigned long long empty = __ballot(g < a.gr.G && a.gr.edge(g + 2) <= a.gr.edge(g + 1));
+    unsigned long long empty = __ballot(lane < 8 && g < a.gr.G && a.gr.edge(g + 2) <= a.gr.edge(g + 1));
     while (empty) {
       const int64_t group = base + __builtin_ctzll(empty);
       empty &= empty - 1;
@@ -972,11 +989,12 @@ template <class T, class TileT>
 __global__ __launch_bounds__(TileT::THREADS, 2) void grouped_wgrad_kernel(const WgradArgs a) {
   typedef typename TileT::OpA OpA;
   extern __shared__ __attribute__((aligned(16))) unsigned char raw_lds[];
-  if (blockIdx.x < ZEROERS) return write_empty_groups(a, blockIdx.x);
-  const int64_t id = xcd_run(blockIdx.x - ZEROERS, gridDim.x - ZEROERS), tile = id % a.tiles, n0 = (tile / a.tiles_k) * TileT::BM, k0 = (tile % a.tiles_k) * TileT::BN;
+  if ((int)blockIdx.x < a.zeroers) return write_empty_groups(a, blockIdx.x);
+  const WgradTile w = wgrad_tile(a);
+  const int64_t n0 = (int64_t)w.n * TileT::BM, k0 = (int64_t)w.k * TileT::BN;
   const bool sums = a.db && k0 == 0;
   constexpr int VEC = Geo<T>::VEC;
-  Segments walk(a, id / a.tiles);
+  Segments walk(a, w.chunk);
   Segment s;
   while (walk.next(s)) {
     TileT t;
@@ -1052,11 +1070,11 @@ __device__ __forceinline__ void wgrad_dma(const WgradArgs& a, int64_t c, int64_t
 template <class TileT>
 __global__ __launch_bounds__(TileT::THREADS, 2) void grouped_wgrad_dma_kernel(const WgradArgs a) {
   extern __shared__ __attribute__((aligned(16))) unsigned char raw_lds[];
-  if (blockIdx.x < ZEROERS) return write_empty_groups(a, blockIdx.x);
-  const int64_t id = xcd_run(blockIdx.x - ZEROERS, gridDim.x - ZEROERS), tile = id % a.tiles, n0 = (tile / a.tiles_k) * TileT::BM;
-  const int64_t k0 = (tile % a.tiles_k) * TileT::BN;
-  if (a.db && k0 == 0) wgrad_dma<TileT, true>(a, id / a.tiles, n0, k0, reinterpret_cast<typename TileT::Elem*>(raw_lds));
-  else wgrad_dma<TileT, false>(a, id / a.tiles, n0, k0, reinterpret_cast<typename TileT::Elem*>(raw_lds));
+  if ((int)blockIdx.x < a.zeroers) return write_empty_groups(a, blockIdx.x);
+  const WgradTile w = wgrad_tile(a);
+  const int64_t n0 = (int64_t)w.n * TileT::BM, k0 = (int64_t)w.k * TileT::BN;
+  if (a.db && w.k == 0) wgrad_dma<TileT, true>(a, w.chunk, n0, k0, reinterpret_cast<typename TileT::Elem*>(raw_lds));
+  else wgrad_dma<TileT, false>(a, w.chunk, n0, k0, reinterpret_cast<typename TileT::Elem*>(raw_lds));
 }
 
 // The parts of every group that spans chunks.  blockIdx.y = c: the group that begins in chunk c and reaches beyond it, if there is one,
@@ -1064,7 +1082,7 @@ __global__ __launch_bounds__(TileT::THREADS, 2) void grouped_wgrad_dma_kernel(co
 __global__ __launch_bounds__(256) void wgrad_join_kernel(const WgradArgs a) {
   const int64_t c0 = blockIdx.y, last = (c0 + 1) * a.chunk - 1;
   const int i = search(a.gr.G + 2, last, [&](int j) { return a.gr.edge(j); });
-  const int64_t start = a.gr.edge(i), end = a.gr.edge(i + 1);
+  const int64_t start = a.gr.shared_edge(i), end = a.gr.shared_edge(i + 1);
   if (i == 0 || i == a.gr.G + 1 || start < c0 * a.chunk || start > last || end <= last + 1) return;
   const int group = i - 1, parts = (int)((end - 1) / a.chunk - c0);  // later ones
   const int64_t nk = a.N * a.K, at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
@@ -1145,11 +1163,12 @@ template <class TileT>
 int forward_dma_launch(const char* me, const FwdArgs& a, hipStream_t st) {
   const int64_t tiles = (a.gr.M / TileT::BM + a.gr.G + 2) * dh::ceil_div(a.N, TileT::BN);
   const int64_t resident = (int64_t)CUS * (160 * 1024 / TileT::LDS_BYTES);
+  if (tiles > MAX_GRID - resident) return dh::fail(DH_ERR_INVALID, "%s: %lld tiles in one launch", me, (long long)tiles);
   static std::atomic<uint64_t> done{0};
   const int allowed = allow_lds(me, reinterpret_cast<const void*>(grouped_forward_dma_kernel<TileT>), TileT::LDS_BYTES, done);
   if (allowed != DH_OK) return allowed;
   hipLaunchKernelGGL((grouped_forward_dma_kernel<TileT>), dim3((unsigned)(tiles < resident ? tiles : resident)), dim3(TileT::THREADS), TileT::LDS_BYTES, st,
-                     a, tiles);
+                     a, (int)tiles);
   return dh::check_launch(me);
 }
 
@@ -1192,20 +1211,22 @@ int forward_pick(const char* me, const FwdArgs& a, hipStream_t st) {
 }
 
 // The tile of the weight gradient and its chunks: as many chunks x tiles as workgroups run at a time, so that all end together; no chunk below
-// 32 rows, which a step of k would not fill.  The large tile reads its operands least often; where it would leave a chunk short (few rows,
+// 32 rows, which a step of k would not fill, or below two groups of the mean size where that is less: a workgroup takes its groups one after
+// the other (1000 rows of 300 types: 81 us with 32 rows a chunk, 44 with 8; 500 rows of 17: 20 with 32, 25 with 8).  The large tile reads its operands least often; where it would leave a chunk short (few rows,
 // or a small dW) the smaller one has more workgroups to share the groups among.
 struct WgradPlan {
   int edge;  // rows and columns of the tile
   int64_t chunk;
 };
-WgradPlan wgrad_plan(int64_t M, int64_t N, int64_t K, int dtype) {
+WgradPlan wgrad_plan(int64_t M, int64_t N, int64_t K, int64_t G, int dtype) {
   const int large = dtype == DH_DTYPE_BF16 ? 256 : 128;
   WgradPlan p{};
   for (int edge : {large, large / 2}) {
     const int64_t tiles = dh::ceil_div(N, edge) * dh::ceil_div(K, edge), resident = edge == 256 ? CUS : 2 * CUS;
     const int64_t chunks = resident / tiles > 1 ? resident / tiles : 1;
-    int64_t rows = dh::ceil_div(dh::ceil_div(M, chunks), 32) * 32;
-    if (rows < 32) rows = 32;
+    const int64_t least = 2 * M / (G > 0 ? G : 1) >= 32 ? 32 : dh::ceil_div(2 * M / (G > 0 ? G : 1) + 1, 8) * 8;
+    int64_t rows = dh::ceil_div(dh::ceil_div(M, chunks), least) * least;
+    if (rows < least) rows = least;
     p = {edge, rows};
     if (rows >= 4096) break;  // (1563 rows a chunk: 50000 x 1000 -> 304 76 us with the 256 tile, 62 with 128)
   }
@@ -1214,9 +1235,11 @@ WgradPlan wgrad_plan(int64_t M, int64_t N, int64_t K, int dtype) {
 
 template <class TileT>
 int wgrad_grid(const char* me, WgradArgs& a) {
-  a.tiles_k = dh::ceil_div(a.K, TileT::BN);
-  a.tiles = dh::ceil_div(a.N, TileT::BM) * a.tiles_k;
-  if (a.chunks * a.tiles > MAX_GRID - ZEROERS) return dh::fail(DH_ERR_INVALID, "%s: %lld tiles in one launch", me, (long long)(a.chunks * a.tiles));
+  const int64_t tiles_k = dh::ceil_div(a.K, TileT::BN), tiles = dh::ceil_div(a.N, TileT::BM) * tiles_k;
+  if (tiles > MAX_GRID || a.chunks * tiles > MAX_GRID - a.zeroers)
+    return dh::fail(DH_ERR_INVALID, "%s: %lld tiles in one launch", me, (long long)(a.chunks * tiles));
+  a.tiles_k = (int)tiles_k;
+  a.tiles = (int)tiles;
   return DH_OK;
 }
 
@@ -1226,7 +1249,7 @@ int wgrad_launch(const char* me, WgradArgs a, hipStream_t st) {
   const int allowed = allow_lds(me, reinterpret_cast<const void*>(grouped_wgrad_kernel<T, TileT>), TileT::LDS_BYTES, done);
   const int rc = allowed == DH_OK ? wgrad_grid<TileT>(me, a) : allowed;
   if (rc != DH_OK) return rc;
-  hipLaunchKernelGGL((grouped_wgrad_kernel<T, TileT>), dim3((unsigned)(a.chunks * a.tiles + ZEROERS)), dim3(TileT::THREADS), TileT::LDS_BYTES, st, a);
+  hipLaunchKernelGGL((grouped_wgrad_kernel<T, TileT>), dim3((unsigned)(a.chunks * a.tiles + a.zeroers)), dim3(TileT::THREADS), TileT::LDS_BYTES, st, a);
   return dh::check_launch(me);
 }
 
@@ -1236,7 +1259,7 @@ int wgrad_dma_launch(const char* me, WgradArgs a, hipStream_t st) {
   const int allowed = allow_lds(me, reinterpret_cast<const void*>(grouped_wgrad_dma_kernel<TileT>), TileT::LDS_BYTES, done);
   const int rc = allowed == DH_OK ? wgrad_grid<TileT>(me, a) : allowed;
   if (rc != DH_OK) return rc;
-  hipLaunchKernelGGL((grouped_wgrad_dma_kernel<TileT>), dim3((unsigned)(a.chunks * a.tiles + ZEROERS)), dim3(TileT::THREADS), TileT::LDS_BYTES, st, a);
+  hipLaunchKernelGGL((grouped_wgrad_dma_kernel<TileT>), dim3((unsigned)(a.chunks * a.tiles + a.zeroers)), dim3(TileT::THREADS), TileT::LDS_BYTES, st, a);
   return dh::check_launch(me);
 }
 
@@ -1270,9 +1293,9 @@ extern "C" int dh_gemm_grouped(int64_t M, int64_t N, int64_t K, int64_t G, int t
   return trans_b ? forward_pick<float, false>(me, a, st) : forward_pick<float, true>(me, a, st);
 }
 
-extern "C" size_t dh_gemm_grouped_wgrad_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype) {
-  if (M <= 0 || N <= 0 || K <= 0) return 16;
-  const int64_t chunks = dh::ceil_div(M, wgrad_plan(M, N, K, dtype).chunk);
+extern "C" size_t dh_gemm_grouped_wgrad_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t G, int dtype) {
+  if (M <= 0 || N <= 0 || K <= 0 || G <= 0) return 16;
+  const int64_t chunks = dh::ceil_div(M, wgrad_plan(M, N, K, G, dtype).chunk);
   return chunks < 2 ? 16 : 16 + (size_t)(2 * chunks) * (size_t)N * (size_t)(K + 1) * 4;
 }
 
@@ -1287,15 +1310,16 @@ extern "C" int dh_gemm_grouped_wgrad(int64_t M, int64_t N, int64_t K, int64_t G,
   if (!dW || !group_ptr || (M > 0 && (!dY || !X))) return dh::fail(DH_ERR_INVALID, "%s: null tensor", me);
   if (ldy < N || ldx < K || ldw < K || (G > 1 && stride_w < (N - 1) * ldw + K) || (db && ld_db < N))
     return dh::fail(DH_ERR_INVALID, "%s: leading dimension below the row length", me);
-  const size_t need = dh_gemm_grouped_wgrad_workspace_bytes(M, N, K, dtype);
+  const size_t need = dh_gemm_grouped_wgrad_workspace_bytes(M, N, K, G, dtype);
   if (!workspace || workspace_bytes < need) return dh::fail(DH_ERR_WORKSPACE, "%s: workspace of %zu bytes, need %zu", me, workspace_bytes, need);
   if (!dh::aligned16(workspace)) return dh::fail(DH_ERR_INVALID, "%s: workspace must be 16-byte aligned", me);
   WgradArgs a{};
   a.gr = {group_ptr, M, (int)G};
   a.N = N; a.K = K; a.dY = dY; a.X = X; a.ldy = ldy; a.ldx = ldx; a.dW = dW; a.ldw = ldw; a.stride_w = stride_w; a.dw_bf16 = dw_dtype == DH_DTYPE_BF16;
   a.db = db; a.ld_db = ld_db;
-  const WgradPlan plan = wgrad_plan(M, N, K, dtype);
+  const WgradPlan plan = wgrad_plan(M, N, K, G, dtype);
   a.chunk = plan.chunk;
+  a.zeroers = G <= 64 ? 8 : 64;
   a.chunks = M > 0 ? dh::ceil_div(M, a.chunk) : 1;
   a.part_w = static_cast<float*>(workspace);
   a.part_b = a.part_w + 2 * a.chunks * N * K;

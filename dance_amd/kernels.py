@@ -842,7 +842,7 @@ def gemm_grouped_wgrad(dY: torch.Tensor, X: torch.Tensor, group_ptr: torch.Tenso
     dW = X.new_empty((G, N, K)) if out_dtype is None or out_dtype is xt else torch.empty((G, N, K), dtype=out_dtype, device=X.device)
     db = torch.empty((G, N), dtype=torch.float32, device=X.device) if want_bias else None
     with _one_device(dY, X, group_ptr):
-        ws_bytes = lib.dh_gemm_grouped_wgrad_workspace_bytes(M, N, K, dt)
+        ws_bytes = lib.dh_gemm_grouped_wgrad_workspace_bytes(M, N, K, G, dt)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=X.device)
         _call("gemm_grouped_bf16_tn" if dt else "gemm_grouped_f32_tn", lib.dh_gemm_grouped_wgrad, M, N, K, G, dt, yp, ldy, xp, ldx, gp, dW.data_ptr(),
               K or 1, N * K, _elem(dW, "dW"), None if db is None else db.data_ptr(), N or 1, ws.data_ptr(), ws_bytes, _stream())

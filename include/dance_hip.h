@@ -902,7 +902,7 @@ DH_API int dh_residual_norm_backward(int64_t M, int64_t D, int dtype, const void
 DH_API int dh_gemm_grouped(int64_t M, int64_t N, int64_t K, int64_t G, int trans_b, int dtype, const void* X, int64_t ldx, const void* W, int64_t ldw,
                     int64_t stride_w, const int32_t* group_ptr, const float* bias, int64_t ld_bias, int act, void* Y, int64_t ldy, int y_dtype,
                     int zero_outside, dh_stream_t stream);
-DH_API size_t dh_gemm_grouped_wgrad_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype);
+DH_API size_t dh_gemm_grouped_wgrad_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t G, int dtype);
 DH_API int dh_gemm_grouped_wgrad(int64_t M, int64_t N, int64_t K, int64_t G, int dtype, const void* dY, int64_t ldy, const void* X, int64_t ldx,
                           const int32_t* group_ptr, void* dW, int64_t ldw, int64_t stride_w, int dw_dtype, float* db, int64_t ld_db,
                           void* workspace, size_t workspace_bytes, dh_stream_t stream);

@@ -50,11 +50,11 @@ def test_grouped_wgrad_refusals(lib, bad):
 
 
 def test_grouped_wgrad_workspace(lib):
-    need = lib.dh_gemm_grouped_wgrad_workspace_bytes(8, 4, 4, 0)
+    need = lib.dh_gemm_grouped_wgrad_workspace_bytes(8, 4, 4, 2, 0)
     assert _wgrad(lib, ws_bytes=need - 1) == WORKSPACE and _wgrad(lib, ws=None) == WORKSPACE
     for dtype in (0, 1):
-        assert lib.dh_gemm_grouped_wgrad_workspace_bytes(31, 512, 2000, dtype) == 16        # one chunk of rows: no partial results
-        assert lib.dh_gemm_grouped_wgrad_workspace_bytes(200003, 512, 2000, dtype) >= 2 * 2 * 512 * 2001 * 4
+        assert lib.dh_gemm_grouped_wgrad_workspace_bytes(31, 512, 2000, 1, dtype) == 16        # one chunk of rows: no partial results
+        assert lib.dh_gemm_grouped_wgrad_workspace_bytes(200003, 512, 2000, 9, dtype) >= 2 * 2 * 512 * 2001 * 4
 
 
 def _norm_fwd(lib, **kw):
@@ -146,16 +146,19 @@ def _segments(ptr, M, chunk, chunks, c):
     """(group, begin, end, partial slot) of a chunk of rows, as Segments walks them."""
     e, G = _edges(ptr, M), len(ptr) - 1
     first, last = c * chunk, min(c * chunk + chunk, M)
-    i = 1 if c == 0 else max(1, max(j for j in range(G + 2) if e[j] <= first))
-    out = []
-    while i <= G:
+    out, at = [], first
+    while at < last:
+        lo = at
+        i = max(j for j in range(G + 2) if e[j] <= lo)
         b, t = e[i], e[i + 1]
-        if b >= last:
+        if t <= lo:  # (bounds that decrease)
             break
-        i += 1
-        lo, hi = max(b, first), min(t, last)
-        if lo < hi:
-            out.append((i - 2, lo, hi, -1 if b >= first and t <= last else 2 * c if b >= first else 2 * c + 1))
+        at = min(t, last)
+        if i == 0:
+            continue
+        if i == G + 1:
+            break
+        out.append((i - 1, lo, at, -1 if b >= first and t <= last else 2 * c if b >= first else 2 * c + 1))
     return out
 
 
@@ -164,7 +167,7 @@ def test_weight_gradient_segments(seed):
     """Every row of a group is in one segment, every group with rows is finished once (in place, or by the join of its parts, which reads
     exactly the slots that were written), and no slot is written twice."""
     rng = np.random.default_rng(seed)
-    M, G, chunk = int(rng.integers(0, 700)), int(rng.integers(1, 60)), int(rng.choice([32, 64, 96, 1000]))
+    M, G, chunk = int(rng.integers(0, 700)), int(rng.integers(1, 60)), int(rng.choice([8, 32, 96, 1000]))
     ptr = np.sort(rng.integers(0, M + 1, G + 1)) if seed % 3 else np.sort(rng.choice([0, M // 3, M // 2, M], G + 1))
     chunks = max(1, -(-M // chunk))
     owner, done, slots = np.full(M, -1), np.zeros(G, int), {}
