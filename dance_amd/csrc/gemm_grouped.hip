@@ -1306,6 +1306,7 @@ extern "C" int dh_gemm_grouped_wgrad(int64_t M, int64_t N, int64_t K, int64_t G,
   const int rc = check_grouped(me, M, N, K, G, dtype);
   if (rc != DH_OK) return rc;
   if (dw_dtype != DH_DTYPE_F32 && dw_dtype != DH_DTYPE_BF16) return dh::fail(DH_ERR_INVALID, "%s: output dtype %d", me, dw_dtype);
+  if (db && G > 0 && N > 0 && K == 0) return dh::fail(DH_ERR_INVALID, "%s: db without a column of X", me);
   if (G == 0 || N == 0 || K == 0) return DH_OK;
   if (!dW || !group_ptr || (M > 0 && (!dY || !X))) return dh::fail(DH_ERR_INVALID, "%s: null tensor", me);
   if (ldy < N || ldx < K || ldw < K || (G > 1 && stride_w < (N - 1) * ldw + K) || (db && ld_db < N))

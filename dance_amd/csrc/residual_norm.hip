@@ -493,11 +493,15 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256) void residual_norm_backw
       const float u = dn * w[i];
       s[0] = __builtin_fmaf(u, f[i], s[0]);
       s[1] += u;
-      s[2] += dg;
       gf[i] = dg;
       dr[i] = u;
     }
     if (FULL && valid && a.dgate) store_row<T, V, CH, TAIL>(a.dgate, row * a.lddg, t, tpr, a.D, gf);
+    if (a.gate_kind == GATE_ROW && a.dgate) {  // (behind the row's end lies a product of zero with some value of the row, which may be infinite)
+      zero_tail<V, CH, TAIL>(t, tpr, a.D, gf);
+#pragma unroll
+      for (int i = 0; i < E; ++i) s[2] += gf[i];
+    }
     if (a.has_post || (a.gate_kind == GATE_ROW && a.dgate)) row_sums<MODE, 3>(s, tpr, lds);
     if (a.gate_kind == GATE_ROW && a.dgate && valid && t == 0) Elem<T>::put(a.dgate, row * a.lddg, s[2]);
     if (a.df && valid) {
@@ -702,6 +706,8 @@ extern "C" int dh_residual_norm_backward(int64_t M, int64_t D, int dtype, const 
   const char* me = "dh_residual_norm_backward";
   const int rc = check_common(me, M, D, dtype, f, x, ldf, ldx, gate, ldg, gate_kind, gate_sigmoid, kind, 0.f);
   if (rc != DH_OK) return rc;
+  if ((!has_post && (dw1 || db1)) || (!has_pre && (dw2 || db2)) || (gate_kind == GATE_NONE && dgate))
+    return dh::fail(DH_ERR_INVALID, "%s: the gradient of a parameter that is not there", me);
   hipStream_t st = dh::as_stream(stream);
   const bool col_gate = gate_kind == GATE_CHANNEL || gate_kind == GATE_SCALAR;
   if (M == 0) {  // no rows: the column gradients are empty sums
@@ -728,7 +734,7 @@ extern "C" int dh_residual_norm_backward(int64_t M, int64_t D, int dtype, const 
   a.df = df; a.dx = dx; a.lddf = lddf; a.lddx = lddx; a.lddg = lddg;
   a.dgate = col_gate ? nullptr : dgate;
   a.partials = static_cast<float*>(workspace);
-  a.want_w1 = has_post && dw1; a.want_b1 = has_post && db1; a.want_w2 = dw2 != nullptr; a.want_b2 = db2 != nullptr;
+  a.want_w1 = dw1 != nullptr; a.want_b1 = db1 != nullptr; a.want_w2 = dw2 != nullptr; a.want_b2 = db2 != nullptr;
   a.want_gate = col_gate && dgate;
   const int vw = dtype == DH_DTYPE_BF16 ? 8 : 4;
   const Split s = split_of(D, vw);

@@ -732,7 +732,7 @@ def _mat(t: Optional[torch.Tensor], dtype, name: str):
         raise ValueError(f"{name} must be 2-d, got shape {tuple(t.shape)}")
     rows, cols = t.shape
     ld, step = t.stride()
-    if step != 1 and rows and cols:
+    if step != 1 and rows and cols > 1:  # (a single column's step means nothing)
         raise ValueError(f"{name} must be contiguous in its last dimension")
     if rows <= 1:
         ld = cols or 1
@@ -756,7 +756,7 @@ def _stack(W: torch.Tensor, dtype, name: str):
         ldw = cols or 1
     if groups <= 1:
         sw = 0
-    if groups and rows and cols and (step != 1 or ldw < cols or sw < 0):
+    if groups and rows and cols and ((step != 1 and cols > 1) or ldw < cols or sw < 0):
         raise ValueError(f"{name}: strides {W.stride()} of shape {tuple(shape)} are not supported")
     return W.data_ptr(), ldw, sw, shape
 
@@ -790,7 +790,8 @@ def gemm_grouped(X: torch.Tensor, W: torch.Tensor, group_ptr: torch.Tensor, *, t
 
     X [M, K] fp32 or bf16 with its rows sorted by group; W [G, N, K] (``trans_b``, torch.nn.Linear's layout) or [G, K, N] of X's dtype;
     ``group_ptr`` int32 [G + 1] on the device, non-decreasing; bias fp32 [G, N].  Groups may be empty, sizes are not read by the host (no
-    synchronisation, capturable).  Rows that belong to no group are zero in a fresh result and left as they are in ``out``."""
+    synchronisation, capturable).  Rows that belong to no group are zero in a fresh result and left as they are in ``out``, whose memory, from
+    its first element to its last, may hold no operand's."""
     lib = _lib_ready()
     xt = X.dtype
     dt = _elem(X, "X")
@@ -837,8 +838,9 @@ def gemm_grouped_wgrad(dY: torch.Tensor, X: torch.Tensor, group_ptr: torch.Tenso
     G = group_ptr.numel() - 1
     if M != My:
         raise ValueError(f"dY and X must have the same rows, got shapes {tuple(dY.shape)} and {tuple(X.shape)}")
-    if K == 0 and want_bias:
-        raise ValueError("gemm_grouped_wgrad: the bias gradient needs at least one input column")
+    if K == 0 and want_bias:  # no products, the column sums all the same
+        db = gemm_grouped_wgrad(dY, dY[:, :1], group_ptr, want_bias=True)[1] if N else torch.empty((G, 0), dtype=torch.float32, device=X.device)
+        return torch.empty((G, N, 0), dtype=out_dtype or xt, device=X.device), db
     dW = X.new_empty((G, N, K)) if out_dtype is None or out_dtype is xt else torch.empty((G, N, K), dtype=out_dtype, device=X.device)
     db = torch.empty((G, N), dtype=torch.float32, device=X.device) if want_bias else None
     with _one_device(dY, X, group_ptr):

@@ -877,7 +877,7 @@ DH_API int dh_grad_clip(int n, const void* const* grads_host, void* const* out_h
  * parameters are f32.  gate_kind: dh_gate; gate_sigmoid: act = sigmoid.  kind: dh_norm.  stats [M, 4] f32 (16-byte aligned; NULL: not
  * kept): mean and rstd of both norms, what the backward needs.  r may be NULL when has_pre.
  * Backward: dr, dh (either may be NULL) -> df, dx, dgate (row / full: dtype; scalar / channel: f32) and the column sums dw1, db1, dw2,
- * db2 (f32), each skipped when NULL; sums over rows in a fixed order.                                                                     */
+ * db2 (f32), each skipped when NULL; sums over rows in a fixed order.  No output may overlap an input.                                    */
 DH_API int dh_residual_norm_forward(int64_t M, int64_t D, int dtype, const void* f, int64_t ldf, const void* x, int64_t ldx, const void* gate,
                              int64_t ldg, int gate_kind, int gate_sigmoid, float scale, int kind, float eps, int has_post, const float* w1,
                              const float* b1, int has_pre, const float* w2, const float* b2, void* r, int64_t ldr, void* h, int64_t ldh,
@@ -897,8 +897,8 @@ DH_API int dh_residual_norm_backward(int64_t M, int64_t D, int dtype, const void
  *                          W_g without (W [G][K][N]); X, W: dtype; Y: y_dtype (rounded once); bias [G][N] f32, row stride ld_bias, or NULL.
  *                          Rows of no group (before ptr[0], from ptr[G] on) are set to zero with zero_outside, left as they are without.
  *   dh_gemm_grouped_wgrad: dW_g = sum_i dY[i]^T X[i] ([G][N][K], dw_dtype) and, db != NULL, db_g = sum_i dY[i] (f32); an empty group's are
- *                          zero; sums over rows in a fixed order.
- * Accumulation in fp32 on the matrix cores; M < 2^31 rows.                                                                                 */
+ *                          zero; sums over rows in a fixed order.  db needs K >= 1.
+ * Accumulation in fp32 on the matrix cores; M < 2^31 rows; no output may overlap an input.                                                 */
 DH_API int dh_gemm_grouped(int64_t M, int64_t N, int64_t K, int64_t G, int trans_b, int dtype, const void* X, int64_t ldx, const void* W, int64_t ldw,
                     int64_t stride_w, const int32_t* group_ptr, const float* bias, int64_t ld_bias, int act, void* Y, int64_t ldy, int y_dtype,
                     int zero_outside, dh_stream_t stream);

@@ -289,3 +289,38 @@ def test_nothing_to_multiply(cuda_device):
         b = torch.randn(1, 5, device=DEV)
         y = kernels.gemm_grouped(z(6, 0), z(1, 5, 0), torch.tensor([0, 6], dtype=torch.int32, device=DEV), bias=b, out_dtype=torch.float32)
         assert torch.equal(y, b.expand(6, 5))  # no columns: the bias
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_single_columns_of_any_stride(cuda_device, dtype):
+    """A matrix of one column is contiguous whatever that dimension's stride: transposes of a row."""
+    from dance_amd.autograd import grouped_linear
+    ptr = torch.tensor([0, 7, 20, 33], dtype=torch.int32, device=DEV)
+    g = torch.Generator().manual_seed(3)
+    draw = lambda *shape: torch.randn(*shape, generator=g).to(DEV, dtype)
+    for K, N in ((1, 5), (24, 1), (1, 1)):
+        odd = lambda t: t.as_strided(t.shape, (*t.stride()[:-1], 7)) if t.shape[-1] == 1 else t
+        x, w, b, dy = draw(33, K), draw(3, N, K), draw(3, N).float(), draw(33, N)
+        results = []
+        for change in (lambda t: t, odd):
+            leaves = [change(t).detach().requires_grad_() for t in (x, w, b)]
+            y = grouped_linear(leaves[0], leaves[1], ptr, leaves[2])
+            y.backward(change(dy))
+            results.append([y] + [t.grad for t in leaves])
+        assert odd(x).stride() != x.stride() or odd(b).stride() != b.stride()
+        assert all(torch.equal(a, c) for a, c in zip(*results))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_bias_gradient_without_input_columns(cuda_device, dtype):
+    from dance_amd.autograd import grouped_linear
+    ptr = torch.tensor([1, 3, 3, 6], dtype=torch.int32, device=DEV)
+    x = torch.zeros(7, 0, dtype=dtype, device=DEV, requires_grad=True)
+    w = torch.zeros(3, 4, 0, dtype=dtype, device=DEV, requires_grad=True)
+    b = torch.ones(3, 4, device=DEV, requires_grad=True)
+    y = grouped_linear(x, w, ptr, b)
+    dy = torch.arange(28, device=DEV).reshape(7, 4).to(dtype)
+    y.backward(dy)
+    d = dy.float()
+    assert torch.equal(b.grad, torch.stack([d[1:3].sum(0), torch.zeros(4, device=DEV), d[3:6].sum(0)]))  # (small integers: exact)
+    assert w.grad.shape == (3, 4, 0) and x.grad.shape == (7, 0)

@@ -231,6 +231,39 @@ def test_rows_do_not_touch_each_other(cuda_device, dtype):
     assert not bool(r.any()) and not bool(h.any())
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("D", [3, 20, 23, 64, 300, 513, 2050])
+def test_infinity_and_row_gate(cuda_device, D, dtype):
+    """An infinite element makes its row's gate gradient infinite, not NaN, wherever in the row it lies: nothing behind a row's end enters."""
+    from dance_amd import kernels
+    for at in {0, D // 2, D - 1}:
+        f, x = torch.ones(5, D, dtype=dtype, device=DEV), torch.ones(5, D, dtype=dtype, device=DEV)
+        dr = torch.ones(5, D, dtype=dtype, device=DEV)
+        f[2, at], f[3, at] = float("inf"), float("-inf")
+        gate = torch.full((5, 1), 0.5, dtype=dtype, device=DEV)
+        r, _, stats = kernels.residual_norm_forward(f, x, gate=gate, want_stats=True)
+        g = kernels.residual_norm_backward(dr, None, f, x, stats, gate=gate, want=("f", "gate"))
+        want = f.double().sum(1, keepdim=True)  # D itself in the finite rows: exact in fp32, one rounding in bf16
+        assert torch.equal(g["gate"], want.to(dtype)) and torch.equal(g["f"], dr * 0.5)
+        assert torch.equal(r, x + f * 0.5)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_row_gate_of_any_stride(cuda_device, dtype):
+    """A [M, 1] gate is contiguous whatever its last stride: the transpose of a row."""
+    from dance_amd.autograd import residual_norm
+    v = _inputs(33, 40, dtype, "none", "layer")
+    row = torch.randn(1, 33, generator=torch.Generator().manual_seed(1)).to(DEV, dtype)
+    gates = [row.reshape(33, 1).clone().requires_grad_(), row.t().detach().requires_grad_()]
+    assert gates[0].stride() != gates[1].stride()
+    results = []
+    for gate in gates:
+        r, h = residual_norm(v["f"], v["x"], gate=gate, pre=(v["w2"], v["b2"]))
+        torch.autograd.backward((r, h), (v["dr"], v["dh"]))
+        results.append((r, h, gate.grad))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
 @pytest.mark.parametrize("D", [40, 512, 2000])
 def test_offset_rows(cuda_device, D):
     """Rows of a large common offset and small differences: the differences are what the norm sees.  mean carries 22 roundings of the row's

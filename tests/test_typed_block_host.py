@@ -44,7 +44,7 @@ def _wgrad(lib, **kw):
 
 
 @pytest.mark.parametrize("bad", [dict(M=-1), dict(G=-1), dict(dtype=9), dict(dw_dtype=9), dict(dY=None), dict(X=None), dict(ptr=None), dict(dW=None),
-                                 dict(ldy=3), dict(ldx=3), dict(ldw=3), dict(stride_w=15), dict(db=P, ld_db=3), dict(ws=P + 4)])
+                                 dict(ldy=3), dict(ldx=3), dict(ldw=3), dict(stride_w=15), dict(db=P, ld_db=3), dict(ws=P + 4), dict(K=0, db=P, ld_db=4)])
 def test_grouped_wgrad_refusals(lib, bad):
     assert _wgrad(lib, **bad) == INVALID
 
@@ -82,7 +82,8 @@ def _norm_bwd(lib, **kw):
 
 
 @pytest.mark.parametrize("bad", [dict(D=0), dict(stats=None), dict(stats=P + 8), dict(pre=0), dict(dr=None, dh=None), dict(lddr=7), dict(lddh=7),
-                                 dict(lddf=7), dict(lddx=7), dict(gk=4, gate=P, ldg=8, dgate=P, lddg=7)])
+                                 dict(lddf=7), dict(lddx=7), dict(gk=4, gate=P, ldg=8, dgate=P, lddg=7), dict(post=0, dw1=P),
+                                 dict(post=0, db1=P), dict(pre=0, dh=None, dw2=P), dict(pre=0, dh=None, db2=P), dict(dgate=P)])
 def test_residual_norm_backward_refusals(lib, bad):
     assert _norm_bwd(lib, **bad) == INVALID
     assert _norm_bwd(lib, ws_bytes=lib.dh_residual_norm_backward_workspace_bytes(4, 8) - 1) == WORKSPACE
