@@ -12,12 +12,16 @@
 //
 // Bound: HBM.  Forward reads f and x and writes r and h; backward reads f, x, dr, dh and writes df, dx: r is recomputed from f, x and the
 // gate (the same bytes as reading it back, and unrounded in the bf16 case), only mean and rstd of each row are kept.
-// Split: a row lives in the registers of 8 .. 64 lanes of a wave (rows up to 512 columns) or of a workgroup of 256 / 512 (up to 4096),
-// 4 or 8 elements per lane (16 spill: the backward holds ten arrays of them), 16 bytes per access whatever the rows' alignment (global memory takes unaligned
-// accesses); a row length that is no multiple of the access reads its last piece from D - V and shifts it down in registers (ODD), so
-// no load is guarded.  The two-pass variance and both reductions of the backward run on registers.  Column gradients are summed in
-// registers over the rows a workgroup walks, joined in its LDS, written once per workgroup and added up by a second kernel in workgroup
-// order: no atomics, the result does not depend on timing.  All arithmetic is fp32; bf16 rounds once, at the stores.
+// Split: a row lives in the registers of 8 .. 64 lanes of a wave (rows up to 512 columns) or of a workgroup of two to eight waves (up to
+// 4096), 4 or 8 elements per lane (16 spill: the backward holds ten arrays of them), 16 bytes per access whatever the rows' alignment
+// (global memory takes unaligned accesses); a row length that is no multiple of the access reads its last piece from D - V and shifts it
+// down in registers (ODD), so no load is guarded.  The two-pass variance and both reductions of the backward run on registers.  Column
+// gradients are summed in registers over the rows a workgroup walks, joined in its LDS, written once per workgroup and added up by a second
+// kernel in workgroup order: no atomics, the result does not depend on timing.  All arithmetic is fp32; bf16 rounds once, at the stores.
+// Measured, layer norms and channel gate, forward / backward: 200003 x 512 bf16 165 / 282 us (5.0 / 4.4 TB/s), fp32 321 / 446 us (5.1 / 5.5);
+// 50001 x 504 bf16 41 / 76 us, x 500 (ODD) 50 / 94, x 501 54 / 101; 50001 x 1000 110 / 188.  The bf16 backward has the arithmetic of twice
+// as many elements to a byte and comes near the vector units' limit.
+#include <algorithm>
 #include <atomic>
 #include <type_traits>
 
@@ -81,6 +85,15 @@ struct Elem<float> {
       put(p, i, v[0]);
     }
   }
+  // the first n (uniform) of four values
+  static __device__ __forceinline__ void store_first(void* p, int64_t i, int n, const float* v) {
+    typedef float f32x2u __attribute__((ext_vector_type(2), aligned(4)));
+    if (n & 2) *reinterpret_cast<f32x2u*>(static_cast<float*>(p) + i) = f32x2u{v[0], v[1]};
+    if (n & 1) {
+      const float last = v[2], first = v[0];
+      put(p, i + (n & 2), (n & 2) ? last : first);
+    }
+  }
 };
 template <>
 struct Elem<uint16_t> {
@@ -97,6 +110,27 @@ struct Elem<uint16_t> {
     } else {
       put(p, i, v[0]);
     }
+  }
+  // the first n (uniform) of eight values
+  static __device__ __forceinline__ void store_first(void* p, int64_t i, int n, const float* v) {
+    typedef uint32_t u32x2u __attribute__((ext_vector_type(2), aligned(2)));
+    typedef uint32_t u32u __attribute__((aligned(2)));
+    uint16_t* to = static_cast<uint16_t*>(p) + i;
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = pack_bf16(v[2 * e], v[2 * e + 1]);
+    if (n & 4) {
+      *reinterpret_cast<u32x2u*>(to) = u32x2u{w[0], w[1]};
+      to += 4;
+      w[0] = w[2];
+      w[1] = w[3];
+    }
+    if (n & 2) {
+      *reinterpret_cast<u32u*>(to) = w[0];
+      to += 2;
+      w[0] = w[1];
+    }
+    if (n & 1) *to = (uint16_t)w[0];
   }
 };
 
@@ -163,12 +197,32 @@ __device__ __forceinline__ void row_sums(float (&v)[N], int tpr, float* lds) {
 
 // A lane's columns: chunk c covers (c * tpr + t) * V .. + V.  Chunks that end behind D read the last V values of the row instead; with
 // ODD their values are shifted down to the columns they belong to.  What lies at columns >= D is some value of the same row.
+// (The two values are read before the choice: a choice between array elements themselves becomes an index into the registers, a chain of
+// compares each; rows of 500 columns took five times as long as rows of 504.)
 template <int V>
 __device__ __forceinline__ void shift_down(int by, float* v) {
 #pragma unroll
   for (int bit = 1; bit < V; bit *= 2)
 #pragma unroll
-    for (int e = 0; e + bit < V; ++e) v[e] = (by & bit) ? v[e + bit] : v[e];
+    for (int e = 0; e + bit < V; ++e) {
+      const float far = v[e + bit], near = v[e];
+      v[e] = (by & bit) ? far : near;
+    }
+}
+// the same of 16 bytes, PER elements to a word
+template <int PER>
+__device__ __forceinline__ void shift_words(int by, uint32_t (&w)[4]) {
+#pragma unroll
+  for (int bit = 1; bit < 4; bit *= 2)
+#pragma unroll
+    for (int e = 0; e + bit < 4; ++e) {
+      const uint32_t far = w[e + bit], near = w[e];
+      w[e] = (by & (bit * PER)) ? far : near;
+    }
+  if (PER == 2) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = __builtin_amdgcn_alignbyte(w[e < 3 ? e + 1 : e], w[e], (by & 1) * 2);
+  }
 }
 // A row's pieces as they lie in memory (requested before any of them is used).
 template <class T, int V, int CH>
@@ -191,9 +245,10 @@ struct RawRow {
     }
   }
   template <int TAIL>
-  __device__ __forceinline__ void unpack(int t, int tpr, int D, float (&v)[V * CH]) const {
+  __device__ __forceinline__ void unpack(int t, int tpr, int D, float (&v)[V * CH]) {
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
+      if constexpr (TAIL == ODD) shift_words<V / 4>(max((c * tpr + t) * V - (D - V), 0), w[c]);
       if constexpr (sizeof(T) == 2) {
 #pragma unroll
         for (int e = 0; e < WORDS; ++e) {
@@ -204,7 +259,6 @@ struct RawRow {
 #pragma unroll
         for (int e = 0; e < WORDS; ++e) v[c * V + e] = __uint_as_float(w[c][e]);
       }
-      if (TAIL == ODD) shift_down<V>(max((c * tpr + t) * V - (D - V), 0), v + c * V);
     }
   }
 };
@@ -236,11 +290,7 @@ __device__ __forceinline__ void store_row(void* p, int64_t row_at, int t, int tp
   for (int c = 0; c < CH; ++c) {
     const int col = (c * tpr + t) * V;
     if (TAIL == WHOLE || (TAIL == ODD ? col + V <= D : col < D)) Elem<T>::template store<V>(p, row_at + col, v + c * V);
-    else if (TAIL == ODD && col < D) {
-#pragma unroll
-      for (int e = 0; e < V; ++e)
-        if (col + e < D) Elem<T>::put(p, row_at + col + e, v[c * V + e]);
-    }
+    else if (TAIL == ODD && col < D) Elem<T>::store_first(p, row_at + col, D % V, v + c * V);
   }
 }
 
@@ -391,30 +441,20 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256) void residual_norm_backw
 #pragma unroll
   for (int i = 0; i < E; ++i) acc_w1[i] = acc_b1[i] = acc_w2[i] = acc_b2[i] = acc_g[i] = 0.f;
   const bool col_gate = !FULL && (a.gate_kind == GATE_CHANNEL || a.gate_kind == GATE_SCALAR);
-  // A wave's rows: the next one is requested while the present one is worked on (200003 x 512 bf16: 371 -> 332 us).  Not where a workgroup
-  // holds a row: there the registers for it cost a wave per SIMD (4099 x 2000 bf16: 38.6 -> 42.0 us), nor in the forward (193 -> 202).
-  constexpr bool AHEAD = MODE != GROUP;
   const bool use_x = a.x && a.dh;  // r enters through the second norm only
-  RawRow<T, V, CH> rf, rx, rr, rh, rg;
-  float4 st_next;
-  float grow_next = 1.f;
-  auto request = [&](int64_t base) __attribute__((always_inline)) {
+  for (int64_t base = (int64_t)blockIdx.x * rows_per_block; base < a.M; base += (int64_t)gridDim.x * rows_per_block) {
     const int64_t row = min(base + sub, a.M - 1);
+    const bool valid = base + sub < a.M;
+    float f[E], x[E], gf[E], dr[E], dh[E], w[E], b[E];
+    RawRow<T, V, CH> rf, rx, rr, rh, rg;
+    float grow = 1.f;
     rf.load(a.f, row * a.ldf, t, tpr, a.D);
     if (use_x) rx.load(a.x, row * a.ldx, t, tpr, a.D);
     if (a.dr) rr.load(a.dr, row * a.lddr, t, tpr, a.D);
     if (a.dh) rh.load(a.dh, row * a.lddh, t, tpr, a.D);
     if (FULL) rg.load(a.gate, row * a.ldg, t, tpr, a.D);
-    else if (a.gate_kind == GATE_ROW) grow_next = Elem<T>::get(a.gate, row * a.ldg);
-    st_next = *reinterpret_cast<const float4*>(a.stats + row * 4);
-  };
-  const int64_t stride = (int64_t)gridDim.x * rows_per_block;
-  if (AHEAD) request((int64_t)blockIdx.x * rows_per_block);
-  for (int64_t base = (int64_t)blockIdx.x * rows_per_block; base < a.M; base += stride) {
-    const int64_t row = min(base + sub, a.M - 1);
-    const bool valid = base + sub < a.M;
-    float f[E], x[E], gf[E], dr[E], dh[E], w[E], b[E];
-    if (!AHEAD) request(base);
+    else if (a.gate_kind == GATE_ROW) grow = Elem<T>::get(a.gate, row * a.ldg);
+    const float4 st = *reinterpret_cast<const float4*>(a.stats + row * 4);
     rf.template unpack<TAIL>(t, tpr, a.D, f);
     if (use_x) rx.template unpack<TAIL>(t, tpr, a.D, x);
     else {
@@ -428,9 +468,6 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256) void residual_norm_backw
     }
     if (a.dh) rh.template unpack<TAIL>(t, tpr, a.D, dh);
     if (FULL) rg.template unpack<TAIL>(t, tpr, a.D, gf);
-    const float4 st = st_next;
-    const float grow = grow_next;
-    if (AHEAD && base + stride < a.M) request(base + stride);
     // the gate and its derivative's factor
     if (!FULL) {
       if (a.gate_kind == GATE_CHANNEL) load_params<V, CH, TAIL>(static_cast<const float*>(a.gate), 1.f, t, tpr, a.D, gf);
@@ -565,7 +602,8 @@ __global__ __launch_bounds__(256) void sum_kernel(const float* __restrict__ v, i
 }
 
 // How a row is split: V elements per access (16 bytes; rows shorter than that: 1), CH accesses per lane, tpr lanes per row.  As many
-// lanes as the row has accesses up to a wave, then up to 8 elements per lane, then a workgroup of 256 or 512 threads per row.
+// lanes as the row has accesses up to a wave, then up to 8 elements per lane, then a workgroup of as many waves as that takes (50001 x 1000
+// bf16 on two waves 107 / 185 us forward / backward, on four 157 / 245).
 struct Split {
   int v, ch, tpr;
   int mode, tail;
@@ -578,7 +616,7 @@ Split split_of(int64_t D, int vec_width) {
   const int64_t eight = 8 / s.v;  // accesses that hold eight elements
   if (n > 64 * eight) {
     s.mode = GROUP;
-    s.tpr = n <= 256 * eight ? 256 : 512;
+    s.tpr = 64 * (int)dh::ceil_div(n, 64 * eight);
   } else {
     s.tpr = 8;
     while (s.tpr < 64 && s.tpr < n) s.tpr *= 2;
@@ -586,15 +624,14 @@ Split split_of(int64_t D, int vec_width) {
   }
   s.ch = 1;
   while ((int64_t)s.ch * s.tpr < n) s.ch *= 2;
-  if (s.mode == GROUP) s.ch = (int)eight;
   s.tail = D % s.v != 0 ? ODD : (int64_t)s.tpr * s.ch == n ? WHOLE : SHORT;
   return s;
 }
 
 int64_t rows_per_block(const Split& s) { return s.mode == GROUP ? 1 : 256 / s.tpr; }
 
-// Workgroups of a launch: what the chip holds at a time, so that no second, partly filled round follows (1024 workgroups where 768 fit took
-// 534 us instead of 400 at 200003 x 512 bf16), and the rows shared out evenly among them.
+// Workgroups of a launch: what the chip holds at a time, so that no second, partly filled round follows (backward, 200003 x 512 bf16: 1024
+// workgroups where 768 fit took 398 us instead of 312), and the rows shared out evenly among them.
 int64_t even_grid(int64_t M, int64_t per_block, int64_t resident) {
   const int64_t need = dh::ceil_div(M, per_block);
   return need <= resident ? need : dh::ceil_div(need, dh::ceil_div(need, resident));
@@ -605,16 +642,17 @@ int64_t launch(bool backward, const Args& a, const Split& s, hipStream_t st) {
   const dim3 b(MODE == GROUP ? a.tpr : 256);
   const void* kernel = backward ? reinterpret_cast<const void*>(residual_norm_backward_kernel<T, V, CH, MODE, FULL, TAIL>)
                                 : reinterpret_cast<const void*>(residual_norm_forward_kernel<T, V, CH, MODE, FULL, TAIL>);
-  // (a row of 257 .. 512 threads is asked for separately: static per direction and width)
-  static std::atomic<int> per_cu[2][2];
-  int fit = per_cu[backward][b.x > 256].load(std::memory_order_relaxed);
+  static std::atomic<int> per_cu[2][9];  // by direction and waves of a workgroup
+  int fit = per_cu[backward][b.x / 64].load(std::memory_order_relaxed);
   if (fit == 0) {
     if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kernel, (int)b.x, 0) != hipSuccess || fit < 1) {
       (void)hipGetLastError();
       fit = 2;
     }
-    per_cu[backward][b.x > 256].store(fit, std::memory_order_relaxed);
+    per_cu[backward][b.x / 64].store(fit, std::memory_order_relaxed);
   }
+  // the forward runs no faster with more than 20 waves on a CU, wide bf16 rows slower (200003 x 512: 174 us with 24, 166 with 20, 185 with 12)
+  if (!backward) fit = std::min(fit, 20 / ((int)b.x / 64));
   int64_t resident = (int64_t)256 * fit;
   if (backward && resident > BWD_BLOCKS) resident = BWD_BLOCKS;
   const int64_t grid = even_grid(a.M, rows_per_block(s), resident);

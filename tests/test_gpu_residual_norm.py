@@ -144,7 +144,7 @@ def _run(M, D, dtype, gate, gate_act="none", kind="layer", post=True, pre=True, 
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("M,D", [(1, 16), (37, 50), (5, 200), (9, 512), (3, 513), (130, 31), (3, 2000), (2, 4096), (3, 4095), (2, 1030)])
+@pytest.mark.parametrize("M,D", [(1, 16), (37, 50), (5, 200), (9, 512), (3, 513), (130, 31), (3, 2000), (2, 4096), (3, 4095), (2, 1030), (3, 2700)])
 @pytest.mark.parametrize("gate", ["none", "scalar", "channel", "row", "full"])
 @pytest.mark.parametrize("kind", ["layer", "rms"])
 def test_shapes(cuda_device, dtype, M, D, gate, kind):
