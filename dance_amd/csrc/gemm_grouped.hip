@@ -8,6 +8,12 @@
 // them: group g owns the row slots [floor(ptr[g] / R) + g, floor(ptr[g + 1] / R) + g + 1), R rows each, always enough for its
 // ceil(len / R) tiles and monotone in g, so a workgroup finds its group with one 64-wide search per 64 groups instead of a prefix sum;
 // at most one slot per group and none of the work is wasted on it.
+//
+// Bound: the matrix cores for many rows (200003 rows of 9 types, 2000 -> 512 bf16: Y 505 us, dX 630, dW and db 470 + 32: 810 / 650 / 870 TFLOP/s;
+// fp32 100003 rows: 125 / 122 / 134 TFLOP/s), latency for few (16 rows of 8 types, 400 -> 200: 7.3 us; 500 rows of 17 types, forward and all
+// gradients: 36 us in four launches).  Four kernels: a tile filled by LDS DMA for aligned operands, one staged through registers for the
+// others (60000 x 401 -> 203 bf16 168 us for the three products, 106 at 400 -> 200), one of 32 x 32 with K split over the waves for few rows,
+// and the weight gradient's, which cuts the rows into equal chunks whatever the groups.
 #include <atomic>
 #include <type_traits>
 
@@ -204,7 +210,7 @@ struct Operand {
 
 // f(m, n, values) for the elements of a workgroup's accumulators, four consecutive n of a row at a time: the B rows are given as the
 // instruction's first operand, so a lane's 32x32 results are row m = lane & 31, n = (r & 3) + 8 (r >> 2) + 4 (lane >> 5), r = 0 .. 15
-// (with A first a lane holds 16 rows of one column: four times as many, two-byte, stores: 818 against 726 us at 200003 x 2000 -> 512 bf16)
+// (with A first a lane holds 16 rows of one column: four times as many, two-byte, stores)
 template <int MI, int NI, int WC, class F>
 __device__ __forceinline__ void each4(const f32x16 (&acc)[MI][NI], int64_t m0, int64_t mlim, int64_t n0, int64_t nlim, F&& f) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -1186,14 +1192,18 @@ int small_launch(const char* me, const FwdArgs& a, hipStream_t st) {
 
 template <class T, bool W_KM>
 int forward_pick(const char* me, const FwdArgs& a, hipStream_t st) {
-  const int64_t tiles = (a.gr.M / 128 + a.gr.G) * dh::ceil_div(a.N, 128);  // of 128 x 128
   constexpr int VEC = 16 / sizeof(T);
   constexpr bool BF16 = sizeof(T) == 2;
   const bool dma = dma_rows(a.X, a.ldx, VEC) && dma_rows(a.W, a.ldw, VEC) && a.stride_w % VEC == 0 && a.K % VEC == 0 && (!W_KM || a.N % VEC == 0);
-  // A handful of tiles (bf16 1000 x 400 -> 200, 18 tiles: 5.9 us against 12.4 of the DMA tile; 3000 x 512 -> 512, 100 tiles: 24.6 against
-  // 14.7; fp32 the same shapes: 8.7 against 15.5 and 44 against 27; 1000 x 2000 -> 512, 32 tiles: 61 against 49), or few rows per group: fp32
-  // 4000 rows of 100 types, 2000 -> 512: 302 us against 383.  (bf16 the same: 148 against 107: there the DMA tile stays ahead.)
-  if (tiles <= (BF16 ? 64 : 24) || (a.gr.M <= (int64_t)48 * a.gr.G && !(BF16 && dma))) return small_launch<T, W_KM>(me, a, st);
+  // Few 32 x 32 tiles, in us, small against DMA tile: bf16 500 rows of 9 types 400 -> 200 (168 tiles) 5.2 / 10.8, 1500 of 30 types (532) 8.5 /
+  // 10.7, 3000 of 3 types 512 -> 256 (768) 15.8 / 12.3; fp32 the first 8.2 / 14.0, 500 of 17 types 200 -> 400 (416) 7.5 / 8.8, 1500 of 30
+  // types 15.5 / 13.3.  Against the staged tile: bf16 1500 of 30 types 401 -> 203 (532) 14.7 / 16.3, 203 -> 401 (988) 14.6 / 12.7; fp32 2000
+  // rows 511 -> 510 (1008) 36 / 46, 3000 of 3 types 255 -> 510 (1536) 28 / 29.
+  const int64_t small_tiles = (a.gr.M / 32 + a.gr.G) * dh::ceil_div(a.N, 32);
+  if (small_tiles <= (BF16 ? 640 : dma ? 420 : 1536)) return small_launch<T, W_KM>(me, a, st);
+  // Few rows per group: fp32 4000 rows of 100 types, 2000 -> 512: 302 us against 383.  (bf16 the same: 148 against 107: there the DMA tile
+  // stays ahead.)
+  if (a.gr.M <= (int64_t)48 * a.gr.G && !(BF16 && dma)) return small_launch<T, W_KM>(me, a, st);
   if (dma) {
     if constexpr (sizeof(T) == 2) {
       // three rounds of 256 x 256 tiles: 200003 x 400 -> 200 (791 tiles) 90 us against 96 of the 128 x 128 one, which has two workgroups on a CU
@@ -1203,7 +1213,7 @@ int forward_pick(const char* me, const FwdArgs& a, hipStream_t st) {
     } else {
       // fp32 with less than a round of workgroups: 64 x 64 (20011 x 512 -> 256, 336 tiles of 128: 68 / 67 us against 78 / 65; 60000 x 400 ->
       // 200, 996 tiles: 141 against 128)
-      if (tiles < 2 * CUS) return forward_dma_launch<DmaTile<T, false, W_KM, 1, 1, 2, 2>>(me, a, st);
+      if ((a.gr.M / 128 + a.gr.G) * dh::ceil_div(a.N, 128) < 2 * CUS) return forward_dma_launch<DmaTile<T, false, W_KM, 1, 1, 2, 2>>(me, a, st);
     }
     return forward_dma_launch<DmaTile<T, false, W_KM, 2, 2, 2, 2>>(me, a, st);
   }
@@ -1212,8 +1222,9 @@ int forward_pick(const char* me, const FwdArgs& a, hipStream_t st) {
 
 // The tile of the weight gradient and its chunks: as many chunks x tiles as workgroups run at a time, so that all end together; no chunk below
 // 32 rows, which a step of k would not fill, or below two groups of the mean size where that is less: a workgroup takes its groups one after
-// the other (1000 rows of 300 types: 81 us with 32 rows a chunk, 44 with 8; 500 rows of 17: 20 with 32, 25 with 8).  The large tile reads its operands least often; where it would leave a chunk short (few rows,
-// or a small dW) the smaller one has more workgroups to share the groups among.
+// the other (1000 rows of 300 types: 81 us with 32 rows a chunk, 44 with 8; 500 rows of 17: 20 with 32, 25 with 8).  The large tile reads its
+// operands least often; where it would leave a chunk short (few rows, or a small dW) the smaller one has more workgroups to share the
+// groups among.
 struct WgradPlan {
   int edge;  // rows and columns of the tile
   int64_t chunk;
