@@ -5,7 +5,7 @@
 //   out_t[i] = g_t[i] * min(1, max_norm / (norm + 1e-6))
 //
 // Bound: HBM.  The scaling cannot start before the norm is known, so a set larger than the caches is read twice and written once: 328 million
-// fp32 elements in 24 tensors 243 us (5.4 TB/s) and 515 us (5.1 TB/s).  The launches and their latencies for small ones: 2000 x 512, 512 x 30
+// fp32 elements in 32 tensors 243 us (5.4 TB/s) and 515 us (5.1 TB/s).  The launches and their latencies for small ones: 2000 x 512, 512 x 30
 // and their biases 9 us, 320 tensors of at most 200 x 64 30 us.
 // Layout: the tensors' addresses travel as kernel arguments, 128 per launch (nothing is uploaded, so a captured call replays with the
 // addresses it was recorded with); a launch walks its tensors in chunks of 16 KB of fp32, up to GRID workgroups striding over the chunks.
