@@ -106,10 +106,16 @@ def _one_device(*tensors: Optional[torch.Tensor]):
 _HERE = contextlib.nullcontext()
 
 
+_ready = None
+
+
 def _lib_ready():
-    lib = _lib.load()
-    _lib.require_device()
-    return lib
+    global _ready
+    if _ready is None:  # (a device that has been there stays)
+        lib = _lib.load()
+        _lib.require_device()
+        _ready = lib
+    return _ready
 
 
 def spmm_csr(rowptr: torch.Tensor, col: torch.Tensor, val: Optional[torch.Tensor], Z: torch.Tensor, *,
@@ -877,11 +883,15 @@ def _norm_params(p, D: int, name: str):
     """(has, weight pointer, bias pointer) of a norm given as None or (weight or None, bias or None)."""
     if p is None:
         return 0, None, None
-    w, b = p
-    for t in (w, b):
-        if t is not None and t.shape != (D, ):
-            raise ValueError(f"{name} weight and bias must be [{D}], got shape {tuple(t.shape)}")
-    return 1, _dev(w, torch.float32, name, 1), _dev(b, torch.float32, name, 1)
+    return 1, _columns(p[0], D, name), _columns(p[1], D, name)
+
+
+def _columns(t: Optional[torch.Tensor], D: int, name: str) -> Optional[int]:
+    if t is None or (t.dtype is torch.float32 and t.is_cuda and t.is_contiguous() and t.shape == (D, )):
+        return None if t is None else t.data_ptr()
+    if t.shape != (D, ):
+        raise ValueError(f"{name} weight and bias must be [{D}], got shape {tuple(t.shape)}")
+    return _dev(t, torch.float32, name, 1)
 
 
 def _gate_args(gate, kind: int, dtype):
@@ -951,27 +961,32 @@ def residual_norm_backward(dr: Optional[torch.Tensor], dh: Optional[torch.Tensor
     has_post, w1, b1 = _norm_params(post, D, "post")
     has_pre, w2, _ = _norm_params(pre, D, "pre")
     gp, ldg = _gate_args(gate, gk, f.dtype)
-    df = f.new_empty((M, D)) if "f" in want else None
-    dx = f.new_empty((M, D)) if x is not None and "x" in want else None
-    dgate = torch.empty_like(gate, memory_format=torch.contiguous_format) if gate is not None and "gate" in want else None
+    out = {}
+    if "f" in want:
+        out["f"] = f.new_empty((M, D))
+    if x is not None and "x" in want:
+        out["x"] = f.new_empty((M, D))
+    if gate is not None and "gate" in want:
+        out["gate"] = torch.empty_like(gate, memory_format=torch.contiguous_format)
     # one allocation for the column gradients of the norms
     names = [n for n, there in (("w1", has_post), ("b1", has_post), ("w2", has_pre), ("b2", has_pre)) if there and n in want]
-    cols = dict(zip(names, torch.empty((len(names), D), dtype=torch.float32, device=f.device).unbind(0))) if names else {}
+    if names:
+        out.update(zip(names, torch.empty((len(names), D), dtype=torch.float32, device=f.device).unbind(0)))
+    p = {n: t.data_ptr() for n, t in out.items()}.get
+    w2_wanted, b2_wanted = p("w2"), p("b2")
     if dh is None:  # nothing flows through the second norm
         for n in ("w2", "b2"):
-            if n in cols:
-                cols[n].zero_()
-    ptr = lambda t: None if t is None else t.data_ptr()
-    pw1, pb1, pw2, pb2 = (ptr(cols.get(n)) for n in ("w1", "b1", "w2", "b2"))
+            if n in out:
+                out[n].zero_()
+        w2_wanted = b2_wanted = None
     with _one_device(f, x, gate, stats, dr, dh, *(post or ()), *(pre or ())):
         ws_bytes = lib.dh_residual_norm_backward_workspace_bytes(M, D)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=f.device)
         _call("residual_norm_backward", lib.dh_residual_norm_backward, M, D, dt, *_mat(f, f.dtype, "f"), *_mat(x, f.dtype, "x"), gp, ldg, gk,
               1 if gate_sigmoid else 0, scale, kind, has_post, w1, b1, has_pre, w2, _dev(stats, torch.float32, "stats", 2), *_mat(dr, f.dtype, "dr"),
-              *_mat(dh, f.dtype, "dh"), ptr(df), D, ptr(dx), D, ptr(dgate), D if gk == GATE_FULL else 1, pw1, pb1, None if dh is None else pw2,
-              None if dh is None else pb2, ws.data_ptr(), ws_bytes, _stream())
-    new = {"f": df, "x": dx, "gate": dgate, **cols}
-    return {n: t for n, t in new.items() if t is not None}
+              *_mat(dh, f.dtype, "dh"), p("f"), D, p("x"), D, p("gate"), D if gk == GATE_FULL else 1, p("w1"), p("b1"), w2_wanted, b2_wanted,
+              ws.data_ptr(), ws_bytes, _stream())
+    return out
 
 
 # ---- graph builders ----------------------------------------------------------------------------------------
