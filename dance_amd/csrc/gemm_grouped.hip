@@ -14,6 +14,7 @@
 // gradients: 36 us in four launches).  Four kernels: a tile filled by LDS DMA for aligned operands, one staged through registers for the
 // others (60000 x 401 -> 203 bf16 168 us for the three products, 106 at 400 -> 200), one of 32 x 32 with K split over the waves for few rows,
 // and the weight gradient's, which cuts the rows into equal chunks whatever the groups.
+#include <algorithm>
 #include <atomic>
 #include <type_traits>
 
@@ -119,14 +120,21 @@ struct Geo<float> {
   static constexpr int VEC = 4, BK = 32, LD_MK = 36;
 };
 
+// The value again, unknown to the compiler: what is computed from it is not kept in registers across the loop over tiles (hoisted, the
+// lane-dependent addresses of all phases together spilled 180 registers).
+__device__ __forceinline__ int anew(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
 // R rows (m or n) x BK of an operand.  KM = false: memory is [row][k]; true: [k][row].  Both stay as they lie in memory in LDS too:
 // a [k][row] image is read back transposed (bf16: ds_read_b64_tr_b16) or by single elements (fp32).
 template <class T, bool KM, int R, int THREADS>
 struct Operand {
   static constexpr int VEC = Geo<T>::VEC, BK = Geo<T>::BK;
-  // [k][row] images: bf16 rows of R + 32 elements (64 bytes past a multiple of 256: the four k rows that one transposing read takes from
+  // [k][row] images: bf16 rows of R + 32 elements, or 32 (an odd number of 64 bytes: the four k rows that one transposing read takes from
   // lie on distinct banks); fp32 rows of R + 8 (the two half waves read rows 4 apart: 32 banks apart)
-  static constexpr int LD = KM ? (sizeof(T) == 2 ? R + 32 : R + 8) : Geo<T>::LD_MK;
+  static constexpr int LD = KM ? (sizeof(T) == 2 ? (R == 32 ? R : R + 32) : R + 8) : Geo<T>::LD_MK;
   static constexpr int ELEMS = KM ? BK * LD : R * LD;
   static constexpr int CPR = KM ? R / VEC : 8;                        // 16-byte pieces per image row
   static constexpr int PIECES = (KM ? BK : R) * CPR / THREADS;        // per thread
@@ -134,47 +142,83 @@ struct Operand {
   static_assert(PIECES >= 1 && PIECES * THREADS == (KM ? BK : R) * CPR, "tile does not divide among the threads");
 
   u32x4 reg[2][PIECES];  // two steps in flight
-  const T* p[PIECES];  // the lane's pieces of the next step
-  int valid[PIECES];   // [k][row] images: values of the piece below rlim
+  const T* p[KM ? 1 : PIECES];  // the lane's pieces of the next step; [k][row] images: the first, the others lie whole rows behind it
+  int valid;                    // [k][row] images: values of the pieces below rlim, negative behind it
+  bool wide;                    // the memory rows hold a whole piece
 
-  static __device__ __forceinline__ u32x4 guarded(const T* p, int64_t n_valid) {
-    if (n_valid >= VEC) return *reinterpret_cast<const u32x4u*>(p);
-    T e[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) e[i] = i < n_valid ? p[i] : T(0);
-    u32x4 v;
-    __builtin_memcpy(&v, e, 16);
-    return v;
-  }
-  // rows [r0, rlim) of the operand from k0 on.  Rows beyond rlim read some row below it (their products are never stored).
-  __device__ __forceinline__ void start(const T* base, int64_t ld, int64_t r0, int64_t rlim, int64_t k0) {
+  // rows [r0, rlim) of the operand from k0 on, up to k_end.  Rows beyond rlim read some row below it (their products are never stored).
+  __device__ __forceinline__ void start(const T* base, int64_t ld, int64_t r0, int64_t rlim, int64_t k0, int64_t k_end) {
     const int tid = threadIdx.x;
+    wide = (KM ? rlim : k_end) >= VEC;
+    const int ir = tid / CPR, ic = (tid % CPR) * VEC;
+    if constexpr (KM) {
+      p[0] = base + (k0 + ir) * ld + r0 + ic;
+      valid = (int)min((int64_t)VEC, rlim - r0 - ic);
+    } else {
 #pragma unroll
-    for (int q = 0; q < PIECES; ++q) {
-      const int ir = tid / CPR + q * ROWS_PER_PASS, ic = (tid % CPR) * VEC;
-      if (!KM) {
-        p[q] = base + min(r0 + ir, rlim - 1) * ld + k0 + ic;
-      } else {
-        p[q] = base + (k0 + ir) * ld + r0 + ic;
-        valid[q] = (int)max((int64_t)0, min((int64_t)VEC, rlim - r0 - ic));
-      }
+      for (int q = 0; q < PIECES; ++q) p[q] = base + min(r0 + ir + q * ROWS_PER_PASS, rlim - 1) * ld + k0 + ic;
     }
   }
-  // the next BK of k, of which `left` exist (the others read as zero).  FULL: all of them (and for KM all R rows).
+  // values of the lane's pieces within their memory rows, of a step that has `left` k
+  __device__ __forceinline__ int inside(int left) const { return KM ? valid : min(VEC, left - (int)(threadIdx.x % CPR) * VEC); }
+
+  // The next BK of k, of which `left` exist.  FULL: all of them (and for KM all R rows).  Otherwise nothing here is guarded, which would
+  // cost a round trip per guard: k rows that do not exist repeat the last one, a piece that passes its memory row's end is fetched from
+  // where it just does not, and finish() moves and clears, when the values have arrived.
   template <bool FULL, int U>
-  __device__ __forceinline__ void load(int64_t ld, int64_t left) {
-    const int tid = threadIdx.x;
+  __device__ __forceinline__ void load(int64_t ld, int left) {
+    const int tid = anew(threadIdx.x);
 #pragma unroll
     for (int q = 0; q < PIECES; ++q) {
-      if (FULL) reg[U][q] = *reinterpret_cast<const u32x4u*>(p[q]);
-      else if (!KM) reg[U][q] = guarded(p[q], left - (tid % CPR) * VEC);
-      else reg[U][q] = guarded(p[q], tid / CPR + q * ROWS_PER_PASS < left ? valid[q] : 0);
-      p[q] += KM ? BK * ld : BK;
+      const T* from = KM ? p[0] + q * ROWS_PER_PASS * ld : p[KM ? 0 : q];
+      if (!FULL) {
+        const int in = inside(left);
+        if (KM) from -= max(0, tid / CPR + q * ROWS_PER_PASS - (left - 1)) * ld;
+        if (wide) {
+          from += min(0, in - VEC);
+        } else {  // a memory row shorter than a piece: its values one by one
+          T e[VEC];
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) e[i] = from[min(i, in - 1)];
+          __builtin_memcpy(&reg[U][q], e, 16);
+        }
+      }
+      if (FULL || wide) reg[U][q] = *reinterpret_cast<const u32x4u*>(from);
+      if (!KM) p[KM ? 0 : q] += BK;
+    }
+    if (KM) p[0] += BK * ld;
+  }
+  // the pieces of a step that was not FULL: into place, zeros behind the memory row's end and in k rows that do not exist
+  template <int U>
+  __device__ __forceinline__ void finish(int left) {
+    constexpr int PER = 4 / sizeof(T);  // values of a word
+#pragma unroll
+    for (int q = 0; q < PIECES; ++q) {
+      const int tid = anew(threadIdx.x), in = inside(left), by = wide ? VEC - in : 0;
+      const int n = !KM || (int)(tid / CPR) + q * ROWS_PER_PASS < left ? in : 0;
+      uint32_t w[4] = {reg[U][q][0], reg[U][q][1], reg[U][q][2], reg[U][q][3]};
+#pragma unroll
+      for (int bit = 1; bit < 4; bit *= 2)
+#pragma unroll
+        for (int e = 0; e + bit < 4; ++e) {
+          const uint32_t far = w[e + bit], near = w[e];
+          w[e] = (by & (bit * PER)) ? far : near;
+        }
+      if (PER == 2) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = __builtin_amdgcn_alignbyte(w[e < 3 ? e + 1 : e], w[e], (by & 1) * 2);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        uint32_t keep = n > e * PER ? 0xffffffffu : 0u;
+        if (PER == 2) keep &= n > e * 2 + 1 ? 0xffffffffu : 0xffffu;
+        reg[U][q][e] = w[e] & keep;
+      }
     }
   }
   template <int U>
   __device__ __forceinline__ void store(T* img) const {
-    const int tid = threadIdx.x;
+    const int tid = anew(threadIdx.x);
 #pragma unroll
     for (int q = 0; q < PIECES; ++q) {
       const int ir = tid / CPR + q * ROWS_PER_PASS, ic = (tid % CPR) * VEC;
@@ -213,7 +257,7 @@ struct Operand {
 // (with A first a lane holds 16 rows of one column: four times as many, two-byte, stores)
 template <int MI, int NI, int WC, class F>
 __device__ __forceinline__ void each4(const f32x16 (&acc)[MI][NI], int64_t m0, int64_t mlim, int64_t n0, int64_t nlim, F&& f) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int tid = anew(threadIdx.x), lane = tid & 63, wave = tid >> 6;
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
     const int64_t m = m0 + (wave / WC) * MI * 32 + i * 32 + (lane & 31);
@@ -290,21 +334,25 @@ struct Tile {
     const bool whole = (!A_KM || m0 + BM <= mlim) && (!B_KM || n0 + BN <= nlim);
     OpA a;
     OpB b;
-    a.start(A, lda, m0, mlim, k_begin);
-    b.start(B, ldb, n0, nlim, k_begin);
+    a.start(A, lda, m0, mlim, k_begin, k_end);
+    b.start(B, ldb, n0, nlim, k_begin, k_end);
+    auto left = [&](int64_t t) { return (int)min((int64_t)BK, k_end - k_begin - t * BK); };
     auto fetch = [&](int64_t t, auto buf) __attribute__((always_inline)) {
       constexpr int U = decltype(buf)::value;
-      const int64_t left = k_end - k_begin - t * BK;
-      if (whole && left >= BK) {
+      if (whole && left(t) == BK) {
         a.template load<true, U>(lda, BK);
         b.template load<true, U>(ldb, BK);
       } else {
-        a.template load<false, U>(lda, left);
-        b.template load<false, U>(ldb, left);
+        a.template load<false, U>(lda, left(t));
+        b.template load<false, U>(ldb, left(t));
       }
     };
-    auto put = [&](auto buf) __attribute__((always_inline)) {  // the buffer's step into the stage of the same parity
+    auto put = [&](int64_t t, auto buf) __attribute__((always_inline)) {  // the buffer's step t into the stage of the same parity
       constexpr int U = decltype(buf)::value;
+      if (!whole || left(t) < BK) {
+        a.template finish<U>(left(t));
+        b.template finish<U>(left(t));
+      }
       a.template store<U>(lds + U * STAGE);
       b.template store<U>(lds + U * STAGE + OpA::ELEMS);
       seen(a.reg[U]);
@@ -314,12 +362,12 @@ struct Tile {
     const int64_t steps = (k_end - k_begin + BK - 1) / BK;
     fetch(0, Even{});
     if (steps > 1) fetch(1, Odd{});
-    put(Even{});
+    put(0, Even{});
     if (steps > 2) fetch(2, Even{});
     __syncthreads();
     auto step = [&](int64_t t, auto mine, auto other) __attribute__((always_inline)) {
       if (t + 1 < steps) {
-        put(other);
+        put(t + 1, other);
         if (t + 3 < steps) fetch(t + 3, other);
       }
       products(lds + decltype(mine)::value * STAGE);
@@ -374,13 +422,6 @@ typedef const __attribute__((address_space(1))) void* global_ptr;
 typedef __attribute__((address_space(3))) void* lds_ptr;
 
 __device__ __attribute__((aligned(16))) const uint32_t zero_piece[4] = {0, 0, 0, 0};
-
-// The value again, unknown to the compiler: what is computed from it is not kept in registers across the loop over tiles (hoisted, the
-// lane-dependent addresses of all phases together spilled 180 registers).
-__device__ __forceinline__ int anew(int v) {
-  asm volatile("" : "+v"(v));
-  return v;
-}
 
 // a lane's share of a 32-row fragment: 16 bytes, 8 bf16 or 4 fp32 of k
 template <class T>
@@ -892,11 +933,14 @@ __global__ __launch_bounds__(512) void grouped_small_kernel(const FwdArgs a) {
 
 // ---- dW, db --------------------------------------------------------------------------------------------------------------------------
 // dW_g [N][K] = sum over the group's rows of dY[i, n] X[i, k]: both operands [k][row] images with the rows as the contraction.  The rows are
-// cut into equal chunks whatever the groups: a workgroup takes one tile of dW through one chunk, group by group, so every workgroup has the
-// same number of rows to multiply however ragged the groups are.  A group that lies inside a chunk is finished in place; of one that spans
+// cut into chunks of equal work whatever the groups: a workgroup takes one tile of dW through one chunk, group by group.  A group costs its
+// rows and, for the start and the end of its tile, about as much as GROUP_ROWS rows: row r of group g lies at position r + g GROUP_ROWS of a
+// line that is cut into equal pieces, a closed form of the bounds again.  A group that lies inside a chunk is finished in place; of one that spans
 // several, chunk c holds either its beginning (partial slot 2 c) or a later part that starts with the chunk (slot 2 c + 1; never two of a
 // kind), which wgrad_join_kernel adds in chunk order (no atomics).  The zeros of empty groups are written by workgroups of their own, the
 // first `zeroers` of the launch.
+constexpr int GROUP_ROWS = 64;
+
 struct WgradArgs {
   Groups gr;
   int64_t N, K;
@@ -909,9 +953,10 @@ struct WgradArgs {
   int64_t ld_db;
   float* part_w;  // [2 chunks][N][K]
   float* part_b;  // [2 chunks][N]
-  int64_t chunk, chunks;
+  int64_t chunk, chunks;  // positions of a chunk
   int tiles_k, tiles;
   int zeroers;  // a multiple of the XCDs: the other workgroups keep their places
+  int slices;
 };
 
 struct WgradTile {
@@ -921,6 +966,17 @@ __device__ __forceinline__ WgradTile wgrad_tile(const WgradArgs& a) {  // of thi
   const int id = xcd_run(blockIdx.x - a.zeroers, gridDim.x - a.zeroers), chunk = __builtin_amdgcn_readfirstlane(id / a.tiles), tile = id - chunk * a.tiles;
   const int n = __builtin_amdgcn_readfirstlane(tile / a.tiles_k);
   return {chunk, n, tile - n * a.tiles_k};
+}
+
+// where a group (of those with the two groups of no weight) begins on the line; the group at position s; the first row at s or behind it
+__device__ __forceinline__ int64_t place_of(int i, int64_t start) { return start + (int64_t)max(i - 1, 0) * GROUP_ROWS; }
+__device__ __forceinline__ int group_at(const Groups& gr, int64_t s) {
+  return search(gr.G + 2, s, [&](int j) { return place_of(j, gr.edge(j)); });
+}
+__device__ __forceinline__ int64_t row_at(const Groups& gr, int64_t s) {
+  const int i = group_at(gr, s);
+  const int64_t start = gr.shared_edge(i);
+  return min(start + max((int64_t)0, s - place_of(i, start)), gr.shared_edge(i + 1));
 }
 
 struct Segment {  // the rows [begin, end) of a group inside a chunk
@@ -936,8 +992,8 @@ struct Segments {
   int64_t at;              // the next row
 
   __device__ __forceinline__ Segments(const WgradArgs& args, int64_t chunk_id) : a(args), c(chunk_id) {
-    first = at = c * a.chunk;
-    last = min(first + a.chunk, a.gr.M);
+    first = at = row_at(a.gr, c * a.chunk);
+    last = row_at(a.gr, (c + 1) * a.chunk);
   }
   __device__ __forceinline__ bool next(Segment& s) {
     while (at < last) {
@@ -955,26 +1011,26 @@ struct Segments {
   }
 };
 
-// dW, db of the empty groups among every zeroers-th eight
+// dW, db of the empty groups: every group cut into `slices` runs of rows, run u of group g written by workgroup (g slices + u) mod zeroers
 __device__ void write_empty_groups(const WgradArgs& a, int part) {
-  const int lane = threadIdx.x & 63;
-  for (int64_t base = (int64_t)part * 8; base < a.gr.G; base += (int64_t)a.zeroers * 8) {
-    const int g = (int)base + lane;
-    unsigned long long empty = __ballot(lane < 8 && g < a.gr.G && a.gr.edge(g + 2) <= a.gr.edge(g + 1));
-    while (empty) {
-      const int64_t group = base + __builtin_ctzll(empty);
-      empty &= empty - 1;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int64_t units = (int64_t)a.gr.G * a.slices;
+  for (int64_t base = part; base < units; base += (int64_t)a.zeroers * 64) {
+    const int64_t unit = base + (int64_t)lane * a.zeroers;
+    const int g = (int)(min(unit, units - 1) / a.slices);
+    for (unsigned long long empty = __ballot(unit < units && a.gr.edge(g + 2) <= a.gr.edge(g + 1)); empty; empty &= empty - 1) {
+      const int64_t mine = base + (int64_t)__builtin_ctzll(empty) * a.zeroers, group = mine / a.slices, u = mine - group * a.slices;
       char* to = static_cast<char*>(a.dW) + group * a.stride_w * (a.dw_bf16 ? 2 : 4);
       const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-      const int pieces = (int)((a.K + 3) / 4), rows = blockDim.x / min(pieces, (int)blockDim.x);  // rows at a time
-      const int r = threadIdx.x / min(pieces, (int)blockDim.x), c = threadIdx.x % min(pieces, (int)blockDim.x);
-      for (int64_t n = r; r < rows && n < a.N; n += rows)
+      const int pieces = (int)min((a.K + 3) / 4, (int64_t)blockDim.x), rows = blockDim.x / pieces, r = tid / pieces, c = tid % pieces;
+      const int64_t end = (u + 1) * a.N / a.slices;
+      for (int64_t n = u * a.N / a.slices + r; r < rows && n < end; n += rows)
         for (int64_t k = (int64_t)c * 4; k < a.K; k += (int64_t)blockDim.x * 4) {
           if (a.dw_bf16) put4<true>(reinterpret_cast<uint16_t*>(to) + n * a.ldw, k, a.K, zero);
           else put4<false>(reinterpret_cast<float*>(to) + n * a.ldw, k, a.K, zero);
         }
-      if (a.db)
-        for (int64_t n = threadIdx.x; n < a.N; n += blockDim.x) a.db[group * a.ld_db + n] = 0.f;
+      if (a.db && u == 0)
+        for (int64_t n = tid; n < a.N; n += blockDim.x) a.db[group * a.ld_db + n] = 0.f;
     }
   }
 }
@@ -1083,14 +1139,14 @@ __global__ __launch_bounds__(TileT::THREADS, 2) void grouped_wgrad_dma_kernel(co
   else wgrad_dma<TileT, false>(a, w.chunk, n0, k0, reinterpret_cast<typename TileT::Elem*>(raw_lds));
 }
 
-// The parts of every group that spans chunks.  blockIdx.y = c: the group that begins in chunk c and reaches beyond it, if there is one,
-// contains the chunk's last row.
+// The parts of every group that spans chunks.  blockIdx.y = c: the group that begins in chunk c and reaches beyond it, if there is one, lies
+// at the chunk's last position.
 __global__ __launch_bounds__(256) void wgrad_join_kernel(const WgradArgs a) {
-  const int64_t c0 = blockIdx.y, last = (c0 + 1) * a.chunk - 1;
-  const int i = search(a.gr.G + 2, last, [&](int j) { return a.gr.edge(j); });
-  const int64_t start = a.gr.shared_edge(i), end = a.gr.shared_edge(i + 1);
-  if (i == 0 || i == a.gr.G + 1 || start < c0 * a.chunk || start > last || end <= last + 1) return;
-  const int group = i - 1, parts = (int)((end - 1) / a.chunk - c0);  // later ones
+  const int64_t c0 = blockIdx.y, next = (c0 + 1) * a.chunk;
+  const int i = group_at(a.gr, next - 1);
+  const int64_t start = a.gr.shared_edge(i), end = a.gr.shared_edge(i + 1), place = place_of(i, start);
+  if (i == 0 || i == a.gr.G + 1 || place < c0 * a.chunk || place > next - 1 || end - start <= next - place) return;
+  const int group = i - 1, parts = (int)((place + end - 1 - start) / a.chunk - c0);  // later ones
   const int64_t nk = a.N * a.K, at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
   // four consecutive values of the parts' sum; part c > 0: slot 2 (c0 + c) + 1; eight in flight, past the last one it is read again and not added
   auto joined = [&](const float* p, int64_t step, int64_t count) __attribute__((always_inline)) {
@@ -1141,6 +1197,7 @@ __global__ __launch_bounds__(256) void wgrad_join_kernel(const WgradArgs a) {
 constexpr int64_t MAX_GRID = 0x7fffffff;
 
 constexpr int CUS = 256;
+constexpr int NARROW = 32;
 
 // Raises a kernel's dynamic LDS limit, once per device: `done` is the kernel's own mask of devices.
 int allow_lds(const char* me, const void* kernel, int bytes, std::atomic<uint64_t>& done) {
@@ -1204,12 +1261,14 @@ int forward_pick(const char* me, const FwdArgs& a, hipStream_t st) {
   // Few rows per group: fp32 4000 rows of 100 types, 2000 -> 512: 302 us against 383.  (bf16 the same: 148 against 107: there the DMA tile
   // stays ahead.)
   if (a.gr.M <= (int64_t)48 * a.gr.G && !(BF16 && dma)) return small_launch<T, W_KM>(me, a, st);
+  if (a.N <= NARROW) return forward_launch<T, Tile<T, false, W_KM, 1, 1, 4, 1>>(me, a, st);
   if (dma) {
     if constexpr (sizeof(T) == 2) {
       // three rounds of 256 x 256 tiles: 200003 x 400 -> 200 (791 tiles) 90 us against 96 of the 128 x 128 one, which has two workgroups on a CU
       // to fill each other's gaps and half the waste at ragged ends: 50000 x 1000 -> 304 (402 tiles) 64 against 70, 8000 x 2000 -> 512 37
       // against 53
-      if (a.N > 128 && (a.gr.M / 256 + a.gr.G) * dh::ceil_div(a.N, 256) >= 3 * CUS) return forward_dma_launch<DmaTile<T, false, W_KM, 4, 2, 2, 4>>(me, a, st);
+      if (a.N > 128 && a.gr.M >= 256 * (int64_t)a.gr.G && (a.gr.M / 256 + a.gr.G) * dh::ceil_div(a.N, 256) >= 3 * CUS)
+        return forward_dma_launch<DmaTile<T, false, W_KM, 4, 2, 2, 4>>(me, a, st);
     } else {
       // fp32 with less than a round of workgroups: 64 x 64 (20011 x 512 -> 256, 336 tiles of 128: 68 / 67 us against 78 / 65; 60000 x 400 ->
       // 200, 996 tiles: 141 against 128)
@@ -1221,25 +1280,25 @@ int forward_pick(const char* me, const FwdArgs& a, hipStream_t st) {
 }
 
 // The tile of the weight gradient and its chunks: as many chunks x tiles as workgroups run at a time, so that all end together; no chunk below
-// 32 rows, which a step of k would not fill, or below two groups of the mean size where that is less: a workgroup takes its groups one after
-// the other (1000 rows of 300 types: 81 us with 32 rows a chunk, 44 with 8; 500 rows of 17: 20 with 32, 25 with 8).  The large tile reads its
-// operands least often; where it would leave a chunk short (few rows, or a small dW) the smaller one has more workgroups to share the
-// groups among.
+// 64 positions.  The large tile reads its operands least often; where it would leave a chunk short (few rows, or a small dW) the smaller
+// one has more workgroups to share the groups among.
 struct WgradPlan {
-  int edge;  // rows and columns of the tile
+  int edge;  // rows and columns of the tile; NARROW: 32 of the narrow side x 128
   int64_t chunk;
 };
+int64_t wgrad_positions(int64_t M, int64_t G) { return M + (G > 1 ? G - 1 : 0) * GROUP_ROWS; }
 WgradPlan wgrad_plan(int64_t M, int64_t N, int64_t K, int64_t G, int dtype) {
   const int large = dtype == DH_DTYPE_BF16 ? 256 : 128;
   WgradPlan p{};
+  const int64_t positions = wgrad_positions(M, G);
+  const bool narrow = N <= NARROW || K <= NARROW;
   for (int edge : {large, large / 2}) {
-    const int64_t tiles = dh::ceil_div(N, edge) * dh::ceil_div(K, edge), resident = edge == 256 ? CUS : 2 * CUS;
+    if (narrow) edge = NARROW;
+    const int64_t tiles = narrow ? dh::ceil_div(std::max(N, K), 128) : dh::ceil_div(N, edge) * dh::ceil_div(K, edge), resident = edge == 256 ? CUS : 2 * CUS;
     const int64_t chunks = resident / tiles > 1 ? resident / tiles : 1;
-    const int64_t least = 2 * M / (G > 0 ? G : 1) >= 32 ? 32 : dh::ceil_div(2 * M / (G > 0 ? G : 1) + 1, 8) * 8;
-    int64_t rows = dh::ceil_div(dh::ceil_div(M, chunks), least) * least;
-    if (rows < least) rows = least;
+    const int64_t rows = std::max<int64_t>(dh::ceil_div(positions, chunks), 64);
     p = {edge, rows};
-    if (rows >= 4096) break;  // (1563 rows a chunk: 50000 x 1000 -> 304 76 us with the 256 tile, 62 with 128)
+    if (narrow || rows >= 4096) break;  // (1563 rows a chunk: 50000 x 1000 -> 304 76 us with the 256 tile, 62 with 128)
   }
   return p;
 }
@@ -1306,7 +1365,7 @@ extern "C" int dh_gemm_grouped(int64_t M, int64_t N, int64_t K, int64_t G, int t
 
 extern "C" size_t dh_gemm_grouped_wgrad_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t G, int dtype) {
   if (M <= 0 || N <= 0 || K <= 0 || G <= 0) return 16;
-  const int64_t chunks = dh::ceil_div(M, wgrad_plan(M, N, K, G, dtype).chunk);
+  const int64_t chunks = dh::ceil_div(wgrad_positions(M, G), wgrad_plan(M, N, K, G, dtype).chunk);
   return chunks < 2 ? 16 : 16 + (size_t)(2 * chunks) * (size_t)N * (size_t)(K + 1) * 4;
 }
 
@@ -1331,15 +1390,22 @@ extern "C" int dh_gemm_grouped_wgrad(int64_t M, int64_t N, int64_t K, int64_t G,
   a.db = db; a.ld_db = ld_db;
   const WgradPlan plan = wgrad_plan(M, N, K, G, dtype);
   a.chunk = plan.chunk;
-  a.zeroers = G <= 64 ? 8 : 64;
-  a.chunks = M > 0 ? dh::ceil_div(M, a.chunk) : 1;
+  // a workgroup writes about 20 GB/s: runs of at most 64 KB (2 rows of 10 types, 328 -> 140 bf16: 38 us with whole groups, 12 so)
+  a.slices = (int)std::min((double)std::min<int64_t>(N, 1 << 20), 1 + (double)N * K * (a.dw_bf16 ? 2 : 4) / 65536);
+  a.zeroers = 8 * (int)std::min<int64_t>(32, dh::ceil_div(G * a.slices, 8));
+  a.chunks = M > 0 ? dh::ceil_div(wgrad_positions(M, G), a.chunk) : 1;
   a.part_w = static_cast<float*>(workspace);
   a.part_b = a.part_w + 2 * a.chunks * N * K;
   hipStream_t st = dh::as_stream(stream);
   const int vec = dtype == DH_DTYPE_BF16 ? 8 : 4;
   const bool dma = dma_rows(dY, ldy, vec) && dma_rows(X, ldx, vec) && N % vec == 0 && K % vec == 0;
   int launched;
-  if (dtype != DH_DTYPE_BF16) {
+  if (plan.edge == NARROW) {
+    if (dtype == DH_DTYPE_BF16)
+      launched = N <= NARROW ? wgrad_launch<uint16_t, Tile<uint16_t, true, true, 1, 1, 1, 4>>(me, a, st) : wgrad_launch<uint16_t, Tile<uint16_t, true, true, 1, 1, 4, 1>>(me, a, st);
+    else
+      launched = N <= NARROW ? wgrad_launch<float, Tile<float, true, true, 1, 1, 1, 4>>(me, a, st) : wgrad_launch<float, Tile<float, true, true, 1, 1, 4, 1>>(me, a, st);
+  } else if (dtype != DH_DTYPE_BF16) {
     if (!dma) launched = plan.edge == 128 ? wgrad_launch<float, Tile<float, true, true, 2, 2, 2, 2>>(me, a, st) : wgrad_launch<float, Tile<float, true, true, 1, 1, 2, 2>>(me, a, st);
     else launched = plan.edge == 128 ? wgrad_dma_launch<DmaTile<float, true, true, 2, 2, 2, 2>>(me, a, st) : wgrad_dma_launch<DmaTile<float, true, true, 1, 1, 2, 2>>(me, a, st);
   } else {

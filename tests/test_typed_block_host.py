@@ -143,10 +143,27 @@ def test_row_slots_cover_every_row_once(seed):
     assert (owner == want).all()
 
 
-def _segments(ptr, M, chunk, chunks, c):
-    """(group, begin, end, partial slot) of a chunk of rows, as Segments walks them."""
+GROUP_ROWS = 64
+
+
+def _place(e, i):
+    """Where group i (of those with the two of no weight) begins on the line of rows and GROUP_ROWS positions behind each group."""
+    return e[i] + max(i - 1, 0) * GROUP_ROWS
+
+
+def _group_at(e, s):
+    return max(j for j in range(len(e) - 1) if _place(e, j) <= s)
+
+
+def _row_at(e, s):
+    i = _group_at(e, s)
+    return min(e[i] + max(0, s - _place(e, i)), e[i + 1])
+
+
+def _segments(ptr, M, chunk, c):
+    """(group, begin, end, partial slot) of a chunk of positions, as Segments walks them."""
     e, G = _edges(ptr, M), len(ptr) - 1
-    first, last = c * chunk, min(c * chunk + chunk, M)
+    first, last = _row_at(e, c * chunk), _row_at(e, (c + 1) * chunk)
     out, at = [], first
     while at < last:
         lo = at
@@ -168,12 +185,12 @@ def test_weight_gradient_segments(seed):
     """Every row of a group is in one segment, every group with rows is finished once (in place, or by the join of its parts, which reads
     exactly the slots that were written), and no slot is written twice."""
     rng = np.random.default_rng(seed)
-    M, G, chunk = int(rng.integers(0, 700)), int(rng.integers(1, 60)), int(rng.choice([8, 32, 96, 1000]))
+    M, G, chunk = int(rng.integers(0, 700)), int(rng.integers(1, 60)), int(rng.choice([8, 64, 96, 1000]))
     ptr = np.sort(rng.integers(0, M + 1, G + 1)) if seed % 3 else np.sort(rng.choice([0, M // 3, M // 2, M], G + 1))
-    chunks = max(1, -(-M // chunk))
+    chunks = max(1, -(-(M + (G - 1) * GROUP_ROWS) // chunk))
     owner, done, slots = np.full(M, -1), np.zeros(G, int), {}
     for c in range(chunks):
-        for group, lo, hi, slot in _segments(ptr, M, chunk, chunks, c):
+        for group, lo, hi, slot in _segments(ptr, M, chunk, c):
             assert (owner[lo:hi] == -1).all() and ptr[group] <= lo < hi <= ptr[group + 1]
             owner[lo:hi] = group
             if slot < 0:
@@ -184,13 +201,13 @@ def test_weight_gradient_segments(seed):
                 slots[slot] = group
     e = _edges(ptr, M)
     for c0 in range(chunks - 1):  # wgrad_join_kernel
-        last = (c0 + 1) * chunk - 1
-        i = max(j for j in range(G + 2) if e[j] <= last)
-        start, end = e[i], e[i + 1]
-        if i in (0, G + 1) or start < c0 * chunk or start > last or end <= last + 1:
+        after = (c0 + 1) * chunk
+        i = _group_at(e, after - 1)
+        start, end, place = e[i], e[i + 1], _place(e, i)
+        if i in (0, G + 1) or place < c0 * chunk or place > after - 1 or end - start <= after - place:
             continue
         done[i - 1] += 1
-        for c in range((end - 1) // chunk - c0 + 1):
+        for c in range((place + end - 1 - start) // chunk - c0 + 1):
             assert slots.pop(2 * (c0 + c) + (c > 0)) == i - 1
     assert not slots and (done == (ptr[1:] > ptr[:-1])).all()
     for g in range(G):
