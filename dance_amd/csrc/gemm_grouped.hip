@@ -11,9 +11,9 @@
 //
 // Bound: the matrix cores for many rows (200003 rows of 9 types, 2000 -> 512 bf16: Y 505 us, dX 630, dW and db 470 + 32: 810 / 650 / 870 TFLOP/s;
 // fp32 100003 rows: 125 / 122 / 134 TFLOP/s), latency for few (16 rows of 8 types, 400 -> 200: 7.3 us; 500 rows of 17 types, forward and all
-// gradients: 36 us in four launches).  Four kernels: a tile filled by LDS DMA for aligned operands, one staged through registers for the
-// others (60000 x 401 -> 203 bf16 168 us for the three products, 106 at 400 -> 200), one of 32 x 32 with K split over the waves for few rows,
-// and the weight gradient's, which cuts the rows into equal chunks whatever the groups.
+// gradients: 33 us in four launches).  Four kernels: a tile filled by LDS DMA for aligned operands, one staged through registers for the
+// others and for few columns (60000 x 401 -> 203 bf16 172 us for the three products, 104 at 400 -> 200), one of 32 x 32 with K split over the
+// waves for few rows, and the weight gradient's, which cuts the rows into chunks of equal work whatever the groups.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -935,7 +935,8 @@ __global__ __launch_bounds__(512) void grouped_small_kernel(const FwdArgs a) {
 // dW_g [N][K] = sum over the group's rows of dY[i, n] X[i, k]: both operands [k][row] images with the rows as the contraction.  The rows are
 // cut into chunks of equal work whatever the groups: a workgroup takes one tile of dW through one chunk, group by group.  A group costs its
 // rows and, for the start and the end of its tile, about as much as GROUP_ROWS rows: row r of group g lies at position r + g GROUP_ROWS of a
-// line that is cut into equal pieces, a closed form of the bounds again.  A group that lies inside a chunk is finished in place; of one that spans
+// line that is cut into equal pieces, a closed form of the bounds again (27630 rows of 476 types, 560 -> 16 bf16: 107 us with pieces of equal
+// rows, 40 so; 52 with 32 positions for a group, 46 with 128).  A group that lies inside a chunk is finished in place; of one that spans
 // several, chunk c holds either its beginning (partial slot 2 c) or a later part that starts with the chunk (slot 2 c + 1; never two of a
 // kind), which wgrad_join_kernel adds in chunk order (no atomics).  The zeros of empty groups are written by workgroups of their own, the
 // first `zeroers` of the launch.
@@ -1197,6 +1198,9 @@ __global__ __launch_bounds__(256) void wgrad_join_kernel(const WgradArgs a) {
 constexpr int64_t MAX_GRID = 0x7fffffff;
 
 constexpr int CUS = 256;
+// Few columns: tiles 32 wide.  Forward, 60833 rows of 172 types 937 -> 12: bf16 31 us against 62 of the 128-wide tile, fp32 78 against 267; 60000 of
+// 9 types 400 -> 32, aligned: 14.1 / 14.9 and 32 / 38; two of them for 64 columns: 24.3 / 15.6 and 60 / 38.  Weight gradient, staged: the first 49
+// / 67 and 125 / 182; against the DMA tile, 400 -> 32: 21.5 / 19.4 and 43 / 39, so only where that cannot be used.
 constexpr int NARROW = 32;
 
 // Raises a kernel's dynamic LDS limit, once per device: `done` is the kernel's own mask of devices.
@@ -1264,9 +1268,9 @@ int forward_pick(const char* me, const FwdArgs& a, hipStream_t st) {
   if (a.N <= NARROW) return forward_launch<T, Tile<T, false, W_KM, 1, 1, 4, 1>>(me, a, st);
   if (dma) {
     if constexpr (sizeof(T) == 2) {
-      // three rounds of 256 x 256 tiles: 200003 x 400 -> 200 (791 tiles) 90 us against 96 of the 128 x 128 one, which has two workgroups on a CU
-      // to fill each other's gaps and half the waste at ragged ends: 50000 x 1000 -> 304 (402 tiles) 64 against 70, 8000 x 2000 -> 512 37
-      // against 53
+      // 256 x 256 with rows enough to fill such tiles (27630 rows of 476 types, 16 -> 560: 42 us against 34) and three rounds of them: 200003 x
+      // 400 -> 200 (791 tiles) 90 us against 96 of the 128 x 128 one, which has two workgroups on a CU to fill each other's gaps and half the
+      // waste at ragged ends: 50000 x 1000 -> 304 (402 tiles) 70 against 64, 8000 x 2000 -> 512 53 against 37
       if (a.N > 128 && a.gr.M >= 256 * (int64_t)a.gr.G && (a.gr.M / 256 + a.gr.G) * dh::ceil_div(a.N, 256) >= 3 * CUS)
         return forward_dma_launch<DmaTile<T, false, W_KM, 4, 2, 2, 4>>(me, a, st);
     } else {
@@ -1291,7 +1295,8 @@ WgradPlan wgrad_plan(int64_t M, int64_t N, int64_t K, int64_t G, int dtype) {
   const int large = dtype == DH_DTYPE_BF16 ? 256 : 128;
   WgradPlan p{};
   const int64_t positions = wgrad_positions(M, G);
-  const bool narrow = N <= NARROW || K <= NARROW;
+  const int vec = dtype == DH_DTYPE_BF16 ? 8 : 4;
+  const bool narrow = (N <= NARROW || K <= NARROW) && (N % vec != 0 || K % vec != 0);
   for (int edge : {large, large / 2}) {
     if (narrow) edge = NARROW;
     const int64_t tiles = narrow ? dh::ceil_div(std::max(N, K), 128) : dh::ceil_div(N, edge) * dh::ceil_div(K, edge), resident = edge == 256 ? CUS : 2 * CUS;

@@ -96,7 +96,7 @@ def test_weight_gradient(cuda_device, layout, dtype, K, N):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("rows,K,N", [(5000, 512, 260), (130, 2000, 512), (3, 400, 200)])
+@pytest.mark.parametrize("rows,K,N", [(5000, 512, 260), (130, 2000, 512), (3, 400, 200), (5000, 511, 331), (52000, 37, 12), (60000, 3, 5), (52000, 24, 16)])
 def test_larger(cuda_device, dtype, rows, K, N):
     from dance_amd import kernels
     gen = torch.Generator().manual_seed(rows)
@@ -289,6 +289,37 @@ def test_nothing_to_multiply(cuda_device):
         b = torch.randn(1, 5, device=DEV)
         y = kernels.gemm_grouped(z(6, 0), z(1, 5, 0), torch.tensor([0, 6], dtype=torch.int32, device=DEV), bias=b, out_dtype=torch.float32)
         assert torch.equal(y, b.expand(6, 5))  # no columns: the bias
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,K,N", [(6000, 333, 331), (52000, 35, 13), (60000, 5, 3), (70, 37, 21)])
+def test_nothing_behind_a_row_enters(cuda_device, dtype, rows, K, N):
+    """NaN behind every row of every operand (up to three columns), in the rows of no group and in front of the first."""
+    from dance_amd import kernels
+    gen = torch.Generator().manual_seed(K)
+    nan = float("nan")
+
+    def padded(*shape):
+        buf = torch.full((*shape[:-1], shape[-1] + 3), nan)
+        buf[..., :shape[-1]] = torch.randn(*shape, generator=gen)
+        return buf.to(dtype).to(DEV)[..., :shape[-1]]
+
+    sizes, lead = [rows // 3, 0, 1, rows // 2], 9
+    ptr = _ptr(sizes, lead)
+    x, dy, w = padded(rows, K), padded(rows, N), padded(4, N, K)
+    outside = torch.ones(rows, dtype=torch.bool)
+    outside[lead:lead + sum(sizes)] = False
+    x[outside.to(DEV)], dy[outside.to(DEV)] = nan, nan
+    bf = dtype == torch.bfloat16
+    clean = [t.cpu().nan_to_num(0.0) for t in (x, dy)]
+    _check(kernels.gemm_grouped(x, w, ptr), *_reference(clean[0], w, None, ptr), K, bf)
+    _check(kernels.gemm_grouped(dy, w, ptr, trans_b=False), *_reference(clean[1], w, None, ptr, False), N, bf)
+    dw, db = kernels.gemm_grouped_wgrad(dy, x, ptr, want_bias=True)
+    p, xd, yd = ptr.tolist(), clean[0].double(), clean[1].double()
+    for g in range(4):
+        i, j = p[g], p[g + 1]
+        _check(dw[g], yd[i:j].t() @ xd[i:j], yd[i:j].abs().t() @ xd[i:j].abs(), j - i, bf)
+        _check(db[g], yd[i:j].sum(0), yd[i:j].abs().sum(0), j - i)
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
