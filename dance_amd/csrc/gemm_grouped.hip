@@ -1259,9 +1259,11 @@ int forward_pick(const char* me, const FwdArgs& a, hipStream_t st) {
   // Few 32 x 32 tiles, in us, small against DMA tile: bf16 500 rows of 9 types 400 -> 200 (168 tiles) 5.2 / 10.8, 1500 of 30 types (532) 8.5 /
   // 10.7, 3000 of 3 types 512 -> 256 (768) 15.8 / 12.3; fp32 the first 8.2 / 14.0, 500 of 17 types 200 -> 400 (416) 7.5 / 8.8, 1500 of 30
   // types 15.5 / 13.3.  Against the staged tile: bf16 1500 of 30 types 401 -> 203 (532) 14.7 / 16.3, 203 -> 401 (988) 14.6 / 12.7; fp32 2000
-  // rows 511 -> 510 (1008) 36 / 46, 3000 of 3 types 255 -> 510 (1536) 28 / 29.
+  // rows 511 -> 510 (1008) 36 / 46, 3000 of 3 types 255 -> 510 (1536) 28 / 29.  Against the narrow tile: bf16 10000 of 5 types 400 -> 16 (317) 6.1 /
+  // 8.4, 15913 of 30 types 872 -> 32 (527) 19.5 / 16.7; fp32 the latter 34 / 43, 30000 of 5 types 100 -> 16 (942) 10.5 / 8.9.
   const int64_t small_tiles = (a.gr.M / 32 + a.gr.G) * dh::ceil_div(a.N, 32);
-  if (small_tiles <= (BF16 ? 640 : dma ? 420 : 1536)) return small_launch<T, W_KM>(me, a, st);
+  const int64_t few = a.N <= NARROW ? (BF16 ? 400 : 700) : BF16 ? 640 : dma ? 420 : 1536;
+  if (small_tiles <= few) return small_launch<T, W_KM>(me, a, st);
   // Few rows per group: fp32 4000 rows of 100 types, 2000 -> 512: 302 us against 383.  (bf16 the same: 148 against 107: there the DMA tile
   // stays ahead.)
   if (a.gr.M <= (int64_t)48 * a.gr.G && !(BF16 && dma)) return small_launch<T, W_KM>(me, a, st);
