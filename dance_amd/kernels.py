@@ -1378,7 +1378,8 @@ def global_norm(tensors, norm_type: float = 2.0) -> torch.Tensor:
 def clip_grads(grads, max_norm: float, *, norm_type: float = 2.0, out=None) -> torch.Tensor:
     """Scale ``grads`` (fp32 / bf16 tensors) by min(1, max_norm / (norm + 1e-6)), norm = their global norm, which is returned as an fp32 scalar
     on the device: in place, or into the tensors of ``out`` (fp32 or bf16 each, as many elements as their gradient: e.g. the views of the
-    flat fp32 buffer that an optimiser works on).  Nothing waits for the device.  See dh_grad_clip."""
+    flat fp32 buffer that an optimiser works on).  Apart from a gradient and its own output no two tensors may share memory (the same one
+    twice is refused).  Nothing waits for the device.  See dh_grad_clip."""
     lib = _lib_ready()
     code = _norm_type(norm_type)
     max_norm = float(max_norm)

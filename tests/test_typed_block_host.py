@@ -226,6 +226,13 @@ def test_row_slots_of_a_wrong_table_stay_inside(seed):
                 begin = e[i] + (index << shift)
                 if begin < e[i + 1]:
                     assert 0 <= begin < min(e[i + 1], begin + (1 << shift)) <= M
+    G, chunk = len(ptr) - 1, int(rng.choice([64, 200]))
+    chunks = -(-(M + (G - 1) * GROUP_ROWS) // chunk)
+    for i in range(G + 2):  # the weight gradient: rows of a chunk, and the slots that the join of a group's parts reads
+        for s in range(0, chunks * chunk + 1, 17):
+            assert 0 <= min(e[i] + max(0, s - _place(e, i)), e[i + 1]) <= M
+        if 0 < i < G + 1 and e[i + 1] > e[i]:
+            assert 0 <= (_place(e, i) + e[i + 1] - 1 - e[i]) // chunk < chunks
 
 
 # ---- wrappers ----
