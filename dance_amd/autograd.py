@@ -770,7 +770,7 @@ class _ResidualNormFn(torch.autograd.Function):
         pre = (params[2], params[3]) if has_pre else None
         r, h, stats = kernels.residual_norm_forward(f, x, post=post, gate=gate, gate_sigmoid=gate_sigmoid, scale=scale, pre=pre, kind=kind, eps=eps,
                                                     want_stats=any(ctx.needs_input_grad))
-        ctx.opts = opts
+        ctx.opts, ctx.gate_kind = opts, kernels.residual_norm_gate_kind(gate, *f.shape)
         ctx.save_for_backward(f, x if has_pre else None, gate, *params, stats)  # (without the second norm the backward does not need r)
         return (r, h) if has_pre else r
 
@@ -783,9 +783,9 @@ class _ResidualNormFn(torch.autograd.Function):
         if dr is None and dh is None:
             return (None, ) * 8
         want = [n for n, need in zip(names, ctx.needs_input_grad) if need and (has_pre or n != "x")]
-        g = kernels.residual_norm_backward(None if dr is None else _rows(dr), None if dh is None else _rows(dh), f, x, stats,
-                                           post=(w1, b1) if has_post else None, gate=gate, gate_sigmoid=gate_sigmoid, scale=scale,
-                                           pre=(w2, b2) if has_pre else None, kind=kind, want=want)
+        g = kernels.residual_norm_backward_unchecked(None if dr is None else _rows(dr), None if dh is None else _rows(dh), f, x, stats,
+                                                     (w1, b1) if has_post else None, gate, ctx.gate_kind, gate_sigmoid, scale,
+                                                     (w2, b2) if has_pre else None, kind, want)
         if not has_pre and ctx.needs_input_grad[1]:
             g["x"] = dr  # r = x + ...
         return (*(g.get(n) for n in names), None)

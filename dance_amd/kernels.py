@@ -945,22 +945,34 @@ def residual_norm_backward(dr: Optional[torch.Tensor], dh: Optional[torch.Tensor
                            pre=None, kind: int = NORM_LAYER, want=("f", "x", "gate", "w1", "b1", "w2", "b2")):
     """Gradients of ``residual_norm_forward`` as a dict over ``want``; see dh_residual_norm_backward.  ``dr`` / ``dh``: the upstream gradients
     of r and h, either may be None."""
-    lib = _lib_ready()
-    dt = _elem(f, "f")
+    _elem(f, "f")
     M, D = f.shape
-    _check_rows(x, f, "x")
-    _check_rows(dr, f, "dr")
-    _check_rows(dh, f, "dh")
+    for name, t in (("x", x), ("dr", dr), ("dh", dh)):
+        _check_rows(t, f, name)
+        _mat(t, f.dtype, name)
+    _mat(f, f.dtype, "f")
     if dr is None and dh is None:
         raise ValueError("residual_norm_backward: neither dr nor dh")
     if dh is not None and pre is None:
         raise ValueError("residual_norm_backward: dh without the second norm")
     if tuple(stats.shape) != (M, 4):
         raise ValueError(f"stats must be [{M}, 4], got shape {tuple(stats.shape)}")
+    _dev(stats, torch.float32, "stats", 2)
     gk = residual_norm_gate_kind(gate, M, D)
-    has_post, w1, b1 = _norm_params(post, D, "post")
-    has_pre, w2, _ = _norm_params(pre, D, "pre")
-    gp, ldg = _gate_args(gate, gk, f.dtype)
+    _norm_params(post, D, "post")
+    _norm_params(pre, D, "pre")
+    _gate_args(gate, gk, f.dtype)
+    with _one_device(f, x, gate, stats, dr, dh, *(post or ()), *(pre or ())):
+        return residual_norm_backward_unchecked(dr, dh, f, x, stats, post, gate, gk, gate_sigmoid, scale, pre, kind, want)
+
+
+def residual_norm_backward_unchecked(dr, dh, f, x, stats, post, gate, gate_kind, gate_sigmoid, scale, pre, kind, want):
+    """``residual_norm_backward`` on operands that have been checked, on the current device: for the autograd node, whose operands its forward
+    has checked (half of the node's time in Python on a batch of few rows)."""
+    lib = _lib_ready()
+    M, D = f.shape
+    w1, b1 = post or (None, None)
+    w2, b2 = pre or (None, None)
     out = {}
     if "f" in want:
         out["f"] = f.new_empty((M, D))
@@ -969,9 +981,9 @@ def residual_norm_backward(dr: Optional[torch.Tensor], dh: Optional[torch.Tensor
     if gate is not None and "gate" in want:
         out["gate"] = torch.empty_like(gate, memory_format=torch.contiguous_format)
     # one allocation for the column gradients of the norms
-    names = [n for n, there in (("w1", has_post), ("b1", has_post), ("w2", has_pre), ("b2", has_pre)) if there and n in want]
+    names = [n for n, norm in (("w1", post), ("b1", post), ("w2", pre), ("b2", pre)) if norm is not None and n in want]
     if names:
-        out.update(zip(names, torch.empty((len(names), D), dtype=torch.float32, device=f.device).unbind(0)))
+        out.update(zip(names, stats.new_empty((len(names), D)).unbind(0)))
     p = {n: t.data_ptr() for n, t in out.items()}.get
     w2_wanted, b2_wanted = p("w2"), p("b2")
     if dh is None:  # nothing flows through the second norm
@@ -979,13 +991,14 @@ def residual_norm_backward(dr: Optional[torch.Tensor], dh: Optional[torch.Tensor
             if n in out:
                 out[n].zero_()
         w2_wanted = b2_wanted = None
-    with _one_device(f, x, gate, stats, dr, dh, *(post or ()), *(pre or ())):
-        ws_bytes = lib.dh_residual_norm_backward_workspace_bytes(M, D)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=f.device)
-        _call("residual_norm_backward", lib.dh_residual_norm_backward, M, D, dt, *_mat(f, f.dtype, "f"), *_mat(x, f.dtype, "x"), gp, ldg, gk,
-              1 if gate_sigmoid else 0, scale, kind, has_post, w1, b1, has_pre, w2, _dev(stats, torch.float32, "stats", 2), *_mat(dr, f.dtype, "dr"),
-              *_mat(dh, f.dtype, "dh"), p("f"), D, p("x"), D, p("gate"), D if gk == GATE_FULL else 1, p("w1"), p("b1"), w2_wanted, b2_wanted,
-              ws.data_ptr(), ws_bytes, _stream())
+    ws_bytes = lib.dh_residual_norm_backward_workspace_bytes(M, D)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=f.device)
+    at = lambda t: None if t is None else t.data_ptr()
+    ld = lambda t: 0 if t is None else t.stride(0) if M > 1 else D
+    _call("residual_norm_backward", lib.dh_residual_norm_backward, M, D, _ELEM[f.dtype], f.data_ptr(), ld(f), at(x), ld(x), at(gate),
+          (ld(gate) if gate_kind == GATE_FULL else gate.stride(0) if M > 1 else 1) if gate_kind >= GATE_ROW else 0, gate_kind, 1 if gate_sigmoid else 0,
+          scale, kind, 0 if post is None else 1, at(w1), at(b1), 0 if pre is None else 1, at(w2), stats.data_ptr(), at(dr), ld(dr), at(dh), ld(dh),
+          p("f"), D, p("x"), D, p("gate"), D if gate_kind == GATE_FULL else 1, p("w1"), p("b1"), w2_wanted, b2_wanted, ws.data_ptr(), ws_bytes, _stream())
     return out
 
 
