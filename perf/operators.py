@@ -63,7 +63,7 @@ def draw(rng):
         types = _log_int(rng, 1, max(2, min(700, int(2e8 / (k * n)))))
         return dict(op=op, dir=rng.choice(["fwd", "train"]), dtype=dtype, rows=rows, types=types, skew=rng.uniform(0.0, 2.0), k=k, n=n)
     if op == "norm":
-        d = _log_int(rng, 16, 4096)
+        d = _log_int(rng, 16, 8192)
         rows = max(1, min(_log_int(rng, 1, 400000), int(1e8 / d)))
         post, pre = rng.choice([(True, True), (True, False), (False, True)])
         return dict(op=op, dir=rng.choice(["fwd", "train"]), dtype=dtype, rows=rows, d=d, kind=rng.choice(["layer", "rms"]),
