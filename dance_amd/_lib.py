@@ -154,11 +154,12 @@ def _declare(lib):
         "dh_grad_norm_workspace_bytes": (c_size_t, [i32, P]),
         "dh_grad_norm": (c_int, [i32, P, P, P, i32, P, P, c_size_t, P]),
         "dh_grad_clip": (c_int, [i32, P, P, P, P, P, i32, c_double, P, P, c_size_t, P]),
-        "dh_residual_norm_forward": (c_int, [i64, i64, i32, P, i64, P, i64, P, i64, i32, i32, c_float, i32, c_float, i32, P, P, i32, P, P, P, i64, P, i64,
-                                             P, P]),
+        **dict.fromkeys(("dh_residual_norm_forward", "dh_residual_norm_wide_forward"),
+                        (c_int, [i64, i64, i32, P, i64, P, i64, P, i64, i32, i32, c_float, i32, c_float, i32, P, P, i32, P, P, P, i64, P, i64, P, P])),
         "dh_residual_norm_backward_workspace_bytes": (c_size_t, [i64, i64]),
-        "dh_residual_norm_backward": (c_int, [i64, i64, i32, P, i64, P, i64, P, i64, i32, i32, c_float, i32, i32, P, P, i32, P, P, P, i64, P, i64, P, i64,
-                                              P, i64, P, i64, P, P, P, P, P, c_size_t, P]),
+        **dict.fromkeys(("dh_residual_norm_backward", "dh_residual_norm_wide_backward"),
+                        (c_int, [i64, i64, i32, P, i64, P, i64, P, i64, i32, i32, c_float, i32, i32, P, P, i32, P, P, P, i64, P, i64, P, i64, P, i64, P, i64,
+                                 P, P, P, P, P, c_size_t, P])),
         "dh_gemm_grouped": (c_int, [i64, i64, i64, i64, i32, i32, P, i64, P, i64, i64, P, P, i64, i32, P, i64, i32, i32, P]),
         "dh_gemm_grouped_wgrad_workspace_bytes": (c_size_t, [i64, i64, i64, i64, i32]),
         "dh_gemm_grouped_wgrad": (c_int, [i64, i64, i64, i64, i32, P, i64, P, i64, P, P, i64, i64, i32, P, i64, P, c_size_t, P]),

@@ -798,7 +798,7 @@ def residual_norm(f: torch.Tensor, x: Optional[torch.Tensor] = None, *, post=Non
         r = x + scale * act(gate) * norm(f; post)        (norm left out without ``post``, x = 0 without x)
         h = norm(r; pre)                                 (None without ``pre``): the next block's input
 
-    Returns (r, h).  f, x [M, D] fp32 or bf16 (D <= 4096); ``post`` / ``pre``: (weight, bias), fp32 [D], None for no weight or no bias;
+    Returns (r, h).  f, x [M, D] fp32 or bf16 (D <= 8192, 4096 without either norm); ``post`` / ``pre``: (weight, bias), fp32 [D], None for no weight or no bias;
     ``kind``: "layer" or "rms"; gate: fp32 [] / [1] (one for all) or [D] (per column), or of f's dtype [M, 1] (per row) or [M, D];
     ``gate_act``: "none" or "sigmoid".  h is computed from the unrounded r.  Gradients of f, x, gate and all parameters."""
     if kind not in ("layer", "rms"):

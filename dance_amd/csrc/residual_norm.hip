@@ -21,6 +21,11 @@
 // Measured, layer norms and channel gate, forward / backward: 200003 x 512 bf16 165 / 282 us (5.0 / 4.4 TB/s), fp32 321 / 446 us (5.1 / 5.5);
 // 50001 x 504 bf16 41 / 76 us, x 500 (ODD) 50 / 94, x 501 54 / 101; 50001 x 1000 110 / 188.  The bf16 backward has the arithmetic of twice
 // as many elements to a byte and comes near the vector units' limit.
+// Wide rows (4097 .. 8192 columns, entries of their own): a workgroup of up to eight waves, sixteen elements a lane.  The backward takes one
+// workgroup for every row, without the column gradients, which would spill, and leaves two numbers a row; a second kernel walks the columns
+// down the rows and reads f, x, dr and dh again, so a training pass moves 14 row lengths instead of 10.  12001 rows, bf16 / fp32, forward and
+// training pass: x 4096 (not wide) 102, 282 / 163, 405 us; x 5000 162, 496 / 236, 772; x 8192 185, 651 / 302, 1124; x 4097 281, 709 / 293, 789
+// (rows that start at odd elements).
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -30,11 +35,12 @@
 namespace {
 
 enum { GATE_NONE = DH_GATE_NONE, GATE_SCALAR = DH_GATE_SCALAR, GATE_CHANNEL = DH_GATE_CHANNEL, GATE_ROW = DH_GATE_ROW, GATE_FULL = DH_GATE_FULL };
-constexpr int64_t MAX_D = 4096;
+constexpr int64_t MAX_D = 4096, WIDE_D = 8192;  // columns of a row; of one in the wide entries
 // who holds a row: part of a wave, a wave, a workgroup;  how the row ends: with the lanes' last access, with an access before, inside one
 enum { SUB = 0, WAVE = 1, GROUP = 2 };
 enum { WHOLE = 0, SHORT = 1, ODD = 2 };
 constexpr int BWD_BLOCKS = 1024;  // workgroups of a backward launch at most = partial rows of the column gradients
+constexpr int WIDE_CHUNKS = 256;  // row chunks of wide rows' column gradients = partial rows; 3 to 8 workgroups side by side in each
 
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(2)));
@@ -57,6 +63,9 @@ struct Args {
   int64_t lddf, lddx, lddg;
   float* partials;  // [n_arrays][gridDim.x][D]
   int want_w1, want_b1, want_w2, want_b2, want_gate;
+  // wide rows
+  float2* terms;  // [M]: <u2 rhat>, <u2> of each row, for the kernel of the column gradients; null: nobody asks
+  int64_t rows;   // of a workgroup of that kernel
 };
 
 __device__ __forceinline__ float bf16_f32(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
@@ -437,9 +446,11 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256) void residual_norm_backw
   const int rows_per_block = MODE == GROUP ? 1 : 256 / tpr;
   // the row within the workgroup's pass; uniform (a scalar, and with it the rows' addresses) where a wave holds one row
   const int sub = MODE == GROUP ? 0 : MODE == WAVE ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : threadIdx.x / tpr;
-  float acc_w1[E], acc_b1[E], acc_w2[E], acc_b2[E], acc_g[E];
+  constexpr bool COLUMNS = E <= 8;  // column gradients: sixteen elements a lane leave no registers for them (wide_columns_kernel)
+  constexpr int A = COLUMNS ? E : 1;
+  float acc_w1[A], acc_b1[A], acc_w2[A], acc_b2[A], acc_g[A];
 #pragma unroll
-  for (int i = 0; i < E; ++i) acc_w1[i] = acc_b1[i] = acc_w2[i] = acc_b2[i] = acc_g[i] = 0.f;
+  for (int i = 0; i < A; ++i) acc_w1[i] = acc_b1[i] = acc_w2[i] = acc_b2[i] = acc_g[i] = 0.f;
   const bool col_gate = !FULL && (a.gate_kind == GATE_CHANNEL || a.gate_kind == GATE_SCALAR);
   const bool use_x = a.x && a.dh;  // r enters through the second norm only
   for (int64_t base = (int64_t)blockIdx.x * rows_per_block; base < a.M; base += (int64_t)gridDim.x * rows_per_block) {
@@ -500,9 +511,11 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256) void residual_norm_backw
       for (int i = 0; i < E; ++i) {
         const float n = __builtin_fmaf(f[i], w[i], b[i]);
         x[i] = (__builtin_fmaf(a.scale * gf[i], n, x[i]) - st.z) * st.w;  // rhat
-        if (valid) {
-          acc_w2[i] = __builtin_fmaf(dh[i], x[i], acc_w2[i]);
-          acc_b2[i] += dh[i];
+        if constexpr (COLUMNS) {
+          if (valid) {
+            acc_w2[i] = __builtin_fmaf(dh[i], x[i], acc_w2[i]);
+            acc_b2[i] += dh[i];
+          }
         }
         dh[i] *= w2[i];
         s[0] = __builtin_fmaf(dh[i], x[i], s[0]);
@@ -510,6 +523,9 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256) void residual_norm_backw
       }
       row_sums<MODE, 2>(s, tpr, lds);
       const float c1 = s[0] * a.inv_d, c0 = a.rms ? 0.f : s[1] * a.inv_d;
+      if constexpr (!COLUMNS) {
+        if (a.terms && t == 0) a.terms[row] = make_float2(c1, c0);
+      }
 #pragma unroll
       for (int i = 0; i < E; ++i) dr[i] = __builtin_fmaf(st.w, __builtin_fmaf(-x[i], c1, dh[i] - c0), dr[i]);
     }
@@ -522,10 +538,12 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256) void residual_norm_backw
       float dg = sd * n;
       if (sig) dg *= gf[i] * (1.f - gf[i]);
       const float dn = sd * gf[i];
-      if (valid) {
-        acc_w1[i] = __builtin_fmaf(dn, f[i], acc_w1[i]);
-        acc_b1[i] += dn;
-        if (col_gate) acc_g[i] += dg;
+      if constexpr (COLUMNS) {
+        if (valid) {
+          acc_w1[i] = __builtin_fmaf(dn, f[i], acc_w1[i]);
+          acc_b1[i] += dn;
+          if (col_gate) acc_g[i] += dg;
+        }
       }
       const float u = dn * w[i];
       s[0] = __builtin_fmaf(u, f[i], s[0]);
@@ -549,13 +567,82 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256) void residual_norm_backw
       }
       store_row<T, V, CH, TAIL>(a.df, row * a.lddf, t, tpr, a.D, dr);
     }
+    if constexpr (!COLUMNS) break;  // one workgroup for every row: no parameters to keep in registers from row to row
+  }
+  if constexpr (COLUMNS) {
+    int slot = 0;
+    if (a.want_w1) put_partials<V, CH, MODE>(a, t, sub, acc_w1, slot++, lds);
+    if (a.want_b1) put_partials<V, CH, MODE>(a, t, sub, acc_b1, slot++, lds);
+    if (a.want_w2) put_partials<V, CH, MODE>(a, t, sub, acc_w2, slot++, lds);
+    if (a.want_b2) put_partials<V, CH, MODE>(a, t, sub, acc_b2, slot++, lds);
+    if (a.want_gate) put_partials<V, CH, MODE>(a, t, sub, acc_g, slot++, lds);
+  }
+}
+
+// The column gradients of wide rows: a thread walks V columns down the rows of its workgroup, with the row's four statistics and the two
+// means of the second norm's gradient that the row kernel left.  f, x, dr and dh are read a second time for it.
+template <class T, int V, bool FULL, int TAIL>
+__global__ __launch_bounds__(256) void wide_columns_kernel(const Args a) {
+  const int t = blockIdx.x * 256 + threadIdx.x;  // the piece of the row
+  if (t * V >= a.D) return;
+  float w1[V], b1[V], w2[V], gc[V], acc_w1[V], acc_b1[V], acc_w2[V], acc_b2[V], acc_g[V];
+  load_params<V, 1, TAIL>(a.has_post ? a.w1 : nullptr, 1.f, t, 0, a.D, w1);
+  load_params<V, 1, TAIL>(a.has_post ? a.b1 : nullptr, 0.f, t, 0, a.D, b1);
+  load_params<V, 1, TAIL>(a.has_pre ? a.w2 : nullptr, 1.f, t, 0, a.D, w2);
+  load_params<V, 1, TAIL>(a.gate_kind == GATE_CHANNEL ? static_cast<const float*>(a.gate) : nullptr,
+                          a.gate_kind == GATE_SCALAR ? *static_cast<const float*>(a.gate) : 1.f, t, 0, a.D, gc);
+#pragma unroll
+  for (int e = 0; e < V; ++e) acc_w1[e] = acc_b1[e] = acc_w2[e] = acc_b2[e] = acc_g[e] = 0.f;
+  const bool sig = a.gate_sigmoid && a.gate_kind != GATE_NONE;
+  const int64_t first = (int64_t)blockIdx.y * a.rows, last = min(first + a.rows, a.M);
+  for (int64_t row = first; row < last; ++row) {
+    RawRow<T, V, 1> rf, rx, rr, rh, rg;
+    float f[V], x[V], dr[V], dh[V], gf[V];
+    rf.load(a.f, row * a.ldf, t, 0, a.D);
+    if (a.x && a.dh) rx.load(a.x, row * a.ldx, t, 0, a.D);
+    if (a.dr) rr.load(a.dr, row * a.lddr, t, 0, a.D);
+    if (a.dh) rh.load(a.dh, row * a.lddh, t, 0, a.D);
+    if (FULL) rg.load(a.gate, row * a.ldg, t, 0, a.D);
+    const float grow = !FULL && a.gate_kind == GATE_ROW ? Elem<T>::get(a.gate, row * a.ldg) : 0.f;
+    const float4 st = *reinterpret_cast<const float4*>(a.stats + row * 4);
+    const float2 c = a.dh ? a.terms[row] : make_float2(0.f, 0.f);
+    rf.template unpack<TAIL>(t, 0, a.D, f);
+    if (a.x && a.dh) rx.template unpack<TAIL>(t, 0, a.D, x);
+    if (a.dr) rr.template unpack<TAIL>(t, 0, a.D, dr);
+    if (a.dh) rh.template unpack<TAIL>(t, 0, a.D, dh);
+    if (FULL) rg.template unpack<TAIL>(t, 0, a.D, gf);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      if (!FULL) gf[e] = a.gate_kind == GATE_ROW ? grow : gc[e];
+      if (sig) gf[e] = sigmoid(gf[e]);
+      const float fhat = a.has_post ? (f[e] - st.x) * st.y : f[e], n = __builtin_fmaf(fhat, w1[e], b1[e]);
+      float d = a.dr ? dr[e] : 0.f;
+      if (a.dh) {
+        const float rhat = (__builtin_fmaf(a.scale * gf[e], n, a.x ? x[e] : 0.f) - st.z) * st.w;
+        acc_w2[e] = __builtin_fmaf(dh[e], rhat, acc_w2[e]);
+        acc_b2[e] += dh[e];
+        d = __builtin_fmaf(st.w, __builtin_fmaf(-rhat, c.x, dh[e] * w2[e] - c.y), d);
+      }
+      const float sd = a.scale * d, dn = sd * gf[e];
+      acc_w1[e] = __builtin_fmaf(dn, fhat, acc_w1[e]);
+      acc_b1[e] += dn;
+      float dg = sd * n;
+      if (sig) dg *= gf[e] * (1.f - gf[e]);
+      acc_g[e] += dg;
+    }
   }
   int slot = 0;
-  if (a.want_w1) put_partials<V, CH, MODE>(a, t, sub, acc_w1, slot++, lds);
-  if (a.want_b1) put_partials<V, CH, MODE>(a, t, sub, acc_b1, slot++, lds);
-  if (a.want_w2) put_partials<V, CH, MODE>(a, t, sub, acc_w2, slot++, lds);
-  if (a.want_b2) put_partials<V, CH, MODE>(a, t, sub, acc_b2, slot++, lds);
-  if (a.want_gate) put_partials<V, CH, MODE>(a, t, sub, acc_g, slot++, lds);
+  auto put = [&](const float (&acc)[V]) __attribute__((always_inline)) {
+    float* out = a.partials + ((int64_t)slot++ * gridDim.y + blockIdx.y) * a.D;
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (t * V + e < a.D) out[t * V + e] = acc[e];
+  };
+  if (a.want_w1) put(acc_w1);
+  if (a.want_b1) put(acc_b1);
+  if (a.want_w2) put(acc_w2);
+  if (a.want_b2) put(acc_b2);
+  if (a.want_gate) put(acc_g);
 }
 
 struct ReduceArgs {
@@ -616,7 +703,7 @@ Split split_of(int64_t D, int vec_width) {
   const int64_t eight = 8 / s.v;  // accesses that hold eight elements
   if (n > 64 * eight) {
     s.mode = GROUP;
-    s.tpr = 64 * (int)dh::ceil_div(n, 64 * eight);
+    s.tpr = 64 * (int)dh::ceil_div(n, 64 * (D > MAX_D ? 2 * eight : eight));  // wide rows: sixteen elements per lane
   } else {
     s.tpr = 8;
     while (s.tpr < 64 && s.tpr < n) s.tpr *= 2;
@@ -655,7 +742,7 @@ int64_t launch(bool backward, const Args& a, const Split& s, hipStream_t st) {
   if (!backward) fit = std::min(fit, 20 / ((int)b.x / 64));
   int64_t resident = (int64_t)256 * fit;
   if (backward && resident > BWD_BLOCKS) resident = BWD_BLOCKS;
-  const int64_t grid = even_grid(a.M, rows_per_block(s), resident);
+  const int64_t grid = backward && V * CH > 8 ? a.M : even_grid(a.M, rows_per_block(s), resident);
   const dim3 g((unsigned)grid);
   if (backward) hipLaunchKernelGGL((residual_norm_backward_kernel<T, V, CH, MODE, FULL, TAIL>), g, b, 0, st, a);
   else hipLaunchKernelGGL((residual_norm_forward_kernel<T, V, CH, MODE, FULL, TAIL>), g, b, 0, st, a);
@@ -680,7 +767,7 @@ template <class T>
 int64_t launch_t(bool backward, const Args& a, const Split& s, hipStream_t st) {
   constexpr int V = Elem<T>::VEC, EIGHT = 8 / V;
   if (s.v == 1) return launch_tail<T, 1, 1, SUB>(backward, a, s, st);
-  if (s.mode == GROUP) return launch_tail<T, V, EIGHT, GROUP>(backward, a, s, st);
+  if (s.mode == GROUP) return s.ch > EIGHT ? launch_tail<T, V, 2 * EIGHT, GROUP>(backward, a, s, st) : launch_tail<T, V, EIGHT, GROUP>(backward, a, s, st);
   if (s.mode == SUB) return launch_tail<T, V, 1, SUB>(backward, a, s, st);
   if constexpr (EIGHT == 2) {
     if (s.ch == 2) return launch_tail<T, V, 2, WAVE>(backward, a, s, st);
@@ -688,9 +775,12 @@ int64_t launch_t(bool backward, const Args& a, const Split& s, hipStream_t st) {
   return launch_tail<T, V, 1, WAVE>(backward, a, s, st);
 }
 
-int check_common(const char* me, int64_t M, int64_t D, int dtype, const void* f, const void* x, int64_t ldf, int64_t ldx, const void* gate,
-                 int64_t ldg, int gate_kind, int gate_sigmoid, int kind, float eps) {
-  if (M < 0 || D < 1 || D > MAX_D) return dh::fail(DH_ERR_INVALID, "%s: %lld rows of %lld columns (1 .. %lld)", me, (long long)M, (long long)D, (long long)MAX_D);
+int check_common(const char* me, bool wide, int64_t M, int64_t D, int dtype, const void* f, const void* x, int64_t ldf, int64_t ldx, const void* gate,
+                 int64_t ldg, int gate_kind, int gate_sigmoid, int kind, float eps, int has_post, int has_pre) {
+  const int64_t least = wide ? MAX_D + 1 : 1, most = wide ? WIDE_D : MAX_D;
+  if (M < 0 || D < least || D > most)
+    return dh::fail(DH_ERR_INVALID, "%s: %lld rows of %lld columns (%lld .. %lld)", me, (long long)M, (long long)D, (long long)least, (long long)most);
+  if (wide && (M > 0x7fffffff || (!has_post && !has_pre))) return dh::fail(DH_ERR_INVALID, "%s: wide rows without a norm, or too many of them", me);
   if (dtype != DH_DTYPE_F32 && dtype != DH_DTYPE_BF16) return dh::fail(DH_ERR_INVALID, "%s: dtype %d", me, dtype);
   if (kind != DH_NORM_LAYER && kind != DH_NORM_RMS) return dh::fail(DH_ERR_INVALID, "%s: norm kind %d", me, kind);
   if (gate_kind < GATE_NONE || gate_kind > GATE_FULL) return dh::fail(DH_ERR_INVALID, "%s: gate kind %d", me, gate_kind);
@@ -703,14 +793,10 @@ int check_common(const char* me, int64_t M, int64_t D, int dtype, const void* f,
   return DH_OK;
 }
 
-}  // namespace
-
-extern "C" int dh_residual_norm_forward(int64_t M, int64_t D, int dtype, const void* f, int64_t ldf, const void* x, int64_t ldx, const void* gate,
-                                        int64_t ldg, int gate_kind, int gate_sigmoid, float scale, int kind, float eps, int has_post,
-                                        const float* w1, const float* b1, int has_pre, const float* w2, const float* b2, void* r, int64_t ldr,
-                                        void* h, int64_t ldh, float* stats, dh_stream_t stream) {
-  const char* me = "dh_residual_norm_forward";
-  const int rc = check_common(me, M, D, dtype, f, x, ldf, ldx, gate, ldg, gate_kind, gate_sigmoid, kind, eps);
+int forward(const char* me, bool wide, int64_t M, int64_t D, int dtype, const void* f, int64_t ldf, const void* x, int64_t ldx, const void* gate, int64_t ldg,
+            int gate_kind, int gate_sigmoid, float scale, int kind, float eps, int has_post, const float* w1, const float* b1, int has_pre,
+            const float* w2, const float* b2, void* r, int64_t ldr, void* h, int64_t ldh, float* stats, dh_stream_t stream) {
+  const int rc = check_common(me, wide, M, D, dtype, f, x, ldf, ldx, gate, ldg, gate_kind, gate_sigmoid, kind, eps, has_post, has_pre);
   if (rc != DH_OK) return rc;
   if (M == 0) return DH_OK;
   if ((!r && !has_pre) || (has_pre && !h)) return dh::fail(DH_ERR_INVALID, "%s: null output", me);
@@ -729,20 +815,30 @@ extern "C" int dh_residual_norm_forward(int64_t M, int64_t D, int dtype, const v
   return dh::check_launch(me);
 }
 
-extern "C" size_t dh_residual_norm_backward_workspace_bytes(int64_t M, int64_t D) {
+// five arrays of one partial row per workgroup, and the per-column sums of a scalar gate
+size_t partials_bytes(int64_t M, int64_t D) { return (size_t)(5 * std::min<int64_t>(M, BWD_BLOCKS) + 1) * (size_t)D * 4; }
+// and, for wide rows, two numbers of each row behind them
+size_t workspace_bytes_of(int64_t M, int64_t D) {
   if (M <= 0 || D <= 0) return 16;
-  const int64_t rows = M < BWD_BLOCKS ? M : BWD_BLOCKS;
-  return (size_t)(5 * rows + 1) * (size_t)D * 4;  // five arrays of one partial row per workgroup, and the per-column sums of a scalar gate
+  return D > MAX_D ? (partials_bytes(M, D) + 15) / 16 * 16 + (size_t)M * 8 : partials_bytes(M, D);
 }
 
-extern "C" int dh_residual_norm_backward(int64_t M, int64_t D, int dtype, const void* f, int64_t ldf, const void* x, int64_t ldx, const void* gate,
-                                         int64_t ldg, int gate_kind, int gate_sigmoid, float scale, int kind, int has_post, const float* w1,
-                                         const float* b1, int has_pre, const float* w2, const float* stats, const void* dr, int64_t lddr,
-                                         const void* dhh, int64_t lddh, void* df, int64_t lddf, void* dx, int64_t lddx, void* dgate, int64_t lddg,
-                                         float* dw1, float* db1, float* dw2, float* db2, void* workspace, size_t workspace_bytes,
-                                         dh_stream_t stream) {
-  const char* me = "dh_residual_norm_backward";
-  const int rc = check_common(me, M, D, dtype, f, x, ldf, ldx, gate, ldg, gate_kind, gate_sigmoid, kind, 0.f);
+template <class T>
+void launch_columns(const Args& a, int64_t chunks, hipStream_t st) {
+  constexpr int V = Elem<T>::VEC;
+  const dim3 g((unsigned)dh::ceil_div(dh::ceil_div(a.D, V), 256), (unsigned)chunks), b(256);
+  const bool odd = a.D % V != 0, full = a.gate_kind == GATE_FULL;
+  if (full && odd) hipLaunchKernelGGL((wide_columns_kernel<T, V, true, ODD>), g, b, 0, st, a);
+  else if (full) hipLaunchKernelGGL((wide_columns_kernel<T, V, true, WHOLE>), g, b, 0, st, a);
+  else if (odd) hipLaunchKernelGGL((wide_columns_kernel<T, V, false, ODD>), g, b, 0, st, a);
+  else hipLaunchKernelGGL((wide_columns_kernel<T, V, false, WHOLE>), g, b, 0, st, a);
+}
+
+int backward(const char* me, bool wide, int64_t M, int64_t D, int dtype, const void* f, int64_t ldf, const void* x, int64_t ldx, const void* gate, int64_t ldg,
+             int gate_kind, int gate_sigmoid, float scale, int kind, int has_post, const float* w1, const float* b1, int has_pre, const float* w2,
+             const float* stats, const void* dr, int64_t lddr, const void* dhh, int64_t lddh, void* df, int64_t lddf, void* dx, int64_t lddx, void* dgate,
+             int64_t lddg, float* dw1, float* db1, float* dw2, float* db2, void* workspace, size_t workspace_bytes, dh_stream_t stream) {
+  const int rc = check_common(me, wide, M, D, dtype, f, x, ldf, ldx, gate, ldg, gate_kind, gate_sigmoid, kind, 0.f, has_post, has_pre);
   if (rc != DH_OK) return rc;
   if ((!has_post && (dw1 || db1)) || (!has_pre && (dw2 || db2)) || (gate_kind == GATE_NONE && dgate))
     return dh::fail(DH_ERR_INVALID, "%s: the gradient of a parameter that is not there", me);
@@ -762,8 +858,9 @@ extern "C" int dh_residual_norm_backward(int64_t M, int64_t D, int dtype, const 
   if ((dr && lddr < D) || (dhh && lddh < D) || (df && lddf < D) || (dx && lddx < D) || (gate_kind == GATE_FULL && dgate && lddg < D) ||
       (gate_kind == GATE_ROW && dgate && lddg < 1))
     return dh::fail(DH_ERR_INVALID, "%s: leading dimension below the row length", me);
-  const size_t need = dh_residual_norm_backward_workspace_bytes(M, D);
+  const size_t need = workspace_bytes_of(M, D);
   if (!workspace || workspace_bytes < need) return dh::fail(DH_ERR_WORKSPACE, "%s: workspace of %zu bytes, need %zu", me, workspace_bytes, need);
+  if (wide && !dh::aligned16(workspace)) return dh::fail(DH_ERR_INVALID, "%s: workspace must be 16-byte aligned", me);
   Args a{};
   a.M = M; a.D = (int)D; a.gate_kind = gate_kind; a.gate_sigmoid = gate_sigmoid; a.rms = kind == DH_NORM_RMS;
   a.has_post = has_post != 0; a.has_pre = has_pre != 0; a.scale = scale; a.inv_d = 1.f / (float)D;
@@ -777,7 +874,15 @@ extern "C" int dh_residual_norm_backward(int64_t M, int64_t D, int dtype, const 
   const int vw = dtype == DH_DTYPE_BF16 ? 8 : 4;
   const Split s = split_of(D, vw);
   a.tpr = s.tpr;
-  const int64_t grid = dtype == DH_DTYPE_BF16 ? launch_t<uint16_t>(true, a, s, st) : launch_t<float>(true, a, s, st);
+  const bool columns = a.want_w1 || a.want_b1 || a.want_w2 || a.want_b2 || a.want_gate;
+  if (wide && columns) a.terms = reinterpret_cast<float2*>(static_cast<char*>(workspace) + (partials_bytes(M, D) + 15) / 16 * 16);
+  int64_t grid = dtype == DH_DTYPE_BF16 ? launch_t<uint16_t>(true, a, s, st) : launch_t<float>(true, a, s, st);
+  if (wide && columns) {
+    a.rows = dh::ceil_div(M, WIDE_CHUNKS);
+    grid = dh::ceil_div(M, a.rows);
+    if (dtype == DH_DTYPE_BF16) launch_columns<uint16_t>(a, grid, st);
+    else launch_columns<float>(a, grid, st);
+  }
   ReduceArgs ra{};
   ra.partials = a.partials; ra.n_blocks = (int)grid; ra.D = (int)D;
   int slots = 0;
@@ -785,10 +890,32 @@ extern "C" int dh_residual_norm_backward(int64_t M, int64_t D, int dtype, const 
   if (a.want_b1) ra.out[slots++] = db1;
   if (a.want_w2) ra.out[slots++] = dw2;
   if (a.want_b2) ra.out[slots++] = db2;
-  float* gate_cols = a.partials + (int64_t)5 * (M < BWD_BLOCKS ? M : BWD_BLOCKS) * D;
+  float* gate_cols = a.partials + 5 * std::min<int64_t>(M, BWD_BLOCKS) * D;
   if (a.want_gate) ra.out[slots++] = gate_kind == GATE_SCALAR ? gate_cols : static_cast<float*>(dgate);
   if (slots > 0) hipLaunchKernelGGL(column_reduce_kernel, dim3((unsigned)dh::ceil_div(D, 64), (unsigned)slots), dim3(1024), 0, st, ra);
   if (a.want_gate && gate_kind == GATE_SCALAR)
     hipLaunchKernelGGL(sum_kernel, dim3(1), dim3(256), 0, st, gate_cols, (int)D, static_cast<float*>(dgate));
   return dh::check_launch(me);
 }
+
+}  // namespace
+
+#define FORWARD_PARAMS                                                                                                                                       \
+  int64_t M, int64_t D, int dtype, const void *f, int64_t ldf, const void *x, int64_t ldx, const void *gate, int64_t ldg, int gate_kind, int gate_sigmoid,   \
+      float scale, int kind, float eps, int has_post, const float *w1, const float *b1, int has_pre, const float *w2, const float *b2, void *r, int64_t ldr, \
+      void *h, int64_t ldh, float *stats, dh_stream_t stream
+#define FORWARD_ARGS M, D, dtype, f, ldf, x, ldx, gate, ldg, gate_kind, gate_sigmoid, scale, kind, eps, has_post, w1, b1, has_pre, w2, b2, r, ldr, h, ldh, stats, stream
+#define BACKWARD_PARAMS                                                                                                                                      \
+  int64_t M, int64_t D, int dtype, const void *f, int64_t ldf, const void *x, int64_t ldx, const void *gate, int64_t ldg, int gate_kind, int gate_sigmoid,   \
+      float scale, int kind, int has_post, const float *w1, const float *b1, int has_pre, const float *w2, const float *stats, const void *dr, int64_t lddr, \
+      const void *dhh, int64_t lddh, void *df, int64_t lddf, void *dx, int64_t lddx, void *dgate, int64_t lddg, float *dw1, float *db1, float *dw2,          \
+      float *db2, void *workspace, size_t workspace_bytes, dh_stream_t stream
+#define BACKWARD_ARGS                                                                                                                                        \
+  M, D, dtype, f, ldf, x, ldx, gate, ldg, gate_kind, gate_sigmoid, scale, kind, has_post, w1, b1, has_pre, w2, stats, dr, lddr, dhh, lddh, df, lddf, dx,     \
+      lddx, dgate, lddg, dw1, db1, dw2, db2, workspace, workspace_bytes, stream
+
+extern "C" int dh_residual_norm_forward(FORWARD_PARAMS) { return forward("dh_residual_norm_forward", false, FORWARD_ARGS); }
+extern "C" int dh_residual_norm_wide_forward(FORWARD_PARAMS) { return forward("dh_residual_norm_wide_forward", true, FORWARD_ARGS); }
+extern "C" size_t dh_residual_norm_backward_workspace_bytes(int64_t M, int64_t D) { return workspace_bytes_of(M, D); }
+extern "C" int dh_residual_norm_backward(BACKWARD_PARAMS) { return backward("dh_residual_norm_backward", false, BACKWARD_ARGS); }
+extern "C" int dh_residual_norm_wide_backward(BACKWARD_PARAMS) { return backward("dh_residual_norm_wide_backward", true, BACKWARD_ARGS); }

@@ -861,6 +861,7 @@ def gemm_grouped_wgrad(dY: torch.Tensor, X: torch.Tensor, group_ptr: torch.Tenso
 NORM_LAYER, NORM_RMS = 0, 1
 GATE_NONE, GATE_SCALAR, GATE_CHANNEL, GATE_ROW, GATE_FULL = 0, 1, 2, 3, 4
 RESIDUAL_NORM_MAX_COLUMNS = 4096
+RESIDUAL_NORM_WIDE_COLUMNS = 8192  # with one of the norms
 
 
 def residual_norm_gate_kind(gate: Optional[torch.Tensor], M: int, D: int) -> int:
@@ -912,15 +913,16 @@ def residual_norm_forward(f: torch.Tensor, x: Optional[torch.Tensor] = None, *, 
                           want_stats: bool = False):
     """(r, h, stats): r = x + scale * act(gate) * post(f), h = pre(r) (None without ``pre``); see dh_residual_norm_forward.
 
-    f, x [M, D] fp32 or bf16, D <= 4096; ``post`` / ``pre``: None or (weight, bias), fp32 [D] or None each; gate: residual_norm_gate_kind
+    f, x [M, D] fp32 or bf16, D <= 8192 (4096 without either norm); ``post`` / ``pre``: None or (weight, bias), fp32 [D] or None each; gate: residual_norm_gate_kind
     (scalar and channel gates fp32, the others of f's dtype).  stats [M, 4] fp32 is what residual_norm_backward needs."""
     lib = _lib_ready()
     dt = _elem(f, "f")
     if f.dim() != 2:
         raise ValueError(f"f must be 2-d, got shape {tuple(f.shape)}")
     M, D = f.shape
-    if not 1 <= D <= RESIDUAL_NORM_MAX_COLUMNS:
-        raise ValueError(f"residual_norm: rows of 1 .. {RESIDUAL_NORM_MAX_COLUMNS} columns, got {D}")
+    most = RESIDUAL_NORM_MAX_COLUMNS if post is None and pre is None else RESIDUAL_NORM_WIDE_COLUMNS
+    if not 1 <= D <= most:
+        raise ValueError(f"residual_norm: rows of 1 .. {most} columns, got {D}")
     if kind not in (NORM_LAYER, NORM_RMS) or not eps >= 0:
         raise ValueError(f"residual_norm: kind {kind}, eps {eps}")
     _check_rows(x, f, "x")
@@ -934,7 +936,8 @@ def residual_norm_forward(f: torch.Tensor, x: Optional[torch.Tensor] = None, *, 
     h = f.new_empty((M, D)) if has_pre else None
     stats = torch.empty((M, 4), dtype=torch.float32, device=f.device) if want_stats else None
     with _one_device(f, x, gate, *(post or ()), *(pre or ())):
-        _call("residual_norm_forward", lib.dh_residual_norm_forward, M, D, dt, fp, ldf, xp, ldx, gp, ldg, gk, 1 if gate_sigmoid else 0, scale, kind, eps,
+        entry = lib.dh_residual_norm_forward if D <= RESIDUAL_NORM_MAX_COLUMNS else lib.dh_residual_norm_wide_forward
+        _call("residual_norm_forward", entry, M, D, dt, fp, ldf, xp, ldx, gp, ldg, gk, 1 if gate_sigmoid else 0, scale, kind, eps,
               has_post, w1, b1, has_pre, w2, b2, r.data_ptr(), D, None if h is None else h.data_ptr(), D,
               None if stats is None else stats.data_ptr(), _stream())
     return r, h, stats
@@ -995,7 +998,8 @@ def residual_norm_backward_unchecked(dr, dh, f, x, stats, post, gate, gate_kind,
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=f.device)
     at = lambda t: None if t is None else t.data_ptr()
     ld = lambda t: 0 if t is None else t.stride(0) if M > 1 else D
-    _call("residual_norm_backward", lib.dh_residual_norm_backward, M, D, _ELEM[f.dtype], f.data_ptr(), ld(f), at(x), ld(x), at(gate),
+    entry = lib.dh_residual_norm_backward if D <= RESIDUAL_NORM_MAX_COLUMNS else lib.dh_residual_norm_wide_backward
+    _call("residual_norm_backward", entry, M, D, _ELEM[f.dtype], f.data_ptr(), ld(f), at(x), ld(x), at(gate),
           (ld(gate) if gate_kind == GATE_FULL else gate.stride(0) if M > 1 else 1) if gate_kind >= GATE_ROW else 0, gate_kind, 1 if gate_sigmoid else 0,
           scale, kind, 0 if post is None else 1, at(w1), at(b1), 0 if pre is None else 1, at(w2), stats.data_ptr(), at(dr), ld(dr), at(dh), ld(dh),
           p("f"), D, p("x"), D, p("gate"), D if gate_kind == GATE_FULL else 1, p("w1"), p("b1"), w2_wanted, b2_wanted, ws.data_ptr(), ws_bytes, _stream())

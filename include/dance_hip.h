@@ -877,17 +877,27 @@ DH_API int dh_grad_clip(int n, const void* const* grads_host, void* const* out_h
  * parameters are f32.  gate_kind: dh_gate; gate_sigmoid: act = sigmoid.  kind: dh_norm.  stats [M, 4] f32 (16-byte aligned; NULL: not
  * kept): mean and rstd of both norms, what the backward needs.  r may be NULL when has_pre.
  * Backward: dr, dh (either may be NULL) -> df, dx, dgate (row / full: dtype; scalar / channel: f32) and the column sums dw1, db1, dw2,
- * db2 (f32), each skipped when NULL; sums over rows in a fixed order.  No output may overlap an input.                                    */
+ * db2 (f32), each skipped when NULL; sums over rows in a fixed order.  No output may overlap an input.
+ * The wide entries are the same for 4096 < D <= 8192 and at least one of the norms (workspace 16-byte aligned).                          */
 DH_API int dh_residual_norm_forward(int64_t M, int64_t D, int dtype, const void* f, int64_t ldf, const void* x, int64_t ldx, const void* gate,
                              int64_t ldg, int gate_kind, int gate_sigmoid, float scale, int kind, float eps, int has_post, const float* w1,
                              const float* b1, int has_pre, const float* w2, const float* b2, void* r, int64_t ldr, void* h, int64_t ldh,
                              float* stats, dh_stream_t stream);
+DH_API int dh_residual_norm_wide_forward(int64_t M, int64_t D, int dtype, const void* f, int64_t ldf, const void* x, int64_t ldx, const void* gate,
+                                  int64_t ldg, int gate_kind, int gate_sigmoid, float scale, int kind, float eps, int has_post, const float* w1,
+                                  const float* b1, int has_pre, const float* w2, const float* b2, void* r, int64_t ldr, void* h, int64_t ldh,
+                                  float* stats, dh_stream_t stream);
 DH_API size_t dh_residual_norm_backward_workspace_bytes(int64_t M, int64_t D);
 DH_API int dh_residual_norm_backward(int64_t M, int64_t D, int dtype, const void* f, int64_t ldf, const void* x, int64_t ldx, const void* gate,
                               int64_t ldg, int gate_kind, int gate_sigmoid, float scale, int kind, int has_post, const float* w1,
                               const float* b1, int has_pre, const float* w2, const float* stats, const void* dr, int64_t lddr, const void* dh,
                               int64_t lddh, void* df, int64_t lddf, void* dx, int64_t lddx, void* dgate, int64_t lddg, float* dw1, float* db1,
                               float* dw2, float* db2, void* workspace, size_t workspace_bytes, dh_stream_t stream);
+DH_API int dh_residual_norm_wide_backward(int64_t M, int64_t D, int dtype, const void* f, int64_t ldf, const void* x, int64_t ldx, const void* gate,
+                                   int64_t ldg, int gate_kind, int gate_sigmoid, float scale, int kind, int has_post, const float* w1,
+                                   const float* b1, int has_pre, const float* w2, const float* stats, const void* dr, int64_t lddr, const void* dh,
+                                   int64_t lddh, void* df, int64_t lddf, void* dx, int64_t lddx, void* dgate, int64_t lddg, float* dw1, float* db1,
+                                   float* dw2, float* db2, void* workspace, size_t workspace_bytes, dh_stream_t stream);
 
 /* ---- products grouped by row type with ragged sizes (gemm_grouped.hip) ---------------------------------------------------------------------
  * dance/models/nn/gnn.py:84-96 and scdeepsort.py:26-88 apply one Linear to every node; with typed nodes (genes / cells, tissues, donors)
