@@ -511,6 +511,12 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256) void residual_norm_backw
       for (int i = 0; i < E; ++i) {
         const float n = __builtin_fmaf(f[i], w[i], b[i]);
         x[i] = (__builtin_fmaf(a.scale * gf[i], n, x[i]) - st.z) * st.w;  // rhat
+      }
+      // behind the end of a bf16 row of odd length the features stand beside other columns' gate and parameters: a product that no column
+      // has, and that may be infinite where all of theirs are finite
+      if constexpr (TAIL == ODD && sizeof(T) == 2) zero_tail<V, CH, TAIL>(t, tpr, a.D, x);
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
         if constexpr (COLUMNS) {
           if (valid) {
             acc_w2[i] = __builtin_fmaf(dh[i], x[i], acc_w2[i]);
