@@ -7,6 +7,7 @@ wrappers never copy to the host and never compute on the CPU.
 from typing import Optional, Tuple
 
 import contextlib
+import math
 import operator
 import os
 
@@ -1358,6 +1359,64 @@ def _refuse_overlap(begins, ends):
         raise ValueError("clip_grads: tensors overlap in memory (the same tensor given twice, or views of one)")
 
 
+def _window(t: torch.Tensor):
+    """(first byte, extent, outer dimensions as (step, count) from the widest on, length of the innermost run) of the memory that a tensor
+    holds, in bytes; dimensions that follow one another without a gap are one, an expanded one holds nothing more.  None without elements."""
+    if t.numel() == 0:
+        return None
+    run, outer = t.element_size(), []
+    for step, count in sorted((s * t.element_size(), n) for n, s in zip(t.shape, t.stride()) if n > 1 and s > 0):
+        if not outer and step == run:
+            run *= count
+        elif outer and step == outer[-1][0] * outer[-1][1]:
+            outer[-1] = (outer[-1][0], outer[-1][1] * count)
+        else:
+            outer.append((step, count))
+    extent, nested = run, True
+    for step, count in outer:
+        nested &= step >= extent
+        extent += step * (count - 1)
+    if not nested:  # rows that run into each other: all that lies between the first and the last element
+        run, outer = extent, []
+    return t.data_ptr(), extent, tuple(reversed(outer)), run, nested
+
+
+def _meet(a: int, dims_a, run_a: int, b: int, dims_b, run_b: int) -> bool:
+    """Whether two windows hold a common byte.  The one with the wider rows is taken apart row by row, against the other's rows that lie there;
+    rows of equal steps are compared by their distance alone."""
+    extent = lambda dims, run: run + sum(step * (count - 1) for step, count in dims)
+    end_a, end_b = a + extent(dims_a, run_a), b + extent(dims_b, run_b)
+    if a >= end_b or b >= end_a:
+        return False
+    if not dims_a and not dims_b:
+        return True
+    if not dims_a or (dims_b and dims_b[0][0] > dims_a[0][0]):
+        a, dims_a, run_a, b, dims_b, run_b, end_b = b, dims_b, run_b, a, dims_a, run_a, end_a
+    step, count = dims_a[0]
+    inner = extent(dims_a[1:], run_a)
+    if dims_b and dims_b[0][0] == step:  # rows i of a and j of b: k = i - j
+        most = count - 1
+        least, end, dims_b = 1 - dims_b[0][1], b + extent(dims_b[1:], run_b), dims_b[1:]
+    else:
+        least, most, end = 0, count - 1, end_b
+        if dims_b:  # the rows repeat their places among b's after `period` of them; twice that many hold every pair of places that occurs
+            period = dims_b[0][0] // math.gcd(step, dims_b[0][0])
+            most = min(most, max(0, (b - a - inner) // step + 1) + 2 * period + 2)
+    first = max(least, (b - a - inner) // step + 1)
+    return any(_meet(a + k * step, dims_a[1:], run_a, b, dims_b, run_b) for k in range(first, min(most, (end - a - 1) // step) + 1))
+
+
+def _refuse_shared_windows(tensors):
+    """No two of the tensors may hold a common byte, whatever their layout; interleaved ones (column slices of one buffer) may stand."""
+    windows = sorted(w for w in map(_window, tensors) if w is not None)
+    for i, (a, extent, dims, run, _) in enumerate(windows):
+        for b, _, dims_b, run_b, _ in windows[i + 1:]:
+            if b >= a + extent:
+                break
+            if _meet(a, dims, run, b, dims_b, run_b):
+                raise ValueError("clip_grads: tensors overlap in memory (the same tensor given twice, or views of one)")
+
+
 def _norm_tables(tensors, name: str):
     """Host tables of a tensor list: addresses, sizes, dtypes."""
     n = len(tensors)
@@ -1396,7 +1455,7 @@ def clip_grads(grads, max_norm: float, *, norm_type: float = 2.0, out=None) -> t
     """Scale ``grads`` (fp32 / bf16 tensors) by min(1, max_norm / (norm + 1e-6)), norm = their global norm, which is returned as an fp32 scalar
     on the device: in place, or into the tensors of ``out`` (fp32 or bf16 each, as many elements as their gradient: e.g. the views of the
     flat fp32 buffer that an optimiser works on).  Apart from a gradient and its own output no two tensors may share memory (the same one
-    twice is refused).  Nothing waits for the device.  See dh_grad_clip."""
+    twice and overlapping slices are refused, slices that only interleave are not).  Nothing waits for the device.  See dh_grad_clip."""
     lib = _lib_ready()
     code = _norm_type(norm_type)
     max_norm = float(max_norm)
@@ -1441,12 +1500,16 @@ def clip_grads(grads, max_norm: float, *, norm_type: float = 2.0, out=None) -> t
 def _consecutive(grads, targets):
     """(inputs, outputs, copies to make afterwards) with consecutive elements in matching order: tensors that are so are taken as they are,
     the others (column slices, outputs in another order than their gradient) go through contiguous copies."""
+    alike = [g is o or (g.data_ptr() == o.data_ptr() and g.dtype == o.dtype and g.shape == o.shape and g.stride() == o.stride())
+             for g, o in zip(grads, targets)]
+    for o in targets:
+        window = _window(o)
+        if any(n > 1 and s == 0 for n, s in zip(o.shape, o.stride())) or (window and not window[-1]):
+            raise ValueError("clip_grads: a tensor whose elements share memory (an expanded one) cannot be written")
+    _refuse_shared_windows([*targets, *(g for g, same in zip(grads, alike) if not same)])  # (the copies below would hide it)
     src, dst, back = [], [], []
-    for g, o in zip(grads, targets):
-        same = g is o or (g.data_ptr() == o.data_ptr() and g.dtype == o.dtype and g.shape == o.shape and g.stride() == o.stride())
+    for g, o, same in zip(grads, targets, alike):
         flat = _is_dense(g)
-        if any(n > 1 and s == 0 for n, s in zip(o.shape, o.stride())):
-            raise ValueError("clip_grads: an expanded tensor cannot be written")
         if flat and (same or (g.is_contiguous() and o.is_contiguous()) or (g.shape == o.shape and g.stride() == o.stride())):
             src.append(g)
             dst.append(g if same else o)
