@@ -1358,7 +1358,7 @@ extern "C" int dh_gemm_grouped(int64_t M, int64_t N, int64_t K, int64_t G, int t
   if (y_dtype != DH_DTYPE_F32 && y_dtype != DH_DTYPE_BF16) return dh::fail(DH_ERR_INVALID, "%s: output dtype %d", me, y_dtype);
   if (act != DH_ACT_NONE && act != DH_ACT_RELU) return dh::fail(DH_ERR_INVALID, "%s: activation %d", me, act);
   if (M == 0 || N == 0) return DH_OK;
-  if (!Y || (G > 0 && !group_ptr) || (K > 0 && (!X || (G > 0 && !W)))) return dh::fail(DH_ERR_INVALID, "%s: null tensor", me);
+  if (!Y || !group_ptr || (K > 0 && (!X || (G > 0 && !W)))) return dh::fail(DH_ERR_INVALID, "%s: null tensor", me);
   const int64_t wc = trans_b ? K : N;
   if (ldx < K || ldw < wc || ldy < N || (bias && ld_bias < N) || (G > 1 && stride_w < 0)) return dh::fail(DH_ERR_INVALID, "%s: leading dimension below the row length", me);
   FwdArgs a{};
