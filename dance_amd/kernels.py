@@ -76,7 +76,7 @@ def _dev(t: Optional[torch.Tensor], dtype, name: str, ndim: Optional[int] = None
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
     if ndim is not None and t.dim() != ndim:
         raise ValueError(f"{name} must be {ndim}-d, got shape {tuple(t.shape)}")
-    if t.dim() >= 1 and t.numel() > 0 and t.stride(-1) != 1:
+    if t.dim() >= 1 and t.numel() > 0 and t.stride(-1) != 1 and (t.dim() == 1 or t.shape[-1] > 1):  # (a single column's step means nothing)
         raise ValueError(f"{name} must be contiguous in its last dimension")
     if t.dim() == 1 and not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
