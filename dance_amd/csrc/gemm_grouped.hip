@@ -506,6 +506,12 @@ __device__ __forceinline__ void images_ready() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LATER) : "memory");
 }
 
+// Between LDS writes of a wave and reads of what its other lanes wrote: the hardware keeps a wave's LDS accesses in order, the compiler is told to.
+__device__ __forceinline__ void lanes_exchange() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 // Schedule of a step: its first fragments are in registers when it begins; the fragments of k group kk + 1 are read while the products of
 // group kk run, the barrier that hands over the next image stands in front of the LAST group, and behind it the next step's first fragments
 // are read and the image just emptied is requested again, STAGES steps ahead: a wave never waits for LDS with nothing to multiply.
@@ -699,6 +705,7 @@ struct DmaTile {
             if (BF16) *reinterpret_cast<u32x2*>(out + r * 128 + (((col >> 3) ^ x) << 4) + (col & 4) * 2) = u32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
             else *reinterpret_cast<f32x4*>(out + r * 128 + (((col >> 2) ^ x) << 4)) = v;
           }
+        lanes_exchange();
 #pragma unroll
         for (int it = 0; it < 4; ++it) {
           const int row = it * 8 + (lane >> 3), c = lane & 7, m = i * 32 + row, n = jj * 32 + c * (16 / SIZE);
@@ -716,6 +723,7 @@ struct DmaTile {
             }
           }
         }
+        lanes_exchange();  // the next rows are written over these
       }
     }
   }
