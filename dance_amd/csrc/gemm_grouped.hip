@@ -80,8 +80,7 @@ __device__ __forceinline__ int search(int n, int64_t s, Key key) {
 
 struct Slot {
   int group;       // -1: rows that belong to no group
-  int64_t begin, end, start;  // the slot's rows; start: the group's first row
-  int index;       // number of the slot within its group
+  int64_t begin, end;  // the slot's rows
   bool live;
 };
 
@@ -93,11 +92,9 @@ __device__ __forceinline__ Slot find_slot(const Groups& gr, int64_t s, int shift
   const int64_t first = (a >> shift) + i;
   Slot r;
   r.group = i == 0 || i == n - 1 ? -1 : i - 1;
-  r.start = a;
-  r.index = (int)(s - first);
-  r.begin = a + ((int64_t)r.index << shift);
+  r.begin = a + ((s - first) << shift);
   r.end = min(b, r.begin + ((int64_t)1 << shift));
-  r.live = r.index >= 0 && r.begin < b;
+  r.live = s >= first && r.begin < b;
   return r;
 }
 
