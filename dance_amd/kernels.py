@@ -1536,8 +1536,8 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_i
     if error_if_nonfinite:
         norm = global_norm(grads, norm_type)
         if not bool(torch.isfinite(norm)):
-            raise RuntimeError(f"The total norm of order {norm_type} for gradients from `parameters` is non-finite, so it cannot be clipped. To "
-                               "disable this error and scale the gradients by the non-finite norm anyway, set `error_if_nonfinite=False`")
+            raise RuntimeError(f"clip_grad_norm_: the gradients' global norm (norm_type {norm_type}) is non-finite; nothing was scaled.  Without "
+                               "error_if_nonfinite a NaN or infinite norm goes into the factor")
     return clip_grads(grads, max_norm, norm_type=norm_type)
 
 
