@@ -9,10 +9,11 @@
 // ceil(len / R) tiles and monotone in g, so a workgroup finds its group with one 64-wide search per 64 groups instead of a prefix sum;
 // at most one slot per group and none of the work is wasted on it.
 //
-// Bound: the matrix cores for many rows (200003 rows of 9 types, 2000 -> 512 bf16: Y 505 us, dX 630, dW and db 470 + 32: 810 / 650 / 870 TFLOP/s;
+// Bound: the matrix cores, and what they wait for at a tile's start and end, for many rows (200003 rows of 9 types, 2000 -> 512 bf16: Y 501 us, dX 616, dW
+// and db 476 + 31: 820 / 665 / 860 TFLOP/s, the cores busy 38 / 30 / 40 % of the cycles;
 // fp32 100003 rows: 125 / 122 / 134 TFLOP/s), latency for few (16 rows of 8 types, 400 -> 200: 7.3 us; 500 rows of 17 types, forward and all
 // gradients: 33 us in four launches).  Four kernels: a tile filled by LDS DMA for aligned operands, one staged through registers for the
-// others and for few columns (60000 x 401 -> 203 bf16 172 us for the three products, 104 at 400 -> 200), one of 32 x 32 with K split over the
+// others and for few columns (60000 x 401 -> 203 bf16 169 us for the three products, 97 at 400 -> 200), one of 32 x 32 with K split over the
 // waves for few rows, and the weight gradient's, which cuts the rows into chunks of equal work whatever the groups.
 #include <algorithm>
 #include <atomic>
@@ -514,7 +515,8 @@ __device__ __forceinline__ void lanes_exchange() {
 // are read and the image just emptied is requested again, STAGES steps ahead: a wave never waits for LDS with nothing to multiply.
 // begin() requests a tile's first steps, main() multiplies, store() writes the result out of an LDS region of its own, so that the next
 // tile's begin() runs before this one's store(): with one workgroup on a CU nothing else would fill these gaps (measured in cycles at
-// 200003 rows, 2000 -> 512, per tile: first request to first product 8500, 32 steps 107000, stores 16000 before they were made cheap).
+// 200003 rows, 2000 -> 512, per tile: first request to first product 8500, 32 steps 107000, stores 16000 before they went out as whole row pieces; dX
+// there, 24.7 tiles a CU of eight steps each, takes 1.33 M cycles, of which its steps at that pace are about half).
 template <class T, bool A_KM, bool B_KM, int MI, int NI, int WR, int WC>
 struct DmaTile {
   static constexpr int STAGES = 2, BM = MI * WR * 32, BN = NI * WC * 32, THREADS = WR * WC * 64, BK = 128 / sizeof(T);
@@ -1270,7 +1272,7 @@ int forward_pick(const char* me, const FwdArgs& a, hipStream_t st) {
   const int64_t few = a.N <= NARROW ? (BF16 ? 400 : 700) : BF16 ? 640 : dma ? 420 : 1536;
   if (small_tiles <= few) return small_launch<T, W_KM>(me, a, st);
   // Few rows per group: fp32 4000 rows of 100 types, 2000 -> 512: 302 us against 383.  (bf16 the same: 148 against 107: there the DMA tile
-  // stays ahead.)
+  // stays ahead.  Measured at that K; with K = 200 and 6 rows a group, 700 groups -> 64, it takes 13.5 us, and 32-row tiles took 12.2.)
   if (a.gr.M <= (int64_t)48 * a.gr.G && !(BF16 && dma)) return small_launch<T, W_KM>(me, a, st);
   if (a.N <= NARROW) return forward_launch<T, Tile<T, false, W_KM, 1, 1, 4, 1>>(me, a, st);
   if (dma) {

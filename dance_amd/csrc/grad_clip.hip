@@ -5,10 +5,10 @@
 //   out_t[i] = g_t[i] * min(1, max_norm / (norm + 1e-6))
 //
 // Bound: HBM.  The scaling cannot start before the norm is known, so a set larger than the caches is read twice and written once: 328 million
-// fp32 elements in 32 tensors 243 us (5.4 TB/s) and 515 us (5.1 TB/s).  The launches and their latencies for small ones: 2000 x 512, 512 x 30
+// fp32 elements in 32 tensors 246 us (5.3 TB/s) and 518 us (5.1 TB/s).  The launches and their latencies for small ones: 2000 x 512, 512 x 30
 // and their biases 9 us, 320 tensors of at most 200 x 64 30 us.
 // Layout: the tensors' addresses travel as kernel arguments, 128 per launch (nothing is uploaded, so a captured call replays with the
-// addresses it was recorded with); a launch walks its tensors in chunks of 16 KB of fp32, up to GRID workgroups striding over the chunks.
+// addresses it was recorded with); a launch walks its tensors in chunks of 16 KB of fp32, up to GRID workgroups (2 GRID for the scaling) striding over the chunks.
 // Sums are double from the first product (the conversions and fp64 FMAs cost 2 of ~16 issue slots that a 16-byte load leaves) and are
 // joined in a fixed order: the result does not depend on timing.  Every workgroup of the scaling launch joins the partial sums itself
 // (<= 8 KB from the L2) instead of waiting for a launch of its own to do it.
@@ -17,7 +17,7 @@
 namespace {
 
 constexpr int MAX_T = 128;        // tensors per launch: 128 x (8 + 8 + 8 + 4) bytes of kernel arguments stay under 4 KB
-constexpr int GRID = 1024;        // workgroups per launch at most = partial sums per launch
+constexpr int GRID = 1024;        // workgroups of a norm launch at most = its partial sums
 constexpr int THREADS = 256;
 constexpr int CHUNK = 4096;       // elements of one workgroup's pass over a chunk: 16 per thread
 constexpr int INLINE_PARTIALS = 1024;  // up to here the scaling workgroups join the partial sums themselves

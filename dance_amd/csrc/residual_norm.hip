@@ -19,7 +19,7 @@
 // gradients are summed in registers over the rows a workgroup walks, joined in its LDS, written once per workgroup and added up by a second
 // kernel in workgroup order: no atomics, the result does not depend on timing.  All arithmetic is fp32; bf16 rounds once, at the stores.
 // Measured, layer norms and channel gate, forward / backward: 200003 x 512 bf16 165 / 282 us (5.0 / 4.4 TB/s), fp32 321 / 446 us (5.1 / 5.5);
-// 50001 x 504 bf16 41 / 76 us, x 500 (ODD) 50 / 94, x 501 54 / 101; 50001 x 1000 110 / 188.  The bf16 backward has the arithmetic of twice
+// 50001 x 504 bf16 37 / 76 us, x 500 (ODD) 50 / 95, x 501 53 / 101; 50001 x 1000 109 / 184.  The bf16 backward has the arithmetic of twice
 // as many elements to a byte and comes near the vector units' limit.
 // Wide rows (4097 .. 8192 columns, entries of their own): a workgroup of up to eight waves, sixteen elements a lane.  The backward takes one
 // workgroup for every row, without the column gradients, which would spill, and leaves two numbers a row; a second kernel walks the columns

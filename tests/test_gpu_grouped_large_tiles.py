@@ -4,7 +4,8 @@ Operands are small integers: every product, every partial sum and every result i
 exactly in whatever order they are added, and the results have to be the float64 ones to the last bit (a bf16 result: that value rounded once).
 
 Which kernel a size takes (gemm_grouped.hip: forward_pick, wgrad_plan): bf16 100003 x 1032 -> 520 both ways over the 256 x 256 tile (at least
-256 rows a type and 768 tiles), its weight gradient too (5913 positions a chunk); fp32 30011 x 1036 -> 1028 over the 128 x 128 tile (5056 positions a chunk); rows that are no multiple of 16 bytes over the tiles staged through registers."""
+256 rows a type and 768 tiles), its weight gradient too (5913 positions a chunk); fp32 30011 x 1036 -> 1028 over the 128 x 128 tile (5056
+positions a chunk); rows that are no multiple of 16 bytes over the tiles staged through registers."""
 import pytest
 import torch
 
