@@ -453,7 +453,8 @@ __global__ __launch_bounds__(MODE == GROUP ? 512 : 256) void residual_norm_backw
   for (int i = 0; i < A; ++i) acc_w1[i] = acc_b1[i] = acc_w2[i] = acc_b2[i] = acc_g[i] = 0.f;
   const bool col_gate = !FULL && (a.gate_kind == GATE_CHANNEL || a.gate_kind == GATE_SCALAR);
   const bool use_x = a.x && a.dh;  // r enters through the second norm only
-  for (int64_t base = (int64_t)blockIdx.x * rows_per_block; base < a.M; base += (int64_t)gridDim.x * rows_per_block) {
+  // (blockIdx.y: wide rows only)
+  for (int64_t base = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * rows_per_block; base < a.M; base += (int64_t)gridDim.x * rows_per_block) {
     const int64_t row = min(base + sub, a.M - 1);
     const bool valid = base + sub < a.M;
     float f[E], x[E], gf[E], dr[E], dh[E], w[E], b[E];
@@ -748,8 +749,9 @@ int64_t launch(bool backward, const Args& a, const Split& s, hipStream_t st) {
   if (!backward) fit = std::min(fit, 20 / ((int)b.x / 64));
   int64_t resident = (int64_t)256 * fit;
   if (backward && resident > BWD_BLOCKS) resident = BWD_BLOCKS;
-  const int64_t grid = backward && V * CH > 8 ? a.M : even_grid(a.M, rows_per_block(s), resident);
-  const dim3 g((unsigned)grid);
+  const bool every_row = backward && V * CH > 8;  // wide rows, in two dimensions: one holds less than 2^32 threads
+  const int64_t grid = every_row ? std::min<int64_t>(a.M, 1 << 20) : even_grid(a.M, rows_per_block(s), resident);
+  const dim3 g((unsigned)grid, every_row ? (unsigned)dh::ceil_div(a.M, grid) : 1u);
   if (backward) hipLaunchKernelGGL((residual_norm_backward_kernel<T, V, CH, MODE, FULL, TAIL>), g, b, 0, st, a);
   else hipLaunchKernelGGL((residual_norm_forward_kernel<T, V, CH, MODE, FULL, TAIL>), g, b, 0, st, a);
   return grid;

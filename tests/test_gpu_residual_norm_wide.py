@@ -135,3 +135,22 @@ def test_no_rows_and_refusals(cuda_device):
         residual_norm(torch.zeros(2, 8193, device=DEV), post=(None, None))
     with pytest.raises(ValueError, match="4096"):
         residual_norm(torch.zeros(2, 5000, device=DEV), torch.zeros(2, 5000, device=DEV), gate=torch.zeros(2, 1, device=DEV))
+
+
+def test_more_rows_than_one_grid_dimension(cuda_device):
+    """The rows of the backward lie on two grid dimensions of 2^20 workgroups in the first: rows on both sides of that border."""
+    from dance_amd import kernels
+    M, D = 2**20 + 3, 4097
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    f = torch.empty(M, D, dtype=torch.bfloat16, device=DEV).normal_(generator=gen)
+    dr = torch.empty_like(f).normal_(generator=gen)
+    gate = torch.full((M, 1), 0.5, dtype=torch.bfloat16, device=DEV)
+    w = torch.ones(D, device=DEV)
+    r, _, stats = kernels.residual_norm_forward(f, post=(w, None), gate=gate, want_stats=True)
+    g = kernels.residual_norm_backward(dr, None, f, None, stats, post=(w, None), gate=gate, want=("f", "gate"))
+    rows = torch.tensor([0, 1, 500_000, 2**20 - 1, 2**20, 2**20 + 1, 2**20 + 2], device=DEV)
+    v = dict(f=f[rows], x=None, gate=gate[rows], w1=w, b1=None, w2=None, b2=None, dr=dr[rows], dh=None)
+    ref = narrow._reference(v, "row", "none", "layer", 1.0, 1e-5)
+    narrow._check(r[rows], ref["r"], narrow.C_FWD, "r")
+    for k in ("f", "gate"):
+        narrow._check(g[k][rows], ref[k], narrow.C_BWD, k)
